@@ -1,0 +1,177 @@
+// w4_convert.cu - a matrix to 4-bit codes with group scales, and its values back.
+//
+// Per row and group m = max |w|, s = bf16(m / 7), code = 8 + clamp(round(w / s), -7, 7), halves to even, both roundings of s to
+// nearest even. The quotient is taken exactly: the product with 1 / s decides, and where it lies near a half the residual w - q s
+// does, which is exact there (q s has 12 significant bits; within half a step of it the difference loses none). A
+// division instead is twenty instructions a weight, as many as the SM can issue while HBM delivers an FP8 weight.
+//
+// Both directions are bound by HBM. A warp takes a piece of a row, a lane eight columns at a time (one word of codes), so that a
+// group is 4, 8 or 16 neighbouring lanes and its maximum two to four shuffles.
+#include "common.cuh"
+#include "w4.h"
+
+namespace g5b {
+
+constexpr int CV_WORDS = 128;      // words of codes (eight columns) a warp takes
+constexpr int CV_WARPS = 8;
+
+// Eight values from column c0 on (zero behind the last column); whole: 16-byte loads of eight that exist
+template <int DT>
+__device__ __forceinline__ void load8(float (&v)[8], const void *src, size_t at, int c0, int cols, bool whole)
+{
+    if (whole && c0 + 8 <= cols) {
+        if (DT == DT_F32) {
+            const float4 a = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at));
+            const float4 b = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at + 4));
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else if (DT == DT_BF16) {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(src) + at));
+            bf16x2_to_f32(a.x, v[0], v[1]); bf16x2_to_f32(a.y, v[2], v[3]); bf16x2_to_f32(a.z, v[4], v[5]); bf16x2_to_f32(a.w, v[6], v[7]);
+        } else {
+            const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(src) + at));
+            e4m3x4_to_f32(a.x, v[0], v[1], v[2], v[3]);
+            e4m3x4_to_f32(a.y, v[4], v[5], v[6], v[7]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = 0.f;
+        if (c0 + i < cols)
+            v[i] = DT == DT_F32 ? static_cast<const float *>(src)[at + i] : DT == DT_BF16 ? bf16_to_f32(static_cast<const uint16_t *>(src)[at + i])
+                                                                                       : e4m3_to_f32(static_cast<const uint8_t *>(src)[at + i]);
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uint8_t *codes, uint16_t *scales, const void *src, const float *inv,
+                                                                    int br, int bc, int scols, int pieces, bool whole)
+{
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * CV_WARPS + (threadIdx.x >> 5);
+    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
+    if (row >= w.rows) return;
+    const int per = w.group / 8, words = w.pitch / 4;
+    float v[CV_WORDS / 32][8];
+#pragma unroll
+    for (int i = 0; i < CV_WORDS / 32; i++) {
+        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
+        load8<DT>(v[i], src, (size_t)row * w.cols + c0, c0, w.cols, whole);
+        if (DT == DT_FP8) {
+            // the weight is the FP32 product of code and block scale
+            const float *irow = inv + (size_t)(row / br) * scols;
+            if (bc % 8 == 0) {
+                const float s = c0 < w.cols ? __ldg(irow + c0 / bc) : 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[i][k] = __fmul_rn(v[i][k], s);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) if (c0 + k < w.cols) v[i][k] = __fmul_rn(v[i][k], __ldg(irow + (c0 + k) / bc));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CV_WORDS / 32; i++) {
+        const int word = piece * CV_WORDS + i * 32 + lane;
+        // the largest magnitude as bits: infinities and NaN are above every number
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) m = max(m, __float_as_uint(v[i][k]) & 0x7fffffffu);
+        for (int o = 1; o < per; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const bool finite = m < 0x7f800000u;
+        const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
+        const float s = __bfloat162float(sb);
+        const bool live = finite && s > 0.f;
+        // 1 / s of a subnormal s may be infinite: the quotient is then taken of both times 2^64
+        const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
+        uint32_t packed = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float x = v[i][k] * up;
+            float q = rintf(__fmul_rn(x, r));
+            const float d = fmaf(-q, su, x), ad = fabsf(d);
+            // one step on where the residual is over half a step, or half a step and q odd
+            if (ad > half || (ad == half && ((int)q & 1))) q += copysignf(1.0f, d);
+            q = fminf(fmaxf(q, -7.0f), 7.0f);
+            packed |= (uint32_t)(live ? (int)q + 8 : 8) << (4 * k);
+        }
+        if (word < words) reinterpret_cast<uint32_t *>(codes + (size_t)row * w.pitch)[word] = packed;
+        const int group = word / per;
+        if ((word & (per - 1)) == 0 && group < w.sp)
+            scales[(size_t)row * w.sp + group] = group >= w.groups ? (uint16_t)0 : finite ? __bfloat16_as_ushort(sb) : (uint16_t)0x7fc0;
+    }
+}
+
+void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const float *scale, int br, int bc)
+{
+    // the pieces cover the codes' and the scales' padding too, so that no byte of either is left undefined
+    const int words = max(w.pitch / 4, w.sp * (w.group / 8)), pieces = (words + CV_WORDS - 1) / CV_WORDS;
+    const long long units = (long long)w.rows * pieces;
+    const int size = dt == DT_F32 ? 4 : dt == DT_BF16 ? 2 : 1;
+    const size_t align = dt == DT_FP8 ? 8 : 16;
+    const bool whole = (reinterpret_cast<uintptr_t>(src) % align) == 0 && ((size_t)w.cols * size) % align == 0;
+    uint8_t *codes = const_cast<uint8_t *>(w.codes);
+    uint16_t *scales = const_cast<uint16_t *>(w.scales);
+    const int grid = (int)((units + CV_WARPS - 1) / CV_WARPS), scols = bc > 0 ? (w.cols + bc - 1) / bc : 0;
+    if (dt == DT_F32)       G5B_LAUNCH(w4_quantize_kernel<DT_F32>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
+    else if (dt == DT_BF16) G5B_LAUNCH(w4_quantize_kernel<DT_BF16>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
+    else                    G5B_LAUNCH(w4_quantize_kernel<DT_FP8>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, void *out, size_t ldo, int pieces, bool whole)
+{
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * CV_WARPS + (threadIdx.x >> 5);
+    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
+    if (row >= w.rows) return;
+    uint32_t word[CV_WORDS / 32];
+    float s[CV_WORDS / 32];
+#pragma unroll
+    for (int i = 0; i < CV_WORDS / 32; i++) {
+        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
+        word[i] = 0; s[i] = 0.f;
+        if (c0 < w.cols) {
+            word[i] = __ldcs(reinterpret_cast<const uint32_t *>(w.codes + (size_t)row * w.pitch) + c0 / 8);
+            s[i] = bf16_to_f32(__ldg(w.scales + (size_t)row * w.sp + c0 / w.group));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CV_WORDS / 32; i++) {
+        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
+        if (c0 >= w.cols) continue;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = __fmul_rn((float)((int)((word[i] >> (4 * k)) & 15u) - 8), s[i]);
+        const size_t at = (size_t)row * ldo + c0;
+        if (DT == DT_F32) {
+            float *o = static_cast<float *>(out) + at;
+            if (whole && c0 + 8 <= w.cols) {
+                __stcs(reinterpret_cast<float4 *>(o), make_float4(v[0], v[1], v[2], v[3]));
+                __stcs(reinterpret_cast<float4 *>(o + 4), make_float4(v[4], v[5], v[6], v[7]));
+            } else
+                for (int k = 0; k < 8 && c0 + k < w.cols; k++) o[k] = v[k];
+        } else {
+            // (3 significant bits times 8: rounded to BF16's 8, halves to even)
+            __align__(16) __nv_bfloat16 h[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) h[k] = __float2bfloat16_rn(v[k]);
+            __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(out) + at;
+            if (whole && c0 + 8 <= w.cols) __stcs(reinterpret_cast<uint4 *>(o), *reinterpret_cast<const uint4 *>(h));
+            else
+                for (int k = 0; k < 8 && c0 + k < w.cols; k++) o[k] = h[k];
+        }
+    }
+}
+
+void w4_dequantize(cudaStream_t st, const W4Mat &w, void *out, int dt, size_t ldo)
+{
+    const int pieces = ((w.cols + 7) / 8 + CV_WORDS - 1) / CV_WORDS, size = dt == DT_F32 ? 4 : 2;
+    const long long units = (long long)w.rows * pieces;
+    const int grid = (int)((units + CV_WARPS - 1) / CV_WARPS);
+    const bool whole = (reinterpret_cast<uintptr_t>(out) % 16) == 0 && (ldo * size) % 16 == 0;
+    if (dt == DT_F32) G5B_LAUNCH(w4_dequantize_kernel<DT_F32>, grid, CV_WARPS * 32, 0, st, w, out, ldo, pieces, whole);
+    else              G5B_LAUNCH(w4_dequantize_kernel<DT_BF16>, grid, CV_WARPS * 32, 0, st, w, out, ldo, pieces, whole);
+}
+
+}  // namespace g5b

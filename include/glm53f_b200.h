@@ -7,7 +7,7 @@
  * that pass is made of (include/glm53f/glm53f.h:136-360). Nothing here takes or returns a
  * torch type; every argument is a plain pointer, size or handle.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *
  *   1. ENGINE      create / load / finalize / forward / reset / free. This is the contract
  *                  of the reference backend ABI (src/gpu/glm53f_gpu.h:38-50) with the
@@ -20,6 +20,9 @@
  *   3. DEVICE OPS  the same hot ops with device pointers and no copies, for callers that
  *                  already hold activations in HBM (the reference's gk_* launcher layer,
  *                  src/gpu/glm53f_gpu_kernels.h:18-93).
+ *   4. 4-BIT OPS   products with 4-bit weights and group scales, the conversion to them, tokens
+ *                  sorted by expert and back, and routed experts in 4 bits: device pointers, a
+ *                  stream and a workspace of the caller's, no engine and no allocation.
  *
  * Error convention (reference: glm53f_model.h:61-64, glm53f_gpu_kernels.cu:668-686): every
  * int function returns 0 on success and -1 on failure; on failure outputs are untouched or
@@ -38,8 +41,9 @@
 extern "C" {
 #endif
 
-/* Storage formats of a weight matrix (reference: enum at glm53f.h:122; int4 is an
- * approximation format of the reference's SSD cache and is not part of this engine). */
+/* Storage formats of a weight matrix (reference: enum at glm53f.h:122; the engine's tensors are never
+ * int4, an approximation format of the reference's SSD cache: 4-bit weights have operators of their own,
+ * group 4 below). */
 #define G5B_DT_F32  0
 #define G5B_DT_BF16 1
 #define G5B_DT_FP8  2   /* E4M3FN codes + FP32 block scales ("weight_scale_inv") */
@@ -393,6 +397,72 @@ int g5b_time_matvec(g5b_engine *e, const char *name, const float *x_dev, int T, 
  * reads the accumulated milliseconds of [router+plan, gate/up, down, combine] and the number of
  * ops they cover, and optionally clears them. */
 int g5b_engine_profile_read(g5b_engine *e, float *ms, int n, long *count, int reset);
+
+/* ---------------------------------------------------------------- 4-BIT OPS ---- */
+/* Matrices of 4-bit codes with group scales, for callers that keep weights in HBM themselves: half of the bytes that
+ * the engine's FP8 experts take (the reference keeps an int4 form of the experts beside the checkpoint too,
+ * src/io/glm53f_i4file.h, in a format of its own).
+ *
+ * Format: W[r][k] = (code - 8) * scale. codes [count][rows][g5b_w4_pitch(cols)] bytes, two codes of 0..15 to a
+ * byte, the even column in the low four bits; scales BF16 [count][rows][g5b_w4_scale_pitch(cols, group)], one
+ * for each row and group of 32, 64 or 128 columns. Both start on a multiple of 16 bytes. Codes behind
+ * the last column and scales behind the last group are never used. Scales are finite: a row of W with
+ * an infinite or NaN scale gives undefined values in its own outputs.
+ *
+ * All of them: pointers are memory of the CURRENT device, the work is enqueued on `stream` (a cudaStream_t
+ * of that device, NULL for the default one) and nothing is waited for, copied to the host or allocated, so
+ * a call can be captured into a graph. Rows are F32 or BF16 (G5B_DT_F32, G5B_DT_BF16), `ld` elements apart, unless noted.
+ * Outputs must not overlap inputs. A workspace (device memory on a multiple of 256 bytes, as many bytes as the
+ * _workspace function says) holds nothing between calls; calls that may run at the same time - on different
+ * streams, or two captured graphs - each need their own. Results do not depend on what else is in a workspace, and are the same in
+ * every run. Calls with no rows (T = 0) do nothing. Limits: 2^22 rows, 2^17 columns, 2^19 activation
+ * rows, G5B_MAX_EXPERTS matrices, G5B_MAX_TOPK picks; beyond them, and for what does not fit together, -1 and a message. */
+typedef struct g5b_w4 {
+    const uint8_t  *codes;
+    const uint16_t *scales;
+    int32_t rows, cols, group;
+    int32_t count;              /* matrices of this shape one behind the other (experts); 1 for a single one */
+} g5b_w4;
+
+size_t g5b_w4_pitch(int cols);                       /* bytes of a row of codes: 16 ceil(cols / 32) */
+size_t g5b_w4_scale_pitch(int cols, int group);      /* scales of a row: ceil(cols / group) rounded up to 8 */
+
+/* src [rows][cols] (g5b_tensor with on_device = 1; F32, BF16, or FP8 with scale blocks of br x bc) into dst's codes and scales, padding
+ * included: per row and group s = bf16(max |w| / 7), code = 8 + round(w / s) clamped to 1..15, halves to even, the quotient
+ * exact; an FP8 weight is the FP32 product of code and block scale. A group of zeros has scale 0 and codes 8; one with
+ * an infinity or NaN scale NaN. dst->count must be 1 (a stack's matrices one by one). */
+int g5b_w4_quantize(const g5b_tensor *src, int br, int bc, const g5b_w4 *dst, void *stream);
+/* The values of a matrix: out [rows][cols] of dtype, BF16 rounded to nearest. */
+int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *stream);
+
+/* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Sums are FP32; F32 activations
+ * enter with 22 significant bits relative to their row's largest, BF16 ones exactly. A row of x with an infinity or NaN
+ * gives NaN in all of its outputs. */
+size_t g5b_w4_matmul_workspace(const g5b_w4 *w, int dtype, int T);
+int g5b_w4_matmul(const g5b_w4 *w, const void *x, int dtype, int T, size_t ldx, void *y, size_t ldy, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/* Tokens sorted by expert. idx [T][topk] holds expert numbers; those outside [0, n_experts) are picks of no expert here
+ * (another rank's) and are left out. Pick p = token * topk + k: order [T * topk] receives the picks by expert, equal experts in
+ * the order of p, -1 behind the last; place [T * topk] each pick's position in it, -1 for one left out; offsets [n_experts + 1]
+ * the first position of every expert, and last their number. */
+int g5b_expert_sort(const int32_t *idx, int T, int topk, int n_experts, int32_t *order, int32_t *place, int32_t *offsets,
+                    void *stream);
+/* rows[i] = x[order[i] / topk] for the offsets[n_experts] sorted picks; rows behind them stay as they were. */
+int g5b_expert_gather(const void *x, int dtype, int T, int cols, size_t ldx, const int32_t *order, const int32_t *offsets,
+                      int topk, int n_experts, void *rows, size_t ldr, void *stream);
+/* out[t] = sum over k of weights[t][k] * rows[place[t][k]], in FP32 in the order of k; a pick left out adds nothing, a token
+ * without picks is zero. weights NULL: all one. */
+int g5b_expert_combine(const void *rows, int dtype, size_t ldr, const int32_t *place, const float *weights, int T, int topk,
+                       int cols, void *out, size_t ldo, void *stream);
+
+/* Routed experts in 4 bits (the routed part of g5b_op_moe): gate and up [count][inter][hidden], down [count][hidden][inter];
+ * out[t] = sum over k of weights[t][k] down_e (silu(min(gate_e x, limit)) clamp(up_e x, -limit, limit)), e = idx[t][k], with the sort
+ * and the sum above. limit: infinity for no clamp. Between the products rows are F32 (22 bits as a factor; BF16 rows: 11). */
+size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *down, int dtype, int T, int topk);
+int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4 *down, const void *x, int dtype, int T, size_t ldx,
+                   const int32_t *idx, const float *weights, int topk, float limit, void *out, size_t ldo, void *workspace,
+                   size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

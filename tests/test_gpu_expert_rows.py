@@ -1,0 +1,192 @@
+"""Tokens sorted by expert and back, and routed experts with 4-bit weights, against plain forms."""
+import pytest
+import torch
+
+import w4_ref as ref
+
+pkg = ref.pkg
+pytestmark = pytest.mark.gpu
+
+
+def _sorted(idx, E):
+    """(order, place, offsets) by definition."""
+    T, K = idx.shape
+    flat = idx.flatten().tolist()
+    by = sorted((p for p, e in enumerate(flat) if 0 <= e < E), key=lambda p: flat[p])
+    place = [-1] * (T * K)
+    for i, p in enumerate(by):
+        place[p] = i
+    offsets = [sum(1 for p in by if flat[p] < e) for e in range(E + 1)] if T * K < 3000 else torch.bincount(
+        torch.tensor([flat[p] for p in by], dtype=torch.int64), minlength=E).cumsum(0).tolist()
+    if len(offsets) == E:
+        offsets = [0] + offsets
+    t = lambda v: torch.tensor(v, dtype=torch.int32)        # noqa: E731
+    return t(by + [-1] * (T * K - len(by))), t(place).view(T, K), t(offsets)
+
+
+def _sort(idx, E):
+    T, K = idx.shape
+    out = [torch.full(s, 77, dtype=torch.int32, device="cuda") for s in ((T * K,), (T, K), (E + 1,))]
+    pkg.expert_sort(idx.cuda(), E, *out)
+    return out
+
+
+def _picks(rng, T, K, E, how):
+    if how == "one":
+        return torch.full((T, K), E - 1, dtype=torch.int32)
+    if how == "none":
+        return torch.full((T, K), -1, dtype=torch.int32)
+    if how == "outside":          # half of them other ranks', on both sides
+        return torch.randint(-E // 2 - 1, E + E // 2 + 1, (T, K), generator=rng, dtype=torch.int32)
+    if how == "skewed":
+        return (E * torch.rand((T, K), generator=rng) ** 4).to(torch.int32).clamp(max=E - 1)
+    return torch.randint(0, E, (T, K), generator=rng, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("T,K,E", [(1, 1, 1), (1, 8, 288), (3, 5, 7), (64, 8, 288), (512, 8, 36), (513, 8, 36), (700, 6, 1024), (4097, 8, 288), (9000, 4, 3)])
+@pytest.mark.parametrize("how", ["even", "skewed", "outside", "one", "none"])
+def test_sort(gpu_lib, T, K, E, how):
+    idx = _picks(torch.Generator().manual_seed(T + E), T, K, E, how)
+    for got, want in zip(_sort(idx, E), _sorted(idx, E)):
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,E,cols,pad,how", [(1, 8, 288, 4096, 0, "even"), (5, 3, 4, 1, 0, "outside"), (37, 8, 36, 255, 1, "outside"),
+                                                (64, 2, 9, 1000, 8, "skewed"), (600, 8, 36, 72, 0, "outside"), (9, 4, 5, 33, 7, "none")])
+def test_gather_and_combine(gpu_lib, T, K, E, cols, pad, how, dtype):
+    rng = torch.Generator().manual_seed(T * cols)
+    idx = _picks(rng, T, K, E, how)
+    x = torch.randn((T, cols), generator=rng).to(dtype)
+    weights = torch.rand((T, K), generator=rng)
+    order, place, offsets = _sort(idx, E)
+    wide = torch.full((T, cols + pad), 3.0, dtype=dtype)
+    wide[:, :cols] = x
+    rows = torch.full((T * K, cols + pad), 9.0, device="cuda", dtype=dtype)
+    pkg.expert_gather(wide.cuda()[:, :cols], order, offsets, rows[:, :cols])
+    n = int(offsets[-1])
+    got = rows.cpu()
+    assert torch.equal(got[:n, :cols], x[order[:n].cpu().long() // K])
+    assert bool((got[n:] == 9.0).all()) and bool((got[:, cols:] == 9.0).all())
+    # rows of their own for every pick, so that a wrong place shows
+    rows[:n, :cols] = torch.randn((n, cols), generator=rng).to(dtype).cuda()
+    for w in (weights, None):
+        out = torch.full((T, cols + pad), 2.0, device="cuda", dtype=dtype)
+        pkg.expert_combine(rows[:, :cols], place, w.cuda() if w is not None else None, out[:, :cols])
+        took = rows.cpu().double()[:, :cols][place.cpu().clamp(min=0).long()] * (place.cpu() >= 0)[..., None]
+        part = took * (w.double() if w is not None else torch.ones(T, K, dtype=torch.float64))[..., None]
+        want = part.sum(1)
+        off = part.abs().sum(1) * K * 2.0 ** -24 + ref.rounded(want, dtype)      # K fused steps, each rounded to half of 2^-23
+        assert bool(((out.cpu()[:, :cols].double() - want).abs() <= off).all())
+        assert bool((out.cpu()[:, cols:] == 2.0).all())
+
+
+def test_combine_does_not_read_rows_left_out(gpu_lib):
+    """NaN in the rows of picks that are not here, and weights that are not numbers beside them, reach nothing."""
+    idx = torch.tensor([[0, -1, 2], [5, 9, -7]], dtype=torch.int32)
+    order, place, offsets = _sort(idx, 4)
+    rows = torch.full((6, 8), float("nan"), device="cuda")
+    rows[:2] = 1.5
+    weights = torch.tensor([[2.0, float("nan"), 1.0], [float("inf")] * 3]).cuda()
+    out = torch.empty((2, 8), device="cuda")
+    pkg.expert_combine(rows, place, weights, out)
+    assert bool((out[0] == 4.5).all()) and bool((out[1] == 0.0).all())
+
+
+def _stack(rng, E, rows, cols, group):
+    codes, scales = ref.make(rng, rows, cols, group, E, scale=0.03)
+    return pkg.W4(codes.cuda(), scales.cuda(), rows, cols, group), ref.values(codes, scales, cols, group)
+
+
+def _experts(handles, x, idx, weights, limit, pad=0):
+    T, H = x.shape
+    ws = torch.full((pkg.w4_experts_workspace(*handles, x, idx) // 4,), float("nan"), device="cuda")
+    out = torch.full((T, H + pad), 6.0, device="cuda", dtype=x.dtype)
+    pkg.w4_experts(*handles, x, idx.cuda(), weights.cuda(), limit, out[:, :H], ws)
+    torch.cuda.synchronize()
+    assert bool((out[:, H:] == 6.0).all())
+    return out[:, :H].cpu()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,E,H,I,group,limit,how", [
+    (1, 8, 12, 256, 128, 128, 10.0, "even"), (1, 1, 1, 33, 17, 32, 1.0, "even"), (5, 4, 6, 200, 96, 64, float("inf"), "outside"),
+    (40, 3, 4, 130, 257, 32, 0.5, "skewed"), (90, 2, 3, 384, 128, 128, 2.0, "even"), (70, 2, 5, 100, 300, 64, 10.0, "one"),
+    (3, 2, 4, 64, 64, 32, 10.0, "none"), (33, 4, 40, 160, 160, 32, 3.0, "outside")])
+def test_experts(gpu_lib, T, K, E, H, I, group, limit, how, dtype):
+    rng = torch.Generator().manual_seed(T * 13 + H)
+    (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, group), _stack(rng, E, I, H, group), _stack(rng, E, H, I, group)
+    idx = _picks(rng, T, K, E, how)                        # the same expert twice in a token among them
+    weights = torch.rand((T, K), generator=rng) * 2 - 0.5
+    x = torch.randn((T, H), generator=rng).to(dtype)
+    got = _experts((gate, up, down), x.cuda(), idx, weights, limit, pad=T % 2)
+    want, off = ref.experts(x.double(), idx, weights, g, u, d, limit, dtype == torch.float32)
+    worst = ((got.double() - want).abs() / (off + ref.rounded(want, dtype))).max()
+    assert worst <= 1.0, float(worst)
+
+
+def test_a_checkpoint_expert_layer_in_four_bits(gpu_lib):
+    """As they are used together: FP8 experts converted one matrix at a time into stacks, a prompt and then single tokens through
+    them; the layer put together from the sort, the gather, the products and the combination gives the same."""
+    rng = torch.Generator().manual_seed(42)
+    E, H, I, K, group = 4, 256, 128, 2, 64
+    src = {}
+    for name, r, c in (("gate", I, H), ("up", I, H), ("down", H, I)):
+        codes = torch.empty((E, r, pkg.w4_pitch(c)), dtype=torch.uint8, device="cuda")
+        scales = torch.empty((E, r, pkg.w4_scale_pitch(c, group)), dtype=torch.bfloat16, device="cuda")
+        one = []
+        for e in range(E):
+            fp8 = torch.randn((r, c), generator=rng).to(torch.float8_e4m3fn).cuda()
+            grid = (0.02 * (1 + torch.rand((-(-r // 128), -(-c // 128)), generator=rng))).cuda()
+            one.append(pkg.W4(codes[e], scales[e], r, c, group))
+            pkg.w4_quantize(fp8, one[e], scale_inv=grid)
+        src[name] = (pkg.W4(codes, scales, r, c, group), one, ref.values(codes.cpu(), scales.cpu(), c, group))
+    handles = [src[n][0] for n in ("gate", "up", "down")]
+    for T in (50, 1, 1):
+        idx = torch.randint(-1, E, (T, K), generator=rng, dtype=torch.int32)
+        weights = torch.rand((T, K), generator=rng)
+        x = torch.randn((T, H), generator=rng).cuda()
+        got = _experts(handles, x, idx, weights, 10.0)
+        want, off = ref.experts(x.cpu().double(), idx, weights, *(src[n][2] for n in ("gate", "up", "down")), 10.0, True)
+        assert bool(((got.double() - want).abs() <= off + ref.rounded(want, torch.float32)).all())
+        order, place, offsets = _sort(idx, E)
+        rows = torch.zeros((T * K, H), device="cuda")
+        pkg.expert_gather(x, order, offsets, rows)
+        at = offsets.tolist()
+        for e in range(E):
+            part = rows[at[e]:at[e + 1]]
+            h = [torch.empty((len(part), I), device="cuda") for _ in range(2)]
+            ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+            for i, n in enumerate(("gate", "up")):
+                pkg.w4_matmul(src[n][1][e], part, h[i], ws)
+            act = ref.swiglu(h[0].double(), h[1].double(), 10.0).float()
+            y = torch.empty_like(part)
+            pkg.w4_matmul(src["down"][1][e], act, y, ws)
+            rows[at[e]:at[e + 1]] = y
+        out = torch.empty_like(x)
+        pkg.expert_combine(rows, place, weights.cuda(), out)
+        assert bool(((out.cpu().double() - want).abs() <= off + ref.rounded(want, torch.float32)).all())
+
+
+def test_experts_repeat_and_replay(gpu_lib):
+    rng = torch.Generator().manual_seed(8)
+    E, H, I, K, T = 6, 256, 192, 3, 20
+    handles = [_stack(rng, E, I, H, 64)[0], _stack(rng, E, I, H, 64)[0], _stack(rng, E, H, I, 64)[0]]
+    idx = _picks(rng, T, K, E, "outside").cuda()
+    weights = torch.rand((T, K), generator=rng).cuda()
+    x = torch.randn((T, H), generator=rng).cuda()
+    first = _experts(handles, x, idx, weights, 10.0)
+    assert torch.equal(_experts(handles, x, idx, weights, 10.0), first)
+    xin, iin, out = torch.zeros_like(x), torch.zeros_like(idx), torch.zeros_like(x)
+    ws = torch.empty(pkg.w4_experts_workspace(*handles, x, idx), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pkg.w4_experts(*handles, xin, iin, weights, 10.0, out, ws)
+    xin.copy_(x)
+    iin.copy_(idx)
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.cpu(), first)

@@ -1,0 +1,204 @@
+"""Products with 4-bit weights and group scales, and the conversion to them, against FP64 on the CPU."""
+import pytest
+import torch
+
+import w4_ref as ref
+
+pkg = ref.pkg
+pytestmark = pytest.mark.gpu
+
+
+def _run(codes, scales, rows, cols, group, x, pad=0, stream=None):
+    """y [T][rows], written into rows `pad` elements further apart whose padding must stay as it was; the workspace starts as NaN."""
+    w = ref.handle(codes, scales, rows, cols, group)
+    T = x.shape[0]
+    buf = torch.full((T + 1, rows + pad), 7.0, device="cuda", dtype=x.dtype)
+    ws = torch.full((pkg.w4_matmul_workspace(w, x) // 4 + 64,), float("nan"), device="cuda")
+    pkg.w4_matmul(w, x, buf[:T, :rows], ws, stream=stream)
+    torch.cuda.synchronize()
+    assert bool((buf[:T, rows:] == 7.0).all()) and bool((buf[T] == 7.0).all())
+    return buf[:T, :rows].cpu()
+
+
+def _check(y, w, x):
+    xd = x.cpu().double()
+    want = xd @ w.t()
+    off = ref.product_bound(w, xd, x.dtype == torch.float32) + ref.rounded(want, x.dtype)
+    worst = ((y.double() - want).abs() / off).max()
+    assert worst <= 1.0, float(worst)
+
+
+SHAPES = [
+    (1, 1, 32, 1), (1, 31, 64, 3), (15, 33, 32, 1), (17, 128, 128, 2), (16, 129, 128, 5), (130, 64, 64, 4), (100, 1000, 32, 8),
+    (128, 256, 128, 16), (129, 257, 64, 17), (300, 1234, 32, 33), (257, 2050, 128, 64), (64, 4096, 64, 65), (520, 512, 128, 130),
+    (1000, 700, 64, 1), (40, 12345, 128, 9), (384, 640, 32, 200), (255, 1152, 128, 257),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,group,T", SHAPES)
+def test_product(gpu_lib, rows, cols, group, T, dtype):
+    rng = torch.Generator().manual_seed(rows * 7919 + cols * 31 + T)
+    codes, scales = ref.make(rng, rows, cols, group)
+    x = torch.randn((T, cols), generator=rng).to(dtype)
+    _check(_run(codes, scales, rows, cols, group, x.cuda(), pad=T % 3), ref.values(codes, scales, cols, group), x)
+
+
+@pytest.mark.parametrize("T", [1, 7, 40, 150])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_apart_and_off_every_alignment(gpu_lib, dtype, T):
+    rng = torch.Generator().manual_seed(T)
+    rows, cols, group = 77, 261, 64
+    codes, scales = ref.make(rng, rows, cols, group)
+    whole = torch.randn((T, cols + 10), generator=rng).to(dtype)
+    on = whole.cuda()
+    for first in (1, 2, 8):
+        y = _run(codes, scales, rows, cols, group, on[:, first:first + cols], pad=5)
+        _check(y, ref.values(codes, scales, cols, group), whole[:, first:first + cols])
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("T", [2, 100])
+def test_magnitudes_far_apart(gpu_lib, T, group):
+    """Rows of x from 2^-120 to 2^60, values of a row over 2^30, scales of a row of W over 2^40."""
+    rng = torch.Generator().manual_seed(3 + T)
+    rows, cols = 130, 640
+    codes, scales = ref.make(rng, rows, cols, group, spread=6.0)
+    x = torch.randn((T, cols), generator=rng) * torch.exp2(torch.randint(-30, 1, (T, cols), generator=rng).float())
+    x = x * torch.exp2(torch.linspace(-120, 60, T))[:, None]
+    _check(_run(codes, scales, rows, cols, group, x.cuda()), ref.values(codes, scales, cols, group), x)
+
+
+@pytest.mark.parametrize("T", [1, 5, 90])
+def test_rows_without_numbers(gpu_lib, T):
+    """A row of zeros is zero; one with an infinity or NaN is NaN in all outputs; its neighbours do not see it."""
+    rng = torch.Generator().manual_seed(5)
+    rows, cols, group = 200, 300, 128
+    codes, scales = ref.make(rng, rows, cols, group)
+    w = ref.values(codes, scales, cols, group)
+    for what in (0.0, float("inf"), float("-inf"), float("nan")):
+        x = torch.randn((T, cols), generator=rng)
+        bad = T // 2
+        if what == 0.0:
+            x[bad] = 0.0
+        else:
+            x[bad, 17] = what
+        y = _run(codes, scales, rows, cols, group, x.cuda())
+        assert bool((y[bad] == 0.0).all()) if what == 0.0 else bool(torch.isnan(y[bad]).all())
+        keep = torch.arange(T) != bad
+        if bool(keep.any()):
+            _check(y[keep], w, x[keep])
+
+
+@pytest.mark.parametrize("T", [1, 6, 70])
+def test_same_bits_every_time_on_any_stream_and_in_a_graph(gpu_lib, T):
+    rng = torch.Generator().manual_seed(11)
+    rows, cols, group = 1000, 2048, 128
+    codes, scales = ref.make(rng, rows, cols, group)
+    x = torch.randn((T, cols), generator=rng).cuda()
+    first = _run(codes, scales, rows, cols, group, x)
+    side = torch.cuda.Stream()
+    assert torch.equal(_run(codes, scales, rows, cols, group, x, stream=side.cuda_stream), first)
+    # two captured calls with workspaces of their own, replayed beside each other with new inputs
+    w = ref.handle(codes, scales, rows, cols, group)
+    graphs, ins, outs, spaces = [], [], [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        ins.append(torch.zeros_like(x))
+        outs.append(torch.zeros((T, rows), device="cuda"))
+        spaces.append(torch.empty(pkg.w4_matmul_workspace(w, x), dtype=torch.uint8, device="cuda"))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            pkg.w4_matmul(w, ins[i], outs[i], spaces[i])
+        graphs.append(g)
+    ins[0].copy_(x)
+    ins[1].copy_(-x)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0].cpu(), first) and torch.equal(outs[1].cpu(), -first)
+
+
+# ------------------------------------------------------------------ conversion ----
+def _quantized(v, group):
+    """(codes as numbers 0..15 [rows][cols], scales [rows][groups]) of FP32 values, quotients in FP64."""
+    rows, cols = v.shape
+    groups = -(-cols // group)
+    p = torch.nn.functional.pad(v.double(), (0, groups * group - cols)).view(rows, groups, group)
+    m = p.abs().amax(2)
+    s = (m / 7.0).float().to(torch.bfloat16)
+    s = torch.where(torch.isfinite(m), s, torch.tensor(float("nan"), dtype=torch.bfloat16))
+    q = (p / s.double()[..., None]).round().clamp(-7, 7)
+    q = torch.where((s.double()[..., None] > 0) & torch.isfinite(q), q, 0.0)
+    return (q + 8).to(torch.uint8).view(rows, -1)[:, :cols], s
+
+
+def _convert(src, rows, cols, group, scale=None, block=(128, 128)):
+    codes = torch.full((rows, pkg.w4_pitch(cols)), 255, dtype=torch.uint8, device="cuda")
+    scales = torch.full((rows, pkg.w4_scale_pitch(cols, group)), float("nan"), dtype=torch.bfloat16, device="cuda")
+    w = pkg.W4(codes, scales, rows, cols, group)
+    pkg.w4_quantize(src.cuda(), w, scale_inv=scale.cuda() if scale is not None else None, block=block)
+    out = {}
+    for dt in (torch.float32, torch.bfloat16):
+        buf = torch.full((rows, cols + 3), 5.0, device="cuda", dtype=dt)
+        pkg.w4_dequantize(w, buf[:, :cols])
+        torch.cuda.synchronize()
+        assert bool((buf[:, cols:] == 5.0).all())
+        out[dt] = buf[:, :cols].cpu()
+    return codes.cpu(), scales.cpu(), out
+
+
+def _compare(v, got, rows, cols, group):
+    codes, scales, out = got
+    want, s = _quantized(v, group)
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
+    assert torch.equal(c[:, :cols], want)
+    assert bool((c[:, cols:] == 8).all()) and bool((scales[:, s.shape[1]:] == 0).all())
+    assert torch.equal(scales[:, :s.shape[1]].view(torch.int16)[~torch.isnan(s)], s.view(torch.int16)[~torch.isnan(s)])
+    assert torch.equal(torch.isnan(scales[:, :s.shape[1]]), torch.isnan(s))
+    y = (want.double() - 8) * s.double().repeat_interleave(group, 1)[:, :cols]
+    for dt, o in out.items():
+        assert torch.equal(torch.nan_to_num(o, nan=123.0), torch.nan_to_num(y.to(dt), nan=123.0))
+
+
+@pytest.mark.parametrize("rows,cols,group", [(1, 1, 32), (3, 33, 32), (5, 64, 64), (7, 200, 128), (64, 1024, 32), (33, 1031, 64), (9, 5000, 128), (2, 4097, 32)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "fp8"])
+def test_quantize_and_back(gpu_lib, rows, cols, group, kind):
+    rng = torch.Generator().manual_seed(rows + cols)
+    v, scale = 0.02 * torch.randn((rows, cols), generator=rng), None
+    if kind == "bf16":
+        src = v.to(torch.bfloat16)
+        v = src.float()
+    elif kind == "fp8":
+        for block in ((128, 128), (16, 12)):
+            scale = 1e-4 * (1 + torch.rand((-(-rows // block[0]), -(-cols // block[1])), generator=rng))
+            src = (v * 5000).to(torch.float8_e4m3fn)
+            vv = src.float() * scale.repeat_interleave(block[0], 0)[:rows].repeat_interleave(block[1], 1)[:, :cols]
+            _compare(vv, _convert(src, rows, cols, group, scale, block), rows, cols, group)
+        return
+    else:
+        src = v
+    _compare(v, _convert(src, rows, cols, group), rows, cols, group)
+
+
+def test_quantize_borders(gpu_lib):
+    """Quotients at, and one FP32 step to either side of, every half; groups of zeros, of subnormal and of huge values, and without numbers."""
+    group, rows = 32, 64
+    v = torch.zeros((rows, 5 * group))
+    for r in range(rows):
+        top = (1.0 + r / 64.0) * 2.0 ** (r % 7 - 20)
+        s = (torch.tensor(top, dtype=torch.float64) / 7).float().to(torch.bfloat16).double()
+        half = torch.tensor([(k + 0.5) * float(s) for k in range(-7, 7)], dtype=torch.float32)
+        inf = torch.tensor(float("inf"))
+        v[r, 0], v[r, group], v[r, 2 * group] = top, -top, top
+        v[r, 1:15] = half
+        v[r, group + 1:group + 15] = torch.nextafter(half, inf)
+        v[r, 2 * group + 1:2 * group + 15] = torch.nextafter(half, -inf)
+        v[r, 4 * group:] = torch.linspace(-1, 1, group) * 2.0 ** (-149 + 2 * r if r < 40 else 127 - (r - 40))
+    v[5, 3 * group + 3], v[6, 3 * group + 31], v[7, 3 * group] = float("nan"), float("inf"), float("-inf")
+    _compare(v, _convert(v, rows, 5 * group, group), rows, 5 * group, group)

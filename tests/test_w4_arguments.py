@@ -1,0 +1,112 @@
+"""What the 4-bit operators and the sort refuse, and their sizes: host logic, no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import synth
+
+pkg = synth.pkg
+
+
+def _err():
+    return (pkg.lib().g5b_last_error() or b"").decode()
+
+
+def test_pitches():
+    for cols in (1, 31, 32, 33, 4096, 4097):
+        assert pkg.w4_pitch(cols) == -(-cols // 32) * 16
+        for group in (32, 64, 128):
+            assert pkg.w4_scale_pitch(cols, group) == -(-(-(-cols // group)) // 8) * 8
+    assert pkg.w4_pitch(0) == 0 and pkg.w4_scale_pitch(64, 48) == 0 and pkg.w4_scale_pitch(-3, 32) == 0
+
+
+def _w4(codes, scales, rows, cols, group, count=1):
+    return pkg._W4(codes, scales, rows, cols, group, count)
+
+
+@pytest.mark.parametrize("rows,cols,group,count,word", [(0, 64, 32, 1, "outside"), (64, 0, 32, 1, "outside"), (1 << 23, 64, 32, 1, "outside"),
+                                                        (64, 1 << 18, 32, 1, "outside"), (64, 64, 48, 1, "32, 64 or 128"), (64, 64, 0, 1, "32, 64 or 128"),
+                                                        (64, 64, 32, 0, "matrices"), (64, 64, 32, 5000, "matrices"), (64, 64, 32, 2, "matrices")])
+def test_matrices_out_of_range(rows, cols, group, count, word):
+    m = _w4(1 << 20, 1 << 20, rows, cols, group, count)
+    assert pkg.lib().g5b_w4_matmul(C.byref(m), 1 << 20, 0, 1, 1 << 20, 1 << 20, 1 << 23, 1 << 20, 1 << 30, None) == -1
+    assert word in _err()
+    assert pkg.lib().g5b_w4_dequantize(C.byref(m), 0, 1 << 20, 1 << 20, None) == -1 and word in _err()
+
+
+def test_addresses():
+    L, a = pkg.lib(), torch.zeros(1 << 16, dtype=torch.uint8)
+    here = (a.data_ptr() + 255) // 256 * 256
+    x = _w4(None, here, 16, 32, 32)
+    assert L.g5b_w4_dequantize(C.byref(x), 0, here, 32, None) == -1 and "null" in _err()
+    x = _w4(here + 8, here, 16, 32, 32)
+    assert L.g5b_w4_dequantize(C.byref(x), 0, here, 32, None) == -1 and "multiple of 16" in _err()
+    # host memory, or no device at all: never launched on
+    x = _w4(here, here, 16, 32, 32)
+    assert L.g5b_w4_dequantize(C.byref(x), 0, here, 32, None) == -1 and ("device" in _err())
+    assert L.g5b_w4_matmul(None, here, 0, 1, 32, here, 16, here, 1 << 16, None) == -1 and "null" in _err()
+    assert L.g5b_expert_sort(here, 1, 1, 1, here, here, here, None) == -1 and "device" in _err()
+
+
+@pytest.mark.parametrize("T,topk,E", [(-1, 1, 1), (1, 0, 1), (1, 65, 1), (1, 1, 0), (1, 1, 1025), (1 << 20, 1, 1)])
+def test_picks_out_of_range(T, topk, E):
+    L, a = pkg.lib(), 1 << 20
+    assert L.g5b_expert_sort(a, T, topk, E, a, a, a, None) == -1 and "outside" in _err()
+    assert L.g5b_expert_gather(a, 0, T, 8, 8, a, a, topk, E, a, 8, None) == -1 and "outside" in _err()
+    if E == 1:
+        assert L.g5b_expert_combine(a, 0, 8, a, a, T, topk, 8, a, 8, None) == -1 and "outside" in _err()
+
+
+def test_rows_out_of_range():
+    L, a = pkg.lib(), 1 << 20
+    assert L.g5b_expert_gather(a, 0, 1, 8, 7, a, a, 1, 1, a, 8, None) == -1 and "apart" in _err()
+    assert L.g5b_expert_gather(a, 0, 1, 8, 8, a, a, 1, 1, a, 7, None) == -1 and "apart" in _err()
+    assert L.g5b_expert_gather(a, 2, 1, 8, 8, a, a, 1, 1, a, 8, None) == -1 and "dtype 2" in _err()
+    assert L.g5b_expert_combine(a, 0, 8, a, a, 1, 1, 8, a, 7, None) == -1 and "apart" in _err()
+
+
+def test_workspace_sizes():
+    m = _w4(1 << 20, 1 << 20, 4096, 4096, 128)
+    L = pkg.lib()
+    small, large = L.g5b_w4_matmul_workspace(C.byref(m), 0, 1), L.g5b_w4_matmul_workspace(C.byref(m), 0, 2048)
+    assert 0 < small < large and small >= 2 * 2 * 4096 and large >= 2048 * 2 * 2 * 4096
+    assert L.g5b_w4_matmul_workspace(C.byref(m), 1, 2048) < large
+    assert L.g5b_w4_matmul_workspace(None, 0, 1) == 0 and L.g5b_w4_matmul_workspace(C.byref(m), 0, -1) == 0
+    assert L.g5b_w4_experts_workspace(C.byref(m), C.byref(m), 0, 1, 0) == 0
+    assert 0 < L.g5b_w4_experts_workspace(C.byref(m), C.byref(m), 0, 1, 8) < L.g5b_w4_experts_workspace(C.byref(m), C.byref(m), 0, 64, 8)
+
+
+def test_python_checks():
+    """Shapes, types and layouts that do not belong together end before the library is called."""
+    rows, cols, group = 8, 70, 32
+    codes, scales = torch.zeros((rows, 48), dtype=torch.uint8), torch.zeros((rows, 8), dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        pkg.W4(codes[:, :40], scales, rows, cols, group)
+    with pytest.raises(TypeError):
+        pkg.W4(codes.int(), scales, rows, cols, group)
+    with pytest.raises(ValueError):
+        pkg.W4(codes, scales, rows, cols, 48)
+    w = pkg.W4(codes, scales, rows, cols, group)
+    assert w.count == 1
+    x, ws = torch.zeros((3, cols)), torch.zeros(16)
+    for bad in (torch.zeros((3, cols + 1)), torch.zeros((4, cols)), torch.zeros(cols), torch.zeros((cols, 3)).t()):
+        with pytest.raises(ValueError):
+            pkg.w4_matmul(w, bad, torch.zeros((3, rows)), ws, stream=0)
+    with pytest.raises(TypeError):
+        pkg.w4_matmul(w, x.half(), torch.zeros((3, rows)).half(), ws, stream=0)
+    with pytest.raises(ValueError):
+        pkg.w4_matmul(w, x, torch.zeros((3, rows), dtype=torch.bfloat16), ws, stream=0)
+    with pytest.raises(RuntimeError):                      # host tensors: refused by the library
+        pkg.w4_matmul(w, x, torch.zeros((3, rows)), ws, stream=0)
+    with pytest.raises(ValueError):
+        pkg.w4_quantize(torch.zeros((rows, cols), dtype=torch.uint8), w, stream=0)
+    with pytest.raises(TypeError):
+        pkg.w4_quantize(torch.zeros((rows, cols), dtype=torch.int32), w, stream=0)
+    idx = torch.zeros((4, 2), dtype=torch.int32)
+    with pytest.raises(TypeError):
+        pkg.expert_sort(idx.long(), 3, idx.flatten(), idx, torch.zeros(4, dtype=torch.int32), stream=0)
+    with pytest.raises(ValueError):
+        pkg.expert_sort(idx, 3, idx.flatten(), idx, torch.zeros(3, dtype=torch.int32), stream=0)
+    with pytest.raises(ValueError):
+        pkg.expert_gather(torch.zeros((4, 8)), idx.flatten(), torch.zeros(4, dtype=torch.int32), torch.zeros((8, 9)), stream=0)
