@@ -615,7 +615,7 @@ def _declare_w4(L):
                             ("expert_sort", [p, i, i, i, p, p, p, p], i),
                             ("expert_gather", [p, i, i, i, z, p, p, i, i, p, z, p], i),
                             ("expert_combine", [p, i, z, p, p, i, i, i, p, z, p], i),
-                            ("w4_experts_workspace", [m, m, i, i, i], z),
+                            ("w4_experts_workspace", [m, m, i, i, i], z), ("w4_status", [p], i),
                             ("w4_experts", [m, m, m, p, i, i, z, p, p, i, C.c_float, p, z, p, z, p], i)):
         fn = getattr(L, "g5b_" + name)
         fn.argtypes, fn.restype = args, res
@@ -797,3 +797,8 @@ def w4_experts(gate: W4, up: W4, down: W4, x, idx, weights, limit: float, out, w
         raise ValueError(f"x {tuple(x.shape)} and out {tuple(out.shape)} do not fit experts of {gate.cols} columns")
     _call_w4("w4_experts", gate.ref, up.ref, down.ref, p, kind, T, ldx, _check("idx", idx, (T, topk), "int32", x),
              _check("weights", weights, (T, topk), "float32", x), topk, limit, q, ldo, workspace.data_ptr(), workspace.nbytes, _stream(stream, x))
+
+
+def w4_status(stream=0):
+    """Waits for the stream and raises if a wait inside a 4-bit product ran out since the last look (g5b_w4_status)."""
+    _call_w4("w4_status", stream)

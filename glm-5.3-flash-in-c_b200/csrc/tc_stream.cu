@@ -1242,6 +1242,16 @@ bool tc_encode(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elt
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The same with boxes of any width and another swizzle.
+bool tc_encode_swizzled(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int dims, const cuuint64_t *size, const cuuint64_t *stride,
+                        const cuuint32_t *box, CUtensorMapSwizzle swizzle)
+{
+    EncodeTiledFn fn = encode_fn();
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return fn && fn(m, dt, (cuuint32_t)dims, const_cast<void *>(base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct TcGemm {
     void *terms = nullptr;          // 16-bit values: [inputs][terms][plane][columns]
     size_t terms_n = 0;             // how many fit

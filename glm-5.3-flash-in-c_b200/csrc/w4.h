@@ -29,8 +29,9 @@ struct W4Terms {
 };
 inline int w4_kp(int cols) { return (cols + 127) / 128 * 128; }
 
-// rows: at most; n_rows (device, may be null): how many of them count
-void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t ldx, int rows, int cols, const int *n_rows, bool early);
+// rows: at most; n_rows (device, may be null): how many of them count; order (may be null): row i is x's row order[i] / topk
+void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t ldx, int rows, int cols, const int *n_rows, const int *order, int topk,
+              bool early);
 
 // Tiles of the experts' rows: slot s multiplies expert[s] with rows first[s] .. first[s] + count[s] of the sorted ones.
 struct W4Slots {
@@ -41,16 +42,23 @@ enum { W4_DENSE = 0, W4_GATEUP = 1, W4_DOWN = 2 };
 struct W4Job {
     int mode;
     W4Mat w, up;                // gate/up: w is the gate
+    int count;                  // matrices of the stack
     W4Terms x;
-    int T;                      // dense: rows of x
-    const int *order; int topk; // gate/up: the activation row of sorted row i is order[i] / topk
+    int T;                      // rows of x (experts: of picks, at most)
+    const int *order; int topk; // gate/up in w4_few: the terms' row of sorted row i is order[i] / topk
     W4Slots slots;
     void *y; size_t ldy; int y_dt;
     float limit;
 };
-// The smallest number of rows past which w4_many takes a product over from w4_few; rows of a tile of each.
-int  w4_few_rows(int n_terms, int rows_each);
+// Which of the two kernels multiplies `rows` activation rows (experts: rows of one expert on average), and how many of them make a tile.
+// w4_few goes past up to 32 columns (terms of rows) at a time.
+inline bool w4_few_takes(int n_terms, int rows) { return rows * n_terms <= 32; }
+int  w4_few_rows(int n_terms, int rows);
 int  w4_few(cudaStream_t st, const W4Job &job);
+constexpr int W4_MANY_ROWS = 64;
+size_t w4_many_part_floats(int rows, int cols, int T);      // room for the sums of a dense product's parts
+int  w4_many(cudaStream_t st, const W4Job &job, float *part);
+int  w4_many_status(cudaStream_t st);
 
 // ---- expert_rows.cu
 int  expert_sort(cudaStream_t st, const int *idx, int T, int topk, int E, int *order, int *place, int *offsets, const W4Slots *slots);

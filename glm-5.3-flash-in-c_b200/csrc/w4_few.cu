@@ -25,14 +25,14 @@ __device__ __forceinline__ float x_value(const uint16_t *p) { return bf16_to_f32
 
 // One CTA per row. The power of two brings the row's largest magnitude below 2^14; what falls below F16's 2^-24 then is 2^-38 of it.
 template <typename IN, int TERMS>
-__global__ void __launch_bounds__(256) w4_split_kernel(W4Terms t, const IN *x, size_t ldx, int cols, const int *n_rows)
+__global__ void __launch_bounds__(256) w4_split_kernel(W4Terms t, const IN *x, size_t ldx, int cols, const int *n_rows, const int *order, int topk)
 {
     __shared__ uint32_t s_max[8];
     pdl_trigger();
     pdl_wait();
     const int row = blockIdx.x;
     if (n_rows && row >= __ldg(n_rows)) return;
-    const IN *xr = x + (size_t)row * ldx;
+    const IN *xr = x + (size_t)(order ? __ldg(order + row) / topk : row) * ldx;
     uint32_t m = 0;
     for (int c = threadIdx.x; c < cols; c += 256) m = max(m, __float_as_uint(x_value(xr + c)) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
@@ -60,14 +60,15 @@ __global__ void __launch_bounds__(256) w4_split_kernel(W4Terms t, const IN *x, s
     }
 }
 
-void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t ldx, int rows, int cols, const int *n_rows, bool early)
+void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t ldx, int rows, int cols, const int *n_rows, const int *order, int topk,
+              bool early)
 {
     const float *f = static_cast<const float *>(x);
     const uint16_t *h = static_cast<const uint16_t *>(x);
 #define SPLIT(IN, TERMS, p)                                                                                             \
     do {                                                                                                                \
-        if (early) G5B_LAUNCH_PDL((w4_split_kernel<IN, TERMS>), dim3(rows), dim3(256), 0, st, t, p, ldx, cols, n_rows); \
-        else       G5B_LAUNCH((w4_split_kernel<IN, TERMS>), rows, 256, 0, st, t, p, ldx, cols, n_rows);                 \
+        if (early) G5B_LAUNCH_PDL((w4_split_kernel<IN, TERMS>), dim3(rows), dim3(256), 0, st, t, p, ldx, cols, n_rows, order, topk); \
+        else       G5B_LAUNCH((w4_split_kernel<IN, TERMS>), rows, 256, 0, st, t, p, ldx, cols, n_rows, order, topk);                 \
     } while (0)
     if (dt == DT_BF16) SPLIT(uint16_t, 1, h);
     else if (t.n_terms == 1) SPLIT(float, 1, f);

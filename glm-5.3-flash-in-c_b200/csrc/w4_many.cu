@@ -1,0 +1,455 @@
+// w4_many.cu - 4-bit weights times many activation rows (a batch, a prompt, an expert's share of one) on the tensor
+// cores of sm_100: tcgen05.mma with the weights as the A operand out of tensor memory.
+//
+// A tile is two blocks of 128 weight rows (gate/up: 128 gate rows and the 128 up rows that go with them) and up to 64
+// activation rows. One CTA per SM walks tiles; its warps have roles:
+//   16     codes by TMA: 2 x 128 rows x 64 bytes (128 columns) a step
+//   17     activation terms by TMA: 64 rows x 128 columns x terms a step
+//   8-15   conversion, four warps to a block, a thread to a row: nibbles become F16 values of (code - 8) * scale in tensor
+//          memory. They are exact: 3 significant bits of the code times 8 of a BF16 scale fit F16's 11, and a power of two
+//          per row of W brings its largest scale to [2^11, 2^12), so that only those of groups 2^28 below it lose bits.
+//   18, 19 products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
+//          same sums one after the other, so that a converted block is used twice.
+//   0-7    four warps to a block: take the sums over 256 columns (F32 rows; 512 of BF16) out of tensor memory and add them
+//          in registers, because the tensor cores cut off when they add; two accumulators in turn. Then the scales come off, and the rows are stored.
+// A converted block and its sums live in tensor memory (256 columns each); shared memory only holds what TMA brings, which it
+// must read for every product anyway: 64 rows of terms, 16 KB per step and term.
+//
+// Few tiles (a small batch, a narrow matrix) are cut along the columns too, into parts whose sums another kernel adds in order.
+// Every wait is bounded: one that runs out sets a flag (g5b_w4_status), and every role drains what it has in flight and ends.
+#include "tc_ptx.cuh"
+#include "w4.h"
+
+namespace g5b {
+
+bool tc_encode_swizzled(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int dims, const cuuint64_t *size, const cuuint64_t *stride,
+                        const cuuint32_t *box, CUtensorMapSwizzle swizzle);
+
+constexpr int WM_ROWS = 64;                         // activation rows of a tile
+constexpr int WM_WS = 4, WM_XS = 3;                 // stages of codes, of terms
+constexpr int WM_W_STAGE = 2 * 128 * 64;
+constexpr int WM_THREADS = 20 * 32;
+constexpr int WM_CTAS = 148;                        // SMs of a B200: what the parts along the columns are chosen for
+constexpr int WM_MAX_PARTS = 8;
+
+static __device__ int g_w4_err;                     // a wait that ran out: its code (0: none)
+
+struct ManyMaps { CUtensorMap w, up, x; };
+struct ManyArgs {
+    W4Mat w, up;
+    const float *inv;
+    int mode, KB, n;               // steps of 128 columns; rows of a box of terms (a multiple of 16)
+    int RT, TT, parts;             // tiles of weight rows; dense: tiles of activation rows, parts along the columns
+    int T;
+    W4Slots slots;
+    void *y;
+    size_t ldy;
+    int y_dt;
+    float *part;                   // [parts][T][rows], parts > 1
+    float limit;
+};
+
+struct ManyTile {
+    int e, rt, first, np, n, k0, k1, part;
+};
+__device__ __forceinline__ int many_tiles(const ManyArgs &a)
+{
+    return a.mode == W4_DENSE ? a.RT * a.TT * a.parts : a.RT * __ldg(a.slots.n);
+}
+__device__ __forceinline__ ManyTile many_tile(const ManyArgs &a, int i)
+{
+    ManyTile t;
+    if (a.mode == W4_DENSE) {
+        const int tt = i % a.TT, rest = i / a.TT;
+        t.e = 0; t.rt = rest % a.RT; t.part = rest / a.RT;
+        t.first = tt * a.n; t.np = min(a.n, a.T - t.first);
+        t.k0 = (int)((long long)a.KB * t.part / a.parts); t.k1 = (int)((long long)a.KB * (t.part + 1) / a.parts);
+    } else {
+        const int slot = i / a.RT;
+        t.rt = i - slot * a.RT; t.part = 0;
+        t.e = __ldg(a.slots.expert + slot); t.first = __ldg(a.slots.first + slot); t.np = __ldg(a.slots.count + slot);
+        t.k0 = 0; t.k1 = a.KB;
+    }
+    t.n = (t.np + 15) & ~15;
+    return t;
+}
+
+// The power of two that brings the largest of a row's scales to [2^11, 2^12).
+__device__ __forceinline__ int many_row_up(const uint16_t *srow, int groups)
+{
+    uint32_t m = 0;
+    int i = 0;
+#pragma unroll 4
+    for (; i + 8 <= groups; i += 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(srow + i));
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+    }
+    for (; i < groups; i++) m = __vmaxu2(m, (uint32_t)__ldg(srow + i) & 0x7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    return min(11 + 127 - max((int)(m >> 7), 1), 126);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+// Eight codes of a word, times the scale (twice in s), as four pairs in the terms' order.
+__device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
+{
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        uint32_t a, b;
+        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(v));       // (v & mask) | 1024
+        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(v));
+        f[2 * i] = h2_bits(__hmul2(__hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f)), s));
+        f[2 * i + 1] = h2_bits(__hmul2(__hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)), s));
+        v >>= 8;
+    }
+}
+
+// True when it is true for all 256 epilogue threads: they go on together or not at all.
+__device__ __forceinline__ bool many_all(bool ok)
+{
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
+}
+
+template <int TERMS>
+__global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
+{
+    constexpr int CHUNK = TERMS == 2 ? 2 : 4;               // steps summed inside the tensor cores
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int XB = 2 * TERMS * a.n * 128;
+    uint8_t *wst = smem;                                                     // [WM_WS][2][128 rows][64]
+    uint8_t *xst = wst + WM_WS * WM_W_STAGE;                                 // [WM_XS][64-column half][term][n rows][128]
+    float *exch = reinterpret_cast<float *>(xst + (size_t)WM_XS * XB);       // gate/up: [n][128]
+    __shared__ uint64_t w_full[WM_WS], w_empty[WM_WS], x_full[WM_XS], x_empty[WM_XS];
+    __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
+    __shared__ uint32_t s_tmem;
+    int *err = &g_w4_err;
+
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < WM_WS; i++) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
+        for (int i = 0; i < WM_XS; i++) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 2); }
+        for (int b = 0; b < 2; b++) {
+            for (int i = 0; i < 2; i++) { mbar_init(&a_full[b][i], 4); mbar_init(&a_empty[b][i], 1); mbar_init(&d_full[b][i], 1); mbar_init(&d_empty[b][i], 4); }
+            mbar_init(&drained[b], 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 18) tmem_alloc(&s_tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    // sums of block b, accumulator i: columns 128 b + 64 i; converted block b of stage s: columns 256 + 128 s + 64 b
+    if (a.mode != W4_DENSE) pdl_wait();                     // (the slots are another kernel's)
+    const int tiles = many_tiles(a);
+    bool ok = true;
+
+    if (warp == 16) {
+        // --------------------------------------------------------------------- codes ----
+        if (elect_one()) {
+            int s = 0, ph = 1, issued = 0;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                const ManyTile t = many_tile(a, i);
+#pragma unroll 1
+                for (int kb = t.k0; kb < t.k1; kb++) {
+                    if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
+                    mbar_expect_tx(&w_full[s], WM_W_STAGE);
+                    uint8_t *dst = wst + (size_t)s * WM_W_STAGE;
+                    if (a.mode == W4_GATEUP) {
+                        tma_load_3d(dst, &maps.w, kb * 64, t.rt * 128, t.e, &w_full[s]);
+                        tma_load_3d(dst + WM_W_STAGE / 2, &maps.up, kb * 64, t.rt * 128, t.e, &w_full[s]);
+                    } else {
+                        tma_load_3d(dst, &maps.w, kb * 64, t.rt * 256, t.e, &w_full[s]);
+                        tma_load_3d(dst + WM_W_STAGE / 2, &maps.w, kb * 64, t.rt * 256 + 128, t.e, &w_full[s]);
+                    }
+                    issued++;
+                    if (++s == WM_WS) { s = 0; ph ^= 1; }
+                }
+            }
+            // copies in flight must land before shared memory goes away
+            for (int j = issued - 1; j >= 0 && j >= issued - WM_WS; j--) mbar_wait(&w_full[j % WM_WS], (uint32_t)(j / WM_WS) & 1, err, 2);
+        }
+        __syncwarp();
+    } else if (warp == 17) {
+        // --------------------------------------------------------------------- terms ----
+        pdl_wait();
+        if (elect_one()) {
+            int s = 0, ph = 1, issued = 0;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                const ManyTile t = many_tile(a, i);
+#pragma unroll 1
+                for (int kb = t.k0; kb < t.k1; kb++) {
+                    if (issued >= WM_XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
+                    mbar_expect_tx(&x_full[s], (uint32_t)XB);
+                    tma_load_4d(xst + (size_t)s * XB, &maps.x, 0, t.first, 0, kb * 2, &x_full[s]);
+                    issued++;
+                    if (++s == WM_XS) { s = 0; ph ^= 1; }
+                }
+            }
+            for (int j = issued - 1; j >= 0 && j >= issued - WM_XS; j--) mbar_wait(&x_full[j % WM_XS], (uint32_t)(j / WM_XS) & 1, err, 4);
+        }
+        __syncwarp();
+    } else if (warp >= 18) {
+        // ------------------------------------------------------------------ products ----
+        if (elect_one()) {
+            const int b = warp - 18;
+            int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
+#pragma unroll 1
+            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                const ManyTile t = many_tile(a, i);
+                const uint32_t idesc = tc_idesc(0, t.n);
+                int c = 0;                                   // steps in the current accumulator
+#pragma unroll 1
+                for (int kb = t.k0; kb < t.k1; kb++) {
+                    const int buf = chunks & 1;
+                    if (c == 0 && chunks >= 2 && !(ok = mbar_wait(&d_empty[b][buf], (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
+                    if (!(ok = mbar_wait(&x_full[xs], (uint32_t)xp, err, 6) && mbar_wait(&a_full[b][as], (uint32_t)ap, err, 7))) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
+                    const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+#pragma unroll
+                        for (int m = 0; m < TERMS; m++) {
+                            const uint64_t bd = tc_smem_desc(xb + (uint32_t)(((k >> 2) * TERMS + m) * a.n * 128)) + 2 * (k & 3);
+                            tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, c || k || m ? 1u : 0u);
+                        }
+                    tc_commit(&a_empty[b][as]);
+                    tc_commit(&x_empty[xs]);
+                    if (++c == CHUNK || kb + 1 == t.k1) { tc_commit(&d_full[b][buf]); chunks++; c = 0; }
+                    if (++as == 2) { as = 0; ap ^= 1; }
+                    if (++xs == WM_XS) { xs = 0; xp ^= 1; }
+                }
+            }
+            // nothing of this thread is in flight, and no arrival still to come, when the CTA ends
+            tc_commit(&drained[b]);
+            mbar_wait(&drained[b], 0, err, 8);
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // --------------------------------------------------- codes -> F16 in tensor memory ----
+        const int b = (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane, x = (r >> 1) & 3;
+        const uint32_t dst = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (uint32_t)(b * 64);
+        const int per = a.w.group == 128 ? 2 : a.w.group == 64 ? 1 : 0;        // a 32-column piece's group: piece >> per
+        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0;
+#pragma unroll 1
+        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+            const ManyTile t = many_tile(a, i);
+            const W4Mat &w = a.mode == W4_GATEUP && b ? a.up : a.w;
+            const int row = a.mode == W4_GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
+            const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
+            const float up = pow2(many_row_up(srow, a.w.groups));
+            // raw scales of a step's four pieces, one step ahead
+            auto fetch = [&](int kb) {
+                uint2 v = make_uint2(0u, 0u);
+                if (kb < t.k1) {
+                    if (per == 2) v.x = __ldg(srow + kb);
+                    else if (per == 1) v.x = __ldg(reinterpret_cast<const uint32_t *>(srow) + kb);
+                    else v = __ldg(reinterpret_cast<const uint2 *>(srow) + kb);
+                }
+                return v;
+            };
+            uint2 next = fetch(t.k0);
+#pragma unroll 1
+            for (int kb = t.k0; kb < t.k1; kb++, steps++) {
+                const uint2 sc = next;
+                next = fetch(kb + 1);
+                if (!(ok = mbar_wait_all(&w_full[ws], (uint32_t)wp, err, 9))) break;
+                if (steps >= 2 && !(ok = mbar_wait_all(&a_empty[b][as], (uint32_t)ap, err, 10))) break;
+                tc_fence_after();
+                const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t f[32];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int piece = h * 2 + c, g = piece >> per;
+                        const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
+                        // (a group behind the last: zero, whatever lies there)
+                        const float s = ((4 * kb + piece) >> per) < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f;
+                        const __half2 s2 = __float2half2_rn(s);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
+                        many_convert(v.x, s2, f + c * 16); many_convert(v.y, s2, f + c * 16 + 4);
+                        many_convert(v.z, s2, f + c * 16 + 8); many_convert(v.w, s2, f + c * 16 + 12);
+                    }
+                    tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
+                }
+                // (handed back only here: the loads' values have arrived when they have been used)
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&w_empty[ws]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[b][as]);
+                if (++ws == WM_WS) { ws = 0; wp ^= 1; }
+                if (++as == 2) { as = 0; ap ^= 1; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ sums, scales, stores ----
+        const int b = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 128);
+        int chunks = 0;
+        bool waited = a.mode != W4_DENSE;
+#pragma unroll 1
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+            const ManyTile t = many_tile(a, i);
+            const W4Mat &w = a.mode == W4_GATEUP && b ? a.up : a.w;
+            const int row = a.mode == W4_GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
+            const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
+            const float down = pow2(-many_row_up(srow, a.w.groups));
+            float acc[WM_ROWS];
+#pragma unroll
+            for (int k = 0; k < WM_ROWS; k++) acc[k] = 0.f;
+            const int uses = (t.k1 - t.k0 + CHUNK - 1) / CHUNK;
+#pragma unroll 1
+            for (int c = 0; c < uses; c++, chunks++) {
+                const int buf = chunks & 1;
+                if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(chunks >> 1) & 1, err, 11))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int g = 0; g < WM_ROWS; g += 8)
+                    if (g < t.n) {
+                        uint32_t v[8];
+                        tmem_ld8(lane_addr + (uint32_t)(buf * 64 + g), v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 8; k++) acc[g + k] = __fadd_rn(acc[g + k], __uint_as_float(v[k]));
+                    }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_empty[b][buf]);
+            }
+            if (!waited) { pdl_wait(); waited = true; }
+            if (!(ok = many_all(ok))) break;
+            const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
+            // (the smaller of the two powers first; NaN stays)
+            auto value = [&](float sum, float inv) { return down < inv ? sum * down * inv : sum * inv * down; };
+            if (a.mode == W4_GATEUP && b) {
+#pragma unroll
+                for (int k = 0; k < WM_ROWS; k++) {
+                    const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
+                    if (k < t.np) exch[k * 128 + r] = value(acc[k], inv);
+                }
+            }
+            if (a.mode == W4_GATEUP) many_all(true);
+            if (a.mode != W4_GATEUP || !b) {
+                const bool live = row < a.w.rows;
+#pragma unroll
+                for (int k = 0; k < WM_ROWS; k++) {
+                    const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
+                    if (k < t.np && live) {
+                        float v = value(acc[k], inv);
+                        if (a.mode == W4_GATEUP) {
+                            float gate = v > a.limit ? a.limit : v, u = exch[k * 128 + r];
+                            u = u > a.limit ? a.limit : (u < -a.limit ? -a.limit : u);
+                            v = gate * sigmoid_near(gate) * u;
+                        }
+                        if (a.parts > 1) a.part[((size_t)t.part * a.T + t.first + k) * a.w.rows + row] = v;
+                        else if (a.y_dt == DT_F32) static_cast<float *>(a.y)[(size_t)(t.first + k) * a.ldy + row] = v;
+                        else static_cast<__nv_bfloat16 *>(a.y)[(size_t)(t.first + k) * a.ldy + row] = __float2bfloat16_rn(v);
+                    }
+                }
+            }
+            if (a.mode == W4_GATEUP) many_all(true);           // the exchange buffer is free again
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 18) { __syncwarp(); tmem_dealloc(tmem, 512); }
+}
+
+// y = the parts' sums in order
+__global__ void __launch_bounds__(256) w4_parts_kernel(const float *part, int parts, int T, int rows, void *y, size_t ldy, int y_dt)
+{
+    pdl_wait();
+    const int t = blockIdx.y, r = blockIdx.x * 256 + threadIdx.x;
+    if (r >= rows) return;
+    float v = 0.f;
+    const float *p = part + (size_t)t * rows + r;
+#pragma unroll 4
+    for (int i = 0; i < parts; i++) v += __ldcs(p + (size_t)i * T * rows);
+    if (y_dt == DT_F32) static_cast<float *>(y)[(size_t)t * ldy + r] = v;
+    else static_cast<__nv_bfloat16 *>(y)[(size_t)t * ldy + r] = __float2bfloat16_rn(v);
+}
+
+// Parts along the columns of a dense product: what takes the fewest steps with one tile at a time on every SM, where a tile's
+// beginning and end count as three steps.
+int w4_many_parts(int rows, int cols, int T)
+{
+    const int KB = w4_kp(cols) / 128, n = T < WM_ROWS ? (T + 15) / 16 * 16 : WM_ROWS;
+    const long long tiles = (long long)((rows + 255) / 256) * ((T + n - 1) / n);
+    int best = 1;
+    long long least = 0;
+    for (int p = 1; p <= WM_MAX_PARTS && (p == 1 || (KB / p >= 2 && tiles * p <= 2 * WM_CTAS)); p++) {
+        const long long cost = (tiles * p + WM_CTAS - 1) / WM_CTAS * ((KB + p - 1) / p + 3) + (p > 1 ? 2 : 0);
+        if (p == 1 || cost < least) { least = cost; best = p; }
+    }
+    return best;
+}
+size_t w4_many_part_floats(int rows, int cols, int T)
+{
+    const int p = w4_many_parts(rows, cols, T);
+    return p > 1 ? (size_t)p * T * rows : 0;
+}
+
+template <int TERMS>
+static int many_launch(cudaStream_t st, const ManyMaps &m, const ManyArgs &a, int grid)
+{
+    static SmemGrant grant;
+    const size_t smem = 1024 + WM_WS * WM_W_STAGE + (size_t)WM_XS * 2 * TERMS * a.n * 128 + (a.mode == W4_GATEUP ? (size_t)a.n * 512 : 0);
+    if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS>, smem, grant)) return -1;
+    G5B_LAUNCH_PDL(w4_many_kernel<TERMS>, dim3(grid), dim3(WM_THREADS), smem, st, m, a);
+    return 0;
+}
+
+int w4_many(cudaStream_t st, const W4Job &j, float *part)
+{
+    ManyMaps m;
+    ManyArgs a{};
+    const int rows_most = j.mode == W4_DENSE ? j.T : j.slots.rows;
+    a.w = j.w; a.up = j.up; a.inv = j.x.inv; a.mode = j.mode; a.KB = j.x.kp / 128; a.T = j.T; a.slots = j.slots;
+    a.n = rows_most < WM_ROWS ? (rows_most + 15) / 16 * 16 : WM_ROWS;
+    a.RT = (j.w.rows + (j.mode == W4_GATEUP ? 127 : 255)) / (j.mode == W4_GATEUP ? 128 : 256);
+    a.TT = (j.T + a.n - 1) / a.n;
+    a.parts = j.mode == W4_DENSE ? w4_many_parts(j.w.rows, j.w.cols, j.T) : 1;
+    a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.part = part; a.limit = j.limit;
+    const cuuint64_t wsize[3] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.rows, (cuuint64_t)j.count};
+    const cuuint64_t wstride[2] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.codes_stride};
+    const cuuint32_t wbox[3] = {64, 128, 1};
+    const cuuint64_t row = (cuuint64_t)j.x.n_terms * j.x.kp * 2;
+    const cuuint64_t xsize[4] = {64, (cuuint64_t)j.T, (cuuint64_t)j.x.n_terms, (cuuint64_t)j.x.kp / 64}, xstride[3] = {row, (cuuint64_t)j.x.kp * 2, 128};
+    const cuuint32_t xbox[4] = {64, (cuuint32_t)a.n, (cuuint32_t)j.x.n_terms, 2};
+    if (!tc_encode_swizzled(&m.w, j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !tc_encode_swizzled(&m.up, j.mode == W4_GATEUP ? j.up.codes : j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !tc_encode_swizzled(&m.x, j.x.terms, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, xsize, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B)) {
+        set_last_error("a tensor map of a 4-bit product was refused");
+        return -1;
+    }
+    const long long tiles = j.mode == W4_DENSE ? (long long)a.RT * a.TT * a.parts : (long long)a.RT * j.slots.max;
+    const int grid = (int)(tiles < dev_sms() ? tiles : dev_sms());
+    if (j.x.n_terms == 2 ? many_launch<2>(st, m, a, grid) : many_launch<1>(st, m, a, grid)) return -1;
+    if (a.parts > 1)
+        G5B_LAUNCH_PDL(w4_parts_kernel, dim3((j.w.rows + 255) / 256, j.T), dim3(256), 0, st, part, a.parts, j.T, j.w.rows, j.y, j.ldy, j.y_dt);
+    return 0;
+}
+
+// The code of a wait that ran out in a kernel of the current device since the last look (and forgets it); -1 where it cannot be read.
+int w4_many_status(cudaStream_t st)
+{
+    int code = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbolAsync(&code, g_w4_err, sizeof code, 0, cudaMemcpyDeviceToHost, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess) return -1;
+    if (code && (cudaMemcpyToSymbolAsync(g_w4_err, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess)) return -1;
+    return code;
+}
+
+}  // namespace g5b

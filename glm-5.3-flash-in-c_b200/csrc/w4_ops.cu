@@ -94,18 +94,20 @@ struct ExpertsWs {
     W4Terms x, h;
     float *act, *rows;
 };
-// rows of a tile for the few-row kernel: from the rows an expert has on average
-int tile_rows(int n_terms, int T, int topk, int E) { return w4_few_rows(n_terms, (T * topk + E - 1) / E); }
+// The kernel and its tiles go by the rows that an expert would have if all picks were here and spread evenly.
+int mean_rows(int T, int topk, int E) { return (T * topk + E - 1) / E; }
 ExpertsWs experts_ws(Pieces &ws, int n_terms, int T, int topk, int E, int H, int I)
 {
     ExpertsWs w;
     const size_t n = (size_t)T * topk;
     w.order = ws.take<int>(n); w.place = ws.take<int>(n); w.offsets = ws.take<int>(E + 1);
-    w.slots.rows = tile_rows(n_terms, T, topk, E);
+    const int mean = mean_rows(T, topk, E);
+    const bool few = w4_few_takes(n_terms, mean);
+    w.slots.rows = few ? w4_few_rows(n_terms, mean) : W4_MANY_ROWS;
     w.slots.max = (int)(n / w.slots.rows + (n < (size_t)E ? n : (size_t)E));
     w.slots.n = ws.take<int>(1);
     w.slots.expert = ws.take<int>(w.slots.max); w.slots.first = ws.take<int>(w.slots.max); w.slots.count = ws.take<int>(w.slots.max);
-    w.x = terms_of(ws, n_terms, H, T);
+    w.x = terms_of(ws, n_terms, H, few ? (size_t)T : n);
     w.h = terms_of(ws, n_terms, I, n);
     w.act = ws.take<float>(n * I);
     w.rows = ws.take<float>(n * H);
@@ -155,7 +157,9 @@ extern "C" size_t g5b_w4_matmul_workspace(const g5b_w4 *m, int dtype, int T)
 {
     if (!m || m->cols < 1 || m->cols > W4_MAX_COLS || T < 0 || T > W4_MAX_TOKENS) return 0;
     Pieces ws{nullptr};
-    terms_of(ws, dtype == DT_BF16 ? 1 : 2, m->cols, T < 1 ? 1 : T);
+    const int n_terms = dtype == DT_BF16 ? 1 : 2;
+    terms_of(ws, n_terms, m->cols, T < 1 ? 1 : T);
+    if (!w4_few_takes(n_terms, T)) ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
     return ws.used;
 }
 
@@ -172,11 +176,11 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     if (check_ws(op, workspace, workspace_bytes, g5b_w4_matmul_workspace(m, dtype, T))) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Pieces ws{static_cast<uint8_t *>(workspace)};
-    j.mode = W4_DENSE; j.T = T;
+    j.mode = W4_DENSE; j.T = T; j.count = 1;
     j.x = terms_of(ws, dtype == DT_BF16 ? 1 : 2, j.w.cols, T);
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
-    w4_split(st, j.x, x, dtype, ldx, T, j.w.cols, nullptr, false);
-    if (w4_few(st, j)) return -1;
+    w4_split(st, j.x, x, dtype, ldx, T, j.w.cols, nullptr, nullptr, 1, false);
+    if (w4_few_takes(j.x.n_terms, T) ? w4_few(st, j) : w4_many(st, j, ws.take<float>(w4_many_part_floats(j.w.rows, j.w.cols, T)))) return -1;
     return launched(op);
 }
 
@@ -253,14 +257,24 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     Pieces pieces{static_cast<uint8_t *>(workspace)};
     const ExpertsWs ws = experts_ws(pieces, dtype == DT_BF16 ? 1 : 2, T, topk, E, H, I);
     if (expert_sort(st, idx, T, topk, E, ws.order, ws.place, ws.offsets, &ws.slots)) return launched(op), -1;
-    w4_split(st, ws.x, x, dtype, ldx, T, H, nullptr, false);
+    // few rows to an expert: terms of the tokens, found through the order; many: terms of the picks in order, as a tile is loaded whole
+    const bool few = w4_few_takes(ws.x.n_terms, mean_rows(T, topk, E));
+    if (few) w4_split(st, ws.x, x, dtype, ldx, T, H, nullptr, nullptr, 1, false);
+    else     w4_split(st, ws.x, x, dtype, ldx, n, H, ws.offsets + E, ws.order, topk, false);
     W4Job j{};
-    j.mode = W4_GATEUP; j.w = wg; j.up = wu; j.x = ws.x; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots;
+    j.mode = W4_GATEUP; j.w = wg; j.up = wu; j.count = E; j.x = ws.x; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots;
     j.y = ws.act; j.ldy = I; j.y_dt = DT_F32; j.limit = limit;
-    if (w4_few(st, j)) return -1;
-    w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, true);
+    if (few ? w4_few(st, j) : w4_many(st, j, nullptr)) return -1;
+    w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, nullptr, 1, true);
     j.mode = W4_DOWN; j.w = wd; j.x = ws.h; j.y = ws.rows; j.ldy = H;
-    if (w4_few(st, j)) return -1;
+    if (few ? w4_few(st, j) : w4_many(st, j, nullptr)) return -1;
     expert_combine(st, ws.rows, DT_F32, H, ws.place, weights, T, topk, H, out, dtype, ldo, true);
     return launched(op);
+}
+
+extern "C" int g5b_w4_status(void *stream)
+{
+    const int code = w4_many_status(static_cast<cudaStream_t>(stream));
+    if (code < 0) return launched("g5b_w4_status"), -1;
+    return code ? fail("g5b_w4_status: a wait of a 4-bit product ran out (code %d): results since the last look are undefined", code) : 0;
 }

@@ -464,6 +464,10 @@ int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4 *down, con
                    const int32_t *idx, const float *weights, int topk, float limit, void *out, size_t ldo, void *workspace,
                    size_t workspace_bytes, void *stream);
 
+/* Waits for `stream`, and says whether a wait inside a kernel of the two products above ran out on the current device since the
+ * last look (all waits are bounded; none is expected to): -1 and a message then, and results since are undefined. */
+int g5b_w4_status(void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,7 @@ def _experts(handles, x, idx, weights, limit, pad=0):
     out = torch.full((T, H + pad), 6.0, device="cuda", dtype=x.dtype)
     pkg.w4_experts(*handles, x, idx.cuda(), weights.cuda(), limit, out[:, :H], ws)
     torch.cuda.synchronize()
+    pkg.w4_status()
     assert bool((out[:, H:] == 6.0).all())
     return out[:, :H].cpu()
 

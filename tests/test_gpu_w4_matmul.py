@@ -16,6 +16,7 @@ def _run(codes, scales, rows, cols, group, x, pad=0, stream=None):
     ws = torch.full((pkg.w4_matmul_workspace(w, x) // 4 + 64,), float("nan"), device="cuda")
     pkg.w4_matmul(w, x, buf[:T, :rows], ws, stream=stream)
     torch.cuda.synchronize()
+    pkg.w4_status()
     assert bool((buf[:T, rows:] == 7.0).all()) and bool((buf[T] == 7.0).all())
     return buf[:T, :rows].cpu()
 
