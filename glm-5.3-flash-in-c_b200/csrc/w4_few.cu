@@ -15,7 +15,7 @@
 // Sums are FP32: in the tensor cores over a group, outside across groups.
 #include "common.cuh"
 #include "mma_stage.cuh"
-#include "w4.h"
+#include "w4.cuh"
 
 namespace g5b {
 
@@ -111,13 +111,6 @@ __device__ __forceinline__ void quad_transpose(uint4 &v, int t)
     x = __shfl_xor_sync(0xffffffffu, a ? v.z : v.w, 1); if (a) v.z = x; else v.w = x;
     x = __shfl_xor_sync(0xffffffffu, b ? v.x : v.z, 2); if (b) v.x = x; else v.z = x;
     x = __shfl_xor_sync(0xffffffffu, b ? v.y : v.w, 2); if (b) v.y = x; else v.w = x;
-}
-
-__device__ __forceinline__ float swiglu_value(float g, float u, float limit)
-{
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : (u < -limit ? -limit : u);
-    return g * sigmoid_near(g) * u;
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }

@@ -18,7 +18,7 @@
 // Few tiles (a small batch, a narrow matrix) are cut along the columns too, into parts whose sums another kernel adds in order.
 // Every wait is bounded: one that runs out sets a flag (g5b_w4_status), and every role drains what it has in flight and ends.
 #include "tc_ptx.cuh"
-#include "w4.h"
+#include "w4.cuh"
 
 namespace g5b {
 
@@ -114,17 +114,17 @@ __device__ __forceinline__ bool many_all(bool ok)
     return all != 0;
 }
 
-template <int TERMS>
+template <int TERMS, bool GATEUP>
 __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
 {
-    constexpr int CHUNK = TERMS == 2 ? 2 : 4;               // steps summed inside the tensor cores
+    constexpr int CHUNK = TERMS == 2 ? 1 : 4;               // steps summed inside the tensor cores
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int XB = 2 * TERMS * a.n * 128;
     uint8_t *wst = smem;                                                     // [WM_WS][2][128 rows][64]
     uint8_t *xst = wst + WM_WS * WM_W_STAGE;                                 // [WM_XS][64-column half][term][n rows][128]
-    float *exch = reinterpret_cast<float *>(xst + (size_t)WM_XS * XB);       // gate/up: [n][128]
+    float *exch = reinterpret_cast<float *>(xst + (size_t)WM_XS * XB);       // [block][64][128]
     __shared__ uint64_t w_full[WM_WS], w_empty[WM_WS], x_full[WM_XS], x_empty[WM_XS];
     __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
     __shared__ uint32_t s_tmem;
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                     if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
                     mbar_expect_tx(&w_full[s], WM_W_STAGE);
                     uint8_t *dst = wst + (size_t)s * WM_W_STAGE;
-                    if (a.mode == W4_GATEUP) {
+                    if (GATEUP) {
                         tma_load_3d(dst, &maps.w, kb * 64, t.rt * 128, t.e, &w_full[s]);
                         tma_load_3d(dst + WM_W_STAGE / 2, &maps.up, kb * 64, t.rt * 128, t.e, &w_full[s]);
                     } else {
@@ -243,8 +243,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll 1
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
             const ManyTile t = many_tile(a, i);
-            const W4Mat &w = a.mode == W4_GATEUP && b ? a.up : a.w;
-            const int row = a.mode == W4_GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
+            const W4Mat &w = GATEUP && b ? a.up : a.w;
+            const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
             const float up = pow2(many_row_up(srow, a.w.groups));
             // raw scales of a step's four pieces, one step ahead
@@ -302,10 +302,9 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll 1
         for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
             const ManyTile t = many_tile(a, i);
-            const W4Mat &w = a.mode == W4_GATEUP && b ? a.up : a.w;
-            const int row = a.mode == W4_GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
-            const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            const float down = pow2(-many_row_up(srow, a.w.groups));
+            const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
+            const size_t srow = (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
+            const float down = pow2(-many_row_up(a.w.scales + srow, a.w.groups)), up_down = GATEUP ? pow2(-many_row_up(a.up.scales + srow, a.w.groups)) : 0.f;
             float acc[WM_ROWS];
 #pragma unroll
             for (int k = 0; k < WM_ROWS; k++) acc[k] = 0.f;
@@ -316,13 +315,13 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(chunks >> 1) & 1, err, 11))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int g = 0; g < WM_ROWS; g += 8)
+                for (int g = 0; g < WM_ROWS; g += 16)
                     if (g < t.n) {
-                        uint32_t v[8];
-                        tmem_ld8(lane_addr + (uint32_t)(buf * 64 + g), v);
+                        uint32_t v[16];
+                        tmem_ld16(lane_addr + (uint32_t)(buf * 64 + g), v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 8; k++) acc[g + k] = __fadd_rn(acc[g + k], __uint_as_float(v[k]));
+                        for (int k = 0; k < 16; k++) acc[g + k] = __fadd_rn(acc[g + k], __uint_as_float(v[k]));
                     }
                 tc_fence_before();
                 __syncwarp();
@@ -331,35 +330,33 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             if (!waited) { pdl_wait(); waited = true; }
             if (!(ok = many_all(ok))) break;
             const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
-            // (the smaller of the two powers first; NaN stays)
-            auto value = [&](float sum, float inv) { return down < inv ? sum * down * inv : sum * inv * down; };
-            if (a.mode == W4_GATEUP && b) {
+            // Through shared memory, so that what comes now is a loop: unrolled over the registers it was 38000 cycles of a cold
+            // instruction cache per tile. A thread reads what it wrote itself (gate/up: what its partner wrote, too).
+            float *mine = exch + b * (WM_ROWS * 128) + r;
 #pragma unroll
-                for (int k = 0; k < WM_ROWS; k++) {
-                    const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
-                    if (k < t.np) exch[k * 128 + r] = value(acc[k], inv);
+            for (int k = 0; k < WM_ROWS; k++) mine[k * 128] = acc[k];
+            if (GATEUP) many_all(true);
+            const bool live = row < a.w.rows && (!GATEUP || !b);
+            const size_t ldy = a.parts > 1 ? (size_t)a.w.rows : a.ldy;
+            char *y = a.parts > 1 ? reinterpret_cast<char *>(a.part + (size_t)t.part * a.T * a.w.rows) : static_cast<char *>(a.y);
+            const bool half = a.parts == 1 && a.y_dt == DT_BF16;
+            size_t at = (size_t)t.first * ldy + row;
+#pragma unroll 4
+            for (int k = 0; k < t.np; k++, at += ldy) {
+                const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
+                // (the smaller of the two powers first; NaN stays)
+                const float lo = down < inv ? down : inv, hi = down < inv ? inv : down;
+                float v = mine[k * 128] * lo * hi;
+                if (GATEUP && !b) {
+                    const float other = mine[WM_ROWS * 128 + k * 128], up = other * (up_down < inv ? up_down : inv) * (up_down < inv ? inv : up_down);
+                    v = swiglu_value(v, up, a.limit);
+                }
+                if (live) {
+                    if (half) reinterpret_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
+                    else reinterpret_cast<float *>(y)[at] = v;
                 }
             }
-            if (a.mode == W4_GATEUP) many_all(true);
-            if (a.mode != W4_GATEUP || !b) {
-                const bool live = row < a.w.rows;
-#pragma unroll
-                for (int k = 0; k < WM_ROWS; k++) {
-                    const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
-                    if (k < t.np && live) {
-                        float v = value(acc[k], inv);
-                        if (a.mode == W4_GATEUP) {
-                            float gate = v > a.limit ? a.limit : v, u = exch[k * 128 + r];
-                            u = u > a.limit ? a.limit : (u < -a.limit ? -a.limit : u);
-                            v = gate * sigmoid_near(gate) * u;
-                        }
-                        if (a.parts > 1) a.part[((size_t)t.part * a.T + t.first + k) * a.w.rows + row] = v;
-                        else if (a.y_dt == DT_F32) static_cast<float *>(a.y)[(size_t)(t.first + k) * a.ldy + row] = v;
-                        else static_cast<__nv_bfloat16 *>(a.y)[(size_t)(t.first + k) * a.ldy + row] = __float2bfloat16_rn(v);
-                    }
-                }
-            }
-            if (a.mode == W4_GATEUP) many_all(true);           // the exchange buffer is free again
+            if (GATEUP) many_all(true);                        // the exchange buffer is free again
         }
     }
     tc_fence_before();
@@ -401,13 +398,13 @@ size_t w4_many_part_floats(int rows, int cols, int T)
     return p > 1 ? (size_t)p * T * rows : 0;
 }
 
-template <int TERMS>
+template <int TERMS, bool GATEUP>
 static int many_launch(cudaStream_t st, const ManyMaps &m, const ManyArgs &a, int grid)
 {
     static SmemGrant grant;
-    const size_t smem = 1024 + WM_WS * WM_W_STAGE + (size_t)WM_XS * 2 * TERMS * a.n * 128 + (a.mode == W4_GATEUP ? (size_t)a.n * 512 : 0);
-    if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS>, smem, grant)) return -1;
-    G5B_LAUNCH_PDL(w4_many_kernel<TERMS>, dim3(grid), dim3(WM_THREADS), smem, st, m, a);
+    const size_t smem = 1024 + WM_WS * WM_W_STAGE + (size_t)WM_XS * 2 * TERMS * a.n * 128 + 2 * WM_ROWS * 128 * 4;
+    if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS, GATEUP>, smem, grant)) return -1;
+    G5B_LAUNCH_PDL((w4_many_kernel<TERMS, GATEUP>), dim3(grid), dim3(WM_THREADS), smem, st, m, a);
     return 0;
 }
 
@@ -436,7 +433,9 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     }
     const long long tiles = j.mode == W4_DENSE ? (long long)a.RT * a.TT * a.parts : (long long)a.RT * j.slots.max;
     const int grid = (int)(tiles < dev_sms() ? tiles : dev_sms());
-    if (j.x.n_terms == 2 ? many_launch<2>(st, m, a, grid) : many_launch<1>(st, m, a, grid)) return -1;
+    const bool pair = j.mode == W4_GATEUP;
+    if (j.x.n_terms == 2 ? (pair ? many_launch<2, true>(st, m, a, grid) : many_launch<2, false>(st, m, a, grid))
+                         : (pair ? many_launch<1, true>(st, m, a, grid) : many_launch<1, false>(st, m, a, grid))) return -1;
     if (a.parts > 1)
         G5B_LAUNCH_PDL(w4_parts_kernel, dim3((j.w.rows + 255) / 256, j.T), dim3(256), 0, st, part, a.parts, j.T, j.w.rows, j.y, j.ldy, j.y_dt);
     return 0;
