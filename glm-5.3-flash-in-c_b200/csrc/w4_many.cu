@@ -46,6 +46,7 @@ struct ManyArgs {
     size_t ldy;
     int y_dt;
     float *part;                   // [parts][T][rows], parts > 1
+    int wide;                      // four rows of an output may be stored at once
     float limit;
 };
 
@@ -105,12 +106,27 @@ __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
     }
 }
 
-// True when it is true for all 256 epilogue threads: they go on together or not at all.
-__device__ __forceinline__ bool many_all(bool ok)
+// Bounded wait for two or three barriers, looked at together: each look takes some 200 cycles even when the phase is long over, one after
+// the other they were most of a step. By one thread, or by a whole warp in step (WARP).
+template <bool WARP = false>
+__device__ __forceinline__ bool many_wait(uint64_t *p, uint32_t pp, uint64_t *q, uint32_t qp, uint64_t *r, uint32_t rp, int *err, int code)
+{
+#pragma unroll 1
+    for (int i = 0; i < ST_WAIT_LIMIT; i++) {
+        const bool a = mbar_test(p, pp), b = !q || mbar_test(q, qp), c = !r || mbar_test(r, rp);
+        if (WARP ? __all_sync(0xffffffffu, a && b && c) : a && b && c) return true;
+    }
+    if (!WARP || (threadIdx.x & 31) == 0) atomicExch(err, code);
+    if (WARP) __syncwarp();
+    return false;
+}
+
+// True when it is true for all `threads` of a barrier: they go on together or not at all.
+__device__ __forceinline__ bool many_all(bool ok, int barrier, int threads)
 {
     uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok), "r"(barrier), "r"(threads) : "memory");
     return all != 0;
 }
 
@@ -200,6 +216,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     } else if (warp >= 18) {
         // ------------------------------------------------------------------ products ----
         if (elect_one()) {
+            // (One warp for both blocks' products waited and issued for 2000 cycles a step, of which the tensor cores work 1184.)
             const int b = warp - 18;
             int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
 #pragma unroll 1
@@ -210,8 +227,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll 1
                 for (int kb = t.k0; kb < t.k1; kb++) {
                     const int buf = chunks & 1;
-                    if (c == 0 && chunks >= 2 && !(ok = mbar_wait(&d_empty[b][buf], (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
-                    if (!(ok = mbar_wait(&x_full[xs], (uint32_t)xp, err, 6) && mbar_wait(&a_full[b][as], (uint32_t)ap, err, 7))) break;
+                    const bool fresh = c == 0 && chunks >= 2;
+                    if (!(ok = many_wait(&x_full[xs], (uint32_t)xp, &a_full[b][as], (uint32_t)ap, fresh ? &d_empty[b][buf] : nullptr, (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
                     const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
@@ -262,8 +279,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             for (int kb = t.k0; kb < t.k1; kb++, steps++) {
                 const uint2 sc = next;
                 next = fetch(kb + 1);
-                if (!(ok = mbar_wait_all(&w_full[ws], (uint32_t)wp, err, 9))) break;
-                if (steps >= 2 && !(ok = mbar_wait_all(&a_empty[b][as], (uint32_t)ap, err, 10))) break;
+                if (!(ok = many_wait<true>(&w_full[ws], (uint32_t)wp, steps >= 2 ? &a_empty[b][as] : nullptr, (uint32_t)ap, nullptr, 0u, err, 9))) break;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
 #pragma unroll
@@ -297,6 +313,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         // ------------------------------------------------------------ sums, scales, stores ----
         const int b = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 128);
+        const int bar = GATEUP ? 1 : 1 + b, bar_threads = GATEUP ? 256 : 128;       // (gate/up: both blocks together)
         int chunks = 0;
         bool waited = a.mode != W4_DENSE;
 #pragma unroll 1
@@ -304,7 +321,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             const ManyTile t = many_tile(a, i);
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const size_t srow = (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            const float down = pow2(-many_row_up(a.w.scales + srow, a.w.groups)), up_down = GATEUP ? pow2(-many_row_up(a.up.scales + srow, a.w.groups)) : 0.f;
+            const float down = pow2(-many_row_up((GATEUP && b ? a.up : a.w).scales + srow, a.w.groups));
             float acc[WM_ROWS];
 #pragma unroll
             for (int k = 0; k < WM_ROWS; k++) acc[k] = 0.f;
@@ -328,35 +345,44 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&d_empty[b][buf]);
             }
             if (!waited) { pdl_wait(); waited = true; }
-            if (!(ok = many_all(ok))) break;
+            if (!(ok = many_all(ok, bar, bar_threads))) break;
             const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
-            // Through shared memory, so that what comes now is a loop: unrolled over the registers it was 38000 cycles of a cold
-            // instruction cache per tile. A thread reads what it wrote itself (gate/up: what its partner wrote, too).
-            float *mine = exch + b * (WM_ROWS * 128) + r;
+            // Through shared memory, so that what comes now is a loop (unrolled over the registers it was 38000 cycles of a cold
+            // instruction cache per tile) in which a warp stores 128 weight rows of one activation row, four to a lane.
+            float *sums = exch + b * (WM_ROWS * 128);
 #pragma unroll
-            for (int k = 0; k < WM_ROWS; k++) mine[k * 128] = acc[k];
-            if (GATEUP) many_all(true);
-            const bool live = row < a.w.rows && (!GATEUP || !b);
-            const size_t ldy = a.parts > 1 ? (size_t)a.w.rows : a.ldy;
-            char *y = a.parts > 1 ? reinterpret_cast<char *>(a.part + (size_t)t.part * a.T * a.w.rows) : static_cast<char *>(a.y);
-            const bool half = a.parts == 1 && a.y_dt == DT_BF16;
-            size_t at = (size_t)t.first * ldy + row;
-#pragma unroll 4
-            for (int k = 0; k < t.np; k++, at += ldy) {
+            for (int k = 0; k < WM_ROWS; k++) sums[k * 128 + r] = acc[k] * down;
+            many_all(true, bar, bar_threads);
+            const int row0 = (GATEUP ? t.rt * 128 : t.rt * 256 + b * 128) + lane * 4;
+#pragma unroll 1
+            for (int k = GATEUP ? warp : quarter; k < t.np; k += GATEUP ? 8 : 4) {
                 const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);
-                // (the smaller of the two powers first; NaN stays)
-                const float lo = down < inv ? down : inv, hi = down < inv ? inv : down;
-                float v = mine[k * 128] * lo * hi;
-                if (GATEUP && !b) {
-                    const float other = mine[WM_ROWS * 128 + k * 128], up = other * (up_down < inv ? up_down : inv) * (up_down < inv ? inv : up_down);
-                    v = swiglu_value(v, up, a.limit);
+                const float4 in = *reinterpret_cast<const float4 *>((GATEUP ? exch : sums) + k * 128 + lane * 4);
+                float v[4] = {in.x * inv, in.y * inv, in.z * inv, in.w * inv};
+                if (GATEUP) {
+                    const float4 up = *reinterpret_cast<const float4 *>(exch + (WM_ROWS + k) * 128 + lane * 4);
+                    const float u[4] = {up.x * inv, up.y * inv, up.z * inv, up.w * inv};
+#pragma unroll
+                    for (int q = 0; q < 4; q++) v[q] = swiglu_value(v[q], u[q], a.limit);
                 }
-                if (live) {
-                    if (half) reinterpret_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
-                    else reinterpret_cast<float *>(y)[at] = v;
+                const size_t at = a.parts > 1 ? ((size_t)t.part * a.T + t.first + k) * a.w.rows + row0 : (size_t)(t.first + k) * a.ldy + row0;
+                if (a.parts > 1 || a.y_dt == DT_F32) {
+                    float *y = (a.parts > 1 ? a.part : static_cast<float *>(a.y)) + at;
+                    if (a.wide && row0 + 3 < a.w.rows) *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+                    else
+#pragma unroll
+                        for (int q = 0; q < 4; q++) if (row0 + q < a.w.rows) y[q] = v[q];
+                } else {
+                    __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(a.y) + at;
+                    __align__(8) const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+                    if (a.wide && row0 + 3 < a.w.rows) *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(h);
+                    else
+#pragma unroll
+                        for (int q = 0; q < 4; q++) if (row0 + q < a.w.rows) y[q] = __float2bfloat16_rn(v[q]);
                 }
             }
-            if (GATEUP) many_all(true);                        // the exchange buffer is free again
+            // the buffer is free again
+            many_all(true, bar, bar_threads);
         }
     }
     tc_fence_before();
@@ -419,6 +445,7 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     a.TT = (j.T + a.n - 1) / a.n;
     a.parts = j.mode == W4_DENSE ? w4_many_parts(j.w.rows, j.w.cols, j.T) : 1;
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.part = part; a.limit = j.limit;
+    a.wide = a.parts > 1 ? j.w.rows % 4 == 0 : j.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(j.y) % (j.y_dt == DT_F32 ? 16 : 8) == 0;
     const cuuint64_t wsize[3] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.rows, (cuuint64_t)j.count};
     const cuuint64_t wstride[2] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.codes_stride};
     const cuuint32_t wbox[3] = {64, 128, 1};
