@@ -26,9 +26,12 @@ bool tc_encode_swizzled(CUtensorMap *m, const void *base, CUtensorMapDataType dt
                         const cuuint32_t *box, CUtensorMapSwizzle swizzle);
 
 constexpr int WM_ROWS = 64;                         // activation rows of a tile
-constexpr int WM_WS = 4, WM_XS = 3;                 // stages of codes, of terms
+constexpr int WM_WS = 3, WM_XS = 3;                 // stages of codes, of terms
 constexpr int WM_W_STAGE = 2 * 128 * 64;
 constexpr int WM_THREADS = 20 * 32;
+constexpr int WM_RING = 8;                          // tiles whose rows' powers of two are kept (two converted steps and two sums ahead of the stores)
+// Registers of a thread: 96 at the launch, of which the other warps give some to those that hold the sums (256 * 120 + 384 * 80 = 640 * 96).
+constexpr int WM_REGS_SUM = 120, WM_REGS_REST = 80;
 constexpr int WM_CTAS = 148;                        // SMs of a B200: what the parts along the columns are chosen for
 constexpr int WM_MAX_PARTS = 8;
 
@@ -92,7 +95,8 @@ __device__ __forceinline__ int many_row_up(const uint16_t *srow, int groups)
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-// Eight codes of a word, times the scale (twice in s), as four pairs in the terms' order.
+// Eight codes of a word (WHOLE), or those times the scale (twice in s), as four pairs in the terms' order.
+template <bool WHOLE>
 __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
 {
 #pragma unroll
@@ -100,20 +104,22 @@ __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
         uint32_t a, b;
         asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(v));       // (v & mask) | 1024
         asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(v));
-        f[2 * i] = h2_bits(__hmul2(__hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f)), s));
-        f[2 * i + 1] = h2_bits(__hmul2(__hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)), s));
+        const __half2 lo = __hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f));
+        const __half2 hi = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+        f[2 * i] = h2_bits(WHOLE ? lo : __hmul2(lo, s));
+        f[2 * i + 1] = h2_bits(WHOLE ? hi : __hmul2(hi, s));
         v >>= 8;
     }
 }
 
 // Bounded wait for two or three barriers, looked at together: each look takes some 200 cycles even when the phase is long over, one after
-// the other they were most of a step. By one thread, or by a whole warp in step (WARP).
+// the other they were most of a step. The first, which is expected to be the last to come, is waited for without polling. By one thread, or by a whole warp in step (WARP).
 template <bool WARP = false>
 __device__ __forceinline__ bool many_wait(uint64_t *p, uint32_t pp, uint64_t *q, uint32_t qp, uint64_t *r, uint32_t rp, int *err, int code)
 {
 #pragma unroll 1
     for (int i = 0; i < ST_WAIT_LIMIT; i++) {
-        const bool a = mbar_test(p, pp), b = !q || mbar_test(q, qp), c = !r || mbar_test(r, rp);
+        const bool b = !q || mbar_test(q, qp), c = !r || mbar_test(r, rp), a = mbar_try_wait(p, pp);
         if (WARP ? __all_sync(0xffffffffu, a && b && c) : a && b && c) return true;
     }
     if (!WARP || (threadIdx.x & 31) == 0) atomicExch(err, code);
@@ -130,10 +136,10 @@ __device__ __forceinline__ bool many_all(bool ok, int barrier, int threads)
     return all != 0;
 }
 
-template <int TERMS, bool GATEUP>
+template <int TERMS, bool GATEUP, bool WHOLE>
 __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
 {
-    constexpr int CHUNK = TERMS == 2 ? 1 : 4;               // steps summed inside the tensor cores
+    constexpr int CHUNK = TERMS == 2 ? 1 : 4;               // steps summed inside the tensor cores (WHOLE: one)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -144,6 +150,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     __shared__ uint64_t w_full[WM_WS], w_empty[WM_WS], x_full[WM_XS], x_empty[WM_XS];
     __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
     __shared__ uint32_t s_tmem;
+    __shared__ float s_up[WM_RING][2][128];                 // what takes a row's power of two off again
     int *err = &g_w4_err;
 
     pdl_trigger();
@@ -166,108 +173,119 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     const int tiles = many_tiles(a);
     bool ok = true;
 
-    if (warp == 16) {
-        // --------------------------------------------------------------------- codes ----
-        if (elect_one()) {
-            int s = 0, ph = 1, issued = 0;
+    // (the four warps of a group change their registers in one place)
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WM_REGS_REST));
+        if (warp == 16) {
+            // --------------------------------------------------------------------- codes ----
+            if (elect_one()) {
+                int s = 0, ph = 1, issued = 0;
 #pragma unroll 1
-            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                const ManyTile t = many_tile(a, i);
+                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                    const ManyTile t = many_tile(a, i);
 #pragma unroll 1
-                for (int kb = t.k0; kb < t.k1; kb++) {
-                    if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
-                    mbar_expect_tx(&w_full[s], WM_W_STAGE);
-                    uint8_t *dst = wst + (size_t)s * WM_W_STAGE;
-                    if (GATEUP) {
-                        tma_load_3d(dst, &maps.w, kb * 64, t.rt * 128, t.e, &w_full[s]);
-                        tma_load_3d(dst + WM_W_STAGE / 2, &maps.up, kb * 64, t.rt * 128, t.e, &w_full[s]);
-                    } else {
-                        tma_load_3d(dst, &maps.w, kb * 64, t.rt * 256, t.e, &w_full[s]);
-                        tma_load_3d(dst + WM_W_STAGE / 2, &maps.w, kb * 64, t.rt * 256 + 128, t.e, &w_full[s]);
-                    }
-                    issued++;
-                    if (++s == WM_WS) { s = 0; ph ^= 1; }
-                }
-            }
-            // copies in flight must land before shared memory goes away
-            for (int j = issued - 1; j >= 0 && j >= issued - WM_WS; j--) mbar_wait(&w_full[j % WM_WS], (uint32_t)(j / WM_WS) & 1, err, 2);
-        }
-        __syncwarp();
-    } else if (warp == 17) {
-        // --------------------------------------------------------------------- terms ----
-        pdl_wait();
-        if (elect_one()) {
-            int s = 0, ph = 1, issued = 0;
-#pragma unroll 1
-            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                const ManyTile t = many_tile(a, i);
-#pragma unroll 1
-                for (int kb = t.k0; kb < t.k1; kb++) {
-                    if (issued >= WM_XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
-                    mbar_expect_tx(&x_full[s], (uint32_t)XB);
-                    tma_load_4d(xst + (size_t)s * XB, &maps.x, 0, t.first, 0, kb * 2, &x_full[s]);
-                    issued++;
-                    if (++s == WM_XS) { s = 0; ph ^= 1; }
-                }
-            }
-            for (int j = issued - 1; j >= 0 && j >= issued - WM_XS; j--) mbar_wait(&x_full[j % WM_XS], (uint32_t)(j / WM_XS) & 1, err, 4);
-        }
-        __syncwarp();
-    } else if (warp >= 18) {
-        // ------------------------------------------------------------------ products ----
-        if (elect_one()) {
-            // (One warp for both blocks' products waited and issued for 2000 cycles a step, of which the tensor cores work 1184.)
-            const int b = warp - 18;
-            int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
-#pragma unroll 1
-            for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                const ManyTile t = many_tile(a, i);
-                const uint32_t idesc = tc_idesc(0, t.n);
-                int c = 0;                                   // steps in the current accumulator
-#pragma unroll 1
-                for (int kb = t.k0; kb < t.k1; kb++) {
-                    const int buf = chunks & 1;
-                    const bool fresh = c == 0 && chunks >= 2;
-                    if (!(ok = many_wait(&x_full[xs], (uint32_t)xp, &a_full[b][as], (uint32_t)ap, fresh ? &d_empty[b][buf] : nullptr, (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
-                    const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-#pragma unroll
-                        for (int m = 0; m < TERMS; m++) {
-                            const uint64_t bd = tc_smem_desc(xb + (uint32_t)(((k >> 2) * TERMS + m) * a.n * 128)) + 2 * (k & 3);
-                            tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, c || k || m ? 1u : 0u);
+                    for (int kb = t.k0; kb < t.k1; kb++) {
+                        if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
+                        mbar_expect_tx(&w_full[s], WM_W_STAGE);
+                        uint8_t *dst = wst + (size_t)s * WM_W_STAGE;
+                        if (GATEUP) {
+                            tma_load_3d(dst, &maps.w, kb * 64, t.rt * 128, t.e, &w_full[s]);
+                            tma_load_3d(dst + WM_W_STAGE / 2, &maps.up, kb * 64, t.rt * 128, t.e, &w_full[s]);
+                        } else {
+                            tma_load_3d(dst, &maps.w, kb * 64, t.rt * 256, t.e, &w_full[s]);
+                            tma_load_3d(dst + WM_W_STAGE / 2, &maps.w, kb * 64, t.rt * 256 + 128, t.e, &w_full[s]);
                         }
-                    tc_commit(&a_empty[b][as]);
-                    tc_commit(&x_empty[xs]);
-                    if (++c == CHUNK || kb + 1 == t.k1) { tc_commit(&d_full[b][buf]); chunks++; c = 0; }
-                    if (++as == 2) { as = 0; ap ^= 1; }
-                    if (++xs == WM_XS) { xs = 0; xp ^= 1; }
+                        issued++;
+                        if (++s == WM_WS) { s = 0; ph ^= 1; }
+                    }
                 }
+                // copies in flight must land before shared memory goes away
+                for (int j = issued - 1; j >= 0 && j >= issued - WM_WS; j--) mbar_wait(&w_full[j % WM_WS], (uint32_t)(j / WM_WS) & 1, err, 2);
             }
-            // nothing of this thread is in flight, and no arrival still to come, when the CTA ends
-            tc_commit(&drained[b]);
-            mbar_wait(&drained[b], 0, err, 8);
+            __syncwarp();
+        } else if (warp == 17) {
+            // --------------------------------------------------------------------- terms ----
+            pdl_wait();
+            if (elect_one()) {
+                int s = 0, ph = 1, issued = 0;
+#pragma unroll 1
+                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                    const ManyTile t = many_tile(a, i);
+#pragma unroll 1
+                    for (int kb = t.k0; kb < t.k1; kb++) {
+                        if (issued >= WM_XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
+                        mbar_expect_tx(&x_full[s], (uint32_t)XB);
+                        tma_load_4d(xst + (size_t)s * XB, &maps.x, 0, t.first, 0, kb * 2, &x_full[s]);
+                        issued++;
+                        if (++s == WM_XS) { s = 0; ph ^= 1; }
+                    }
+                }
+                for (int j = issued - 1; j >= 0 && j >= issued - WM_XS; j--) mbar_wait(&x_full[j % WM_XS], (uint32_t)(j / WM_XS) & 1, err, 4);
+            }
+            __syncwarp();
+        } else if (warp >= 18) {
+            // ------------------------------------------------------------------ products ----
+            if (elect_one()) {
+                // (One warp for both blocks' products waited and issued for 2000 cycles a step, of which the tensor cores work 1184.)
+                const int b = warp - 18;
+                int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
+#pragma unroll 1
+                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+                    const ManyTile t = many_tile(a, i);
+                    const uint32_t idesc = tc_idesc(0, t.n);
+                    int c = 0;                                   // steps in the current accumulator
+#pragma unroll 1
+                    for (int kb = t.k0; kb < t.k1; kb++) {
+                        const int buf = chunks & 1;
+                        const bool fresh = c == 0 && chunks >= 2;
+                        if (!(ok = many_wait(&a_full[b][as], (uint32_t)ap, &x_full[xs], (uint32_t)xp, fresh ? &d_empty[b][buf] : nullptr, (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
+                        tc_fence_after();
+                        const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
+                        const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+#pragma unroll
+                            for (int m = 0; m < TERMS; m++) {
+                                const uint64_t bd = tc_smem_desc(xb + (uint32_t)(((k >> 2) * TERMS + m) * a.n * 128)) + 2 * (k & 3);
+                                tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, c || k || m ? 1u : 0u);
+                            }
+                        tc_commit(&a_empty[b][as]);
+                        tc_commit(&x_empty[xs]);
+                        if (++c == CHUNK || kb + 1 == t.k1) { tc_commit(&d_full[b][buf]); chunks++; c = 0; }
+                        if (++as == 2) { as = 0; ap ^= 1; }
+                        if (++xs == WM_XS) { xs = 0; xp ^= 1; }
+                    }
+                }
+                // nothing of this thread is in flight, and no arrival still to come, when the CTA ends
+                tc_commit(&drained[b]);
+                mbar_wait(&drained[b], 0, err, 8);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else if (warp >= 8) {
         // --------------------------------------------------- codes -> F16 in tensor memory ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WM_REGS_REST));
         const int b = (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane, x = (r >> 1) & 3;
         const uint32_t dst = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (uint32_t)(b * 64);
         const int per = a.w.group == 128 ? 2 : a.w.group == 64 ? 1 : 0;        // a 32-column piece's group: piece >> per
-        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0;
+        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0, n_tile = 0;
 #pragma unroll 1
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
             const ManyTile t = many_tile(a, i);
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            const float up = pow2(many_row_up(srow, a.w.groups));
+            float up = 0.f;
+            if (!WHOLE) {
+                const int e = many_row_up(srow, a.w.groups);
+                up = pow2(e);
+                s_up[n_tile & (WM_RING - 1)][b][r] = pow2(-e);
+                n_tile++;
+            }
             // raw scales of a step's four pieces, one step ahead
             auto fetch = [&](int kb) {
                 uint2 v = make_uint2(0u, 0u);
-                if (kb < t.k1) {
+                if (!WHOLE && kb < t.k1) {
                     if (per == 2) v.x = __ldg(srow + kb);
                     else if (per == 1) v.x = __ldg(reinterpret_cast<const uint32_t *>(srow) + kb);
                     else v = __ldg(reinterpret_cast<const uint2 *>(srow) + kb);
@@ -279,7 +297,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             for (int kb = t.k0; kb < t.k1; kb++, steps++) {
                 const uint2 sc = next;
                 next = fetch(kb + 1);
-                if (!(ok = many_wait<true>(&w_full[ws], (uint32_t)wp, steps >= 2 ? &a_empty[b][as] : nullptr, (uint32_t)ap, nullptr, 0u, err, 9))) break;
+                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) break;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
 #pragma unroll
@@ -290,11 +308,11 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                         const int piece = h * 2 + c, g = piece >> per;
                         const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
                         // (a group behind the last: zero, whatever lies there)
-                        const float s = ((4 * kb + piece) >> per) < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f;
-                        const __half2 s2 = __float2half2_rn(s);
-                        const uint4 v = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
-                        many_convert(v.x, s2, f + c * 16); many_convert(v.y, s2, f + c * 16 + 4);
-                        many_convert(v.z, s2, f + c * 16 + 8); many_convert(v.w, s2, f + c * 16 + 12);
+                        const float v = !WHOLE && ((4 * kb + piece) >> per) < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f;
+                        const __half2 s2 = __float2half2_rn(v);
+                        const uint4 q = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
+                        many_convert<WHOLE>(q.x, s2, f + c * 16); many_convert<WHOLE>(q.y, s2, f + c * 16 + 4);
+                        many_convert<WHOLE>(q.z, s2, f + c * 16 + 8); many_convert<WHOLE>(q.w, s2, f + c * 16 + 12);
                     }
                     tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
                 }
@@ -311,47 +329,63 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         }
     } else {
         // ------------------------------------------------------------ sums, scales, stores ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WM_REGS_SUM));
         const int b = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 128);
         const int bar = GATEUP ? 1 : 1 + b, bar_threads = GATEUP ? 256 : 128;       // (gate/up: both blocks together)
         int chunks = 0;
-        bool waited = a.mode != W4_DENSE;
+        int n_tile = 0;
+        pdl_wait();
 #pragma unroll 1
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x, n_tile++) {
             const ManyTile t = many_tile(a, i);
-            const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
-            const size_t srow = (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            const float down = pow2(-many_row_up((GATEUP && b ? a.up : a.w).scales + srow, a.w.groups));
-            float acc[WM_ROWS];
+            const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
+            F2 acc[WM_ROWS / 2];
 #pragma unroll
-            for (int k = 0; k < WM_ROWS; k++) acc[k] = 0.f;
+            for (int k = 0; k < WM_ROWS / 2; k++) acc[k] = f2(0.f, 0.f);
+            // WHOLE: a step's scale, one step ahead
+            const W4Mat &w = GATEUP && b ? a.up : a.w;
+            const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
+            const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
+            uint16_t next = 0;
+            if (WHOLE) next = __ldg(srow + t.k0);
             const int uses = (t.k1 - t.k0 + CHUNK - 1) / CHUNK;
 #pragma unroll 1
             for (int c = 0; c < uses; c++, chunks++) {
                 const int buf = chunks & 1;
+                const float sc = bf16_to_f32(next);
+                if (WHOLE && c + 1 < uses) next = __ldg(srow + t.k0 + c + 1);
                 if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(chunks >> 1) & 1, err, 11))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int g = 0; g < WM_ROWS; g += 16)
-                    if (g < t.n) {
-                        uint32_t v[16];
-                        tmem_ld16(lane_addr + (uint32_t)(buf * 64 + g), v);
+                for (int g = 0; g < WM_ROWS; g += 32)
+                    if (g < t.n) {                                     // (columns past the rows hold nothing that is stored)
+                        uint32_t v[2][16];
+                        tmem_ld16(lane_addr + (uint32_t)(buf * 64 + g), v[0]);
+                        tmem_ld16(lane_addr + (uint32_t)(buf * 64 + g + 16), v[1]);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 16; k++) acc[g + k] = __fadd_rn(acc[g + k], __uint_as_float(v[k]));
+                        for (int k = 0; k < 16; k++) {
+                            const F2 in = f2(__uint_as_float(v[k >> 3][2 * (k & 7)]), __uint_as_float(v[k >> 3][2 * (k & 7) + 1]));
+                            acc[g / 2 + k] = WHOLE ? f2_fma(in, f2(sc, sc), acc[g / 2 + k]) : f2_add(acc[g / 2 + k], in);
+                        }
                     }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d_empty[b][buf]);
             }
-            if (!waited) { pdl_wait(); waited = true; }
             if (!(ok = many_all(ok, bar, bar_threads))) break;
-            const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
             // Through shared memory, so that what comes now is a loop (unrolled over the registers it was 38000 cycles of a cold
             // instruction cache per tile) in which a warp stores 128 weight rows of one activation row, four to a lane.
             float *sums = exch + b * (WM_ROWS * 128);
+            const float down = WHOLE ? 1.0f : s_up[n_tile & (WM_RING - 1)][b][r];
 #pragma unroll
-            for (int k = 0; k < WM_ROWS; k++) sums[k * 128 + r] = acc[k] * down;
+            for (int k = 0; k < WM_ROWS; k += 2) {
+                float x, y;
+                f2_get(acc[k / 2], x, y);
+                sums[k * 128 + r] = x * down;
+                sums[k * 128 + 128 + r] = y * down;
+            }
             many_all(true, bar, bar_threads);
             const int row0 = (GATEUP ? t.rt * 128 : t.rt * 256 + b * 128) + lane * 4;
 #pragma unroll 1
@@ -424,13 +458,13 @@ size_t w4_many_part_floats(int rows, int cols, int T)
     return p > 1 ? (size_t)p * T * rows : 0;
 }
 
-template <int TERMS, bool GATEUP>
+template <int TERMS, bool GATEUP, bool WHOLE>
 static int many_launch(cudaStream_t st, const ManyMaps &m, const ManyArgs &a, int grid)
 {
     static SmemGrant grant;
     const size_t smem = 1024 + WM_WS * WM_W_STAGE + (size_t)WM_XS * 2 * TERMS * a.n * 128 + 2 * WM_ROWS * 128 * 4;
-    if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS, GATEUP>, smem, grant)) return -1;
-    G5B_LAUNCH_PDL((w4_many_kernel<TERMS, GATEUP>), dim3(grid), dim3(WM_THREADS), smem, st, m, a);
+    if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS, GATEUP, WHOLE>, smem, grant)) return -1;
+    G5B_LAUNCH_PDL((w4_many_kernel<TERMS, GATEUP, WHOLE>), dim3(grid), dim3(WM_THREADS), smem, st, m, a);
     return 0;
 }
 
@@ -460,9 +494,11 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     }
     const long long tiles = j.mode == W4_DENSE ? (long long)a.RT * a.TT * a.parts : (long long)a.RT * j.slots.max;
     const int grid = (int)(tiles < dev_sms() ? tiles : dev_sms());
-    const bool pair = j.mode == W4_GATEUP;
-    if (j.x.n_terms == 2 ? (pair ? many_launch<2, true>(st, m, a, grid) : many_launch<2, false>(st, m, a, grid))
-                         : (pair ? many_launch<1, true>(st, m, a, grid) : many_launch<1, false>(st, m, a, grid))) return -1;
+    const bool pair = j.mode == W4_GATEUP, whole = j.w.group == 128;
+    const int rc = j.x.n_terms == 1 ? (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
+                   : whole ? (pair ? many_launch<2, true, true>(st, m, a, grid) : many_launch<2, false, true>(st, m, a, grid))
+                           : (pair ? many_launch<2, true, false>(st, m, a, grid) : many_launch<2, false, false>(st, m, a, grid));
+    if (rc) return -1;
     if (a.parts > 1)
         G5B_LAUNCH_PDL(w4_parts_kernel, dim3((j.w.rows + 255) / 256, j.T), dim3(256), 0, st, part, a.parts, j.T, j.w.rows, j.y, j.ldy, j.y_dt);
     return 0;
