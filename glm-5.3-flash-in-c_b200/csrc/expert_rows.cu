@@ -169,7 +169,7 @@ __device__ __forceinline__ void row_store(uint16_t *p, float v) { *p = __bfloat1
 
 // A CTA: one token, 256 * V columns. V values of a row are one load.
 template <typename IN, typename OUT, int V>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, size_t ldr, const int *place, const float *w, int topk, int cols,
+__global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, size_t ldr, const int *place, int E, const float *w, int topk, int cols,
                                                              OUT *out, size_t ldo)
 {
     pdl_wait();
@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, siz
     for (int i = 0; i < V; i++) sum[i] = 0.f;
 #pragma unroll 8
     for (int k = 0; k < topk; k++) {
-        const int p = __ldg(at + k);
+        int p = __ldg(at + k);
+        if (E) p = p >= 0 && p < E ? t * topk + k : -1;
         if (p < 0) continue;
         const float f = wt ? __ldg(wt + k) : 1.0f;
         const InV in = *reinterpret_cast<const InV *>(rows + (size_t)p * ldr + c);
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, siz
 }
 
 template <typename IN, typename OUT>
-static void combine_as(cudaStream_t st, const void *rows, size_t ldr, const int *place, const float *w, int T, int topk, int cols, void *out, size_t ldo, bool early)
+static void combine_as(cudaStream_t st, const void *rows, size_t ldr, const int *place, int E, const float *w, int T, int topk, int cols, void *out, size_t ldo, bool early)
 {
     constexpr int V = 16 / (sizeof(IN) > sizeof(OUT) ? sizeof(IN) : sizeof(OUT));
     const IN *in = static_cast<const IN *>(rows);
@@ -206,17 +207,17 @@ static void combine_as(cudaStream_t st, const void *rows, size_t ldr, const int 
     const bool wide = reinterpret_cast<uintptr_t>(rows) % (V * sizeof(IN)) == 0 && reinterpret_cast<uintptr_t>(out) % (V * sizeof(OUT)) == 0 &&
                       ldr % V == 0 && ldo % V == 0 && cols % V == 0;
     const dim3 grid(T, (cols + 256 * (wide ? V : 1) - 1) / (256 * (wide ? V : 1)));
-    if (wide && early)  G5B_LAUNCH_PDL((expert_combine_kernel<IN, OUT, V>), grid, dim3(256), 0, st, in, ldr, place, w, topk, cols, o, ldo);
-    else if (wide)      G5B_LAUNCH((expert_combine_kernel<IN, OUT, V>), grid, 256, 0, st, in, ldr, place, w, topk, cols, o, ldo);
-    else                G5B_LAUNCH((expert_combine_kernel<IN, OUT, 1>), grid, 256, 0, st, in, ldr, place, w, topk, cols, o, ldo);
+    if (wide && early)  G5B_LAUNCH_PDL((expert_combine_kernel<IN, OUT, V>), grid, dim3(256), 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
+    else if (wide)      G5B_LAUNCH((expert_combine_kernel<IN, OUT, V>), grid, 256, 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
+    else                G5B_LAUNCH((expert_combine_kernel<IN, OUT, 1>), grid, 256, 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
 }
 
-void expert_combine(cudaStream_t st, const void *rows, int rows_dt, size_t ldr, const int *place, const float *w, int T, int topk, int cols,
+void expert_combine(cudaStream_t st, const void *rows, int rows_dt, size_t ldr, const int *place, int E, const float *w, int T, int topk, int cols,
                     void *out, int out_dt, size_t ldo, bool early)
 {
-    if (rows_dt == DT_F32 && out_dt == DT_F32) combine_as<float, float>(st, rows, ldr, place, w, T, topk, cols, out, ldo, early);
-    else if (rows_dt == DT_F32)                combine_as<float, uint16_t>(st, rows, ldr, place, w, T, topk, cols, out, ldo, early);
-    else                                       combine_as<uint16_t, uint16_t>(st, rows, ldr, place, w, T, topk, cols, out, ldo, early);
+    if (rows_dt == DT_F32 && out_dt == DT_F32) combine_as<float, float>(st, rows, ldr, place, E, w, T, topk, cols, out, ldo, early);
+    else if (rows_dt == DT_F32)                combine_as<float, uint16_t>(st, rows, ldr, place, E, w, T, topk, cols, out, ldo, early);
+    else                                       combine_as<uint16_t, uint16_t>(st, rows, ldr, place, E, w, T, topk, cols, out, ldo, early);
 }
 
 }  // namespace g5b

@@ -43,18 +43,21 @@ struct W4Job {
     int mode;
     W4Mat w, up;                // gate/up: w is the gate
     int count;                  // matrices of the stack
-    W4Terms x;
-    int T;                      // rows of x (experts: of picks, at most)
-    const int *order; int topk; // gate/up in w4_few: the terms' row of sorted row i is order[i] / topk
+    int n_terms;                // terms of an activation
+    int T;                      // rows of activations (experts: picks, at most)
+    const void *x; int x_dt; size_t ldx;        // w4_few: the activations (dense, gate/up: the caller's; down: F32 rows of picks)
+    const int *order; int topk;                 // w4_few, gate/up: the activation row of sorted row i is order[i] / topk
+    const int *idx;             // w4_few: not sorted, every pick a slot of its own (slots and order are not used then)
+    bool early;                 // w4_few: may be scheduled while the kernel before it drains
+    W4Terms terms;              // w4_many: the activations as terms, in the order of the rows
     W4Slots slots;
     void *y; size_t ldy; int y_dt;
     float limit;
 };
-// Which of the two kernels multiplies `rows` activation rows (experts: rows of one expert on average), and how many of them make a tile.
-// w4_few goes past up to 32 columns (terms of rows) at a time.
-inline bool w4_few_takes(int n_terms, int rows) { return rows * n_terms <= 32; }
-int  w4_few_rows(int n_terms, int rows);
+// w4_few takes up to eight columns of terms at a time: rows of a tile for matrices of so many columns (0: none).
+int  w4_few_rows(int n_terms, int cols);
 int  w4_few(cudaStream_t st, const W4Job &job);
+int  w4_few_status(cudaStream_t st);
 constexpr int W4_MANY_ROWS = 64;
 size_t w4_many_part_floats(int rows, int cols, int T);      // room for the sums of a dense product's parts
 int  w4_many(cudaStream_t st, const W4Job &job, float *part);
@@ -64,7 +67,8 @@ int  w4_many_status(cudaStream_t st);
 int  expert_sort(cudaStream_t st, const int *idx, int T, int topk, int E, int *order, int *place, int *offsets, const W4Slots *slots);
 void expert_gather(cudaStream_t st, const void *x, size_t row_bytes, size_t x_bytes, size_t out_bytes, const int *order, const int *offsets,
                    int n, int topk, int E, void *rows);
-void expert_combine(cudaStream_t st, const void *rows, int rows_dt, size_t ldr, const int *place, const float *w, int T, int topk, int cols,
+// place, or (E > 0) picks as they came: row p is pick p's, if its expert is one of E
+void expert_combine(cudaStream_t st, const void *rows, int rows_dt, size_t ldr, const int *place, int E, const float *w, int T, int topk, int cols,
                     void *out, int out_dt, size_t ldo, bool early);
 
 // ---- w4_convert.cu

