@@ -22,7 +22,6 @@
 // Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
 
-#include "mma_stage.cuh"
 #include "tc_ptx.cuh"
 #include "w4.cuh"
 
@@ -54,6 +53,7 @@ struct FewArgs {
     float limit;
     int whole_rows;                // rows of codes are whole chunks: one load brings all of a stage's
     int chunks, scale_cols;        // of a stage at most
+    int scale_pitch;               // scales of a stage's row: eight more, so that eight rows lie in different banks
     int stages, stage_bytes, stage_tx;
 };
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
@@ -80,6 +80,12 @@ __device__ __forceinline__ void nibbles(uint32_t v, uint32_t &lo, uint32_t &hi)
     const __half2 h = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
     lo = *reinterpret_cast<const uint32_t *>(&l);
     hi = *reinterpret_cast<const uint32_t *>(&h);
+}
+// (not volatile: two blocks' chains of these are put side by side)
+__device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&g)[4], const uint32_t (&h)[4], int k, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(g[k]), "r"(h[k]), "r"(g[k + 1]), "r"(h[k + 1]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
@@ -111,7 +117,7 @@ __device__ __forceinline__ void few_load8<uint16_t>(float (&v)[8], const uint16_
 
 // The 512 consumer threads: rows of an item as terms. terms: [block][j][column][t] 16 bytes, as the lanes read them; inv: 2^-e of each row.
 // The power of two brings the row's largest magnitude below 2^14; what falls below F16's 2^-24 then is 2^-38 of it.
-template <int TERMS, int MODE, bool WHOLE, typename IN>
+template <int TERMS, int MODE, bool WHOLE, int NS, typename IN>
 __device__ __forceinline__ void few_terms(const FewArgs &a, const FewItem &it, uint4 *terms, float *inv, uint32_t *s_max)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,7 +144,6 @@ __device__ __forceinline__ void few_terms(const FewArgs &a, const FewItem &it, u
     const int e = max((int)(m >> 23), 1) - 126, up = min(14 - e, 126);
     const float scale = __int_as_float((up + 127) << 23);
     if (live && (threadIdx.x & (per * 32 - 1)) == 0) inv[i] = finite ? __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
-    const int n = it.count * TERMS;
     if (live)
         for (int c = c_first; c < a.blocks * 128; c += c_step) {
             float v[8];
@@ -152,15 +157,15 @@ __device__ __forceinline__ void few_terms(const FewArgs &a, const FewItem &it, u
                 l[to] = __float2half_rn(f - __half2float(h[to]));
             }
             const int w = (c & 127) >> 3, j = WHOLE ? w & 3 : w >> 2, t = WHOLE ? w >> 2 : w & 3;
-            uint4 *to = terms + (size_t)(((c >> 7) * 4 + j) * n + i * TERMS) * 4 + t;
+            uint4 *to = terms + (((c >> 7) * 4 + j) * NS + i * TERMS) * 4 + t;
             to[0] = *reinterpret_cast<const uint4 *>(h);
             if (TERMS == 2) to[4] = *reinterpret_cast<const uint4 *>(l);
         }
     bar_sync(1, FW_WARPS * 32);
 }
 
-// WHOLE: groups of 128.
-template <int TERMS, int MODE, bool WHOLE>
+// WHOLE: groups of 128. NS: columns that the terms have room for.
+template <int TERMS, int MODE, bool WHOLE, int NS>
 __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_constant__ FewMaps maps, const FewArgs a)
 {
     constexpr int HALVES = MODE == W4_GATEUP ? 2 : 1, HALF_ROWS = 16 / HALVES;
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                             else
                                 for (int c = 0; c < a.chunks; c++)
                                     tma_load_3d(half + c * (HALF_ROWS * 128), &maps.codes[h], p * (FW_PIECE / 2) + c * 128, it.tile * HALF_ROWS, it.e, &full[s]);
-                            tma_load_3d(to + a.chunks * 2048 + h * (HALF_ROWS * 2) * a.scale_cols, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, &full[s]);
+                            tma_load_3d(to + a.chunks * 2048 + h * (HALF_ROWS * 2) * a.scale_pitch, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, &full[s]);
                         }
                         issued++;
                         if (++s == a.stages) { s = 0; ph ^= 1; }
@@ -228,69 +233,86 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), turn = 0, uses = 0;
     bool fresh = true;
     FewItem it{};
+    // Lane row g is weight row wr: the two rows of a quarter of a warp are four apart, so that their pieces lie in different banks.
+    const int wr = (g >> 1) | ((g & 1) << 2);
+    int off[4];                                           // of this lane's pieces (words) in a chunk
+#pragma unroll
+    for (int j = 0; j < 4; j++) off[j] = WHOLE ? (((gw & 1) * 4 + t) ^ wr) * 16 : (((gw & 1) * 4 + j) ^ wr) * 16 + 4 * t;
+    // (lanes of columns behind the last read the last one's: what comes of it is not used)
+    const uint4 *xt = terms + min(g, NS - 1) * 4 + t;
 #pragma unroll 1
     for (long long i = i0; i < i1; i++) {
         if (fresh) {
             it = few_item<MODE>(a, slot, tile);
             if (it.count) {
-                if (MODE == W4_DOWN || a.x_dt == DT_F32) few_terms<TERMS, MODE, WHOLE, float>(a, it, terms, s_inv, s_max);
-                else                                     few_terms<TERMS, MODE, WHOLE, uint16_t>(a, it, terms, s_inv, s_max);
+                if (MODE == W4_DOWN || a.x_dt == DT_F32) few_terms<TERMS, MODE, WHOLE, NS, float>(a, it, terms, s_inv, s_max);
+                else                                     few_terms<TERMS, MODE, WHOLE, NS, uint16_t>(a, it, terms, s_inv, s_max);
             }
             fresh = false;
         }
         it.tile = tile;
         if (it.count) {
             if (turn == team) {
-                const int n = it.count * TERMS;
-                const bool live = g < n;
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int p = 0; p < pieces; p++) {
                     const uint8_t *st = ring + (size_t)s * a.stage_bytes;
                     if (!(ok = ok && mbar_wait_all(&full[s], (uint32_t)ph, err, 3))) break;      // (the barriers below are met all the same)
                     const int nb = min(FW_PIECE / 128, a.blocks - p * (FW_PIECE / 128));
-                    // a row's chunks of 128 bytes are HALF_ROWS * 128 apart, its 16-byte pieces at piece ^ (row & 7)
-                    const uint8_t *cg = st + g * 128, *ch = cg + (MODE == W4_GATEUP ? a.chunks * 1024 : 1024);
-                    const uint16_t *sg = reinterpret_cast<const uint16_t *>(st + a.chunks * 2048) + g * a.scale_cols, *sh = sg + 8 * a.scale_cols;
-                    const uint4 *xp = terms + ((size_t)p * (FW_PIECE / 128) * 4 * n + g) * 4 + t;
-#pragma unroll 2
-                    for (int b = gw; b < nb; b += 8) {
-                        const int at = (b >> 1) * (HALF_ROWS * 128), half = (b & 1) * 4;
-                        uint4 vg, vh;
-                        if (WHOLE) {
-                            const int o = at + ((half + t) ^ g) * 16;
-                            vg = *reinterpret_cast<const uint4 *>(cg + o);
-                            vh = *reinterpret_cast<const uint4 *>(ch + o);
-                        } else {
-                            int o[4];
+                    // This warp's blocks are gw, gw + 8, ...: half a chunk of 128 bytes each, chunks HALF_ROWS * 128 apart, a row's 16-byte
+                    // pieces at piece ^ (row & 7). Whatever does not change from block to block is taken out of the loop.
+                    const uint8_t *cg = st + (gw >> 1) * (HALF_ROWS * 128) + wr * 128, *ch = cg + (MODE == W4_GATEUP ? a.chunks * 1024 : 1024);
+                    const uint16_t *sg = reinterpret_cast<const uint16_t *>(st + a.chunks * 2048) + wr * a.scale_pitch + (WHOLE ? gw : (4 * gw) >> wlog), *sh = sg + 8 * a.scale_pitch;
+                    const uint4 *xp = xt + (p * (FW_PIECE / 128) + gw) * (4 * NS * 4);
+                    const int first_group = (4 * (p * (FW_PIECE / 128) + gw)) >> wlog;
+                    // two blocks at a time (the second may not be there): their chains of eight dependent products side by side
+                    auto pair = [&](int i, bool both) {
+                        uint4 vg[2], vh[2];
+                        float c[2][4];
 #pragma unroll
-                            for (int j = 0; j < 4; j++) o[j] = at + ((half + j) ^ g) * 16 + 4 * t;
-                            vg = make_uint4(*reinterpret_cast<const uint32_t *>(cg + o[0]), *reinterpret_cast<const uint32_t *>(cg + o[1]),
-                                            *reinterpret_cast<const uint32_t *>(cg + o[2]), *reinterpret_cast<const uint32_t *>(cg + o[3]));
-                            vh = make_uint4(*reinterpret_cast<const uint32_t *>(ch + o[0]), *reinterpret_cast<const uint32_t *>(ch + o[1]),
-                                            *reinterpret_cast<const uint32_t *>(ch + o[2]), *reinterpret_cast<const uint32_t *>(ch + o[3]));
-                        }
-                        float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                            if (live) x = xp[(size_t)(b * 4 + j) * n * 4];
-                            uint32_t pg[4], ph_[4];
-                            const uint32_t wg = word_of(vg, j), wh = word_of(vh, j);
-                            nibbles(wg, pg[0], pg[1]); nibbles(wg >> 8, pg[2], pg[3]);
-                            nibbles(wh, ph_[0], ph_[1]); nibbles(wh >> 8, ph_[2], ph_[3]);
-                            mma_f16(c, pg[0], ph_[0], pg[1], ph_[1], x.x, x.y);
-                            mma_f16(d, pg[2], ph_[2], pg[3], ph_[3], x.z, x.w);
-                            if (!WHOLE || j == 3) {
-                                // (a group behind the last: zero, whatever lies there)
-                                const int k = WHOLE ? b : (4 * b + j) >> wlog, group = WHOLE ? p * (FW_PIECE / 128) + b : (4 * (p * (FW_PIECE / 128) + b) + j) >> wlog;
-                                const float fg = group < a.w.groups ? bf16_to_f32(sg[k]) : 0.f, fh = group < a.w.groups ? bf16_to_f32(sh[k]) : 0.f;
-                                acc[0] = fmaf(c[0] + d[0], fg, acc[0]); acc[1] = fmaf(c[1] + d[1], fg, acc[1]);
-                                acc[2] = fmaf(c[2] + d[2], fh, acc[2]); acc[3] = fmaf(c[3] + d[3], fh, acc[3]);
-#pragma unroll
-                                for (int q = 0; q < 4; q++) { c[q] = 0.f; d[q] = 0.f; }
+                        for (int u = 0; u < 2; u++) {
+                            if (u && !both) break;
+                            const uint8_t *pg = cg + (i + u) * (4 * HALF_ROWS * 128), *ph_ = ch + (i + u) * (4 * HALF_ROWS * 128);
+                            if (WHOLE) {
+                                vg[u] = *reinterpret_cast<const uint4 *>(pg + off[0]);
+                                vh[u] = *reinterpret_cast<const uint4 *>(ph_ + off[0]);
+                            } else {
+                                vg[u] = make_uint4(*reinterpret_cast<const uint32_t *>(pg + off[0]), *reinterpret_cast<const uint32_t *>(pg + off[1]),
+                                                   *reinterpret_cast<const uint32_t *>(pg + off[2]), *reinterpret_cast<const uint32_t *>(pg + off[3]));
+                                vh[u] = make_uint4(*reinterpret_cast<const uint32_t *>(ph_ + off[0]), *reinterpret_cast<const uint32_t *>(ph_ + off[1]),
+                                                   *reinterpret_cast<const uint32_t *>(ph_ + off[2]), *reinterpret_cast<const uint32_t *>(ph_ + off[3]));
                             }
+#pragma unroll
+                            for (int q = 0; q < 4; q++) c[u][q] = 0.f;
                         }
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                if (u && !both) break;
+                                const uint4 x = xp[((i + u) * 8 * 4 + j) * (NS * 4)];
+                                uint32_t wg[4], wh[4];
+                                const uint32_t rg = word_of(vg[u], j), rh = word_of(vh[u], j);
+                                nibbles(rg, wg[0], wg[1]); nibbles(rg >> 8, wg[2], wg[3]);
+                                nibbles(rh, wh[0], wh[1]); nibbles(rh >> 8, wh[2], wh[3]);
+                                few_mma(c[u], wg, wh, 0, x.x, x.y);
+                                few_mma(c[u], wg, wh, 2, x.z, x.w);
+                                if (!WHOLE || j == 3) {
+                                    // (groups smaller than a block: one behind the last is zero, whatever lies there)
+                                    const int k = WHOLE ? 8 * (i + u) : (32 * (i + u) + j) >> wlog;
+                                    const bool here = WHOLE || first_group + k < a.w.groups;
+                                    const float fg = here ? bf16_to_f32(sg[k]) : 0.f, fh = here ? bf16_to_f32(sh[k]) : 0.f;
+                                    acc[0] = fmaf(c[u][0], fg, acc[0]); acc[1] = fmaf(c[u][1], fg, acc[1]);
+                                    acc[2] = fmaf(c[u][2], fh, acc[2]); acc[3] = fmaf(c[u][3], fh, acc[3]);
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) c[u][q] = 0.f;
+                                }
+                            }
+                    };
+#pragma unroll
+                    for (int i = 0; i < FW_PIECE / 1024; i += 2) {
+                        if (gw + 8 * (i + 1) < nb) pair(i, true);
+                        else if (gw + 8 * i < nb) pair(i, false);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[s]);
@@ -298,8 +320,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                 }
                 float (*sum)[16][FW_COLS] = s_sum[team][uses & 1];
                 uses++;
-                *reinterpret_cast<float2 *>(&sum[gw][g][2 * t]) = make_float2(acc[0], acc[1]);
-                *reinterpret_cast<float2 *>(&sum[gw][g + 8][2 * t]) = make_float2(acc[2], acc[3]);
+                *reinterpret_cast<float2 *>(&sum[gw][wr][2 * t]) = make_float2(acc[0], acc[1]);
+                *reinterpret_cast<float2 *>(&sum[gw][wr + 8][2 * t]) = make_float2(acc[2], acc[3]);
                 bar_sync(2 + team, 256);
                 constexpr int OUT = MODE == W4_GATEUP ? 8 : 16;           // outputs of a row of x
                 if (gt < OUT * it.count) {
@@ -333,30 +355,36 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     }
 }
 
-template <int TERMS, int MODE, bool WHOLE>
+template <int TERMS, int MODE, bool WHOLE, int NS>
 static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
     static SmemGrant grant;
-    const int n = MODE == W4_DENSE ? a.rows : a.idx ? 1 : a.slots.rows, term_bytes = n * TERMS * a.blocks * 256;
+    const int term_bytes = NS * a.blocks * 256;
     a.stages = std::min((FW_SMEM - term_bytes) / a.stage_bytes, FW_MAX_STAGES);
     const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + term_bytes;
     if (a.stages < 2) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
     // (what counts is this and the 17 KB of sums: more than 48 KB of them must be asked for)
-    if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
+    if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
     const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
-    if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
-    else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE>), grid, FW_THREADS, smem, st, m, a);
+    if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
+    else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS>), grid, FW_THREADS, smem, st, m, a);
     return 0;
 }
 template <int TERMS, int MODE>
 static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
-    return a.w.group == 128 ? few_launch<TERMS, MODE, true>(st, m, a, early) : few_launch<TERMS, MODE, false>(st, m, a, early);
+    const bool one = MODE == W4_DENSE ? a.rows == 1 : a.idx != nullptr;              // a row at a time
+    if (a.w.group == 128) return one ? few_launch<TERMS, MODE, true, TERMS>(st, m, a, early) : few_launch<TERMS, MODE, true, FW_COLS>(st, m, a, early);
+    return one ? few_launch<TERMS, MODE, false, TERMS>(st, m, a, early) : few_launch<TERMS, MODE, false, FW_COLS>(st, m, a, early);
 }
 
-// Rows of a tile: eight columns of terms, as many as there is room for.
-int w4_few_rows(int n_terms, int cols) { return std::min(FW_COLS, FW_TERM_BYTES / (2 * w4_kp(cols))) / n_terms; }
+// Rows of a tile: eight columns of terms if there is room for them, else one row if there is for that.
+int w4_few_rows(int n_terms, int cols)
+{
+    const int kp = w4_kp(cols);
+    return 2 * kp * FW_COLS <= FW_TERM_BYTES ? FW_COLS / n_terms : 2 * kp * n_terms <= FW_TERM_BYTES ? 1 : 0;
+}
 
 int w4_few(cudaStream_t st, const W4Job &j)
 {
@@ -371,7 +399,8 @@ int w4_few(cudaStream_t st, const W4Job &j)
     a.whole_rows = j.w.pitch % 128 == 0;
     a.chunks = std::min(16, (j.w.pitch + 127) / 128);
     a.scale_cols = std::min(FW_PIECE / j.w.group, j.w.sp);
-    a.stage_tx = a.chunks * 2048 + 32 * a.scale_cols;
+    a.scale_pitch = a.scale_cols + 8;
+    a.stage_tx = a.chunks * 2048 + 32 * a.scale_pitch;
     a.stage_bytes = (a.stage_tx + 1023) / 1024 * 1024;
     FewMaps m;
     for (int h = 0; h < 2; h++) {
@@ -381,7 +410,7 @@ int w4_few(cudaStream_t st, const W4Job &j)
         const cuuint64_t size4[4] = {128, rows, pitch / 128, count}, stride4[3] = {pitch, 128, (cuuint64_t)w.codes_stride}, size3[3] = {pitch, rows, count}, stride3[2] = {pitch, (cuuint64_t)w.codes_stride};
         const cuuint32_t box4[4] = {128, (cuuint32_t)half_rows, (cuuint32_t)a.chunks, 1}, box3[3] = {128, (cuuint32_t)half_rows, 1};
         const cuuint64_t ssize[3] = {(cuuint64_t)w.sp, rows, count}, sstride[2] = {(cuuint64_t)w.sp * 2, (cuuint64_t)w.scales_stride * 2};
-        const cuuint32_t sbox[3] = {(cuuint32_t)a.scale_cols, (cuuint32_t)half_rows, 1};
+        const cuuint32_t sbox[3] = {(cuuint32_t)a.scale_pitch, (cuuint32_t)half_rows, 1};
         const bool codes = a.whole_rows ? tc_encode_swizzled(&m.codes[h], w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, size4, stride4, box4, CU_TENSOR_MAP_SWIZZLE_128B)
                                         : tc_encode_swizzled(&m.codes[h], w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, size3, stride3, box3, CU_TENSOR_MAP_SWIZZLE_128B);
         if (!codes || !tc_encode_swizzled(&m.scales[h], w.scales, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, ssize, sstride, sbox, CU_TENSOR_MAP_SWIZZLE_NONE)) {

@@ -97,7 +97,7 @@ ExpertsPlan experts_plan(int n_terms, int T, int topk, int E, int H, int I)
 {
     const int n = T * topk, mean = (n + E - 1) / E, rows_h = w4_few_rows(n_terms, H), rows_i = w4_few_rows(n_terms, I), rows = rows_h < rows_i ? rows_h : rows_i;
     if (rows && n <= PICKS_MOST) return {PICKS, 1};
-    if (mean * 2 <= rows) return {FEW, rows};
+    if (rows > 1 && mean * 2 <= rows) return {FEW, rows};
     return {MANY, W4_MANY_ROWS};
 }
 struct ExpertsWs {
