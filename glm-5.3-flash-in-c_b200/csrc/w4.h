@@ -48,14 +48,15 @@ struct W4Job {
     const void *x; int x_dt; size_t ldx;        // w4_few: the activations (dense, gate/up: the caller's; down: F32 rows of picks)
     const int *order; int topk;                 // w4_few, gate/up: the activation row of sorted row i is order[i] / topk
     const int *idx;             // w4_few: not sorted, every pick a slot of its own (slots and order are not used then)
+    bool half;                  // w4_few, down: the caller's rows are BF16
     bool early;                 // w4_few: may be scheduled while the kernel before it drains
     W4Terms terms;              // w4_many: the activations as terms, in the order of the rows
     W4Slots slots;
     void *y; size_t ldy; int y_dt;
     float limit;
 };
-// w4_few takes up to eight columns of terms at a time: rows of a tile for matrices of so many columns (0: none).
-int  w4_few_rows(int n_terms, int cols);
+// Rows that w4_few takes at a time, of a matrix of so many columns (0: none).
+int  w4_few_rows(int dt, int cols);
 int  w4_few(cudaStream_t st, const W4Job &job);
 int  w4_few_status(cudaStream_t st);
 constexpr int W4_MANY_ROWS = 64;

@@ -1,25 +1,27 @@
-// w4_few.cu - 4-bit weights times at most eight columns of activations (terms of rows): one decoded token, a few sequences, the few
-// tokens of an expert in a batch.
+// w4_few.cu - 4-bit weights times at most eight columns of activations (digits of rows): one or two rows of F32, up to four of BF16 - a
+// decoded token, the few tokens of an expert in a batch.
 //
-// Bound by HBM: half a byte and a scale's share per weight. The legacy matrix instruction does the products (16 weight rows x 16
-// columns x 8 activation columns); the 5th-generation tensor cores would need 128 rows at a time and hand-overs of their sums.
+// Bound by HBM: half a byte and a scale's share per weight. The integer matrix instruction does the products (16 weight rows x 32
+// columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand as they are, two AND to eight of them, where
+// F16 values took five logical and four packed operations; activations are 8-bit digits of a fixed-point number; sums are exact.
 // One CTA per SM, persistent. Work comes in items of 16 weight rows (gate/up: eight gate rows and the eight up rows that go with them),
 // in pieces of 4096 columns; a CTA takes a contiguous share of them.
 //   warp 16   brings an item's rows into a ring in shared memory, one TMA load for the codes and one for the scales (gate/up: two
 //             each), as many ahead as fit: they wait for nothing but room, so HBM is busy while sums are put together and rows change.
 //             (A bulk copy per row was 125 cycles of issue each: 2.3 TB/s.)
-//   0-7, 8-15 take items in turn; the eight warps of a team share an item's blocks of 128 columns, and their sums meet in shared
+//   0-7, 8-15 take items in turn, from rings of their own; the eight warps of a team share an item's blocks of 128 columns, and their sums meet in shared
 //             memory in a fixed order
-//   codes     a lane takes 16 bytes of rows g and g + 8 (lane = 4 g + t), a quad 64 bytes: 128 columns of each. Nibbles become F16
-//             pairs without a conversion: (code | 0x6400) is 1024 + code, (16 code | 0x6400) is 1024 + 16 code, and one packed operation
-//             takes the offset (and the 16) off, exactly. A pair is columns i and i + 4 of a word's eight; which column stands for
-//             which k of an MMA does not matter as long as both operands agree, and the activations lie in that order.
+//   codes     a lane takes 16 bytes of rows g and g + 8 (lane = 4 g + t), a quad 64 bytes: 128 columns of each. Low nibbles are one
+//             operand, high nibbles - in place, 16 times their value - another with sums of its own. Which column stands for which
+//             k of an MMA does not matter as long as both operands agree, and the digits lie in that order. What the codes' offset of
+//             8 adds is the digits' sum times 8: the sums start at minus that.
 //   scales    in FP32, once per group, on the sums of the group. A quad's 128 columns are one group of 128; for smaller groups
-//             a lane takes its words 16 bytes apart, so that every pair of MMAs is 32 columns of one group.
-//   x         becomes F16 terms in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
-//             which the lanes read them: F32 rows two terms (22 significant bits of the row's largest), BF16 rows one, exact.
-// Sums are FP32: in the tensor cores over a group, outside across groups.
-// Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
+//             a lane takes its words 16 bytes apart, so that an MMA is 32 columns of one group.
+//   x         becomes digits in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
+//             which the lanes read them: per row and block of 128 columns the power of two below which its values lie, and
+//             integers of 22 bits and a sign in three digits (BF16 rows: 14 bits in two, 2^-15 of the block's largest).
+// Group sums are exact integers, taken into FP32 by the exponent trick (they start at the bits of 1.5 2^23, so that their bits are the
+// float 1.5 2^23 + sum, |sum| < 2^22); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
 
 #include "tc_ptx.cuh"
@@ -28,11 +30,11 @@
 namespace g5b {
 
 constexpr int FW_WARPS = 16, FW_THREADS = (FW_WARPS + 1) * 32;
-constexpr int FW_COLS = 8;                           // activation columns
-constexpr int FW_PIECE = 4096;                       // weight columns of a stage: 16 chunks of 256 (128 bytes)
-constexpr int FW_TERM_BYTES = 64 * 1024;             // room for the terms
+constexpr int FW_COLS = 8;                           // activation columns of an MMA
+constexpr int FW_PIECE = 4096;                       // weight columns of a stage at most (half of them where that leaves too few stages): 16 chunks of 128 bytes
+constexpr int FW_DIGIT_BYTES = 88 * 1024;            // room for the digits
 constexpr int FW_MAX_STAGES = 12;
-constexpr int FW_SMEM = 206 * 1024;                  // for stages and terms (17 KB of sums beside them)
+constexpr int FW_SMEM = 206 * 1024;                  // for stages and digits (17 KB of sums beside them)
 
 static __device__ int g_few_err;                     // a wait that ran out: its code (0: none)
 
@@ -52,9 +54,10 @@ struct FewArgs {
     int y_dt;
     float limit;
     int whole_rows;                // rows of codes are whole chunks: one load brings all of a stage's
+    int piece;                     // blocks of 128 columns of a stage
     int chunks, scale_cols;        // of a stage at most
     int scale_pitch;               // scales of a stage's row: eight more, so that eight rows lie in different banks
-    int stages, stage_bytes, stage_tx;
+    int stages, stage_bytes, stage_tx;      // (stages of a team)
 };
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
 template <int MODE>
@@ -70,23 +73,15 @@ __device__ __forceinline__ FewItem few_item(const FewArgs &a, int slot, int tile
     return FewItem{__ldg(a.slots.expert + slot), __ldg(a.slots.first + slot), __ldg(a.slots.count + slot), tile};
 }
 
-// the two F16 pairs (low nibbles, high nibbles) of a word's bytes 0 and 2, as code - 8
-__device__ __forceinline__ void nibbles(uint32_t v, uint32_t &lo, uint32_t &hi)
-{
-    uint32_t a, b;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(v));       // (v & mask) | 1024
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(v));
-    const __half2 l = __hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f));
-    const __half2 h = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-}
 // (not volatile: two blocks' chains of these are put side by side)
-__device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&g)[4], const uint32_t (&h)[4], int k, uint32_t b0, uint32_t b1)
+__device__ __forceinline__ void few_mma(int (&c)[4], uint32_t g0, uint32_t h0, uint32_t g1, uint32_t h1, uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(g[k]), "r"(h[k]), "r"(g[k + 1]), "r"(h[k + 1]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(g0), "r"(h0), "r"(g1), "r"(h1), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float few_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+constexpr int FW_MAGIC = 0x4b400000;                 // the bits of 1.5 2^23
+__device__ __forceinline__ float few_float(int v) { return __fsub_rn(__int_as_float(v), 12582912.0f); }
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -115,114 +110,144 @@ __device__ __forceinline__ void few_load8<uint16_t>(float (&v)[8], const uint16_
         for (int i = 0; i < 8; i++) v[i] = c + i < cols ? bf16_to_f32(row[c + i]) : 0.f;
 }
 
-// The 512 consumer threads: rows of an item as terms. terms: [block][j][column][t] 16 bytes, as the lanes read them; inv: 2^-e of each row.
-// The power of two brings the row's largest magnitude below 2^14; what falls below F16's 2^-24 then is 2^-38 of it.
+// A block of 128 columns: [part][column][t] 16 bytes of digits as the lanes read them, then for each of the eight columns where the sums
+// start (WHOLE: of the block; else of each 32 columns, with groups of 64 those of both halves in the first) and what a digit stands for.
+template <int NS, bool WHOLE> struct FewBlock {
+    uint4 digits[2][NS][4];
+    int   start[WHOLE ? 1 : 4][FW_COLS];
+    float worth[FW_COLS];
+};
+
+// The 512 consumer threads: rows of an item as digits; 16 lanes hold a block.
 template <int TERMS, int MODE, bool WHOLE, int NS, typename IN>
-__device__ __forceinline__ void few_terms(const FewArgs &a, const FewItem &it, uint4 *terms, float *inv, uint32_t *s_max)
+__device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, FewBlock<NS, WHOLE> *blocks)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = it.count <= 1 ? 1 : it.count <= 2 ? 2 : it.count <= 4 ? 4 : 8, per = FW_WARPS / rows;    // warps to a row
-    const int i = warp / per, c_first = ((warp - i * per) * 32 + lane) * 8, c_step = per * 256;
-    const bool live = i < it.count;
-    const int at = it.first + (live ? i : 0);
-    const int src = MODE != W4_GATEUP ? at : (a.idx ? at : __ldg(a.order + at)) / a.topk;
-    const IN *row = static_cast<const IN *>(a.x) + (size_t)src * a.ldx;
-    uint32_t m = 0;
-    if (live)
-        for (int c = c_first; c < a.cols; c += c_step) {
+    const int rows = it.count <= 1 ? 1 : it.count <= 2 ? 2 : 4, per = FW_WARPS / rows;    // warps to a row
+    const int i = warp / per;
+    bar_sync(1, FW_WARPS * 32);                          // nobody reads the digits of the rows before any more
+    if (i < it.count) {
+        const int at = it.first + i;
+        const int src = MODE != W4_GATEUP ? at : (a.idx ? at : __ldg(a.order + at)) / a.topk;
+        const IN *row = static_cast<const IN *>(a.x) + (size_t)src * a.ldx;
+        const int col = i * TERMS;
+        for (int c0 = (warp - i * per) * 256; c0 < a.blocks * 128; c0 += per * 256) {
+            const int c = c0 + lane * 8;
             float v[8];
             few_load8<IN>(v, row, c, a.cols, a.wide);
+            uint32_t m = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
-        }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) s_max[warp] = m;
-    bar_sync(1, FW_WARPS * 32);                          // (and nobody reads the terms of the rows before any more)
-    for (int k = 0; k < per; k++) m = max(m, s_max[i * per + k]);
-    const bool finite = m < 0x7f800000u;
-    // 2^(e - 1) <= max < 2^e (a subnormal one counts as 2^-126)
-    const int e = max((int)(m >> 23), 1) - 126, up = min(14 - e, 126);
-    const float scale = __int_as_float((up + 127) << 23);
-    if (live && (threadIdx.x & (per * 32 - 1)) == 0) inv[i] = finite ? __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
-    if (live)
-        for (int c = c_first; c < a.blocks * 128; c += c_step) {
-            float v[8];
-            few_load8<IN>(v, row, c, a.cols, a.wide);
-            __align__(16) __half h[8], l[8];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const bool finite = m < 0x7f800000u;
+            // 2^(e - 1) <= max < 2^e (a subnormal one counts as 2^-126)
+            const int e = max((int)(m >> 23), 1) - 126, up = (TERMS == 3 ? 22 : 14) - e;               // -114 <= up <= 147
+            const float scale = few_pow2(up >> 1), scale2 = few_pow2(up - (up >> 1));
+            uint32_t even[TERMS] = {}, odd[TERMS] = {};  // digits of columns 0 2 4 6 and 1 3 5 7
+            int sum[TERMS] = {};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int to = (k & 3) * 2 + (k >> 2);                  // 0 4 1 5 2 6 3 7
-                const float f = finite ? v[k] * scale : 0.f;
-                h[to] = __float2half_rn(f);
-                l[to] = __float2half_rn(f - __half2float(h[to]));
+                int x = finite ? __float2int_rn(v[k] * scale * scale2) : 0;
+#pragma unroll
+                for (int d = 0; d < TERMS; d++) {
+                    const int digit = d + 1 < TERMS ? (int)(int8_t)x : x;
+                    x = (x - digit) >> 8;
+                    sum[d] += digit;
+                    (k & 1 ? odd : even)[d] |= (uint32_t)(digit & 255) << (8 * (k >> 1));
+                }
             }
+            FewBlock<NS, WHOLE> &b = blocks[min(c >> 7, a.blocks - 1)];
+            const bool here = c < a.blocks * 128;
             const int w = (c & 127) >> 3, j = WHOLE ? w & 3 : w >> 2, t = WHOLE ? w >> 2 : w & 3;
-            uint4 *to = terms + (((c >> 7) * 4 + j) * NS + i * TERMS) * 4 + t;
-            to[0] = *reinterpret_cast<const uint4 *>(h);
-            if (TERMS == 2) to[4] = *reinterpret_cast<const uint4 *>(l);
+            const int span = a.w.group == 128 ? 16 : a.w.group == 64 ? 8 : 4;          // lanes of a group
+#pragma unroll
+            for (int d = 0; d < TERMS; d++) {
+                for (int o = 1; o < span; o <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], o);
+                if (!here) continue;
+                if (WHOLE) {
+                    reinterpret_cast<uint32_t *>(&b.digits[0][col + d][t])[j] = even[d];
+                    reinterpret_cast<uint32_t *>(&b.digits[1][col + d][t])[j] = odd[d];
+                    if (w == 0) b.start[0][col + d] = -8 * sum[d];
+                } else {
+                    reinterpret_cast<uint2 *>(&b.digits[j >> 1][col + d][t])[j & 1] = make_uint2(even[d], odd[d]);
+                    if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = FW_MAGIC - 8 * sum[d];
+                }
+                // (2^-147 at least, a subnormal FP32 number)
+                if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(-(up - (up >> 1))) * (d == 0 ? 1.0f : d == 1 ? 256.0f : 65536.0f)
+                                                            : __int_as_float(0x7fc00000);
+            }
         }
+    }
+    __syncwarp();
     bar_sync(1, FW_WARPS * 32);
 }
 
-// WHOLE: groups of 128. NS: columns that the terms have room for.
+// TERMS: digits of an activation. WHOLE: groups of 128. NS: columns that there is room for.
 template <int TERMS, int MODE, bool WHOLE, int NS>
 __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_constant__ FewMaps maps, const FewArgs a)
 {
     constexpr int HALVES = MODE == W4_GATEUP ? 2 : 1, HALF_ROWS = 16 / HALVES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
-    uint8_t *ring = smem;                                                             // [stages][half][chunk][row][128] codes, [half][row][scale_cols] scales
-    uint4 *terms = reinterpret_cast<uint4 *>(smem + (size_t)a.stages * a.stage_bytes);
-    __shared__ uint64_t full[FW_MAX_STAGES], empty[FW_MAX_STAGES];
-    __shared__ float s_sum[2][2][8][16][FW_COLS];                                     // [team][item's parity][warp][row][column]
-    __shared__ float s_inv[FW_COLS];
-    __shared__ uint32_t s_max[FW_WARPS];
+    uint8_t *ring = smem;                                                             // [team][stages][half][chunk][row][128] codes, [half][row][scale_pitch] scales
+    using Block = FewBlock<NS, WHOLE>;
+    Block *blocks = reinterpret_cast<Block *>(smem + (size_t)2 * a.stages * a.stage_bytes);
+    // A team waits for every use of its stages, so none of its waits can take an earlier use's phase for the one it waits for.
+    __shared__ uint64_t full[2][FW_MAX_STAGES], empty[2][FW_MAX_STAGES];
+    __shared__ float s_sum[2][2][8][16][FW_COLS];                                // [team][item's parity][warp][row][column]
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     int *err = &g_few_err;
     pdl_trigger();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < a.stages; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 8); }
+        for (int i = 0; i < a.stages; i++)
+            for (int k = 0; k < 2; k++) { mbar_init(&full[k][i], 1); mbar_init(&empty[k][i], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     if (MODE != W4_DENSE && !a.idx) pdl_wait();           // (the slots are another kernel's)
-    const int pieces = (a.blocks + FW_PIECE / 128 - 1) / (FW_PIECE / 128);
+    const int pieces = (a.blocks + a.piece - 1) / a.piece;
     const long long items = (long long)few_slots<MODE>(a) * a.tiles;
     const long long i0 = items * blockIdx.x / gridDim.x, i1 = items * (blockIdx.x + 1) / gridDim.x;
     bool ok = true;
-    int s = 0, ph = 0;                                    // stage, and the parity of its uses
+    int turn = 0;                                         // the team that takes the item
 
     if (warp == FW_WARPS) {
         // ------------------------------------------------------------------- weights ----
         if (elect_one()) {
-            int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), issued = 0;
+            int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), stage[2] = {0, 0}, parity[2] = {1, 1}, issued[2] = {0, 0};
             FewItem it = i0 < i1 ? few_item<MODE>(a, slot, tile) : FewItem{};
 #pragma unroll 1
             for (long long i = i0; i < i1 && ok; i++) {
                 if (it.count) {
+                    // (the parity that the stage's `empty` must have passed: that of the use before)
+                    int &st = stage[turn];
 #pragma unroll 1
                     for (int p = 0; p < pieces; p++) {
-                        if (issued >= a.stages && !(ok = mbar_wait(&empty[s], (uint32_t)(ph ^ 1), err, 1))) break;
-                        uint8_t *to = ring + (size_t)s * a.stage_bytes;
-                        mbar_expect_tx(&full[s], (uint32_t)a.stage_tx);
+                        if (issued[turn] >= a.stages && !(ok = mbar_wait(&empty[turn][st], (uint32_t)parity[turn], err, 1))) break;
+                        uint8_t *to = ring + (size_t)(turn * a.stages + st) * a.stage_bytes;
+                        uint64_t *bar = &full[turn][st];
+                        mbar_expect_tx(bar, (uint32_t)a.stage_tx);
 #pragma unroll
                         for (int h = 0; h < HALVES; h++) {
                             uint8_t *half = to + h * a.chunks * (HALF_ROWS * 128);
-                            if (a.whole_rows) tma_load_4d(half, &maps.codes[h], 0, it.tile * HALF_ROWS, p * 16, it.e, &full[s]);
+                            if (a.whole_rows) tma_load_4d(half, &maps.codes[h], 0, it.tile * HALF_ROWS, p * (a.piece / 2), it.e, bar);
                             else
                                 for (int c = 0; c < a.chunks; c++)
-                                    tma_load_3d(half + c * (HALF_ROWS * 128), &maps.codes[h], p * (FW_PIECE / 2) + c * 128, it.tile * HALF_ROWS, it.e, &full[s]);
-                            tma_load_3d(to + a.chunks * 2048 + h * (HALF_ROWS * 2) * a.scale_pitch, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, &full[s]);
+                                    tma_load_3d(half + c * (HALF_ROWS * 128), &maps.codes[h], p * (a.piece * 64) + c * 128, it.tile * HALF_ROWS, it.e, bar);
+                            tma_load_3d(to + a.chunks * 2048 + h * (HALF_ROWS * 2) * a.scale_pitch, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, bar);
                         }
-                        issued++;
-                        if (++s == a.stages) { s = 0; ph ^= 1; }
+                        issued[turn]++;
+                        if (++st == a.stages) { st = 0; parity[turn] ^= 1; }
                     }
+                    turn ^= 1;
                 }
                 if (++tile == a.tiles && i + 1 < i1) { tile = 0; it = few_item<MODE>(a, ++slot, 0); }
                 it.tile = tile;
             }
             // copies in flight must land before shared memory goes away
-            for (int j = issued - 1; j >= 0 && j >= issued - a.stages; j--) mbar_wait(&full[j % a.stages], (uint32_t)(j / a.stages) & 1, err, 2);
+            for (int k = 0; k < 2; k++)
+                for (int j = issued[k] - 1; j >= 0 && j >= issued[k] - a.stages; j--) mbar_wait(&full[k][j % a.stages], (uint32_t)(j / a.stages) & 1, err, 2);
         }
         return;
     }
@@ -230,7 +255,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     const int team = warp >> 3, gw = warp & 7, g = lane >> 2, t = lane & 3, gt = threadIdx.x & 255;
     const int wlog = a.w.group == 64 ? 1 : 0;
     pdl_wait();
-    int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), turn = 0, uses = 0;
+    int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), uses = 0, s = 0, ph = 0;      // s, ph: the team's stage, and the parity of its uses
     bool fresh = true;
     FewItem it{};
     // Lane row g is weight row wr: the two rows of a quarter of a warp are four apart, so that their pieces lie in different banks.
@@ -238,15 +263,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     int off[4];                                           // of this lane's pieces (words) in a chunk
 #pragma unroll
     for (int j = 0; j < 4; j++) off[j] = WHOLE ? (((gw & 1) * 4 + t) ^ wr) * 16 : (((gw & 1) * 4 + j) ^ wr) * 16 + 4 * t;
-    // (lanes of columns behind the last read the last one's: what comes of it is not used)
-    const uint4 *xt = terms + min(g, NS - 1) * 4 + t;
+    const int gx = min(g, NS - 1);                        // (lanes of columns behind the last read the last one's: what comes of it is not used)
 #pragma unroll 1
     for (long long i = i0; i < i1; i++) {
         if (fresh) {
             it = few_item<MODE>(a, slot, tile);
             if (it.count) {
-                if (MODE == W4_DOWN || a.x_dt == DT_F32) few_terms<TERMS, MODE, WHOLE, NS, float>(a, it, terms, s_inv, s_max);
-                else                                     few_terms<TERMS, MODE, WHOLE, NS, uint16_t>(a, it, terms, s_inv, s_max);
+                if (MODE == W4_DOWN || TERMS == 3) few_digits<TERMS, MODE, WHOLE, NS, float>(a, it, blocks);
+                else                               few_digits<TERMS, MODE, WHOLE, NS, uint16_t>(a, it, blocks);
             }
             fresh = false;
         }
@@ -256,66 +280,73 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int p = 0; p < pieces; p++) {
-                    const uint8_t *st = ring + (size_t)s * a.stage_bytes;
-                    if (!(ok = ok && mbar_wait_all(&full[s], (uint32_t)ph, err, 3))) break;      // (the barriers below are met all the same)
-                    const int nb = min(FW_PIECE / 128, a.blocks - p * (FW_PIECE / 128));
+                    const uint8_t *st = ring + (size_t)(team * a.stages + s) * a.stage_bytes;
+                    if (!(ok = ok && mbar_wait_all(&full[team][s], (uint32_t)ph, err, 3))) break;      // (the barriers below are met all the same)
+                    const int nb = min(a.piece, a.blocks - p * a.piece);
                     // This warp's blocks are gw, gw + 8, ...: half a chunk of 128 bytes each, chunks HALF_ROWS * 128 apart, a row's 16-byte
                     // pieces at piece ^ (row & 7). Whatever does not change from block to block is taken out of the loop.
                     const uint8_t *cg = st + (gw >> 1) * (HALF_ROWS * 128) + wr * 128, *ch = cg + (MODE == W4_GATEUP ? a.chunks * 1024 : 1024);
                     const uint16_t *sg = reinterpret_cast<const uint16_t *>(st + a.chunks * 2048) + wr * a.scale_pitch + (WHOLE ? gw : (4 * gw) >> wlog), *sh = sg + 8 * a.scale_pitch;
-                    const uint4 *xp = xt + (p * (FW_PIECE / 128) + gw) * (4 * NS * 4);
-                    const int first_group = (4 * (p * (FW_PIECE / 128) + gw)) >> wlog;
-                    // two blocks at a time (the second may not be there): their chains of eight dependent products side by side
-                    auto pair = [&](int i, bool both) {
-                        uint4 vg[2], vh[2];
-                        float c[2][4];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            if (u && !both) break;
-                            const uint8_t *pg = cg + (i + u) * (4 * HALF_ROWS * 128), *ph_ = ch + (i + u) * (4 * HALF_ROWS * 128);
-                            if (WHOLE) {
-                                vg[u] = *reinterpret_cast<const uint4 *>(pg + off[0]);
-                                vh[u] = *reinterpret_cast<const uint4 *>(ph_ + off[0]);
-                            } else {
-                                vg[u] = make_uint4(*reinterpret_cast<const uint32_t *>(pg + off[0]), *reinterpret_cast<const uint32_t *>(pg + off[1]),
-                                                   *reinterpret_cast<const uint32_t *>(pg + off[2]), *reinterpret_cast<const uint32_t *>(pg + off[3]));
-                                vh[u] = make_uint4(*reinterpret_cast<const uint32_t *>(ph_ + off[0]), *reinterpret_cast<const uint32_t *>(ph_ + off[1]),
-                                                   *reinterpret_cast<const uint32_t *>(ph_ + off[2]), *reinterpret_cast<const uint32_t *>(ph_ + off[3]));
-                            }
-#pragma unroll
-                            for (int q = 0; q < 4; q++) c[u][q] = 0.f;
+                    const Block *bp = blocks + p * a.piece + gw;
+                    const int first_group = (4 * (p * a.piece + gw)) >> wlog;
+                    auto block = [&](int i) {
+                        const uint8_t *pg = cg + i * (4 * HALF_ROWS * 128), *ph_ = ch + i * (4 * HALF_ROWS * 128);
+                        const Block &x = bp[8 * i];
+                        uint4 vg, vh;
+                        if (WHOLE) {
+                            vg = *reinterpret_cast<const uint4 *>(pg + off[0]);
+                            vh = *reinterpret_cast<const uint4 *>(ph_ + off[0]);
+                        } else {
+                            vg = make_uint4(*reinterpret_cast<const uint32_t *>(pg + off[0]), *reinterpret_cast<const uint32_t *>(pg + off[1]),
+                                            *reinterpret_cast<const uint32_t *>(pg + off[2]), *reinterpret_cast<const uint32_t *>(pg + off[3]));
+                            vh = make_uint4(*reinterpret_cast<const uint32_t *>(ph_ + off[0]), *reinterpret_cast<const uint32_t *>(ph_ + off[1]),
+                                            *reinterpret_cast<const uint32_t *>(ph_ + off[2]), *reinterpret_cast<const uint32_t *>(ph_ + off[3]));
                         }
+                        constexpr uint32_t LOW = 0x0f0f0f0fu, HIGH = 0xf0f0f0f0u;
+                        constexpr float UNIT = WHOLE ? 0.0625f : 1.0f;              // (WHOLE: the sums are 16 times theirs)
+                        const uint4 x0 = x.digits[0][gx][t], x1 = x.digits[1][gx][t];
+                        const float2 worth = *reinterpret_cast<const float2 *>(&x.worth[2 * t]);
+                        // one group's sums times its scales
+                        auto take = [&](const int (&c)[4], int k) {
+                            // (groups smaller than a block: one behind the last is zero, whatever lies there)
+                            const bool here = WHOLE || first_group + k < a.w.groups;
+                            const float fg = here ? bf16_to_f32(sg[k]) * UNIT : 0.f, fh = here ? bf16_to_f32(sh[k]) * UNIT : 0.f;
+                            // (in this order: a digit's worth alone times a scale may be too small for FP32)
+                            acc[0] = fmaf(few_float(c[0]) * fg, worth.x, acc[0]); acc[1] = fmaf(few_float(c[1]) * fg, worth.y, acc[1]);
+                            acc[2] = fmaf(few_float(c[2]) * fh, worth.x, acc[2]); acc[3] = fmaf(few_float(c[3]) * fh, worth.y, acc[3]);
+                        };
+                        if (WHOLE) {
+                            const int2 start = *reinterpret_cast<const int2 *>(&x.start[0][2 * t]);
+                            int lo[4] = {start.x, start.y, start.x, start.y}, hi[4] = {FW_MAGIC, FW_MAGIC, FW_MAGIC, FW_MAGIC};
+                            few_mma(lo, vg.x & LOW, vh.x & LOW, vg.y & LOW, vh.y & LOW, x0.x, x0.y);
+                            few_mma(hi, vg.x & HIGH, vh.x & HIGH, vg.y & HIGH, vh.y & HIGH, x1.x, x1.y);
+                            few_mma(lo, vg.z & LOW, vh.z & LOW, vg.w & LOW, vh.w & LOW, x0.z, x0.w);
+                            few_mma(hi, vg.z & HIGH, vh.z & HIGH, vg.w & HIGH, vh.w & HIGH, x1.z, x1.w);
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
+                            for (int q = 0; q < 4; q++) hi[q] += 16 * lo[q];
+                            take(hi, 8 * i);
+                        } else {
+                            int c[4];
 #pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                if (u && !both) break;
-                                const uint4 x = xp[((i + u) * 8 * 4 + j) * (NS * 4)];
-                                uint32_t wg[4], wh[4];
-                                const uint32_t rg = word_of(vg[u], j), rh = word_of(vh[u], j);
-                                nibbles(rg, wg[0], wg[1]); nibbles(rg >> 8, wg[2], wg[3]);
-                                nibbles(rh, wh[0], wh[1]); nibbles(rh >> 8, wh[2], wh[3]);
-                                few_mma(c[u], wg, wh, 0, x.x, x.y);
-                                few_mma(c[u], wg, wh, 2, x.z, x.w);
-                                if (!WHOLE || j == 3) {
-                                    // (groups smaller than a block: one behind the last is zero, whatever lies there)
-                                    const int k = WHOLE ? 8 * (i + u) : (32 * (i + u) + j) >> wlog;
-                                    const bool here = WHOLE || first_group + k < a.w.groups;
-                                    const float fg = here ? bf16_to_f32(sg[k]) : 0.f, fh = here ? bf16_to_f32(sh[k]) : 0.f;
-                                    acc[0] = fmaf(c[u][0], fg, acc[0]); acc[1] = fmaf(c[u][1], fg, acc[1]);
-                                    acc[2] = fmaf(c[u][2], fh, acc[2]); acc[3] = fmaf(c[u][3], fh, acc[3]);
-#pragma unroll
-                                    for (int q = 0; q < 4; q++) c[u][q] = 0.f;
+                            for (int j = 0; j < 4; j++) {
+                                const uint32_t rg = word_of(vg, j), rh = word_of(vh, j);
+                                if (wlog == 0 || !(j & 1)) {
+                                    const int2 start = *reinterpret_cast<const int2 *>(&x.start[WHOLE ? 0 : j][2 * t]);
+                                    c[0] = start.x; c[1] = start.y; c[2] = start.x; c[3] = start.y;
                                 }
+                                const uint4 &d = j < 2 ? x0 : x1;
+                                few_mma(c, rg & LOW, rh & LOW, (rg >> 4) & LOW, (rh >> 4) & LOW, j & 1 ? d.z : d.x, j & 1 ? d.w : d.y);
+                                if (wlog == 0 || (j & 1)) take(c, (32 * i + j) >> wlog);
                             }
+                        }
                     };
 #pragma unroll
-                    for (int i = 0; i < FW_PIECE / 1024; i += 2) {
-                        if (gw + 8 * (i + 1) < nb) pair(i, true);
-                        else if (gw + 8 * i < nb) pair(i, false);
+                    for (int i = 0; i < FW_PIECE / 1024; i++) {
+                        if (gw + 8 * i >= nb) break;
+                        block(i);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&empty[s]);
+                    if (lane == 0) mbar_arrive(&empty[team][s]);
                     if (++s == a.stages) { s = 0; ph ^= 1; }
                 }
                 float (*sum)[16][FW_COLS] = s_sum[team][uses & 1];
@@ -325,18 +356,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                 bar_sync(2 + team, 256);
                 constexpr int OUT = MODE == W4_GATEUP ? 8 : 16;           // outputs of a row of x
                 if (gt < OUT * it.count) {
-                    const int r = gt & (OUT - 1), k = gt / OUT;
+                    const int r = gt & (OUT - 1), k = gt / OUT, col = k * TERMS;
                     float v = 0.f, u = 0.f;
 #pragma unroll
                     for (int w = 0; w < 8; w++)
 #pragma unroll
-                        for (int m = TERMS - 1; m >= 0; m--) {
-                            v += sum[w][r][k * TERMS + m];
-                            if (MODE == W4_GATEUP) u += sum[w][r + 8][k * TERMS + m];
+                        for (int m = 0; m < TERMS; m++) {
+                            v += sum[w][r][col + m];
+                            if (MODE == W4_GATEUP) u += sum[w][r + 8][col + m];
                         }
-                    const float inv = s_inv[k];
-                    v *= inv;
-                    if (MODE == W4_GATEUP) v = swiglu_value(v, u * inv, a.limit);
+                    if (MODE == W4_GATEUP) v = swiglu_value(v, u, a.limit);
                     const int row = it.tile * OUT + r;
                     const size_t at = (size_t)(it.first + k) * a.ldy + row;
                     if (row < a.w.rows) {
@@ -344,10 +373,6 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                         else static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(v);
                     }
                 }
-            } else {
-                // the other eight warps' item
-                s += pieces;
-                while (s >= a.stages) { s -= a.stages; ph ^= 1; }
             }
             turn ^= 1;
         }
@@ -359,11 +384,11 @@ template <int TERMS, int MODE, bool WHOLE, int NS>
 static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
     static SmemGrant grant;
-    const int term_bytes = NS * a.blocks * 256;
-    a.stages = std::min((FW_SMEM - term_bytes) / a.stage_bytes, FW_MAX_STAGES);
-    const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + term_bytes;
-    if (a.stages < 2) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
-    // (what counts is this and the 17 KB of sums: more than 48 KB of them must be asked for)
+    const int digit_bytes = (int)sizeof(FewBlock<NS, WHOLE>) * a.blocks;
+    a.stages = std::min((FW_SMEM - digit_bytes) / a.stage_bytes / 2, FW_MAX_STAGES);
+    const size_t smem = 1024 + (size_t)2 * a.stages * a.stage_bytes + digit_bytes;
+    if (a.stages < 1) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
+    // (what counts is this and the sums: more than 48 KB of them must be asked for)
     if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
     const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
@@ -371,24 +396,32 @@ static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
     else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS>), grid, FW_THREADS, smem, st, m, a);
     return 0;
 }
+constexpr int few_one(int terms) { return terms == 3 ? 4 : 2; }          // columns of a single row, with one to spare
+template <int TERMS, int MODE, bool WHOLE>
+static int few_columns(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
+{
+    const int rows = MODE == W4_DENSE ? a.rows : a.idx ? 1 : a.slots.rows;
+    return rows == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS)>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS>(st, m, a, early);
+}
 template <int TERMS, int MODE>
 static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
-    const bool one = MODE == W4_DENSE ? a.rows == 1 : a.idx != nullptr;              // a row at a time
-    if (a.w.group == 128) return one ? few_launch<TERMS, MODE, true, TERMS>(st, m, a, early) : few_launch<TERMS, MODE, true, FW_COLS>(st, m, a, early);
-    return one ? few_launch<TERMS, MODE, false, TERMS>(st, m, a, early) : few_launch<TERMS, MODE, false, FW_COLS>(st, m, a, early);
+    return a.w.group == 128 ? few_columns<TERMS, MODE, true>(st, m, a, early) : few_columns<TERMS, MODE, false>(st, m, a, early);
 }
 
-// Rows of a tile: eight columns of terms if there is room for them, else one row if there is for that.
-int w4_few_rows(int n_terms, int cols)
+// Rows of a tile for a matrix of so many columns: what eight columns hold if there is room for it, else one row if there is for that.
+int w4_few_rows(int dt, int cols)
 {
-    const int kp = w4_kp(cols);
-    return 2 * kp * FW_COLS <= FW_TERM_BYTES ? FW_COLS / n_terms : 2 * kp * n_terms <= FW_TERM_BYTES ? 1 : 0;
+    const int blocks = w4_kp(cols) / 128, terms = dt == DT_F32 ? 3 : 2;
+    const size_t one = dt == DT_F32 ? sizeof(FewBlock<few_one(3), false>) : sizeof(FewBlock<few_one(2), false>);
+    return blocks * sizeof(FewBlock<FW_COLS, false>) <= (size_t)FW_DIGIT_BYTES ? FW_COLS / terms : blocks * one <= (size_t)FW_DIGIT_BYTES ? 1 : 0;
 }
 
 int w4_few(cudaStream_t st, const W4Job &j)
 {
     FewArgs a{};
+    const bool bf16 = j.x_dt == DT_BF16 || (j.mode == W4_DOWN && j.half);
+    const int rows = j.mode == W4_DENSE ? j.T : j.idx ? 1 : j.slots.rows;
     const int size = j.x_dt == DT_F32 ? 4 : 2;
     a.w = j.w; a.x = j.x; a.ldx = j.ldx; a.x_dt = j.x_dt; a.cols = j.w.cols; a.blocks = w4_kp(j.w.cols) / 128;
     a.wide = reinterpret_cast<uintptr_t>(j.x) % 16 == 0 && j.ldx * size % 16 == 0;
@@ -397,11 +430,16 @@ int w4_few(cudaStream_t st, const W4Job &j)
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.limit = j.limit;
     const int half_rows = j.mode == W4_GATEUP ? 8 : 16;
     a.whole_rows = j.w.pitch % 128 == 0;
-    a.chunks = std::min(16, (j.w.pitch + 127) / 128);
-    a.scale_cols = std::min(FW_PIECE / j.w.group, j.w.sp);
-    a.scale_pitch = a.scale_cols + 8;
-    a.stage_tx = a.chunks * 2048 + 32 * a.scale_pitch;
-    a.stage_bytes = (a.stage_tx + 1023) / 1024 * 1024;
+    // Two stages of each team at least: with many digits beside them in pieces of half the columns.
+    const size_t digits = (size_t)a.blocks * (rows == 1 ? sizeof(FewBlock<4, false>) : sizeof(FewBlock<FW_COLS, false>));
+    for (a.piece = FW_PIECE / 128;; a.piece /= 2) {
+        a.chunks = std::min(a.piece / 2, (j.w.pitch + 127) / 128);
+        a.scale_cols = std::min(a.piece * 128 / j.w.group, j.w.sp);
+        a.scale_pitch = a.scale_cols + 8;
+        a.stage_tx = a.chunks * 2048 + 32 * a.scale_pitch;
+        a.stage_bytes = (a.stage_tx + 1023) / 1024 * 1024;
+        if (a.piece < FW_PIECE / 128 || 4 * (size_t)a.stage_bytes + digits <= FW_SMEM) break;
+    }
     FewMaps m;
     for (int h = 0; h < 2; h++) {
         const W4Mat &w = h && j.mode == W4_GATEUP ? j.up : j.w;
@@ -418,9 +456,9 @@ int w4_few(cudaStream_t st, const W4Job &j)
             return -1;
         }
     }
-    if (j.n_terms == 1)
-        return j.mode == W4_DENSE ? few_group<1, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<1, W4_GATEUP>(st, m, a, j.early) : few_group<1, W4_DOWN>(st, m, a, j.early);
-    return j.mode == W4_DENSE ? few_group<2, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<2, W4_GATEUP>(st, m, a, j.early) : few_group<2, W4_DOWN>(st, m, a, j.early);
+    if (bf16)
+        return j.mode == W4_DENSE ? few_group<2, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<2, W4_GATEUP>(st, m, a, j.early) : few_group<2, W4_DOWN>(st, m, a, j.early);
+    return j.mode == W4_DENSE ? few_group<3, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<3, W4_GATEUP>(st, m, a, j.early) : few_group<3, W4_DOWN>(st, m, a, j.early);
 }
 
 int w4_few_status(cudaStream_t st) { return w4_flag(g_few_err, st); }

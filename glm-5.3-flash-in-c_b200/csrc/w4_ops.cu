@@ -93,11 +93,12 @@ int check_ws(const char *op, const void *ws, size_t have, size_t need)
 enum { PICKS, FEW, MANY };
 struct ExpertsPlan { int how, rows; };           // rows of a slot at most
 constexpr int PICKS_MOST = 16;
-ExpertsPlan experts_plan(int n_terms, int T, int topk, int E, int H, int I)
+constexpr int FEW_MOST = 1;                      // rows of an expert, in tiles of w4_few
+ExpertsPlan experts_plan(int dt, int T, int topk, int E, int H, int I)
 {
-    const int n = T * topk, mean = (n + E - 1) / E, rows_h = w4_few_rows(n_terms, H), rows_i = w4_few_rows(n_terms, I), rows = rows_h < rows_i ? rows_h : rows_i;
+    const int n = T * topk, h = w4_few_rows(dt, H), i = w4_few_rows(dt, I), rows = h < i ? h : i;
     if (rows && n <= PICKS_MOST) return {PICKS, 1};
-    if (rows > 1 && mean * 2 <= rows) return {FEW, rows};
+    if (rows > 1 && n <= rows * FEW_MOST * E) return {FEW, rows};
     return {MANY, W4_MANY_ROWS};
 }
 struct ExpertsWs {
@@ -170,7 +171,7 @@ extern "C" size_t g5b_w4_matmul_workspace(const g5b_w4 *m, int dtype, int T)
     if (!m || m->cols < 1 || m->cols > W4_MAX_COLS || T < 0 || T > W4_MAX_TOKENS) return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2;
-    if (T <= w4_few_rows(n_terms, m->cols)) return WS_ALIGN;
+    if (T <= w4_few_rows(dtype, m->cols)) return WS_ALIGN;
     terms_of(ws, n_terms, m->cols, T);
     ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
     return ws.used;
@@ -191,7 +192,7 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     Pieces ws{static_cast<uint8_t *>(workspace)};
     j.mode = W4_DENSE; j.T = T; j.count = 1; j.n_terms = dtype == DT_BF16 ? 1 : 2;
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
-    if (T <= w4_few_rows(j.n_terms, j.w.cols)) {
+    if (T <= w4_few_rows(dtype, j.w.cols)) {
         j.x = x; j.x_dt = dtype; j.ldx = ldx;
         return w4_few(st, j) ? -1 : launched(op);
     }
@@ -250,7 +251,7 @@ extern "C" size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *dow
         return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2, rows = T < 1 ? 1 : T;
-    experts_ws(ws, experts_plan(n_terms, rows, topk, gate->count, gate->cols, down->cols), n_terms, rows, topk, gate->count, gate->cols, down->cols);
+    experts_ws(ws, experts_plan(dtype, rows, topk, gate->count, gate->cols, down->cols), n_terms, rows, topk, gate->count, gate->cols, down->cols);
     return ws.used;
 }
 
@@ -272,7 +273,7 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int E = gate->count, H = wg.cols, I = wg.rows, n = T * topk, n_terms = dtype == DT_BF16 ? 1 : 2;
     Pieces pieces{static_cast<uint8_t *>(workspace)};
-    const ExpertsPlan plan = experts_plan(n_terms, T, topk, E, H, I);
+    const ExpertsPlan plan = experts_plan(dtype, T, topk, E, H, I);
     const ExpertsWs ws = experts_ws(pieces, plan, n_terms, T, topk, E, H, I);
     W4Job j{};
     j.count = E; j.n_terms = n_terms; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
@@ -286,7 +287,7 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
     if (plan.how == MANY) w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, nullptr, 1, true);
     j.mode = W4_DOWN; j.w = wd; j.y = ws.rows; j.ldy = H;
-    j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true;
+    j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true; j.half = dtype == DT_BF16;
     if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
     expert_combine(st, ws.rows, DT_F32, H, plan.how == PICKS ? idx : ws.place, plan.how == PICKS ? E : 0, weights, T, topk, H, out, dtype, ldo, true);
     return launched(op);

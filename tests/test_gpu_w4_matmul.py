@@ -97,7 +97,7 @@ def test_same_bits_every_time_on_any_stream_and_in_a_graph(gpu_lib, T):
     rows, cols, group = 1000, 2048, 128
     codes, scales = ref.make(rng, rows, cols, group)
     x = torch.randn((T, cols), generator=rng).cuda()
-    first = _run(codes, scales, rows, cols, group, x)
+    first, second = _run(codes, scales, rows, cols, group, x), _run(codes, scales, rows, cols, group, -x)
     side = torch.cuda.Stream()
     assert torch.equal(_run(codes, scales, rows, cols, group, x, stream=side.cuda_stream), first)
     # two captured calls with workspaces of their own, replayed beside each other with new inputs
@@ -122,7 +122,7 @@ def test_same_bits_every_time_on_any_stream_and_in_a_graph(gpu_lib, T):
         with torch.cuda.stream(other):
             graphs[1].replay()
     torch.cuda.synchronize()
-    assert torch.equal(outs[0].cpu(), first) and torch.equal(outs[1].cpu(), -first)
+    assert torch.equal(outs[0].cpu(), first) and torch.equal(outs[1].cpu(), second)
 
 
 # ------------------------------------------------------------------ conversion ----

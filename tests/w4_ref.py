@@ -30,16 +30,18 @@ def handle(codes, scales, rows, cols, group):
     return pkg.W4(codes.cuda(), scales.cuda(), rows, cols, group)
 
 
-# What a product may be off, relative to sum_k |w_k x_k|. The terms of a value hold it to half of 2^-21 (F32 rows: 11 + 11
-# bits, 2^-22 of the value; BF16: exactly) and to 2^-38 of the row's largest where they run out of F16's range. Products are exact.
-# Every addition is off by at most 2^-23 of the partial sum (the tensor cores cut, elsewhere half of it); a matrix
-# instruction takes 16 columns with at most two such cuts, and each group of 32 columns is one more addition: at most
-# cols / 16 * 2 + cols / 32 + 16 in a row, whatever order they are taken in.
-def product_bound(w, x, f32=True):
+# What a product may be off. Additions: each is off by at most 2^-23 of the partial sum (the tensor cores cut, elsewhere half of
+# it); a matrix instruction takes 16 columns with at most two such cuts (or is exact in integers), and each group of 32 columns is one
+# more addition: at most cols / 16 * 2 + cols / 32 + 16 in a row, whatever order they are taken in; a partial sum is at most the sum of
+# |w_k x_k|. Activations: fixed-point numbers of 22 bits (BF16 rows: 14) below the power of two over the largest of their 128
+# columns, off by half a step, 2^-23 (2^-15) of that power, so 2^-22 (2^-14) of the largest; or floating ones of 22 bits, off by less
+# (BF16: exact). `own` adds what one F16 term is off, 2^-12 of the value.
+def product_bound(w, x, f32=True, own=0.0):
     cols = x.shape[-1]
-    sums = x.abs() @ w.abs().t()
     steps = 2 * (cols // 16 + 1) + cols // 32 + 16
-    return sums * (steps * 2.0 ** -23 + (2.0 ** -22 if f32 else 0.0)) + x.abs().amax(-1, keepdim=True) * 2.0 ** -38 * w.abs().sum(-1)
+    block = torch.nn.functional.pad(x.abs(), (0, up(cols, 128) - cols)).view(x.shape[0], -1, 128).amax(2).repeat_interleave(128, 1)[:, :cols]
+    held = block * (2.0 ** -22 if f32 else 2.0 ** -14) + x.abs() * own
+    return (x.abs() @ w.abs().t()) * (steps * 2.0 ** -23) + held @ w.abs().t()
 
 
 def rounded(y, dtype):
@@ -68,10 +70,8 @@ def experts(x, idx, weights, gate, up_, down, limit, f32):
             cu = u.abs().clamp(max=limit) + eu
             # |d silu / d g| <= 1.1 where the clamp lets it through; the sigmoid is 1.53 units of 2^-23 off, two products round
             eh = 1.1 * cu * eg + (g.clamp(max=limit) * torch.sigmoid(g.clamp(max=limit))).abs() * eu + h.abs() * 3 * 2.0 ** -23
-            # between the products a row is two F16 terms, or one for BF16 rows (2^-12 of the value)
-            eh = eh + h.abs() * (0.0 if f32 else 2.0 ** -12) + h.abs().amax() * 2.0 ** -38
             y = h @ down[e].t()
-            ey = eh @ down[e].abs().t() + product_bound(down[e], h.abs() + eh, True)
+            ey = eh @ down[e].abs().t() + product_bound(down[e], h.abs() + eh, f32, 0.0 if f32 else 2.0 ** -12)
             wt = float(weights[t, k])
             out[t] += wt * y[0]
             # the sum over the picks: one rounding each, of a partial sum that is no larger than the sum of magnitudes
