@@ -1,5 +1,6 @@
-// w4_few.cu - 4-bit weights times at most eight columns of activations (digits of rows): one or two rows of F32, up to four of BF16 - a
-// decoded token, the few tokens of an expert in a batch.
+// w4_few.cu - 4-bit weights times a few rows of activations: a decoded token or two, the few tokens of an expert in a batch. Eight columns at
+// a time: two F32 rows, four of BF16. (Four F32 rows in sixteen columns were slower than the weights twice: the second product's branch
+// keeps blocks apart. Experts of 64 tokens 805 us against 700.)
 //
 // Bound by HBM: half a byte and a scale's share per weight. The integer matrix instruction does the products (16 weight rows x 32
 // columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand as they are, two AND to eight of them, where
@@ -34,7 +35,7 @@ constexpr int FW_COLS = 8;                           // activation columns of an
 constexpr int FW_PIECE = 4096;                       // weight columns of a stage at most (half of them where that leaves too few stages): 16 chunks of 128 bytes
 constexpr int FW_DIGIT_BYTES = 88 * 1024;            // room for the digits
 constexpr int FW_MAX_STAGES = 12;
-constexpr int FW_SMEM = 206 * 1024;                  // for stages and digits (17 KB of sums beside them)
+constexpr int FW_SMEM = 206 * 1024;                  // for stages and digits with 16 KB of sums beside them
 
 static __device__ int g_few_err;                     // a wait that ran out: its code (0: none)
 
@@ -45,7 +46,7 @@ struct FewArgs {
     size_t ldx;
     int x_dt, cols, blocks;        // columns of x, blocks of 128 of them
     int wide;                      // x may be read 16 bytes at a time
-    int tiles, rows;               // row tiles; dense: rows of x
+    int tiles, rows, per;          // row tiles; dense: rows of x; rows of a slot at most
     const int *order, *idx;        // experts: sorted picks, or (idx) the picks themselves, each a slot of its own
     int topk, E, n;
     W4Slots slots;
@@ -61,11 +62,11 @@ struct FewArgs {
 };
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
 template <int MODE>
-__device__ __forceinline__ int few_slots(const FewArgs &a) { return MODE == W4_DENSE ? 1 : a.idx ? a.n : __ldg(a.slots.n); }
+__device__ __forceinline__ int few_slots(const FewArgs &a) { return MODE == W4_DENSE ? (a.rows + a.per - 1) / a.per : a.idx ? a.n : __ldg(a.slots.n); }
 template <int MODE>
 __device__ __forceinline__ FewItem few_item(const FewArgs &a, int slot, int tile)
 {
-    if (MODE == W4_DENSE) return FewItem{0, 0, a.rows, tile};
+    if (MODE == W4_DENSE) return FewItem{0, slot * a.per, min(a.per, a.rows - slot * a.per), tile};
     if (a.idx) {
         const int e = __ldg(a.idx + slot);
         return FewItem{e, slot, e >= 0 && e < a.E ? 1 : 0, tile};
@@ -303,18 +304,29 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                                             *reinterpret_cast<const uint32_t *>(ph_ + off[2]), *reinterpret_cast<const uint32_t *>(ph_ + off[3]));
                         }
                         constexpr uint32_t LOW = 0x0f0f0f0fu, HIGH = 0xf0f0f0f0u;
-                        constexpr float UNIT = WHOLE ? 0.0625f : 1.0f;              // (WHOLE: the sums are 16 times theirs)
+                        // the block's scales (of four, two or one group) of rows g and g + 8
+                        float fg[4], fh[4];
+                        if (WHOLE) {
+                            fg[0] = bf16_to_f32(sg[8 * i]) * 0.0625f; fh[0] = bf16_to_f32(sh[8 * i]) * 0.0625f;      // (the sums are 16 times theirs)
+                        } else if (wlog) {
+                            const uint32_t g2 = *reinterpret_cast<const uint32_t *>(sg + 16 * i), h2 = *reinterpret_cast<const uint32_t *>(sh + 16 * i);
+                            bf16x2_to_f32(g2, fg[0], fg[1]); bf16x2_to_f32(h2, fh[0], fh[1]);
+                        } else {
+                            const uint2 g4 = *reinterpret_cast<const uint2 *>(sg + 32 * i), h4 = *reinterpret_cast<const uint2 *>(sh + 32 * i);
+                            bf16x2_to_f32(g4.x, fg[0], fg[1]); bf16x2_to_f32(g4.y, fg[2], fg[3]);
+                            bf16x2_to_f32(h4.x, fh[0], fh[1]); bf16x2_to_f32(h4.y, fh[2], fh[3]);
+                        }
+                        if (!WHOLE) {
+                            // a group behind the last (in a row's last block): zero, whatever lies there
+                            const int left = a.w.groups - first_group - ((32 * i) >> wlog);
+                            if (left < (4 >> wlog)) {
+#pragma unroll
+                                for (int k = 0; k < 4; k++) if (k >= left) { fg[k] = 0.f; fh[k] = 0.f; }
+                            }
+                        }
                         const uint4 x0 = x.digits[0][gx][t], x1 = x.digits[1][gx][t];
                         const float2 worth = *reinterpret_cast<const float2 *>(&x.worth[2 * t]);
-                        // one group's sums times its scales
-                        auto take = [&](const int (&c)[4], int k) {
-                            // (groups smaller than a block: one behind the last is zero, whatever lies there)
-                            const bool here = WHOLE || first_group + k < a.w.groups;
-                            const float fg = here ? bf16_to_f32(sg[k]) * UNIT : 0.f, fh = here ? bf16_to_f32(sh[k]) * UNIT : 0.f;
-                            // (in this order: a digit's worth alone times a scale may be too small for FP32)
-                            acc[0] = fmaf(few_float(c[0]) * fg, worth.x, acc[0]); acc[1] = fmaf(few_float(c[1]) * fg, worth.y, acc[1]);
-                            acc[2] = fmaf(few_float(c[2]) * fh, worth.x, acc[2]); acc[3] = fmaf(few_float(c[3]) * fh, worth.y, acc[3]);
-                        };
+                        float sum[4];
                         if (WHOLE) {
                             const int2 start = *reinterpret_cast<const int2 *>(&x.start[0][2 * t]);
                             int lo[4] = {start.x, start.y, start.x, start.y}, hi[4] = {FW_MAGIC, FW_MAGIC, FW_MAGIC, FW_MAGIC};
@@ -323,10 +335,11 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                             few_mma(lo, vg.z & LOW, vh.z & LOW, vg.w & LOW, vh.w & LOW, x0.z, x0.w);
                             few_mma(hi, vg.z & HIGH, vh.z & HIGH, vg.w & HIGH, vh.w & HIGH, x1.z, x1.w);
 #pragma unroll
-                            for (int q = 0; q < 4; q++) hi[q] += 16 * lo[q];
-                            take(hi, 8 * i);
+                            for (int q = 0; q < 4; q++) sum[q] = few_float(hi[q] + 16 * lo[q]) * (q < 2 ? fg[0] : fh[0]);
                         } else {
                             int c[4];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) sum[q] = 0.f;
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
                                 const uint32_t rg = word_of(vg, j), rh = word_of(vh, j);
@@ -336,9 +349,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                                 }
                                 const uint4 &d = j < 2 ? x0 : x1;
                                 few_mma(c, rg & LOW, rh & LOW, (rg >> 4) & LOW, (rh >> 4) & LOW, j & 1 ? d.z : d.x, j & 1 ? d.w : d.y);
-                                if (wlog == 0 || (j & 1)) take(c, (32 * i + j) >> wlog);
+                                if (wlog == 0 || (j & 1)) {
+                                    const float sg_ = wlog ? fg[j >> 1] : fg[j], sh_ = wlog ? fh[j >> 1] : fh[j];
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) sum[q] = fmaf(few_float(c[q]), q < 2 ? sg_ : sh_, sum[q]);
+                                }
                             }
                         }
+                        // (a digit's worth comes last: times a scale alone it may be too small for FP32)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) acc[q] = fmaf(sum[q], q & 1 ? worth.y : worth.x, acc[q]);
                     };
 #pragma unroll
                     for (int i = 0; i < FW_PIECE / 1024; i++) {
@@ -390,7 +410,7 @@ static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
     if (a.stages < 1) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
     // (what counts is this and the sums: more than 48 KB of them must be asked for)
     if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
-    const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
+    const long long items = (long long)a.tiles * (MODE == W4_DENSE ? (a.rows + a.per - 1) / a.per : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
     if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
     else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS>), grid, FW_THREADS, smem, st, m, a);
@@ -400,8 +420,7 @@ constexpr int few_one(int terms) { return terms == 3 ? 4 : 2; }          // colu
 template <int TERMS, int MODE, bool WHOLE>
 static int few_columns(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
-    const int rows = MODE == W4_DENSE ? a.rows : a.idx ? 1 : a.slots.rows;
-    return rows == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS)>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS>(st, m, a, early);
+    return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS)>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS>(st, m, a, early);
 }
 template <int TERMS, int MODE>
 static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
@@ -409,36 +428,40 @@ static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
     return a.w.group == 128 ? few_columns<TERMS, MODE, true>(st, m, a, early) : few_columns<TERMS, MODE, false>(st, m, a, early);
 }
 
-// Rows of a tile for a matrix of so many columns: what eight columns hold if there is room for it, else one row if there is for that.
+// What a block's digits take: of one row (with a column to spare), of what eight columns hold.
+static size_t few_block(int dt, int rows)
+{
+    return rows > 1 ? sizeof(FewBlock<FW_COLS, false>) : dt == DT_F32 ? sizeof(FewBlock<few_one(3), false>) : sizeof(FewBlock<few_one(2), false>);
+}
+// Rows of a tile for a matrix of so many columns: what eight columns hold if there is room for their digits, else one row or none.
 int w4_few_rows(int dt, int cols)
 {
-    const int blocks = w4_kp(cols) / 128, terms = dt == DT_F32 ? 3 : 2;
-    const size_t one = dt == DT_F32 ? sizeof(FewBlock<few_one(3), false>) : sizeof(FewBlock<few_one(2), false>);
-    return blocks * sizeof(FewBlock<FW_COLS, false>) <= (size_t)FW_DIGIT_BYTES ? FW_COLS / terms : blocks * one <= (size_t)FW_DIGIT_BYTES ? 1 : 0;
+    const size_t blocks = w4_kp(cols) / 128;
+    return blocks * few_block(dt, 2) <= (size_t)FW_DIGIT_BYTES ? (dt == DT_F32 ? 2 : 4) : blocks * few_block(dt, 1) <= (size_t)FW_DIGIT_BYTES ? 1 : 0;
 }
 
 int w4_few(cudaStream_t st, const W4Job &j)
 {
     FewArgs a{};
     const bool bf16 = j.x_dt == DT_BF16 || (j.mode == W4_DOWN && j.half);
-    const int rows = j.mode == W4_DENSE ? j.T : j.idx ? 1 : j.slots.rows;
     const int size = j.x_dt == DT_F32 ? 4 : 2;
     a.w = j.w; a.x = j.x; a.ldx = j.ldx; a.x_dt = j.x_dt; a.cols = j.w.cols; a.blocks = w4_kp(j.w.cols) / 128;
     a.wide = reinterpret_cast<uintptr_t>(j.x) % 16 == 0 && j.ldx * size % 16 == 0;
     a.tiles = (j.w.rows + (j.mode == W4_GATEUP ? 7 : 15)) / (j.mode == W4_GATEUP ? 8 : 16);
-    a.rows = j.T; a.order = j.order; a.idx = j.idx; a.topk = j.topk; a.E = j.count; a.n = j.T; a.slots = j.slots;
+    const int most = w4_few_rows(bf16 ? DT_BF16 : DT_F32, j.w.cols);
+    a.rows = j.T; a.per = j.mode == W4_DENSE ? std::min(j.T, most) : j.idx ? 1 : j.slots.rows; a.order = j.order; a.idx = j.idx; a.topk = j.topk; a.E = j.count; a.n = j.T; a.slots = j.slots;
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.limit = j.limit;
     const int half_rows = j.mode == W4_GATEUP ? 8 : 16;
     a.whole_rows = j.w.pitch % 128 == 0;
     // Two stages of each team at least: with many digits beside them in pieces of half the columns.
-    const size_t digits = (size_t)a.blocks * (rows == 1 ? sizeof(FewBlock<4, false>) : sizeof(FewBlock<FW_COLS, false>));
+    const size_t digits = (size_t)a.blocks * few_block(bf16 ? DT_BF16 : DT_F32, a.per);
     for (a.piece = FW_PIECE / 128;; a.piece /= 2) {
         a.chunks = std::min(a.piece / 2, (j.w.pitch + 127) / 128);
         a.scale_cols = std::min(a.piece * 128 / j.w.group, j.w.sp);
         a.scale_pitch = a.scale_cols + 8;
         a.stage_tx = a.chunks * 2048 + 32 * a.scale_pitch;
         a.stage_bytes = (a.stage_tx + 1023) / 1024 * 1024;
-        if (a.piece < FW_PIECE / 128 || 4 * (size_t)a.stage_bytes + digits <= FW_SMEM) break;
+        if (a.piece < FW_PIECE / 128 || 4 * (size_t)a.stage_bytes + digits <= (size_t)FW_SMEM) break;
     }
     FewMaps m;
     for (int h = 0; h < 2; h++) {

@@ -93,12 +93,11 @@ int check_ws(const char *op, const void *ws, size_t have, size_t need)
 enum { PICKS, FEW, MANY };
 struct ExpertsPlan { int how, rows; };           // rows of a slot at most
 constexpr int PICKS_MOST = 16;
-constexpr int FEW_MOST = 1;                      // rows of an expert, in tiles of w4_few
 ExpertsPlan experts_plan(int dt, int T, int topk, int E, int H, int I)
 {
     const int n = T * topk, h = w4_few_rows(dt, H), i = w4_few_rows(dt, I), rows = h < i ? h : i;
     if (rows && n <= PICKS_MOST) return {PICKS, 1};
-    if (rows > 1 && n <= rows * FEW_MOST * E) return {FEW, rows};
+    if (rows > 1 && n <= rows * E) return {FEW, rows};
     return {MANY, W4_MANY_ROWS};
 }
 struct ExpertsWs {
@@ -171,7 +170,7 @@ extern "C" size_t g5b_w4_matmul_workspace(const g5b_w4 *m, int dtype, int T)
     if (!m || m->cols < 1 || m->cols > W4_MAX_COLS || T < 0 || T > W4_MAX_TOKENS) return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2;
-    if (T <= w4_few_rows(dtype, m->cols)) return WS_ALIGN;
+    if (w4_few_takes(dtype, m->cols, T)) return WS_ALIGN;
     terms_of(ws, n_terms, m->cols, T);
     ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
     return ws.used;
@@ -192,7 +191,7 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     Pieces ws{static_cast<uint8_t *>(workspace)};
     j.mode = W4_DENSE; j.T = T; j.count = 1; j.n_terms = dtype == DT_BF16 ? 1 : 2;
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
-    if (T <= w4_few_rows(dtype, j.w.cols)) {
+    if (w4_few_takes(dtype, j.w.cols, T)) {
         j.x = x; j.x_dt = dtype; j.ldx = ldx;
         return w4_few(st, j) ? -1 : launched(op);
     }
