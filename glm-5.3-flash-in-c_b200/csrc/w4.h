@@ -55,14 +55,14 @@ struct W4Job {
     void *y; size_t ldy; int y_dt;
     float limit;
 };
-// Rows that w4_few takes at a time, of a matrix of so many columns (0: none). Dense products of up to twice as many are its: the weights
-// twice, 154880 x 4096 past four rows 108 us, where w4_many takes 146.
+// Rows that w4_few takes at a time, of a matrix of so many columns (0: none). Dense products of up to as many are its (past three
+// or four F32 rows the weights twice take 20.8 us for 12288 x 4096 in groups of 32, w4_many 17.6).
 int  w4_few_rows(int dt, int cols);
-inline bool w4_few_takes(int dt, int cols, int T) { return T <= 2 * w4_few_rows(dt, cols); }
+inline bool w4_few_takes(int dt, int cols, int T) { return T <= w4_few_rows(dt, cols); }
 int  w4_few(cudaStream_t st, const W4Job &job);
 int  w4_few_status(cudaStream_t st);
 constexpr int W4_MANY_ROWS = 64;
-size_t w4_many_part_floats(int rows, int cols, int T);      // room for the sums of a dense product's parts
+size_t w4_many_part_floats(int rows, int cols, int T);                           // room for the sums of a dense product's parts
 int  w4_many(cudaStream_t st, const W4Job &job, float *part);
 int  w4_many_status(cudaStream_t st);
 

@@ -62,11 +62,11 @@ struct FewArgs {
 };
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
 template <int MODE>
-__device__ __forceinline__ int few_slots(const FewArgs &a) { return MODE == W4_DENSE ? (a.rows + a.per - 1) / a.per : a.idx ? a.n : __ldg(a.slots.n); }
+__device__ __forceinline__ int few_slots(const FewArgs &a) { return MODE == W4_DENSE ? 1 : a.idx ? a.n : __ldg(a.slots.n); }
 template <int MODE>
 __device__ __forceinline__ FewItem few_item(const FewArgs &a, int slot, int tile)
 {
-    if (MODE == W4_DENSE) return FewItem{0, slot * a.per, min(a.per, a.rows - slot * a.per), tile};
+    if (MODE == W4_DENSE) return FewItem{0, 0, a.rows, tile};
     if (a.idx) {
         const int e = __ldg(a.idx + slot);
         return FewItem{e, slot, e >= 0 && e < a.E ? 1 : 0, tile};
@@ -410,7 +410,7 @@ static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
     if (a.stages < 1) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
     // (what counts is this and the sums: more than 48 KB of them must be asked for)
     if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
-    const long long items = (long long)a.tiles * (MODE == W4_DENSE ? (a.rows + a.per - 1) / a.per : a.idx ? a.n : a.slots.max);
+    const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
     if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
     else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS>), grid, FW_THREADS, smem, st, m, a);
@@ -448,8 +448,7 @@ int w4_few(cudaStream_t st, const W4Job &j)
     a.w = j.w; a.x = j.x; a.ldx = j.ldx; a.x_dt = j.x_dt; a.cols = j.w.cols; a.blocks = w4_kp(j.w.cols) / 128;
     a.wide = reinterpret_cast<uintptr_t>(j.x) % 16 == 0 && j.ldx * size % 16 == 0;
     a.tiles = (j.w.rows + (j.mode == W4_GATEUP ? 7 : 15)) / (j.mode == W4_GATEUP ? 8 : 16);
-    const int most = w4_few_rows(bf16 ? DT_BF16 : DT_F32, j.w.cols);
-    a.rows = j.T; a.per = j.mode == W4_DENSE ? std::min(j.T, most) : j.idx ? 1 : j.slots.rows; a.order = j.order; a.idx = j.idx; a.topk = j.topk; a.E = j.count; a.n = j.T; a.slots = j.slots;
+    a.rows = j.T; a.per = j.mode == W4_DENSE ? j.T : j.idx ? 1 : j.slots.rows; a.order = j.order; a.idx = j.idx; a.topk = j.topk; a.E = j.count; a.n = j.T; a.slots = j.slots;
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.limit = j.limit;
     const int half_rows = j.mode == W4_GATEUP ? 8 : 16;
     a.whole_rows = j.w.pitch % 128 == 0;

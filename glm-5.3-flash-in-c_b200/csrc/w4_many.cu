@@ -15,8 +15,12 @@
 // A converted block and its sums live in tensor memory (256 columns each); shared memory only holds what TMA brings, which it
 // must read for every product anyway: 64 rows of terms, 16 KB per step and term.
 //
-// Few tiles (a small batch, a narrow matrix) are cut along the columns too, into parts whose sums another kernel adds in order.
+// A dense product's tiles are dealt out in rounds, whole; those of a last round that would leave SMs idle are cut along the columns, into
+// parts whose sums a second kernel adds in order (605 tiles are 4 rounds of 148 and 13 tiles, which are cut into eleven). Equal shares of all
+// steps instead, whatever the tiles, gave every CTA two tiles' beginnings and ends: 64 rows past 12288 x 4096 30.4 us against 27.3.
 // Every wait is bounded: one that runs out sets a flag (g5b_w4_status), and every role drains what it has in flight and ends.
+#include <algorithm>
+
 #include "tc_ptx.cuh"
 #include "w4.cuh"
 
@@ -29,8 +33,8 @@ constexpr int WM_THREADS = 20 * 32;
 constexpr int WM_RING = 8;                          // tiles whose rows' powers of two are kept (two converted steps and two sums ahead of the stores)
 // Registers of a thread: 96 at the launch, of which the other warps give some to those that hold the sums (256 * 120 + 384 * 80 = 640 * 96).
 constexpr int WM_REGS_SUM = 120, WM_REGS_REST = 80;
-constexpr int WM_CTAS = 148;                        // SMs of a B200: what the parts along the columns are chosen for
-constexpr int WM_MAX_PARTS = 8;
+constexpr int WM_CTAS = 148;                        // SMs of a B200: what the cuts are chosen for
+constexpr int WM_PARTS = 16;
 
 static __device__ int g_many_err;                     // a wait that ran out: its code (0: none)
 
@@ -39,40 +43,52 @@ struct ManyArgs {
     W4Mat w, up;
     const float *inv;
     int mode, KB, n;               // steps of 128 columns; rows of a box of terms (a multiple of 16)
-    int RT, TT, parts;             // tiles of weight rows; dense: tiles of activation rows, parts along the columns
+    int RT, TT;                    // tiles of weight rows; dense: tiles of activation rows
+    int whole, parts;              // dense: tiles that are not cut, parts of the others
     int T;
     W4Slots slots;
     void *y;
     size_t ldy;
     int y_dt;
-    float *part;                   // [parts][T][rows], parts > 1
+    float *part;                   // dense: sums of the tiles that are cut, [tile][part][n][256]
     int wide;                      // four rows of an output may be stored at once
     float limit;
 };
 
 struct ManyTile {
-    int e, rt, first, np, n, k0, k1, part;
+    int e, rt, first, np, n, k0, k1;
+    int part;              // -1: the tile is not cut; else the place of its sums
 };
-__device__ __forceinline__ int many_tiles(const ManyArgs &a)
+// A CTA's work: items u, u + grid, ... (dense: whole tiles, then the others' parts; experts: tiles).
+struct ManyWalk { int u, end; };
+__device__ __forceinline__ ManyWalk many_walk(const ManyArgs &a)
 {
-    return a.mode == W4_DENSE ? a.RT * a.TT * a.parts : a.RT * __ldg(a.slots.n);
+    return ManyWalk{(int)blockIdx.x, a.mode == W4_DENSE ? a.whole + (a.RT * a.TT - a.whole) * a.parts : a.RT * __ldg(a.slots.n)};
 }
-__device__ __forceinline__ ManyTile many_tile(const ManyArgs &a, int i)
+__device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTile &t)
 {
-    ManyTile t;
+    if (w.u >= w.end) return false;
+    t.part = -1; t.k0 = 0; t.k1 = a.KB;
     if (a.mode == W4_DENSE) {
-        const int tt = i % a.TT, rest = i / a.TT;
-        t.e = 0; t.rt = rest % a.RT; t.part = rest / a.RT;
+        int tile = w.u;
+        if (tile >= a.whole) {
+            // the same part of all tiles, then the next
+            const int cut = a.RT * a.TT - a.whole, i = w.u - a.whole, q = i / cut, c = i - q * cut;
+            tile = a.whole + c;
+            t.k0 = a.KB * q / a.parts; t.k1 = a.KB * (q + 1) / a.parts;
+            if (a.parts > 1) t.part = c * a.parts + q;
+        }
+        const int tt = tile % a.TT;
+        t.e = 0; t.rt = tile / a.TT;
         t.first = tt * a.n; t.np = min(a.n, a.T - t.first);
-        t.k0 = (int)((long long)a.KB * t.part / a.parts); t.k1 = (int)((long long)a.KB * (t.part + 1) / a.parts);
     } else {
-        const int slot = i / a.RT;
-        t.rt = i - slot * a.RT; t.part = 0;
+        const int slot = w.u / a.RT;
+        t.rt = w.u - slot * a.RT;
         t.e = __ldg(a.slots.expert + slot); t.first = __ldg(a.slots.first + slot); t.np = __ldg(a.slots.count + slot);
-        t.k0 = 0; t.k1 = a.KB;
     }
     t.n = (t.np + 15) & ~15;
-    return t;
+    w.u += gridDim.x;
+    return true;
 }
 
 // The power of two that brings the largest of a row's scales to [2^11, 2^12).
@@ -167,7 +183,8 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     const uint32_t tmem = s_tmem;
     // sums of block b, accumulator i: columns 128 b + 64 i; converted block b of stage s: columns 256 + 128 s + 64 b
     if (a.mode != W4_DENSE) pdl_wait();                     // (the slots are another kernel's)
-    const int tiles = many_tiles(a);
+    ManyWalk walk = many_walk(a);
+    ManyTile t;
     bool ok = true;
 
     // (the four warps of a group change their registers in one place)
@@ -178,8 +195,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             if (elect_one()) {
                 int s = 0, ph = 1, issued = 0;
 #pragma unroll 1
-                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                    const ManyTile t = many_tile(a, i);
+                while (ok && many_next(a, walk, t)) {
 #pragma unroll 1
                     for (int kb = t.k0; kb < t.k1; kb++) {
                         if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
@@ -206,8 +222,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             if (elect_one()) {
                 int s = 0, ph = 1, issued = 0;
 #pragma unroll 1
-                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                    const ManyTile t = many_tile(a, i);
+                while (ok && many_next(a, walk, t)) {
 #pragma unroll 1
                     for (int kb = t.k0; kb < t.k1; kb++) {
                         if (issued >= WM_XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
@@ -227,8 +242,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 const int b = warp - 18;
                 int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
 #pragma unroll 1
-                for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-                    const ManyTile t = many_tile(a, i);
+                while (ok && many_next(a, walk, t)) {
                     const uint32_t idesc = tc_idesc(0, t.n);
                     int c = 0;                                   // steps in the current accumulator
 #pragma unroll 1
@@ -267,8 +281,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         const int per = a.w.group == 128 ? 2 : a.w.group == 64 ? 1 : 0;        // a 32-column piece's group: piece >> per
         int ws = 0, wp = 0, as = 0, ap = 1, steps = 0, n_tile = 0;
 #pragma unroll 1
-        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
-            const ManyTile t = many_tile(a, i);
+        while (ok && many_next(a, walk, t)) {
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
@@ -334,8 +347,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         int n_tile = 0;
         pdl_wait();
 #pragma unroll 1
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x, n_tile++) {
-            const ManyTile t = many_tile(a, i);
+        for (; many_next(a, walk, t); n_tile++) {
             const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
             F2 acc[WM_ROWS / 2];
 #pragma unroll
@@ -396,9 +408,11 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll
                     for (int q = 0; q < 4; q++) v[q] = swiglu_value(v[q], u[q], a.limit);
                 }
-                const size_t at = a.parts > 1 ? ((size_t)t.part * a.T + t.first + k) * a.w.rows + row0 : (size_t)(t.first + k) * a.ldy + row0;
-                if (a.parts > 1 || a.y_dt == DT_F32) {
-                    float *y = (a.parts > 1 ? a.part : static_cast<float *>(a.y)) + at;
+                const size_t at = (size_t)(t.first + k) * a.ldy + row0;
+                if (!GATEUP && t.part >= 0)
+                    *reinterpret_cast<float4 *>(a.part + ((size_t)t.part * a.n + k) * 256 + b * 128 + lane * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                else if (a.y_dt == DT_F32) {
+                    float *y = static_cast<float *>(a.y) + at;
                     if (a.wide && row0 + 3 < a.w.rows) *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
                     else
 #pragma unroll
@@ -421,38 +435,53 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     if (warp == 18) { __syncwarp(); tmem_dealloc(tmem, 512); }
 }
 
-// y = the parts' sums in order
-__global__ void __launch_bounds__(256) w4_parts_kernel(const float *part, int parts, int T, int rows, void *y, size_t ldy, int y_dt)
+// The tiles that were cut: their parts' sums in order. A CTA takes four rows of x of one tile.
+__global__ void __launch_bounds__(256) w4_parts_kernel(const float *part, int parts, int whole, int TT, int n, int T, int rows, void *y, size_t ldy, int y_dt, int wide)
 {
     pdl_wait();
-    const int t = blockIdx.y, r = blockIdx.x * 256 + threadIdx.x;
-    if (r >= rows) return;
-    float v = 0.f;
-    const float *p = part + (size_t)t * rows + r;
+    const int tile = whole + blockIdx.x, tt = tile % TT, k = blockIdx.y * 4 + (threadIdx.x >> 6), r = (threadIdx.x & 63) * 4, row = tile / TT * 256 + r;
+    if (k >= n || tt * n + k >= T || row >= rows) return;
+    const float *p = part + ((size_t)blockIdx.x * parts * n + k) * 256 + r;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = 0; i < parts; i++) v += __ldcs(p + (size_t)i * T * rows);
-    if (y_dt == DT_F32) static_cast<float *>(y)[(size_t)t * ldy + r] = v;
-    else static_cast<__nv_bfloat16 *>(y)[(size_t)t * ldy + r] = __float2bfloat16_rn(v);
+    for (int q = 0; q < parts; q++) {
+        const float4 in = __ldcs(reinterpret_cast<const float4 *>(p + (size_t)q * n * 256));
+        v.x += in.x; v.y += in.y; v.z += in.z; v.w += in.w;
+    }
+    const size_t at = (size_t)(tt * n + k) * ldy + row;
+    const float o[4] = {v.x, v.y, v.z, v.w};
+    if (wide && row + 3 < rows && y_dt == DT_F32) *reinterpret_cast<float4 *>(static_cast<float *>(y) + at) = v;
+    else
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (row + q < rows) {
+                if (y_dt == DT_F32) static_cast<float *>(y)[at + q] = o[q];
+                else static_cast<__nv_bfloat16 *>(y)[at + q] = __float2bfloat16_rn(o[q]);
+            }
 }
 
-// Parts along the columns of a dense product: what takes the fewest steps with one tile at a time on every SM, where a tile's
-// beginning and end count as three steps.
-int w4_many_parts(int rows, int cols, int T)
+static int many_box(int T) { return T < WM_ROWS ? (T + 15) / 16 * 16 : WM_ROWS; }
+// Which tiles of a dense product are cut, and into how many parts: what takes the fewest steps of 128 columns, where the beginning and end of
+// an item count as three and the second kernel as two.
+struct ManyCut { int whole, parts; };
+static ManyCut many_cut(int rows, int cols, int T)
 {
-    const int KB = w4_kp(cols) / 128, n = T < WM_ROWS ? (T + 15) / 16 * 16 : WM_ROWS;
-    const long long tiles = (long long)((rows + 255) / 256) * ((T + n - 1) / n);
-    int best = 1;
+    const int KB = w4_kp(cols) / 128, tiles = (rows + 255) / 256 * ((T + many_box(T) - 1) / many_box(T)), rounds = tiles / WM_CTAS;
+    ManyCut best{tiles, 1};
     long long least = 0;
-    for (int p = 1; p <= WM_MAX_PARTS && (p == 1 || (KB / p >= 2 && tiles * p <= 2 * WM_CTAS)); p++) {
-        const long long cost = (tiles * p + WM_CTAS - 1) / WM_CTAS * ((KB + p - 1) / p + 3) + (p > 1 ? 2 : 0);
-        if (p == 1 || cost < least) { least = cost; best = p; }
-    }
+    for (int r = rounds; r >= 0 && r >= rounds - 1; r--)
+        for (int p = 1; p <= WM_PARTS && (p == 1 || KB / p >= 2); p++) {
+            const long long left = tiles - (long long)r * WM_CTAS;
+            const long long cost = r * (KB + 3ll) + (left * p + WM_CTAS - 1) / WM_CTAS * ((KB + p - 1) / p + 3) + (p > 1 ? 2 : 0);
+            if ((r == rounds && p == 1) || cost < least) { least = cost; best = p > 1 ? ManyCut{r * WM_CTAS, p} : ManyCut{tiles, 1}; }
+        }
     return best;
 }
 size_t w4_many_part_floats(int rows, int cols, int T)
 {
-    const int p = w4_many_parts(rows, cols, T);
-    return p > 1 ? (size_t)p * T * rows : 0;
+    const ManyCut c = many_cut(rows, cols, T);
+    const size_t tiles = (size_t)((rows + 255) / 256) * ((T + many_box(T) - 1) / many_box(T));
+    return (tiles - c.whole) * c.parts * many_box(T) * 256;
 }
 
 template <int TERMS, bool GATEUP, bool WHOLE>
@@ -471,12 +500,11 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     ManyArgs a{};
     const int rows_most = j.mode == W4_DENSE ? j.T : j.slots.rows;
     a.w = j.w; a.up = j.up; a.inv = j.terms.inv; a.mode = j.mode; a.KB = j.terms.kp / 128; a.T = j.T; a.slots = j.slots;
-    a.n = rows_most < WM_ROWS ? (rows_most + 15) / 16 * 16 : WM_ROWS;
+    a.n = many_box(rows_most);
     a.RT = (j.w.rows + (j.mode == W4_GATEUP ? 127 : 255)) / (j.mode == W4_GATEUP ? 128 : 256);
     a.TT = (j.T + a.n - 1) / a.n;
-    a.parts = j.mode == W4_DENSE ? w4_many_parts(j.w.rows, j.w.cols, j.T) : 1;
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.part = part; a.limit = j.limit;
-    a.wide = a.parts > 1 ? j.w.rows % 4 == 0 : j.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(j.y) % (j.y_dt == DT_F32 ? 16 : 8) == 0;
+    a.wide = j.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(j.y) % (j.y_dt == DT_F32 ? 16 : 8) == 0;
     const cuuint64_t wsize[3] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.rows, (cuuint64_t)j.count};
     const cuuint64_t wstride[2] = {(cuuint64_t)j.w.pitch, (cuuint64_t)j.w.codes_stride};
     const cuuint32_t wbox[3] = {64, 128, 1};
@@ -489,15 +517,21 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
         set_last_error("a tensor map of a 4-bit product was refused");
         return -1;
     }
-    const long long tiles = j.mode == W4_DENSE ? (long long)a.RT * a.TT * a.parts : (long long)a.RT * j.slots.max;
-    const int grid = (int)(tiles < dev_sms() ? tiles : dev_sms());
+    const int tiles = a.RT * a.TT;
+    long long items = (long long)a.RT * j.slots.max;
+    if (j.mode == W4_DENSE) {
+        const ManyCut cut = many_cut(j.w.rows, j.w.cols, j.T);
+        a.whole = cut.whole; a.parts = cut.parts;
+        items = a.whole + (long long)(tiles - a.whole) * a.parts;
+    }
+    const int grid = (int)std::min<long long>(items, dev_sms());
     const bool pair = j.mode == W4_GATEUP, whole = j.w.group == 128;
     const int rc = j.terms.n_terms == 1 ? (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
                    : whole ? (pair ? many_launch<2, true, true>(st, m, a, grid) : many_launch<2, false, true>(st, m, a, grid))
                            : (pair ? many_launch<2, true, false>(st, m, a, grid) : many_launch<2, false, false>(st, m, a, grid));
     if (rc) return -1;
-    if (a.parts > 1)
-        G5B_LAUNCH_PDL(w4_parts_kernel, dim3((j.w.rows + 255) / 256, j.T), dim3(256), 0, st, part, a.parts, j.T, j.w.rows, j.y, j.ldy, j.y_dt);
+    if (j.mode == W4_DENSE && a.parts > 1)
+        G5B_LAUNCH_PDL(w4_parts_kernel, dim3(tiles - a.whole, (a.n + 3) / 4), dim3(256), 0, st, part, a.parts, a.whole, a.TT, a.n, j.T, j.w.rows, j.y, j.ldy, j.y_dt, a.wide);
     return 0;
 }
 

@@ -157,7 +157,7 @@ def test_a_checkpoint_expert_layer_in_four_bits(gpu_lib):
         for e in range(E):
             part = rows[at[e]:at[e + 1]]
             h = [torch.empty((len(part), I), device="cuda") for _ in range(2)]
-            ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+            ws = torch.empty(max(pkg.w4_matmul_workspace(src["gate"][1][e], part), pkg.w4_matmul_workspace(src["down"][1][e], h[0])), dtype=torch.uint8, device="cuda")
             for i, n in enumerate(("gate", "up")):
                 pkg.w4_matmul(src[n][1][e], part, h[i], ws)
             act = ref.swiglu(h[0].double(), h[1].double(), 10.0).float()
