@@ -91,17 +91,17 @@ __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTi
     return true;
 }
 
-// The power of two that brings the largest of a row's scales to [2^11, 2^12).
-__device__ __forceinline__ int many_row_up(const uint16_t *srow, int groups)
+// The power of two that brings the largest of a row's scales from group `first` to `end` to [2^11, 2^12).
+__device__ __forceinline__ int many_row_up(const uint16_t *srow, int first, int end)
 {
     uint32_t m = 0;
-    int i = 0;
-#pragma unroll 4
-    for (; i + 8 <= groups; i += 8) {
+    int i = first & ~7;                                      // (16-byte loads; a few groups before the first do no harm)
+#pragma unroll 8
+    for (; i + 8 <= end; i += 8) {
         const uint4 v = __ldg(reinterpret_cast<const uint4 *>(srow + i));
         m = __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
     }
-    for (; i < groups; i++) m = __vmaxu2(m, (uint32_t)__ldg(srow + i) & 0x7fffu);
+    for (; i < end; i++) m = __vmaxu2(m, (uint32_t)__ldg(srow + i) & 0x7fffu);
     m = max(m & 0xffffu, m >> 16);
     return min(11 + 127 - max((int)(m >> 7), 1), 126);
 }
@@ -287,27 +287,29 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
             float up = 0.f;
             if (!WHOLE) {
-                const int e = many_row_up(srow, a.w.groups);
+                const int e = many_row_up(srow, (4 * t.k0) >> per, min((4 * t.k1) >> per, a.w.groups));
                 up = pow2(e);
                 s_up[n_tile & (WM_RING - 1)][b][r] = pow2(-e);
                 n_tile++;
             }
-            // raw scales of a step's four pieces, one step ahead
+            // Raw scales of a step's four pieces (the four that they are among), two steps ahead: one load whatever the group's size, because
+            // what comes out of branches is put together behind them, and two sets of registers that are not moved, because a move waits.
             auto fetch = [&](int kb) {
-                uint2 v = make_uint2(0u, 0u);
-                if (!WHOLE && kb < t.k1) {
-                    if (per == 2) v.x = __ldg(srow + kb);
-                    else if (per == 1) v.x = __ldg(reinterpret_cast<const uint32_t *>(srow) + kb);
-                    else v = __ldg(reinterpret_cast<const uint2 *>(srow) + kb);
-                }
-                return v;
+                return WHOLE ? make_uint2(0u, 0u) : __ldg(reinterpret_cast<const uint2 *>(srow + ((4 * min(kb, t.k1 - 1) >> per) & ~3)));
             };
-            uint2 next = fetch(t.k0);
-#pragma unroll 1
-            for (int kb = t.k0; kb < t.k1; kb++, steps++) {
-                const uint2 sc = next;
-                next = fetch(kb + 1);
-                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) break;
+            uint2 even = fetch(t.k0), odd = fetch(t.k0 + 1);
+            auto step = [&](int kb, uint2 &sc) {
+                __half2 s2[4];
+#pragma unroll
+                for (int piece = 0; piece < 4; piece++) {
+                    const int g = (4 * kb + piece) >> per;
+                    const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
+                    // (a group behind the last: zero, whatever lies there)
+                    s2[piece] = __float2half2_rn(!WHOLE && g < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f);
+                }
+                sc = fetch(kb + 2);
+                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) return;
+                steps++;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
 #pragma unroll
@@ -315,14 +317,10 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                     uint32_t f[32];
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const int piece = h * 2 + c, g = piece >> per;
-                        const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
-                        // (a group behind the last: zero, whatever lies there)
-                        const float v = !WHOLE && ((4 * kb + piece) >> per) < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f;
-                        const __half2 s2 = __float2half2_rn(v);
+                        const int piece = h * 2 + c;
                         const uint4 q = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
-                        many_convert<WHOLE>(q.x, s2, f + c * 16); many_convert<WHOLE>(q.y, s2, f + c * 16 + 4);
-                        many_convert<WHOLE>(q.z, s2, f + c * 16 + 8); many_convert<WHOLE>(q.w, s2, f + c * 16 + 12);
+                        many_convert<WHOLE>(q.x, s2[piece], f + c * 16); many_convert<WHOLE>(q.y, s2[piece], f + c * 16 + 4);
+                        many_convert<WHOLE>(q.z, s2[piece], f + c * 16 + 8); many_convert<WHOLE>(q.w, s2[piece], f + c * 16 + 12);
                     }
                     tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
                 }
@@ -335,6 +333,11 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&a_full[b][as]);
                 if (++ws == WM_WS) { ws = 0; wp ^= 1; }
                 if (++as == 2) { as = 0; ap ^= 1; }
+            };
+#pragma unroll 1
+            for (int kb = t.k0; kb < t.k1 && ok; kb += 2) {
+                step(kb, even);
+                if (ok && kb + 1 < t.k1) step(kb + 1, odd);
             }
         }
     } else {
