@@ -7,7 +7,9 @@
 //   17     activation terms by TMA: 64 rows x 128 columns x terms a step
 //   8-15   conversion, four warps to a block, a thread to a row: nibbles become F16 values of (code - 8) * scale in tensor
 //          memory. They are exact: 3 significant bits of the code times 8 of a BF16 scale fit F16's 11, and a power of two
-//          per row of W brings its largest scale to [2^11, 2^12), so that only those of groups 2^28 below it lose bits.
+//          per row of W and four steps brings the largest of their scales to [2^11, 2^12), so that only those of groups 2^28 below
+//          it lose bits. (One for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
+//          F32 rows past groups of 128: the codes alone, and the scale on a step's sums.
 //   18, 19 products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
 //          same sums one after the other, so that a converted block is used twice.
 //   0-7    four warps to a block: take the sums over 256 columns (F32 rows; 512 of BF16) out of tensor memory and add them
@@ -30,7 +32,8 @@ constexpr int WM_ROWS = 64;                         // activation rows of a tile
 constexpr int WM_WS = 3, WM_XS = 3;                 // stages of codes, of terms
 constexpr int WM_W_STAGE = 2 * 128 * 64;
 constexpr int WM_THREADS = 20 * 32;
-constexpr int WM_RING = 8;                          // tiles whose rows' powers of two are kept (two converted steps and two sums ahead of the stores)
+constexpr int WM_SPAN = 4;                          // steps with one power of two
+constexpr int WM_RING = 8;                          // spans whose powers of two are kept (the conversion is two steps and two accumulators ahead of the sums)
 // Registers of a thread: 96 at the launch, of which the other warps give some to those that hold the sums (256 * 120 + 384 * 80 = 640 * 96).
 constexpr int WM_REGS_SUM = 120, WM_REGS_REST = 80;
 constexpr int WM_CTAS = 148;                        // SMs of a B200: what the cuts are chosen for
@@ -91,20 +94,6 @@ __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTi
     return true;
 }
 
-// The power of two that brings the largest of a row's scales from group `first` to `end` to [2^11, 2^12).
-__device__ __forceinline__ int many_row_up(const uint16_t *srow, int first, int end)
-{
-    uint32_t m = 0;
-    int i = first & ~7;                                      // (16-byte loads; a few groups before the first do no harm)
-#pragma unroll 8
-    for (; i + 8 <= end; i += 8) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(srow + i));
-        m = __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-    }
-    for (; i < end; i++) m = __vmaxu2(m, (uint32_t)__ldg(srow + i) & 0x7fffu);
-    m = max(m & 0xffffu, m >> 16);
-    return min(11 + 127 - max((int)(m >> 7), 1), 126);
-}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
@@ -152,7 +141,7 @@ __device__ __forceinline__ bool many_all(bool ok, int barrier, int threads)
 template <int TERMS, bool GATEUP, bool WHOLE>
 __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
 {
-    constexpr int CHUNK = TERMS == 2 ? 1 : 4;               // steps summed inside the tensor cores (WHOLE: one)
+    constexpr int CHUNK = TERMS == 2 ? 1 : WM_SPAN;         // steps summed inside the tensor cores
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -163,7 +152,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     __shared__ uint64_t w_full[WM_WS], w_empty[WM_WS], x_full[WM_XS], x_empty[WM_XS];
     __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
     __shared__ uint32_t s_tmem;
-    __shared__ float s_up[WM_RING][2][128];                 // what takes a row's power of two off again
+    __shared__ float s_down[WM_RING][2][128];               // what takes a row's power of two off again
     int *err = &g_many_err;
 
     pdl_trigger();
@@ -279,37 +268,56 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         const int b = (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane, x = (r >> 1) & 3;
         const uint32_t dst = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (uint32_t)(b * 64);
         const int per = a.w.group == 128 ? 2 : a.w.group == 64 ? 1 : 0;        // a 32-column piece's group: piece >> per
-        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0, n_tile = 0;
+        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0, spans = 0;
 #pragma unroll 1
         while (ok && many_next(a, walk, t)) {
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            float up = 0.f;
-            if (!WHOLE) {
-                const int e = many_row_up(srow, (4 * t.k0) >> per, min((4 * t.k1) >> per, a.w.groups));
-                up = pow2(e);
-                s_up[n_tile & (WM_RING - 1)][b][r] = pow2(-e);
-                n_tile++;
-            }
-            // Raw scales of a step's four pieces (the four that they are among), two steps ahead: one load whatever the group's size, because
-            // what comes out of branches is put together behind them, and two sets of registers that are not moved, because a move waits.
-            auto fetch = [&](int kb) {
-                return WHOLE ? make_uint2(0u, 0u) : __ldg(reinterpret_cast<const uint2 *>(srow + ((4 * min(kb, t.k1 - 1) >> per) & ~3)));
-            };
-            uint2 even = fetch(t.k0), odd = fetch(t.k0 + 1);
-            auto step = [&](int kb, uint2 &sc) {
-                __half2 s2[4];
+            // Raw scales of a step's four pieces (the four that they are among), a span ahead: one load whatever the group's size, because
+            // what comes out of branches is put together behind them, and waits there.
+            uint2 next[WM_SPAN];
+            auto fetch = [&](int kb0) {
 #pragma unroll
-                for (int piece = 0; piece < 4; piece++) {
-                    const int g = (4 * kb + piece) >> per;
-                    const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
-                    // (a group behind the last: zero, whatever lies there)
-                    s2[piece] = __float2half2_rn(!WHOLE && g < a.w.groups ? bf16_to_f32((uint16_t)raw) * up : 0.f);
+                for (int i = 0; i < WM_SPAN; i++) next[i] = __ldg(reinterpret_cast<const uint2 *>(srow + ((4 * min(kb0 + i, t.k1 - 1) >> per) & ~3)));
+            };
+            if (!WHOLE) fetch(t.k0);
+            uint2 now[WM_SPAN];
+            float up = 0.f;
+#pragma unroll 1
+            for (int kb = t.k0; kb < t.k1; kb++, steps++) {
+                const int i = (kb - t.k0) & (WM_SPAN - 1);
+                __half2 s2[4];
+                if (!WHOLE) {
+                    if (i == 0) {
+                        // (a group behind the last: zero, whatever lies there)
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int k = 0; k < WM_SPAN; k++) {
+                            now[k] = next[k];
+                            const int last = a.w.groups - ((4 * min(kb + k, t.k1 - 1) >> per) & ~3);       // of the four, how many are groups
+                            if (last < 4) {
+                                now[k].x &= last > 1 ? 0xffffffffu : 0xffffu;
+                                now[k].y &= last > 3 ? 0xffffffffu : last > 2 ? 0xffffu : 0u;
+                            }
+                            m = __vmaxu2(m, __vmaxu2(now[k].x & 0x7fff7fffu, now[k].y & 0x7fff7fffu));
+                        }
+                        fetch(kb + WM_SPAN);
+                        m = max(m & 0xffffu, m >> 16);
+                        const int e = min(11 + 127 - max((int)(m >> 7), 1), 126);
+                        up = pow2(e);
+                        s_down[spans & (WM_RING - 1)][b][r] = pow2(-e);
+                        spans++;
+                    }
+                    const uint2 sc = i == 0 ? now[0] : i == 1 ? now[1] : i == 2 ? now[2] : now[3];
+#pragma unroll
+                    for (int piece = 0; piece < 4; piece++) {
+                        const int g = (4 * kb + piece) >> per;
+                        const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
+                        s2[piece] = __float2half2_rn(bf16_to_f32((uint16_t)raw) * up);
+                    }
                 }
-                sc = fetch(kb + 2);
-                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) return;
-                steps++;
+                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) break;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
 #pragma unroll
@@ -333,11 +341,6 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&a_full[b][as]);
                 if (++ws == WM_WS) { ws = 0; wp ^= 1; }
                 if (++as == 2) { as = 0; ap ^= 1; }
-            };
-#pragma unroll 1
-            for (int kb = t.k0; kb < t.k1 && ok; kb += 2) {
-                step(kb, even);
-                if (ok && kb + 1 < t.k1) step(kb + 1, odd);
             }
         }
     } else {
@@ -347,15 +350,15 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 128);
         const int bar = GATEUP ? 1 : 1 + b, bar_threads = GATEUP ? 256 : 128;       // (gate/up: both blocks together)
         int chunks = 0;
-        int n_tile = 0;
+        int spans = 0;
         pdl_wait();
 #pragma unroll 1
-        for (; many_next(a, walk, t); n_tile++) {
+        while (many_next(a, walk, t)) {
             const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
             F2 acc[WM_ROWS / 2];
 #pragma unroll
             for (int k = 0; k < WM_ROWS / 2; k++) acc[k] = f2(0.f, 0.f);
-            // WHOLE: a step's scale, one step ahead
+            // what a chunk's sums are multiplied by: a step's scale, one step ahead (WHOLE), or what takes the power of two off
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
@@ -365,9 +368,13 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll 1
             for (int c = 0; c < uses; c++, chunks++) {
                 const int buf = chunks & 1;
-                const float sc = bf16_to_f32(next);
+                float sc = bf16_to_f32(next);
                 if (WHOLE && c + 1 < uses) next = __ldg(srow + t.k0 + c + 1);
                 if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(chunks >> 1) & 1, err, 11))) break;
+                if (!WHOLE) {
+                    sc = s_down[spans & (WM_RING - 1)][b][r];
+                    spans += CHUNK == WM_SPAN || (c & (WM_SPAN - 1)) == WM_SPAN - 1 || c + 1 == uses;
+                }
                 tc_fence_after();
 #pragma unroll
                 for (int g = 0; g < WM_ROWS; g += 32)
@@ -379,7 +386,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll
                         for (int k = 0; k < 16; k++) {
                             const F2 in = f2(__uint_as_float(v[k >> 3][2 * (k & 7)]), __uint_as_float(v[k >> 3][2 * (k & 7) + 1]));
-                            acc[g / 2 + k] = WHOLE ? f2_fma(in, f2(sc, sc), acc[g / 2 + k]) : f2_add(acc[g / 2 + k], in);
+                            acc[g / 2 + k] = f2_fma(in, f2(sc, sc), acc[g / 2 + k]);
                         }
                     }
                 tc_fence_before();
@@ -390,13 +397,12 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             // Through shared memory, so that what comes now is a loop (unrolled over the registers it was 38000 cycles of a cold
             // instruction cache per tile) in which a warp stores 128 weight rows of one activation row, four to a lane.
             float *sums = exch + b * (WM_ROWS * 128);
-            const float down = WHOLE ? 1.0f : s_up[n_tile & (WM_RING - 1)][b][r];
 #pragma unroll
             for (int k = 0; k < WM_ROWS; k += 2) {
                 float x, y;
                 f2_get(acc[k / 2], x, y);
-                sums[k * 128 + r] = x * down;
-                sums[k * 128 + 128 + r] = y * down;
+                sums[k * 128 + r] = x;
+                sums[k * 128 + 128 + r] = y;
             }
             many_all(true, bar, bar_threads);
             const int row0 = (GATEUP ? t.rt * 128 : t.rt * 256 + b * 128) + lane * 4;
