@@ -6,9 +6,12 @@
 //   16     codes by TMA: 2 x 128 rows x 64 bytes (128 columns) a step
 //   17     activation terms by TMA: 64 rows x 128 columns x terms a step
 //   8-15   conversion, four warps to a block, a thread to a row: nibbles become F16 values of (code - 8) * scale in tensor
-//          memory. They are exact: 3 significant bits of the code times 8 of a BF16 scale fit F16's 11, and a power of two
-//          per row of W and four steps brings the largest of their scales to [2^11, 2^12), so that only those of groups 2^28 below
-//          it lose bits. (One for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
+//          memory. They are exact: 3 significant bits of the code times 8 of a BF16 scale fit F16's 11, with a power of two per row
+//          of W and four steps. A masked nibble is the subnormal number code * 2^-24 (or 2^-20), and one fused operation makes it
+//          (code - 8) * scale while the four steps' scales are within 2^8 of each other: the largest times 2^24 lies below 2^16, the
+//          smallest's products above F16's last bit. Otherwise 1024 + code, minus 1032, times the scale, whose largest is brought below
+//          2^12: two operations, exact over 2^28 (groups of 32, eight rows past 154880 x 4096: 132 us).
+//          (A power of two for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
 //          F32 rows past groups of 128: the codes alone, and the scale on a step's sums.
 //   18, 19 products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
 //          same sums one after the other, so that a converted block is used twice.
@@ -97,7 +100,7 @@ __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTi
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-// Eight codes of a word (WHOLE), or those times the scale (twice in s), as four pairs in the terms' order.
+// Eight codes of a word as four pairs in the terms' order: (code - 8) (WHOLE), or times the scale (twice in s).
 template <bool WHOLE>
 __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
 {
@@ -110,6 +113,17 @@ __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
         const __half2 hi = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
         f[2 * i] = h2_bits(WHOLE ? lo : __hmul2(lo, s));
         f[2 * i + 1] = h2_bits(WHOLE ? hi : __hmul2(hi, s));
+        v >>= 8;
+    }
+}
+// The same from subnormal numbers. lo: the scale times 2^24; hi: times 2^20; off: times -8.
+__device__ __forceinline__ void many_convert_fused(uint32_t v, __half2 lo, __half2 hi, __half2 off, uint32_t *f)
+{
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        uint32_t a = v & 0x000f000fu, b = v & 0x00f000f0u;
+        f[2 * i] = h2_bits(__hfma2(*reinterpret_cast<__half2 *>(&a), lo, off));
+        f[2 * i + 1] = h2_bits(__hfma2(*reinterpret_cast<__half2 *>(&b), hi, off));
         v >>= 8;
     }
 }
@@ -284,6 +298,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             if (!WHOLE) fetch(t.k0);
             uint2 now[WM_SPAN];
             float up = 0.f;
+            bool fused = false;
 #pragma unroll 1
             for (int kb = t.k0; kb < t.k1; kb++, steps++) {
                 const int i = (kb - t.k0) & (WM_SPAN - 1);
@@ -291,7 +306,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (!WHOLE) {
                     if (i == 0) {
                         // (a group behind the last: zero, whatever lies there)
-                        uint32_t m = 0;
+                        uint32_t m = 0, least = 0xffffffffu;                 // (least: of those that are not zero, less one)
 #pragma unroll
                         for (int k = 0; k < WM_SPAN; k++) {
                             now[k] = next[k];
@@ -300,13 +315,19 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                                 now[k].x &= last > 1 ? 0xffffffffu : 0xffffu;
                                 now[k].y &= last > 3 ? 0xffffffffu : last > 2 ? 0xffffu : 0u;
                             }
-                            m = __vmaxu2(m, __vmaxu2(now[k].x & 0x7fff7fffu, now[k].y & 0x7fff7fffu));
+                            const uint32_t x0 = now[k].x & 0x7fff7fffu, y0 = now[k].y & 0x7fff7fffu;
+                            m = __vmaxu2(m, __vmaxu2(x0, y0));
+                            least = __vminu2(least, __vminu2(__vsub2(x0, 0x00010001u), __vsub2(y0, 0x00010001u)));
                         }
                         fetch(kb + WM_SPAN);
                         m = max(m & 0xffffu, m >> 16);
-                        const int e = min(11 + 127 - max((int)(m >> 7), 1), 126);
+                        least = min(least & 0xffffu, least >> 16);
+                        // exponents of the largest scale and the smallest that is not zero; far from FP32's ends, so that no power of two leaves it
+                        const int top = max((int)(m >> 7), 1), low = (int)((least + 1) >> 7);
+                        fused = __all_sync(0xffffffffu, top - low <= 8 && top >= 40 && top <= 220);
+                        const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 126);
                         up = pow2(e);
-                        s_down[spans & (WM_RING - 1)][b][r] = pow2(-e);
+                        s_down[spans & (WM_RING - 1)][b][r] = fused ? pow2(24 - e) : pow2(-e);
                         spans++;
                     }
                     const uint2 sc = i == 0 ? now[0] : i == 1 ? now[1] : i == 2 ? now[2] : now[3];
@@ -320,17 +341,33 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) break;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
+                if (!WHOLE && fused) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t f[32];
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t f[32];
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int piece = h * 2 + c;
-                        const uint4 q = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
-                        many_convert<WHOLE>(q.x, s2[piece], f + c * 16); many_convert<WHOLE>(q.y, s2[piece], f + c * 16 + 4);
-                        many_convert<WHOLE>(q.z, s2[piece], f + c * 16 + 8); many_convert<WHOLE>(q.w, s2[piece], f + c * 16 + 12);
+                        for (int c = 0; c < 2; c++) {
+                            const int piece = h * 2 + c;
+                            const __half2 hi = __hmul2(s2[piece], __float2half2_rn(0.0625f)), off = __hmul2(s2[piece], __float2half2_rn(-0x1p-21f));
+                            const uint4 q = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
+                            many_convert_fused(q.x, s2[piece], hi, off, f + c * 16); many_convert_fused(q.y, s2[piece], hi, off, f + c * 16 + 4);
+                            many_convert_fused(q.z, s2[piece], hi, off, f + c * 16 + 8); many_convert_fused(q.w, s2[piece], hi, off, f + c * 16 + 12);
+                        }
+                        tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
                     }
-                    tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t f[32];
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const int piece = h * 2 + c;
+                            const uint4 q = *reinterpret_cast<const uint4 *>(src + ((piece ^ x) << 4));
+                            many_convert<WHOLE>(q.x, s2[piece], f + c * 16); many_convert<WHOLE>(q.y, s2[piece], f + c * 16 + 4);
+                            many_convert<WHOLE>(q.z, s2[piece], f + c * 16 + 8); many_convert<WHOLE>(q.w, s2[piece], f + c * 16 + 12);
+                        }
+                        tmem_st32(dst + (uint32_t)(as * 128 + h * 32), f);
+                    }
                 }
                 // (handed back only here: the loads' values have arrived when they have been used)
                 __syncwarp();
