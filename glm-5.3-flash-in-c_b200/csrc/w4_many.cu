@@ -3,20 +3,23 @@
 //
 // A tile is two blocks of 128 weight rows (gate/up: 128 gate rows and the 128 up rows that go with them) and up to 64
 // activation rows. One CTA per SM walks tiles; its warps have roles:
-//   16     codes by TMA: 2 x 128 rows x 64 bytes (128 columns) a step
-//   17     activation terms by TMA: 64 rows x 128 columns x terms a step
-//   8-15   conversion, four warps to a block, a thread to a row: nibbles become F16 values of (code - 8) * scale in tensor
+//   codes by TMA: 2 x 128 rows x 64 bytes (128 columns) a step
+//   activation terms by TMA: 64 rows x 128 columns x terms a step
+//   conversion, four warps to a block, a thread to a row: nibbles become F16 values of (code - 8) * scale in tensor
 //          memory. They are exact: 3 significant bits of the code times 8 of a BF16 scale fit F16's 11, with a power of two per row
-//          of W and four steps. A masked nibble is the subnormal number code * 2^-24 (or 2^-20), and one fused operation makes it
-//          (code - 8) * scale while the four steps' scales are within 2^8 of each other: the largest times 2^24 lies below 2^16, the
+//          of W and step. A masked nibble is the subnormal number code * 2^-24 (or 2^-20), and one fused operation makes it
+//          (code - 8) * scale while the step's scales are within 2^8 of each other: the largest times 2^24 lies below 2^16, the
 //          smallest's products above F16's last bit. Otherwise 1024 + code, minus 1032, times the scale, whose largest is brought below
 //          2^12: two operations, exact over 2^28 (groups of 32, eight rows past 154880 x 4096: 132 us).
 //          (A power of two for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
 //          F32 rows past groups of 128: the codes alone, and the scale on a step's sums.
-//   18, 19 products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
+//   products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
 //          same sums one after the other, so that a converted block is used twice.
-//   0-7    four warps to a block: take the sums over 256 columns (F32 rows; 512 of BF16) out of tensor memory and add them
-//          in registers, because the tensor cores cut off when they add; two accumulators in turn. Then the scales come off, and the rows are stored.
+//   sums, four warps to a block: take a step's sums out of tensor memory, take the power of two off (F32 or BF16 rows past groups of
+//          128: put the scale on) and add them in registers, because the tensor cores cut off when they add; two accumulators in turn.
+//          At a tile's end the rows' powers of two come off, and the rows are stored.
+// BF16 rows have one term, a converted block is used once, and the conversion is most of a step: two groups of warps take steps in turn (2048
+// rows past 12288 x 4096 288 -> 226 us; of F32 rows, whose sums then lack registers, 300 -> 327).
 // A converted block and its sums live in tensor memory (256 columns each); shared memory only holds what TMA brings, which it
 // must read for every product anyway: 64 rows of terms, 16 KB per step and term.
 //
@@ -32,13 +35,15 @@
 namespace g5b {
 
 constexpr int WM_ROWS = 64;                         // activation rows of a tile
-constexpr int WM_WS = 3, WM_XS = 3;                 // stages of codes, of terms
+// Groups of warps that convert, stages of codes (with two groups an even number, so that each stage belongs to one of them, and none of
+// their waits can take another use's phase for its own) and of terms. Registers of a thread: what the launch gives all of them, and what
+// those that hold the sums, convert and wait have of it then (256 * 120 + 384 * 80 = 640 * 96; 256 * 104 + 512 * 56 + 128 * 72 = 896 * 72).
+template <int TERMS> struct ManyRoles;
+template <> struct ManyRoles<2> { static constexpr int GROUPS = 1, WS = 3, XS = 3, SUM = 120, CONVERT = 80, REST = 80; };
+template <> struct ManyRoles<1> { static constexpr int GROUPS = 2, WS = 4, XS = 3, SUM = 104, CONVERT = 56, REST = 72; };
+template <int TERMS> constexpr int many_threads() { return (8 + 8 * ManyRoles<TERMS>::GROUPS + 4) * 32; }
 constexpr int WM_W_STAGE = 2 * 128 * 64;
-constexpr int WM_THREADS = 20 * 32;
-constexpr int WM_SPAN = 4;                          // steps with one power of two
-constexpr int WM_RING = 8;                          // spans whose powers of two are kept (the conversion is two steps and two accumulators ahead of the sums)
-// Registers of a thread: 96 at the launch, of which the other warps give some to those that hold the sums (256 * 120 + 384 * 80 = 640 * 96).
-constexpr int WM_REGS_SUM = 120, WM_REGS_REST = 80;
+constexpr int WM_RING = 8;                          // steps whose powers of two are kept (the conversion is two stages and two accumulators ahead of the sums)
 constexpr int WM_CTAS = 148;                        // SMs of a B200: what the cuts are chosen for
 constexpr int WM_PARTS = 16;
 
@@ -153,17 +158,18 @@ __device__ __forceinline__ bool many_all(bool ok, int barrier, int threads)
 }
 
 template <int TERMS, bool GATEUP, bool WHOLE>
-__global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
+__global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const __grid_constant__ ManyMaps maps, const ManyArgs a)
 {
-    constexpr int CHUNK = TERMS == 2 ? 1 : WM_SPAN;         // steps summed inside the tensor cores
+    using Roles = ManyRoles<TERMS>;
+    constexpr int WS = Roles::WS, XS = Roles::XS, GROUPS = Roles::GROUPS, REST = 8 + 8 * GROUPS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int XB = 2 * TERMS * a.n * 128;
-    uint8_t *wst = smem;                                                     // [WM_WS][2][128 rows][64]
-    uint8_t *xst = wst + WM_WS * WM_W_STAGE;                                 // [WM_XS][64-column half][term][n rows][128]
-    float *exch = reinterpret_cast<float *>(xst + (size_t)WM_XS * XB);       // [block][64][128]
-    __shared__ uint64_t w_full[WM_WS], w_empty[WM_WS], x_full[WM_XS], x_empty[WM_XS];
+    uint8_t *wst = smem;                                                     // [WS][2][128 rows][64]
+    uint8_t *xst = wst + WS * WM_W_STAGE;                                 // [XS][64-column half][term][n rows][128]
+    float *exch = reinterpret_cast<float *>(xst + (size_t)XS * XB);       // [block][64][128]
+    __shared__ uint64_t w_full[WS], w_empty[WS], x_full[XS], x_empty[XS];
     __shared__ uint64_t a_full[2][2], a_empty[2][2], d_full[2][2], d_empty[2][2], drained[2];     // [block][stage]
     __shared__ uint32_t s_tmem;
     __shared__ float s_down[WM_RING][2][128];               // what takes a row's power of two off again
@@ -171,15 +177,15 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 
     pdl_trigger();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < WM_WS; i++) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
-        for (int i = 0; i < WM_XS; i++) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 2); }
+        for (int i = 0; i < WS; i++) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
+        for (int i = 0; i < XS; i++) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 2); }
         for (int b = 0; b < 2; b++) {
             for (int i = 0; i < 2; i++) { mbar_init(&a_full[b][i], 4); mbar_init(&a_empty[b][i], 1); mbar_init(&d_full[b][i], 1); mbar_init(&d_empty[b][i], 4); }
             mbar_init(&drained[b], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 18) tmem_alloc(&s_tmem, 512);
+    if (warp == REST + 2) tmem_alloc(&s_tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -191,9 +197,9 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     bool ok = true;
 
     // (the four warps of a group change their registers in one place)
-    if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WM_REGS_REST));
-        if (warp == 16) {
+    if (warp >= REST) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles::REST));
+        if (warp == REST) {
             // --------------------------------------------------------------------- codes ----
             if (elect_one()) {
                 int s = 0, ph = 1, issued = 0;
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 while (ok && many_next(a, walk, t)) {
 #pragma unroll 1
                     for (int kb = t.k0; kb < t.k1; kb++) {
-                        if (issued >= WM_WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
+                        if (issued >= WS && !(ok = mbar_wait(&w_empty[s], (uint32_t)ph, err, 1))) break;
                         mbar_expect_tx(&w_full[s], WM_W_STAGE);
                         uint8_t *dst = wst + (size_t)s * WM_W_STAGE;
                         if (GATEUP) {
@@ -212,14 +218,14 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                             tma_load_3d(dst + WM_W_STAGE / 2, &maps.w, kb * 64, t.rt * 256 + 128, t.e, &w_full[s]);
                         }
                         issued++;
-                        if (++s == WM_WS) { s = 0; ph ^= 1; }
+                        if (++s == WS) { s = 0; ph ^= 1; }
                     }
                 }
                 // copies in flight must land before shared memory goes away
-                for (int j = issued - 1; j >= 0 && j >= issued - WM_WS; j--) mbar_wait(&w_full[j % WM_WS], (uint32_t)(j / WM_WS) & 1, err, 2);
+                for (int j = issued - 1; j >= 0 && j >= issued - WS; j--) mbar_wait(&w_full[j % WS], (uint32_t)(j / WS) & 1, err, 2);
             }
             __syncwarp();
-        } else if (warp == 17) {
+        } else if (warp == REST + 1) {
             // --------------------------------------------------------------------- terms ----
             pdl_wait();
             if (elect_one()) {
@@ -228,31 +234,29 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 while (ok && many_next(a, walk, t)) {
 #pragma unroll 1
                     for (int kb = t.k0; kb < t.k1; kb++) {
-                        if (issued >= WM_XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
+                        if (issued >= XS && !(ok = mbar_wait(&x_empty[s], (uint32_t)ph, err, 3))) break;
                         mbar_expect_tx(&x_full[s], (uint32_t)XB);
                         tma_load_4d(xst + (size_t)s * XB, &maps.x, 0, t.first, 0, kb * 2, &x_full[s]);
                         issued++;
-                        if (++s == WM_XS) { s = 0; ph ^= 1; }
+                        if (++s == XS) { s = 0; ph ^= 1; }
                     }
                 }
-                for (int j = issued - 1; j >= 0 && j >= issued - WM_XS; j--) mbar_wait(&x_full[j % WM_XS], (uint32_t)(j / WM_XS) & 1, err, 4);
+                for (int j = issued - 1; j >= 0 && j >= issued - XS; j--) mbar_wait(&x_full[j % XS], (uint32_t)(j / XS) & 1, err, 4);
             }
             __syncwarp();
-        } else if (warp >= 18) {
+        } else {
             // ------------------------------------------------------------------ products ----
             if (elect_one()) {
                 // (One warp for both blocks' products waited and issued for 2000 cycles a step, of which the tensor cores work 1184.)
-                const int b = warp - 18;
-                int as = 0, ap = 0, xs = 0, xp = 0, chunks = 0;
+                const int b = warp - REST - 2;
+                int as = 0, ap = 0, xs = 0, xp = 0, steps = 0;
 #pragma unroll 1
                 while (ok && many_next(a, walk, t)) {
                     const uint32_t idesc = tc_idesc(0, t.n);
-                    int c = 0;                                   // steps in the current accumulator
 #pragma unroll 1
                     for (int kb = t.k0; kb < t.k1; kb++) {
-                        const int buf = chunks & 1;
-                        const bool fresh = c == 0 && chunks >= 2;
-                        if (!(ok = many_wait(&a_full[b][as], (uint32_t)ap, &x_full[xs], (uint32_t)xp, fresh ? &d_empty[b][buf] : nullptr, (uint32_t)((chunks >> 1) - 1) & 1, err, 5))) break;
+                        const int buf = steps & 1;
+                        if (!(ok = many_wait(&a_full[b][as], (uint32_t)ap, &x_full[xs], (uint32_t)xp, steps >= 2 ? &d_empty[b][buf] : nullptr, (uint32_t)((steps >> 1) - 1) & 1, err, 5))) break;
                         tc_fence_after();
                         const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
                         const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
@@ -261,13 +265,14 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
 #pragma unroll
                             for (int m = 0; m < TERMS; m++) {
                                 const uint64_t bd = tc_smem_desc(xb + (uint32_t)(((k >> 2) * TERMS + m) * a.n * 128)) + 2 * (k & 3);
-                                tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, c || k || m ? 1u : 0u);
+                                tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, k || m ? 1u : 0u);
                             }
                         tc_commit(&a_empty[b][as]);
                         tc_commit(&x_empty[xs]);
-                        if (++c == CHUNK || kb + 1 == t.k1) { tc_commit(&d_full[b][buf]); chunks++; c = 0; }
+                        tc_commit(&d_full[b][buf]);
+                        steps++;
                         if (++as == 2) { as = 0; ap ^= 1; }
-                        if (++xs == WM_XS) { xs = 0; xp ^= 1; }
+                        if (++xs == XS) { xs = 0; xp ^= 1; }
                     }
                 }
                 // nothing of this thread is in flight, and no arrival still to come, when the CTA ends
@@ -278,59 +283,43 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
         }
     } else if (warp >= 8) {
         // --------------------------------------------------- codes -> F16 in tensor memory ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WM_REGS_REST));
-        const int b = (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane, x = (r >> 1) & 3;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles::CONVERT));
+        // A step's parity (of all tiles' in a row) is the stage that it is converted to; two groups take one each.
+        const int group = GROUPS == 2 ? ((warp - 8) >> 2) & 1 : 0, b = GROUPS == 2 ? (warp - 8) >> 3 : (warp - 8) >> 2, quarter = warp & 3, r = quarter * 32 + lane, x = (r >> 1) & 3;
         const uint32_t dst = tmem + ((uint32_t)(quarter * 32) << 16) + 256u + (uint32_t)(b * 64);
         const int per = a.w.group == 128 ? 2 : a.w.group == 64 ? 1 : 0;        // a 32-column piece's group: piece >> per
-        int ws = 0, wp = 0, as = 0, ap = 1, steps = 0, spans = 0;
+        int steps = 0;                                                          // before the tile
 #pragma unroll 1
         while (ok && many_next(a, walk, t)) {
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
-            // Raw scales of a step's four pieces (the four that they are among), a span ahead: one load whatever the group's size, because
+            // Raw scales of a step's four pieces (the four that they are among), two steps ahead: one load whatever the group's size, because
             // what comes out of branches is put together behind them, and waits there.
-            uint2 next[WM_SPAN];
-            auto fetch = [&](int kb0) {
-#pragma unroll
-                for (int i = 0; i < WM_SPAN; i++) next[i] = __ldg(reinterpret_cast<const uint2 *>(srow + ((4 * min(kb0 + i, t.k1 - 1) >> per) & ~3)));
-            };
-            if (!WHOLE) fetch(t.k0);
-            uint2 now[WM_SPAN];
-            float up = 0.f;
-            bool fused = false;
-#pragma unroll 1
-            for (int kb = t.k0; kb < t.k1; kb++, steps++) {
-                const int i = (kb - t.k0) & (WM_SPAN - 1);
+            auto first_of = [&](int kb) { return (4 * min(kb, t.k1 - 1) >> per) & ~3; };
+            auto fetch = [&](int kb) { return WHOLE ? make_uint2(0u, 0u) : __ldg(reinterpret_cast<const uint2 *>(srow + first_of(kb))); };
+            int kb = t.k0 + (GROUPS == 2 ? (steps ^ group) & 1 : 0);
+            uint2 next = fetch(kb), next1 = GROUPS == 1 ? fetch(kb + 1) : make_uint2(0u, 0u);
+            auto convert = [&](int kb, uint2 &next) {
+                const int step = steps + kb - t.k0, ws = step % WS, as = step & 1;
                 __half2 s2[4];
+                bool fused = false;
                 if (!WHOLE) {
-                    if (i == 0) {
-                        // (a group behind the last: zero, whatever lies there)
-                        uint32_t m = 0, least = 0xffffffffu;                 // (least: of those that are not zero, less one)
-#pragma unroll
-                        for (int k = 0; k < WM_SPAN; k++) {
-                            now[k] = next[k];
-                            const int last = a.w.groups - ((4 * min(kb + k, t.k1 - 1) >> per) & ~3);       // of the four, how many are groups
-                            if (last < 4) {
-                                now[k].x &= last > 1 ? 0xffffffffu : 0xffffu;
-                                now[k].y &= last > 3 ? 0xffffffffu : last > 2 ? 0xffffu : 0u;
-                            }
-                            const uint32_t x0 = now[k].x & 0x7fff7fffu, y0 = now[k].y & 0x7fff7fffu;
-                            m = __vmaxu2(m, __vmaxu2(x0, y0));
-                            least = __vminu2(least, __vminu2(__vsub2(x0, 0x00010001u), __vsub2(y0, 0x00010001u)));
-                        }
-                        fetch(kb + WM_SPAN);
-                        m = max(m & 0xffffu, m >> 16);
-                        least = min(least & 0xffffu, least >> 16);
-                        // exponents of the largest scale and the smallest that is not zero; far from FP32's ends, so that no power of two leaves it
-                        const int top = max((int)(m >> 7), 1), low = (int)((least + 1) >> 7);
-                        fused = __all_sync(0xffffffffu, top - low <= 8 && top >= 40 && top <= 220);
-                        const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 126);
-                        up = pow2(e);
-                        s_down[spans & (WM_RING - 1)][b][r] = fused ? pow2(24 - e) : pow2(-e);
-                        spans++;
+                    uint2 sc = next;
+                    next = fetch(kb + 2);
+                    // (a group behind the last: zero, whatever lies there)
+                    const int last = a.w.groups - first_of(kb);              // of the four, how many are groups
+                    if (last < 4) {
+                        sc.x &= last > 1 ? 0xffffffffu : 0xffffu;
+                        sc.y &= last > 3 ? 0xffffffffu : last > 2 ? 0xffffu : 0u;
                     }
-                    const uint2 sc = i == 0 ? now[0] : i == 1 ? now[1] : i == 2 ? now[2] : now[3];
+                    // exponents of the largest scale and the smallest that is not zero; far from FP32's ends, so that no power of two leaves it
+                    const uint32_t x0 = sc.x & 0x7fff7fffu, y0 = sc.y & 0x7fff7fffu, m2 = __vmaxu2(x0, y0), l2 = __vminu2(__vsub2(x0, 0x00010001u), __vsub2(y0, 0x00010001u));
+                    const int top = max((int)(max(m2 & 0xffffu, m2 >> 16) >> 7), 1), low = (int)((min(l2 & 0xffffu, l2 >> 16) + 1) >> 7);
+                    fused = __all_sync(0xffffffffu, top - low <= 8 && top >= 40 && top <= 220);
+                    const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 126);
+                    const float up = pow2(e);
+                    s_down[step & (WM_RING - 1)][b][r] = fused ? pow2(24 - e) : pow2(-e);
 #pragma unroll
                     for (int piece = 0; piece < 4; piece++) {
                         const int g = (4 * kb + piece) >> per;
@@ -338,7 +327,9 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                         s2[piece] = __float2half2_rn(bf16_to_f32((uint16_t)raw) * up);
                     }
                 }
-                if (!(ok = many_wait<true>(steps >= 2 ? &a_empty[b][as] : &w_full[ws], (uint32_t)(steps >= 2 ? ap : wp), &w_full[ws], (uint32_t)wp, nullptr, 0u, err, 9))) break;
+                uint64_t *full = &w_full[ws], *free_ = &a_empty[b][as];
+                const uint32_t full_parity = (uint32_t)(step / WS) & 1;
+                if (!(ok = many_wait<true>(step >= 2 ? free_ : full, step >= 2 ? (uint32_t)((step >> 1) - 1) & 1 : full_parity, full, full_parity, nullptr, 0u, err, 9))) return;
                 tc_fence_after();
                 const uint8_t *src = wst + (size_t)ws * WM_W_STAGE + b * (WM_W_STAGE / 2) + r * 64;
                 if (!WHOLE && fused) {
@@ -376,18 +367,22 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&a_full[b][as]);
-                if (++ws == WM_WS) { ws = 0; wp ^= 1; }
-                if (++as == 2) { as = 0; ap ^= 1; }
+            };
+            // (two sets of registers for the scales that are on their way: moved from one to the other they would be waited for)
+#pragma unroll 1
+            for (; kb < t.k1 && ok; kb += 2) {
+                convert(kb, next);
+                if (GROUPS == 1 && ok && kb + 1 < t.k1) convert(kb + 1, next1);
             }
+            steps += t.k1 - t.k0;
         }
     } else {
         // ------------------------------------------------------------ sums, scales, stores ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WM_REGS_SUM));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles::SUM));
         const int b = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * 128);
         const int bar = GATEUP ? 1 : 1 + b, bar_threads = GATEUP ? 256 : 128;       // (gate/up: both blocks together)
-        int chunks = 0;
-        int spans = 0;
+        int steps = 0;
         pdl_wait();
 #pragma unroll 1
         while (many_next(a, walk, t)) {
@@ -395,23 +390,19 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
             F2 acc[WM_ROWS / 2];
 #pragma unroll
             for (int k = 0; k < WM_ROWS / 2; k++) acc[k] = f2(0.f, 0.f);
-            // what a chunk's sums are multiplied by: a step's scale, one step ahead (WHOLE), or what takes the power of two off
+            // what a step's sums are multiplied by: a step's scale, one step ahead (WHOLE), or what takes the power of two off
             const W4Mat &w = GATEUP && b ? a.up : a.w;
             const int row = GATEUP ? t.rt * 128 + r : t.rt * 256 + b * 128 + r;
             const uint16_t *srow = w.scales + (size_t)t.e * a.w.scales_stride + (size_t)min(row, a.w.rows - 1) * a.w.sp;
             uint16_t next = 0;
             if (WHOLE) next = __ldg(srow + t.k0);
-            const int uses = (t.k1 - t.k0 + CHUNK - 1) / CHUNK;
 #pragma unroll 1
-            for (int c = 0; c < uses; c++, chunks++) {
-                const int buf = chunks & 1;
+            for (int kb = t.k0; kb < t.k1; kb++, steps++) {
+                const int buf = steps & 1;
                 float sc = bf16_to_f32(next);
-                if (WHOLE && c + 1 < uses) next = __ldg(srow + t.k0 + c + 1);
-                if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(chunks >> 1) & 1, err, 11))) break;
-                if (!WHOLE) {
-                    sc = s_down[spans & (WM_RING - 1)][b][r];
-                    spans += CHUNK == WM_SPAN || (c & (WM_SPAN - 1)) == WM_SPAN - 1 || c + 1 == uses;
-                }
+                if (WHOLE && kb + 1 < t.k1) next = __ldg(srow + kb + 1);
+                if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(steps >> 1) & 1, err, 11))) break;
+                if (!WHOLE) sc = s_down[steps & (WM_RING - 1)][b][r];
                 tc_fence_after();
 #pragma unroll
                 for (int g = 0; g < WM_ROWS; g += 32)
@@ -478,7 +469,7 @@ __global__ void __launch_bounds__(WM_THREADS, 1) w4_many_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 18) { __syncwarp(); tmem_dealloc(tmem, 512); }
+    if (warp == REST + 2) { __syncwarp(); tmem_dealloc(tmem, 512); }
 }
 
 // The tiles that were cut: their parts' sums in order. A CTA takes four rows of x of one tile.
@@ -534,9 +525,9 @@ template <int TERMS, bool GATEUP, bool WHOLE>
 static int many_launch(cudaStream_t st, const ManyMaps &m, const ManyArgs &a, int grid)
 {
     static SmemGrant grant;
-    const size_t smem = 1024 + WM_WS * WM_W_STAGE + (size_t)WM_XS * 2 * TERMS * a.n * 128 + 2 * WM_ROWS * 128 * 4;
+    const size_t smem = 1024 + ManyRoles<TERMS>::WS * WM_W_STAGE + (size_t)ManyRoles<TERMS>::XS * 2 * TERMS * a.n * 128 + 2 * WM_ROWS * 128 * 4;
     if (!dev_opt_in_smem((const void *)w4_many_kernel<TERMS, GATEUP, WHOLE>, smem, grant)) return -1;
-    G5B_LAUNCH_PDL((w4_many_kernel<TERMS, GATEUP, WHOLE>), dim3(grid), dim3(WM_THREADS), smem, st, m, a);
+    G5B_LAUNCH_PDL((w4_many_kernel<TERMS, GATEUP, WHOLE>), dim3(grid), dim3(many_threads<TERMS>()), smem, st, m, a);
     return 0;
 }
 
@@ -572,9 +563,10 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     }
     const int grid = (int)std::min<long long>(items, dev_sms());
     const bool pair = j.mode == W4_GATEUP, whole = j.w.group == 128;
-    const int rc = j.terms.n_terms == 1 ? (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
-                   : whole ? (pair ? many_launch<2, true, true>(st, m, a, grid) : many_launch<2, false, true>(st, m, a, grid))
-                           : (pair ? many_launch<2, true, false>(st, m, a, grid) : many_launch<2, false, false>(st, m, a, grid));
+    const int rc = j.terms.n_terms == 1 ? whole ? (pair ? many_launch<1, true, true>(st, m, a, grid) : many_launch<1, false, true>(st, m, a, grid))
+                                                : (pair ? many_launch<1, true, false>(st, m, a, grid) : many_launch<1, false, false>(st, m, a, grid))
+                                        : whole ? (pair ? many_launch<2, true, true>(st, m, a, grid) : many_launch<2, false, true>(st, m, a, grid))
+                                                : (pair ? many_launch<2, true, false>(st, m, a, grid) : many_launch<2, false, false>(st, m, a, grid));
     if (rc) return -1;
     if (j.mode == W4_DENSE && a.parts > 1)
         G5B_LAUNCH_PDL(w4_parts_kernel, dim3(tiles - a.whole, (a.n + 3) / 4), dim3(256), 0, st, part, a.parts, a.whole, a.TT, a.n, j.T, j.w.rows, j.y, j.ldy, j.y_dt, a.wide);
