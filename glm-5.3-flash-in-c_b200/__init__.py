@@ -597,9 +597,8 @@ def sample_host(logits, temperature: float, top_p: float, seed: int, step: int, 
 
 
 # ------------------------------------------------------------------ 4-bit operators (device memory) ----
-# Arguments are tensors that live on the current CUDA device: any object with data_ptr(), shape, stride(), dtype and device
-# (torch.Tensor; this module does not import torch). `stream` is a cudaStream_t as a number; None takes torch's
-# current stream of the tensors' device. Nothing is copied, allocated or waited for.
+# Arguments are torch tensors that live on the current CUDA device (this module does not import torch). `stream` is a
+# cudaStream_t as a number; None takes torch's current stream of the tensors' device. Nothing is copied, allocated or waited for.
 
 class _W4(C.Structure):
     """g5b_w4 (include/glm53f_b200.h)."""
@@ -634,46 +633,57 @@ def _dtype(t) -> str:
 _ROW_TYPES = {"float32": DT_F32, "bfloat16": DT_BF16}
 
 
-def _check(name, t, shape, dtype, like=None):
-    """A dense tensor of this shape and type (None: any), on the device of `like`."""
+def _check(name, t, shape, dtype, device=None):
+    """Address of a dense tensor of this shape and type (None: any), on this device."""
     if dtype is not None and _dtype(t) != dtype:
         raise TypeError(f"{name} is {_dtype(t)}, not {dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} is not dense")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} lies on {t.device}, not on {like.device}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} lies on device {t.get_device()}, not on {device} (-1: the host)")
     return t.data_ptr()
 
 
-def _rows(name, t, like=None):
-    """A matrix of F32 or BF16 rows: (address, dtype, rows, columns, elements between rows)."""
+def _rows(name, t, device, like=None):
+    """A matrix of F32 or BF16 rows (of the type of `like`) on a device: (address, dtype, rows, columns, elements between rows)."""
     kind = _ROW_TYPES.get(_dtype(t))
     if kind is None:
         raise TypeError(f"{name} is {_dtype(t)}, not float32 or bfloat16")
-    if len(t.shape) != 2:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not two dimensions")
-    rows, cols = t.shape
+    if like is not None and t.dtype != like.dtype:
+        raise ValueError(f"{name} is {_dtype(t)}, not {_dtype(like)}")
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} has shape {tuple(shape)}, not two dimensions")
+    rows, cols = shape
     ld, step = t.stride()
     if (cols > 1 and step != 1) or (rows > 1 and ld < cols):
         raise ValueError(f"{name}: rows must be dense (strides {ld}, {step})")
-    if like is not None and (t.device != like.device or t.dtype != like.dtype):
-        raise ValueError(f"{name} is {_dtype(t)} on {t.device}, not {_dtype(like)} on {like.device}")
-    return t.data_ptr(), kind, rows, cols, max(ld, cols)
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} lies on device {t.get_device()}, not on {device} (-1: the host)")
+    return t.data_ptr(), kind, rows, cols, ld if ld > cols else cols
 
 
-def _stream(stream, t):
+_raw_stream = None                                  # torch's quick way to a device's current stream, where it has one
+
+
+def _stream(stream, device):
+    global _raw_stream
     if stream is not None:
         return stream
-    import sys
-    torch = sys.modules.get("torch")
-    return torch.cuda.current_stream(t.device).cuda_stream if torch is not None else 0
+    if device < 0:                                  # host tensors: the library refuses them
+        return 0
+    if _raw_stream is None:
+        import sys
+        torch = sys.modules["torch"]
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 def _call_w4(name, *args):
-    if getattr(lib(), "g5b_" + name)(*args) != 0:
-        raise RuntimeError(f"g5b_{name} failed: " + (lib().g5b_last_error() or b"").decode())
+    if getattr(_lib or lib(), name)(*args) != 0:
+        raise RuntimeError(f"{name} failed: " + (lib().g5b_last_error() or b"").decode())
 
 
 def w4_pitch(cols: int) -> int:
@@ -697,17 +707,20 @@ class W4:
         if group not in (32, 64, 128) or rows < 1 or cols < 1:
             raise ValueError(f"{rows} x {cols} in groups of {group}")
         self.count = lead[0] if lead else 1
+        self.device = codes.get_device()
         a = _check("codes", codes, lead + (rows, w4_pitch(cols)), "uint8")
-        b = _check("scales", scales, lead + (rows, w4_scale_pitch(cols, group)), "bfloat16", codes)
+        b = _check("scales", scales, lead + (rows, w4_scale_pitch(cols, group)), "bfloat16", self.device)
         self.codes, self.scales, self.rows, self.cols, self.group = codes, scales, rows, cols, group
-        self.device = codes.device
         self.c = _W4(a, b, rows, cols, group, self.count)
         self.ref = C.byref(self.c)
 
 
-def _on(w: W4, name, t):
-    if t.device != w.device:
-        raise ValueError(f"{name} lies on {t.device}, the weights on {w.device}")
+def _workspace(t, device):
+    if t.get_device() != device:
+        raise ValueError(f"the workspace lies on device {t.get_device()}, not on {device} (-1: the host)")
+    if not t.is_contiguous():
+        raise ValueError("the workspace is not dense")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def w4_quantize(src, w: W4, scale_inv=None, block=(128, 128), stream=None):
@@ -715,90 +728,91 @@ def w4_quantize(src, w: W4, scale_inv=None, block=(128, 128), stream=None):
     kind = {"float32": DT_F32, "bfloat16": DT_BF16, "float8_e4m3fn": DT_FP8, "uint8": DT_FP8}.get(_dtype(src))
     if kind is None:
         raise TypeError(f"a source of {_dtype(src)}")
-    _on(w, "the source", src)
-    data, grid = _check("the source", src, (w.rows, w.cols), None), None
+    data, grid = _check("the source", src, (w.rows, w.cols), None, w.device), None
     if kind == DT_FP8:
         if scale_inv is None:
             raise ValueError("an FP8 source needs its scale grid")
-        grid = _check("scale_inv", scale_inv, (-(-w.rows // block[0]), -(-w.cols // block[1])), "float32", src)
+        grid = _check("scale_inv", scale_inv, (-(-w.rows // block[0]), -(-w.cols // block[1])), "float32", w.device)
     t = Tensor(data, grid, kind, w.rows, w.cols, 1)
-    _call_w4("w4_quantize", C.byref(t), block[0], block[1], w.ref, _stream(stream, src))
+    _call_w4("g5b_w4_quantize", C.byref(t), block[0], block[1], w.ref, _stream(stream, w.device))
 
 
 def w4_dequantize(w: W4, out, stream=None):
     """The values of w into out [rows][cols], float32 or bfloat16 (g5b_w4_dequantize)."""
-    _on(w, "out", out)
-    p, kind, rows, cols, ld = _rows("out", out)
-    if (rows, cols) != (w.rows, w.cols):
+    p, kind, rows, cols, ld = _rows("out", out, w.device)
+    if rows != w.rows or cols != w.cols:
         raise ValueError(f"out of {rows} x {cols} for a matrix of {w.rows} x {w.cols}")
-    _call_w4("w4_dequantize", w.ref, kind, p, ld, _stream(stream, out))
+    _call_w4("g5b_w4_dequantize", w.ref, kind, p, ld, _stream(stream, w.device))
 
 
 def w4_matmul_workspace(w: W4, x) -> int:
     """Bytes of workspace of w4_matmul for this x (g5b_w4_matmul_workspace)."""
-    return lib().g5b_w4_matmul_workspace(w.ref, _rows("x", x)[1], x.shape[0])
+    return lib().g5b_w4_matmul_workspace(w.ref, _rows("x", x, None)[1], x.shape[0])
 
 
 def w4_matmul(w: W4, x, y, workspace, stream=None):
     """y [T][rows] = W x [T][cols], float32 or bfloat16 (g5b_w4_matmul). workspace: a dense tensor of any type."""
-    _on(w, "x", x)
-    p, kind, T, cols, ldx = _rows("x", x)
-    q, _, ty, rows, ldy = _rows("y", y, x)
+    device = w.device
+    p, kind, T, cols, ldx = _rows("x", x, device)
+    q, _, ty, rows, ldy = _rows("y", y, device, x)
     if cols != w.cols or rows != w.rows or ty != T:
         raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} do not fit a matrix of {w.rows} x {w.cols}")
-    _on(w, "the workspace", workspace)
-    _call_w4("w4_matmul", w.ref, p, kind, T, ldx, q, ldy, workspace.data_ptr(), workspace.nbytes, _stream(stream, x))
+    space, size = _workspace(workspace, device)
+    _call_w4("g5b_w4_matmul", w.ref, p, kind, T, ldx, q, ldy, space, size, _stream(stream, device))
 
 
 def expert_sort(idx, n_experts: int, order, place, offsets, stream=None):
     """Picks idx int32 [T][topk] sorted by expert: order [T * topk], place [T][topk], offsets [n_experts + 1] (g5b_expert_sort)."""
     T, topk = idx.shape
-    _call_w4("expert_sort", _check("idx", idx, (T, topk), "int32"), T, topk, n_experts, _check("order", order, (T * topk,), "int32", idx),
-             _check("place", place, (T, topk), "int32", idx), _check("offsets", offsets, (n_experts + 1,), "int32", idx), _stream(stream, idx))
+    device = idx.get_device()
+    _call_w4("g5b_expert_sort", _check("idx", idx, (T, topk), "int32"), T, topk, n_experts, _check("order", order, (T * topk,), "int32", device),
+             _check("place", place, (T, topk), "int32", device), _check("offsets", offsets, (n_experts + 1,), "int32", device), _stream(stream, device))
 
 
 def expert_gather(x, order, offsets, rows, stream=None):
     """rows[i] = the x row of sorted pick i (g5b_expert_gather); rows [len(order)][cols] of x's type."""
-    p, kind, T, cols, ldx = _rows("x", x)
-    q, _, n, rc, ldr = _rows("rows", rows, x)
+    device = x.get_device()
+    p, kind, T, cols, ldx = _rows("x", x, None)
+    q, _, n, rc, ldr = _rows("rows", rows, device, x)
     topk = order.shape[0] // T if T else 1
     if rc != cols or n != T * topk:
         raise ValueError(f"rows {tuple(rows.shape)} for {T} tokens of {cols} columns and {order.shape[0]} picks")
-    _call_w4("expert_gather", p, kind, T, cols, ldx, _check("order", order, (T * topk,), "int32", x),
-             _check("offsets", offsets, offsets.shape[:1], "int32", x), topk, offsets.shape[0] - 1, q, ldr, _stream(stream, x))
+    _call_w4("g5b_expert_gather", p, kind, T, cols, ldx, _check("order", order, (T * topk,), "int32", device),
+             _check("offsets", offsets, offsets.shape[:1], "int32", device), topk, offsets.shape[0] - 1, q, ldr, _stream(stream, device))
 
 
 def expert_combine(rows, place, weights, out, stream=None):
     """out[t] = the weighted sum of the token's rows (g5b_expert_combine); weights float32 [T][topk], or None for ones."""
-    p, kind, n, cols, ldr = _rows("rows", rows)
-    q, _, T, oc, ldo = _rows("out", out, rows)
+    device = rows.get_device()
+    p, kind, n, cols, ldr = _rows("rows", rows, None)
+    q, _, T, oc, ldo = _rows("out", out, device, rows)
     topk = place.shape[1]
     if oc != cols or n != T * topk:
         raise ValueError(f"out {tuple(out.shape)} for rows {tuple(rows.shape)} and places {tuple(place.shape)}")
-    _call_w4("expert_combine", p, kind, ldr, _check("place", place, (T, topk), "int32", rows),
-             _check("weights", weights, (T, topk), "float32", rows) if weights is not None else None, T, topk, cols, q, ldo, _stream(stream, rows))
+    _call_w4("g5b_expert_combine", p, kind, ldr, _check("place", place, (T, topk), "int32", device),
+             _check("weights", weights, (T, topk), "float32", device) if weights is not None else None, T, topk, cols, q, ldo, _stream(stream, device))
 
 
 def w4_experts_workspace(gate: W4, up: W4, down: W4, x, idx) -> int:
     """Bytes of workspace of w4_experts for this x and idx (g5b_w4_experts_workspace)."""
-    return lib().g5b_w4_experts_workspace(gate.ref, down.ref, _rows("x", x)[1], x.shape[0], idx.shape[1])
+    return lib().g5b_w4_experts_workspace(gate.ref, down.ref, _rows("x", x, None)[1], x.shape[0], idx.shape[1])
 
 
 def w4_experts(gate: W4, up: W4, down: W4, x, idx, weights, limit: float, out, workspace, stream=None):
     """Routed experts in 4 bits (g5b_w4_experts): x and out [T][hidden], idx int32 and weights float32 [T][topk]."""
-    _on(gate, "x", x)
-    _on(gate, "up", up)
-    _on(gate, "down", down)
-    _on(gate, "the workspace", workspace)
-    p, kind, T, cols, ldx = _rows("x", x)
-    q, _, to, oc, ldo = _rows("out", out, x)
+    device = gate.device
+    p, kind, T, cols, ldx = _rows("x", x, device)
+    q, _, to, oc, ldo = _rows("out", out, device, x)
     topk = idx.shape[1]
     if cols != gate.cols or oc != cols or to != T:
         raise ValueError(f"x {tuple(x.shape)} and out {tuple(out.shape)} do not fit experts of {gate.cols} columns")
-    _call_w4("w4_experts", gate.ref, up.ref, down.ref, p, kind, T, ldx, _check("idx", idx, (T, topk), "int32", x),
-             _check("weights", weights, (T, topk), "float32", x), topk, limit, q, ldo, workspace.data_ptr(), workspace.nbytes, _stream(stream, x))
+    if up.device != device or down.device != device:
+        raise ValueError("the experts' matrices lie on different devices")
+    space, size = _workspace(workspace, device)
+    _call_w4("g5b_w4_experts", gate.ref, up.ref, down.ref, p, kind, T, ldx, _check("idx", idx, (T, topk), "int32", device),
+             _check("weights", weights, (T, topk), "float32", device), topk, limit, q, ldo, space, size, _stream(stream, device))
 
 
 def w4_status(stream=0):
     """Waits for the stream and raises if a wait inside a 4-bit product ran out since the last look (g5b_w4_status)."""
-    _call_w4("w4_status", stream)
+    _call_w4("g5b_w4_status", stream)

@@ -17,6 +17,7 @@ namespace g5b {
 
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_CLUSTER = 8;
 constexpr int SORT_ALONE = 4096;
+constexpr int SORT_HELD = SORT_ALONE / (SORT_WARPS * 32);      // picks of a lane that stay in registers
 
 __device__ __forceinline__ int ld_cluster_s32(const int *p, uint32_t rank)
 {
@@ -39,18 +40,27 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
     const int share = (n + ctas * SORT_WARPS * 32 - 1) / (ctas * SORT_WARPS * 32) * 32;
     const long long p0 = (long long)share * (rank * SORT_WARPS + warp), p1 = p0 + share < n ? p0 + share : n;
     int *mine = count + warp * E;
-    for (int e = lane; e < E; e += 32) mine[e] = 0;
-    __syncwarp();
     auto expert_of = [&](long long p) {
         const int e = p < p1 ? __ldg(idx + p) : -1;
         return e >= 0 && e < E ? e : -1;
     };
-    for (long long p = p0; p < p1; p += 32) {
-        const int e = expert_of(p + lane);
+    // the first picks are asked for together and stay in registers
+    int held[SORT_HELD];
+#pragma unroll
+    for (int i = 0; i < SORT_HELD; i++) held[i] = expert_of(p0 + 32 * i + lane);
+    for (int e = lane; e < E; e += 32) mine[e] = 0;
+    __syncwarp();
+    auto rounds = [&](auto &&step) {
+#pragma unroll
+        for (int i = 0; i < SORT_HELD; i++)
+            if (p0 + 32 * i < p1) step(p0 + 32 * i, held[i]);
+        for (long long p = p0 + 32 * SORT_HELD; p < p1; p += 32) step(p, expert_of(p + lane));
+    };
+    rounds([&](long long, int e) {
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
-    }
+    });
     __syncthreads();
     // places of the warps within the CTA, and the CTA's sum
     for (int e = tid; e < E; e += SORT_THREADS) {
@@ -104,8 +114,7 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
     __syncthreads();
     int valid = 0;
     for (int w = 0; w < SORT_WARPS; w++) valid += s_part[0][w];
-    for (long long p = p0; p < p1; p += 32) {
-        const int e = expert_of(p + lane);
+    rounds([&](long long p, int e) {
         const uint32_t same = __match_any_sync(0xffffffffu, e), below = same & ((1u << lane) - 1u);
         int at = -1;
         if (e >= 0) at = total[e] + mine[e] + __popc(below);
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
             if (at >= 0) order[at] = (int)(p + lane);
             if (p + lane >= valid) order[p + lane] = -1;
         }
-    }
+    });
 }
 
 int expert_sort(cudaStream_t st, const int *idx, int T, int topk, int E, int *order, int *place, int *offsets, const W4Slots *slots)

@@ -5,15 +5,15 @@
 // does, which is exact there (q s has 12 significant bits; within half a step of it the difference loses none). A
 // division instead is twenty instructions a weight, as many as the SM can issue while HBM delivers an FP8 weight.
 //
-// Both directions are bound by HBM. A warp takes a piece of a row, a lane eight columns at a time (one word of codes), so that a
-// group is 4, 8 or 16 neighbouring lanes and its maximum two to four shuffles.
-#include "common.cuh"
-#include "w4.h"
+// Both directions are bound by HBM, the first nearly by the instructions a weight takes (14). There a lane takes 32 columns, so that what
+// is paid per group - the division, the reciprocal, the maximum's shuffles - is paid once for 32 weights, and its codes are one store;
+// eight columns a lane paid it four times, converted to integers by the slow instruction, and took 72 us for 12288 x 4096 BF16 weights.
+#include "w4.cuh"
 
 namespace g5b {
 
-constexpr int CV_WORDS = 128;      // words of codes (eight columns) a warp takes
 constexpr int CV_WARPS = 8;
+constexpr int CV_COLS = 1024;      // columns a warp takes
 
 // Eight values from column c0 on (zero behind the last column); whole: 16-byte loads of eight that exist
 template <int DT>
@@ -45,67 +45,68 @@ __device__ __forceinline__ void load8(float (&v)[8], const void *src, size_t at,
 
 template <int DT>
 __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uint8_t *codes, uint16_t *scales, const void *src, const float *inv,
-                                                                    int br, int bc, int scols, int pieces, bool whole)
+                                                                    int br, int bc, int scols, unsigned pieces, bool whole)
 {
     const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * CV_WARPS + (threadIdx.x >> 5);
-    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
+    const unsigned unit = blockIdx.x * CV_WARPS + (threadIdx.x >> 5), row_ = unit / pieces;
+    const int row = (int)row_, c0 = (int)(unit - row_ * pieces) * CV_COLS + lane * 32, per = w.group / 32;
     if (row >= w.rows) return;
-    const int per = w.group / 8, words = w.pitch / 4;
-    float v[CV_WORDS / 32][8];
+    float v[4][8];
 #pragma unroll
-    for (int i = 0; i < CV_WORDS / 32; i++) {
-        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
-        load8<DT>(v[i], src, (size_t)row * w.cols + c0, c0, w.cols, whole);
+    for (int i = 0; i < 4; i++) {
+        const int c = c0 + 8 * i;
+        load8<DT>(v[i], src, (size_t)row * w.cols + c, c, w.cols, whole);
         if (DT == DT_FP8) {
             // the weight is the FP32 product of code and block scale
             const float *irow = inv + (size_t)(row / br) * scols;
             if (bc % 8 == 0) {
-                const float s = c0 < w.cols ? __ldg(irow + c0 / bc) : 0.f;
+                const float s = c < w.cols ? __ldg(irow + c / bc) : 0.f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[i][k] = __fmul_rn(v[i][k], s);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) if (c0 + k < w.cols) v[i][k] = __fmul_rn(v[i][k], __ldg(irow + (c0 + k) / bc));
+                for (int k = 0; k < 8; k++) if (c + k < w.cols) v[i][k] = __fmul_rn(v[i][k], __ldg(irow + (c + k) / bc));
             }
         }
     }
+    // the largest magnitude as bits: infinities and NaN are above every number
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < CV_WORDS / 32; i++) {
-        const int word = piece * CV_WORDS + i * 32 + lane;
-        // the largest magnitude as bits: infinities and NaN are above every number
-        uint32_t m = 0;
+    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int k = 0; k < 8; k++) m = max(m, __float_as_uint(v[i][k]) & 0x7fffffffu);
-        for (int o = 1; o < per; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const bool finite = m < 0x7f800000u;
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
-        const float s = __bfloat162float(sb);
-        const bool live = finite && s > 0.f;
-        // 1 / s of a subnormal s may be infinite: the quotient is then taken of both times 2^64
-        const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
-        uint32_t packed = 0;
+    for (int o = 1; o < per; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool finite = m < 0x7f800000u;
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
+    const float s = __bfloat162float(sb);
+    const bool live = finite && s > 0.f;
+    // 1 / s of a small s may be infinite: the quotient is then taken of both times 2^64
+    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
+    __align__(16) uint32_t packed[4];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float x = v[i][k] * up;
-            float q = rintf(__fmul_rn(x, r));
-            const float d = fmaf(-q, su, x), ad = fabsf(d);
-            // one step on where the residual is over half a step, or half a step and q odd
-            if (ad > half || (ad == half && ((int)q & 1))) q += copysignf(1.0f, d);
-            q = fminf(fmaxf(q, -7.0f), 7.0f);
-            packed |= (uint32_t)(live ? (int)q + 8 : 8) << (4 * k);
-        }
-        if (word < words) reinterpret_cast<uint32_t *>(codes + (size_t)row * w.pitch)[word] = packed;
-        const int group = word / per;
-        if ((word & (per - 1)) == 0 && group < w.sp)
-            scales[(size_t)row * w.sp + group] = group >= w.groups ? (uint16_t)0 : finite ? __bfloat16_as_ushort(sb) : (uint16_t)0x7fc0;
+    for (int i = 0; i < 4; i++) {
+        packed[i] = live ? 0u : 0x88888888u;
+        if (live)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                // rounded by adding 1.5 2^23, in whose low bits the integer (and whether it is odd) then lies; |w / s| <= 10 (a subnormal scale)
+                const float x = v[i][k] * up, t = fmaf(x, r, 12582912.0f), q = t - 12582912.0f, d = fmaf(-q, su, x), ad = fabsf(d);
+                int n = __float_as_int(t) - 0x4b400000;
+                // one step on where the residual is over half a step, or half a step and the integer odd
+                if (ad > half || (ad == half && (n & 1))) n += d > 0.f ? 1 : -1;
+                packed[i] |= (uint32_t)(min(max(n, -7), 7) + 8) << (4 * k);
+            }
     }
+    if (c0 / 2 < w.pitch) *reinterpret_cast<uint4 *>(codes + (size_t)row * w.pitch + c0 / 2) = *reinterpret_cast<const uint4 *>(packed);
+    const int group = c0 / w.group;
+    if ((lane & (per - 1)) == 0 && group < w.sp)
+        scales[(size_t)row * w.sp + group] = group >= w.groups ? (uint16_t)0 : finite ? __bfloat16_as_ushort(sb) : (uint16_t)0x7fc0;
 }
 
 void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const float *scale, int br, int bc)
 {
     // the pieces cover the codes' and the scales' padding too, so that no byte of either is left undefined
-    const int words = max(w.pitch / 4, w.sp * (w.group / 8)), pieces = (words + CV_WORDS - 1) / CV_WORDS;
+    const unsigned pieces = (max(w.pitch * 2, w.sp * w.group) + CV_COLS - 1) / CV_COLS;
     const long long units = (long long)w.rows * pieces;
     const int size = dt == DT_F32 ? 4 : dt == DT_BF16 ? 2 : 1;
     const size_t align = dt == DT_FP8 ? 8 : 16;
@@ -118,58 +119,57 @@ void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const
     else                    G5B_LAUNCH(w4_quantize_kernel<DT_FP8>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
 }
 
+// A lane takes four columns at a time, so that a warp's store is 512 contiguous bytes of FP32 (eight columns a lane: 52 us for 12288 x 4096).
 template <int DT>
-__global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, void *out, size_t ldo, int pieces, bool whole)
+__global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, void *out, size_t ldo, unsigned pieces, bool whole)
 {
     const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * CV_WARPS + (threadIdx.x >> 5);
-    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
+    const unsigned unit = blockIdx.x * CV_WARPS + (threadIdx.x >> 5), row_ = unit / pieces;
+    const int row = (int)row_, c_first = (int)(unit - row_ * pieces) * CV_COLS + lane * 4, log = w.group == 128 ? 7 : w.group == 64 ? 6 : 5;
     if (row >= w.rows) return;
-    uint32_t word[CV_WORDS / 32];
-    float s[CV_WORDS / 32];
+    uint32_t code[CV_COLS / 128];
+    float s[CV_COLS / 128];
 #pragma unroll
-    for (int i = 0; i < CV_WORDS / 32; i++) {
-        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
-        word[i] = 0; s[i] = 0.f;
+    for (int i = 0; i < CV_COLS / 128; i++) {
+        const int c0 = c_first + 128 * i;
+        code[i] = 0; s[i] = 0.f;
         if (c0 < w.cols) {
-            word[i] = __ldcs(reinterpret_cast<const uint32_t *>(w.codes + (size_t)row * w.pitch) + c0 / 8);
-            s[i] = bf16_to_f32(__ldg(w.scales + (size_t)row * w.sp + c0 / w.group));
+            code[i] = __ldg(reinterpret_cast<const uint16_t *>(w.codes + (size_t)row * w.pitch) + c0 / 4);
+            s[i] = bf16_to_f32(__ldg(w.scales + (size_t)row * w.sp + (c0 >> log)));
         }
     }
 #pragma unroll
-    for (int i = 0; i < CV_WORDS / 32; i++) {
-        const int c0 = (piece * CV_WORDS + i * 32 + lane) * 8;
+    for (int i = 0; i < CV_COLS / 128; i++) {
+        const int c0 = c_first + 128 * i;
         if (c0 >= w.cols) continue;
-        float v[8];
+        float v[4];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = __fmul_rn((float)((int)((word[i] >> (4 * k)) & 15u) - 8), s[i]);
+        for (int k = 0; k < 4; k++) v[k] = __fmul_rn((float)((int)((code[i] >> (4 * k)) & 15u) - 8), s[i]);
         const size_t at = (size_t)row * ldo + c0;
         if (DT == DT_F32) {
             float *o = static_cast<float *>(out) + at;
-            if (whole && c0 + 8 <= w.cols) {
-                __stcs(reinterpret_cast<float4 *>(o), make_float4(v[0], v[1], v[2], v[3]));
-                __stcs(reinterpret_cast<float4 *>(o + 4), make_float4(v[4], v[5], v[6], v[7]));
-            } else
-                for (int k = 0; k < 8 && c0 + k < w.cols; k++) o[k] = v[k];
+            if (whole && c0 + 4 <= w.cols) __stcs(reinterpret_cast<float4 *>(o), make_float4(v[0], v[1], v[2], v[3]));
+            else
+                for (int k = 0; k < 4 && c0 + k < w.cols; k++) o[k] = v[k];
         } else {
             // (3 significant bits times 8: rounded to BF16's 8, halves to even)
-            __align__(16) __nv_bfloat16 h[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) h[k] = __float2bfloat16_rn(v[k]);
             __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(out) + at;
-            if (whole && c0 + 8 <= w.cols) __stcs(reinterpret_cast<uint4 *>(o), *reinterpret_cast<const uint4 *>(h));
-            else
-                for (int k = 0; k < 8 && c0 + k < w.cols; k++) o[k] = h[k];
+            if (whole && c0 + 4 <= w.cols) {
+                __align__(8) const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+                __stcs(reinterpret_cast<uint2 *>(o), *reinterpret_cast<const uint2 *>(h));
+            } else
+                for (int k = 0; k < 4 && c0 + k < w.cols; k++) o[k] = __float2bfloat16_rn(v[k]);
         }
     }
 }
 
 void w4_dequantize(cudaStream_t st, const W4Mat &w, void *out, int dt, size_t ldo)
 {
-    const int pieces = ((w.cols + 7) / 8 + CV_WORDS - 1) / CV_WORDS, size = dt == DT_F32 ? 4 : 2;
+    const unsigned pieces = (w.cols + CV_COLS - 1) / CV_COLS;
+    const int size = dt == DT_F32 ? 4 : 2;
     const long long units = (long long)w.rows * pieces;
     const int grid = (int)((units + CV_WARPS - 1) / CV_WARPS);
-    const bool whole = (reinterpret_cast<uintptr_t>(out) % 16) == 0 && (ldo * size) % 16 == 0;
+    const bool whole = (reinterpret_cast<uintptr_t>(out) % (4 * size)) == 0 && ldo % 4 == 0;
     if (dt == DT_F32) G5B_LAUNCH(w4_dequantize_kernel<DT_F32>, grid, CV_WARPS * 32, 0, st, w, out, ldo, pieces, whole);
     else              G5B_LAUNCH(w4_dequantize_kernel<DT_BF16>, grid, CV_WARPS * 32, 0, st, w, out, ldo, pieces, whole);
 }

@@ -20,7 +20,7 @@
 //             a lane takes its words 16 bytes apart, so that an MMA is 32 columns of one group.
 //   x         becomes digits in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
 //             which the lanes read them: per row and block of 128 columns the power of two below which its values lie, and
-//             integers of 22 bits and a sign in three digits (BF16 rows: 14 bits in two, 2^-15 of the block's largest).
+//             integers of 23 bits and a sign in three digits (BF16 rows: 15 bits in two), one bit less where the largest needs it.
 // Group sums are exact integers, taken into FP32 by the exponent trick (they start at the bits of 1.5 2^23, so that their bits are the
 // float 1.5 2^23 + sum, |sum| < 2^22); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
@@ -87,30 +87,6 @@ __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j ==
 
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// Eight values from column c on, zero behind the last.
-template <typename IN>
-__device__ __forceinline__ void few_load8(float (&v)[8], const IN *row, int c, int cols, bool wide);
-template <>
-__device__ __forceinline__ void few_load8<float>(float (&v)[8], const float *row, int c, int cols, bool wide)
-{
-    if (wide && c + 8 <= cols) {
-        const float4 a = *reinterpret_cast<const float4 *>(row + c), b = *reinterpret_cast<const float4 *>(row + c + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = c + i < cols ? row[c + i] : 0.f;
-}
-template <>
-__device__ __forceinline__ void few_load8<uint16_t>(float (&v)[8], const uint16_t *row, int c, int cols, bool wide)
-{
-    if (wide && c + 8 <= cols) {
-        const uint4 a = *reinterpret_cast<const uint4 *>(row + c);
-        bf16x2_to_f32(a.x, v[0], v[1]); bf16x2_to_f32(a.y, v[2], v[3]); bf16x2_to_f32(a.z, v[4], v[5]); bf16x2_to_f32(a.w, v[6], v[7]);
-    } else
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = c + i < cols ? bf16_to_f32(row[c + i]) : 0.f;
-}
-
 // A block of 128 columns: [part][column][t] 16 bytes of digits as the lanes read them, then for each of the eight columns where the sums
 // start (WHOLE: of the block; else of each 32 columns, with groups of 64 those of both halves in the first) and what a digit stands for.
 template <int NS, bool WHOLE> struct FewBlock {
@@ -135,7 +111,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
         for (int c0 = (warp - i * per) * 256; c0 < a.blocks * 128; c0 += per * 256) {
             const int c = c0 + lane * 8;
             float v[8];
-            few_load8<IN>(v, row, c, a.cols, a.wide);
+            w4_load8(v, row, c, a.cols, a.wide);
             uint32_t m = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
@@ -143,7 +119,10 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
             for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             const bool finite = m < 0x7f800000u;
             // 2^(e - 1) <= max < 2^e (a subnormal one counts as 2^-126)
-            const int e = max((int)(m >> 23), 1) - 126, up = (TERMS == 3 ? 22 : 14) - e;               // -114 <= up <= 147
+            // One more bit where the largest leaves the highest digit below 128.
+            const int e = max((int)(m >> 23), 1) - 126, bits = TERMS == 3 ? 22 : 14;
+            const float most = TERMS == 3 ? 127.0f * 65536.0f + 127.0f * 256.0f + 127.0f : 127.0f * 256.0f + 127.0f;
+            const int up = bits - e + (__uint_as_float(m) * few_pow2((bits + 1 - e) >> 1) * few_pow2(bits + 1 - e - ((bits + 1 - e) >> 1)) <= most);   // -114 <= up <= 148
             const float scale = few_pow2(up >> 1), scale2 = few_pow2(up - (up >> 1));
             uint32_t even[TERMS] = {}, odd[TERMS] = {};  // digits of columns 0 2 4 6 and 1 3 5 7
             int sum[TERMS] = {};
@@ -174,7 +153,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
                     reinterpret_cast<uint2 *>(&b.digits[j >> 1][col + d][t])[j & 1] = make_uint2(even[d], odd[d]);
                     if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = FW_MAGIC - 8 * sum[d];
                 }
-                // (2^-147 at least, a subnormal FP32 number)
+                // (2^-148 at least, a subnormal FP32 number)
                 if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(-(up - (up >> 1))) * (d == 0 ? 1.0f : d == 1 ? 256.0f : 65536.0f)
                                                             : __int_as_float(0x7fc00000);
             }

@@ -549,7 +549,7 @@ int w4_many(cudaStream_t st, const W4Job &j, float *part)
     const cuuint64_t xsize[4] = {64, (cuuint64_t)j.T, (cuuint64_t)j.terms.n_terms, (cuuint64_t)j.terms.kp / 64}, xstride[3] = {row, (cuuint64_t)j.terms.kp * 2, 128};
     const cuuint32_t xbox[4] = {64, (cuuint32_t)a.n, (cuuint32_t)j.terms.n_terms, 2};
     if (!tc_encode_swizzled(&m.w, j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
-        !tc_encode_swizzled(&m.up, j.mode == W4_GATEUP ? j.up.codes : j.w.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B) ||
+        (j.mode == W4_GATEUP && !tc_encode_swizzled(&m.up, j.up.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, wsize, wstride, wbox, CU_TENSOR_MAP_SWIZZLE_64B)) ||
         !tc_encode_swizzled(&m.x, j.terms.terms, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, xsize, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B)) {
         set_last_error("a tensor map of a 4-bit product was refused");
         return -1;

@@ -4,6 +4,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <cuda.h>
+
 #include "common.cuh"
 #include "w4.h"
 
@@ -29,20 +31,46 @@ int launched(const char *op)
     return rc == cudaSuccess ? 0 : fail("%s: launch failed: %s", op, cudaGetErrorString(rc));
 }
 
+// Whether p is memory of the device `dev`: 1 yes, 0 no (`at`: which device's it is, -1 for the host's), -1 unknown. The driver's call takes a
+// fifth of the runtime's 0.35 us, and a product asks about five addresses.
+typedef CUresult (*PointerAttributesFn)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
+int on_device(const void *p, int dev, int &at)
+{
+    static const PointerAttributesFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); f = nullptr; }
+        return reinterpret_cast<PointerAttributesFn>(f);
+    }();
+    unsigned type = 0, managed = 0;
+    int ordinal = -1;
+    CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, CU_POINTER_ATTRIBUTE_IS_MANAGED};
+    void *to[3] = {&type, &ordinal, &managed};
+    at = -1;
+    if (fn && fn(3, what, to, reinterpret_cast<CUdeviceptr>(p)) == CUDA_SUCCESS) {
+        if (managed) return 1;
+        if (type != CU_MEMORYTYPE_DEVICE) return 0;
+        at = ordinal;
+        return ordinal == dev;
+    }
+    cudaPointerAttributes a;                             // (a thread without a context, for instance)
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) { cudaGetLastError(); return -1; }
+    if (a.type == cudaMemoryTypeManaged) return 1;
+    if (a.type != cudaMemoryTypeDevice) return 0;
+    at = a.device;
+    return a.device == dev;
+}
 // Memory of the current device (where the launches go); `align`: what the kernels need of the address.
 int check_ptr(const char *op, const char *what, const void *p, size_t align)
 {
     if (!p) return fail("%s: %s is null", op, what);
     if (reinterpret_cast<uintptr_t>(p) % align) return fail("%s: %s must lie on a multiple of %zu bytes", op, what, align);
-    cudaPointerAttributes at;
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();
-        return fail("%s: no usable current CUDA device", op);
-    }
-    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) return fail("%s: %s is not device memory", op, what);
-    if (at.type == cudaMemoryTypeDevice && at.device != dev) return fail("%s: %s lies on device %d, the current one is %d", op, what, at.device, dev);
-    return 0;
+    int dev = -1, at = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return fail("%s: no usable current CUDA device", op); }
+    const int here = on_device(p, dev, at);
+    if (here == 1) return 0;
+    if (here < 0) return fail("%s: no usable current CUDA device", op);
+    return at < 0 ? fail("%s: %s is not device memory", op, what) : fail("%s: %s lies on device %d, the current one is %d", op, what, at, dev);
 }
 int elt(int dt) { return dt == DT_F32 ? 4 : 2; }
 int check_dtype(const char *op, int dt) { return dt == DT_F32 || dt == DT_BF16 ? 0 : fail("%s: rows are F32 or BF16, not dtype %d", op, dt); }
