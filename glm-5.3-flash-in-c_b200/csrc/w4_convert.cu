@@ -5,7 +5,7 @@
 // does, which is exact there (q s has 12 significant bits; within half a step of it the difference loses none). A
 // division instead is twenty instructions a weight, as many as the SM can issue while HBM delivers an FP8 weight.
 //
-// Both directions are bound by HBM, the first nearly by the instructions a weight takes (14). There a lane takes 32 columns, so that what
+// Both directions are bound by HBM, the first nearly by the instructions a weight takes (9). There a lane takes 32 columns, so that what
 // is paid per group - the division, the reciprocal, the maximum's shuffles - is paid once for 32 weights, and its codes are one store;
 // eight columns a lane paid it four times, converted to integers by the slow instruction, and took 72 us for 12288 x 4096 BF16 weights.
 #include "w4.cuh"
@@ -82,20 +82,34 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
     const bool live = finite && s > 0.f;
     // 1 / s of a small s may be infinite: the quotient is then taken of both times 2^64
     const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
+    // Rounded by adding 1.5 2^23 + 8, in whose low bits the code then lies; eight codes are put together by multiplications, the same pipe. A
+    // quotient over 7.5 (of a scale rounded to a few bits) and residuals from half a step on take the long way, eight weights at a time.
+    constexpr float MAGIC = 12582912.0f + 8.0f;
+    constexpr uint32_t MAGIC_BITS = 0x4b400000u, ONES = 0x11111111u;
+    const bool clamp = __uint_as_float(m) * up > 7.5f * su;
     __align__(16) uint32_t packed[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        packed[i] = live ? 0u : 0x88888888u;
-        if (live)
+        uint32_t word = 0u - MAGIC_BITS * ONES;
+        float far = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float x = v[i][k] * up, t = fmaf(x, r, MAGIC), q = t - MAGIC;
+            far = fmaxf(far, fabsf(fmaf(-q, su, x)));
+            word += __float_as_uint(t) << (4 * k);
+        }
+        if (clamp || far >= half) {
+            word = 0u;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                // rounded by adding 1.5 2^23, in whose low bits the integer (and whether it is odd) then lies; |w / s| <= 10 (a subnormal scale)
-                const float x = v[i][k] * up, t = fmaf(x, r, 12582912.0f), q = t - 12582912.0f, d = fmaf(-q, su, x), ad = fabsf(d);
-                int n = __float_as_int(t) - 0x4b400000;
+                const float x = v[i][k] * up, t = fmaf(x, r, MAGIC), q = t - MAGIC, d = fmaf(-q, su, x), ad = fabsf(d);
+                int n = (int)(__float_as_uint(t) - MAGIC_BITS);                   // the code
                 // one step on where the residual is over half a step, or half a step and the integer odd
                 if (ad > half || (ad == half && (n & 1))) n += d > 0.f ? 1 : -1;
-                packed[i] |= (uint32_t)(min(max(n, -7), 7) + 8) << (4 * k);
+                word |= (uint32_t)min(max(n, 1), 15) << (4 * k);
             }
+        }
+        packed[i] = live ? word : 0x88888888u;
     }
     if (c0 / 2 < w.pitch) *reinterpret_cast<uint4 *>(codes + (size_t)row * w.pitch + c0 / 2) = *reinterpret_cast<const uint4 *>(packed);
     const int group = c0 / w.group;
