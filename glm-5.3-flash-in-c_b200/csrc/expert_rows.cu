@@ -10,6 +10,8 @@
 // experts is that of the picks), counts become first places by sums over warps, CTAs and experts, and a second pass over the
 // stretch places the picks. One launch: a CTA alone up to SORT_ALONE picks, beyond a cluster of eight whose CTAs read each
 // other's counts through distributed shared memory. Bound by the latency of those steps.
+#include <type_traits>
+
 #include "common.cuh"
 #include "w4.h"
 
@@ -23,8 +25,8 @@ __device__ __forceinline__ int ld_cluster_s32(const int *p, uint32_t rank)
 {
     uint32_t theirs;
     int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(theirs) : "memory");
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(theirs));
     return v;
 }
 
@@ -64,8 +66,11 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
     __syncthreads();
     // places of the warps within the CTA, and the CTA's sum
     for (int e = tid; e < E; e += SORT_THREADS) {
-        int sum = 0;
-        for (int w = 0; w < SORT_WARPS; w++) { const int c = count[w * E + e]; count[w * E + e] = sum; sum += c; }
+        int sum = 0, c[SORT_WARPS];
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; w++) c[w] = count[w * E + e];
+#pragma unroll
+        for (int w = 0; w < SORT_WARPS; w++) { count[w * E + e] = sum; sum += c[w]; }
         total[e] = sum;
     }
     if (ctas > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
@@ -74,10 +79,16 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
     int before[2] = {0, 0}, all[2] = {0, 0};
     for (int i = 0; i < 2; i++)
         if (e0 + i < E)
-            for (int r = 0; r < ctas; r++) {
-                const int c = ctas > 1 ? ld_cluster_s32(total + e0 + i, (uint32_t)r) : total[e0 + i];
-                all[i] += c;
-                if (r < rank) before[i] += c;
+            if (ctas == 1) all[i] = total[e0 + i];
+            else {
+                int c[SORT_CLUSTER];                            // (asked for together)
+#pragma unroll
+                for (int r = 0; r < SORT_CLUSTER; r++) c[r] = ld_cluster_s32(total + e0 + i, (uint32_t)r);
+#pragma unroll
+                for (int r = 0; r < SORT_CLUSTER; r++) {
+                    all[i] += c[r];
+                    if (r < rank) before[i] += c[r];
+                }
             }
     // sums over the experts: of the picks, and of the tiles they make
     const int rows = slots.n ? slots.rows : 1;
@@ -146,18 +157,24 @@ int expert_sort(cudaStream_t st, const int *idx, int T, int topk, int E, int *or
     return cudaLaunchKernelEx(&cfg, expert_sort_kernel, idx, n, E, ctas, order, place, offsets, slots ? *slots : none) == cudaSuccess ? 0 : -1;
 }
 
-// One CTA per sorted row. PIECE: bytes of one load
+// Rows one after the other by CTAs that fill the GPU once (a CTA for each of 16384 picks, of which 2048 were here, took 14 us). PIECE:
+// bytes of one load, four of which a thread has on their way.
 template <typename PIECE>
 __global__ void __launch_bounds__(256) expert_gather_kernel(const uint8_t *x, size_t row_bytes, size_t ldx, size_t ldr, const int *order,
                                                             const int *offsets, int topk, int E, uint8_t *rows)
 {
-    const int i = blockIdx.x;
-    if (i >= __ldg(offsets + E)) return;
-    const PIECE *src = reinterpret_cast<const PIECE *>(x + (size_t)(__ldg(order + i) / topk) * ldx);
-    PIECE *dst = reinterpret_cast<PIECE *>(rows + (size_t)i * ldr);
-    const int pieces = (int)(row_bytes / sizeof(PIECE));
-#pragma unroll 4
-    for (int c = threadIdx.x; c < pieces; c += 256) dst[c] = __ldg(src + c);
+    const int n = __ldg(offsets + E), pieces = (int)(row_bytes / sizeof(PIECE));
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const PIECE *src = reinterpret_cast<const PIECE *>(x + (size_t)(__ldg(order + i) / topk) * ldx);
+        PIECE *dst = reinterpret_cast<PIECE *>(rows + (size_t)i * ldr);
+        for (int c0 = threadIdx.x; c0 < pieces; c0 += 1024) {
+            PIECE v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) if (c0 + 256 * k < pieces) v[k] = __ldg(src + c0 + 256 * k);
+#pragma unroll
+            for (int k = 0; k < 4; k++) if (c0 + 256 * k < pieces) dst[c0 + 256 * k] = v[k];
+        }
+    }
 }
 
 void expert_gather(cudaStream_t st, const void *x, size_t row_bytes, size_t x_bytes, size_t out_bytes, const int *order, const int *offsets,
@@ -166,9 +183,10 @@ void expert_gather(cudaStream_t st, const void *x, size_t row_bytes, size_t x_by
     const size_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows) | row_bytes | x_bytes | out_bytes;
     const uint8_t *src = static_cast<const uint8_t *>(x);
     uint8_t *dst = static_cast<uint8_t *>(rows);
-    if (all % 16 == 0) G5B_LAUNCH(expert_gather_kernel<uint4>, n, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
-    else if (all % 4 == 0) G5B_LAUNCH(expert_gather_kernel<uint32_t>, n, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
-    else G5B_LAUNCH(expert_gather_kernel<uint16_t>, n, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
+    const int grid = n < 8 * dev_sms() ? n : 8 * dev_sms();
+    if (all % 16 == 0) G5B_LAUNCH(expert_gather_kernel<uint4>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
+    else if (all % 4 == 0) G5B_LAUNCH(expert_gather_kernel<uint32_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
+    else G5B_LAUNCH(expert_gather_kernel<uint16_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
 }
 
 __device__ __forceinline__ float row_value(const float *p) { return *p; }
@@ -176,35 +194,51 @@ __device__ __forceinline__ float row_value(const uint16_t *p) { return bf16_to_f
 __device__ __forceinline__ void row_store(float *p, float v) { *p = v; }
 __device__ __forceinline__ void row_store(uint16_t *p, float v) { *p = __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 
-// A CTA: one token, 256 * V columns. V values of a row are one load.
-template <typename IN, typename OUT, int V>
+// A CTA: one token, up to 256 * V * CH columns. V values of a row are one load, CH of which a thread has on their way for each pick.
+template <typename IN, typename OUT, int V, int CH>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, size_t ldr, const int *place, int E, const float *w, int topk, int cols,
                                                              OUT *out, size_t ldo)
 {
+    __shared__ int s_at[G5B_MAX_TOPK];
+    __shared__ float s_w[G5B_MAX_TOPK];
     pdl_wait();
     struct __align__(sizeof(IN) * V) InV { IN v[V]; };
     struct __align__(sizeof(OUT) * V) OutV { OUT v[V]; };
-    const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
-    if (c >= cols) return;
-    const int *at = place + (size_t)t * topk;
-    const float *wt = w ? w + (size_t)t * topk : nullptr;
-    float sum[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) sum[i] = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < topk; k++) {
-        int p = __ldg(at + k);
-        if (E) p = p >= 0 && p < E ? t * topk + k : -1;
-        if (p < 0) continue;
-        const float f = wt ? __ldg(wt + k) : 1.0f;
-        const InV in = *reinterpret_cast<const InV *>(rows + (size_t)p * ldr + c);
-#pragma unroll
-        for (int i = 0; i < V; i++) sum[i] = fmaf(f, row_value(&in.v[i]), sum[i]);
+    const int t = blockIdx.x, c0 = (blockIdx.y * 256 * CH + threadIdx.x) * V;
+    if (threadIdx.x < topk) {
+        int p = __ldg(place + (size_t)t * topk + threadIdx.x);
+        if (E) p = p >= 0 && p < E ? t * topk + (int)threadIdx.x : -1;
+        s_at[threadIdx.x] = p;
+        s_w[threadIdx.x] = w ? __ldg(w + (size_t)t * topk + threadIdx.x) : 1.0f;
     }
-    OutV o;
+    __syncthreads();
+    float sum[CH][V];
 #pragma unroll
-    for (int i = 0; i < V; i++) row_store(&o.v[i], sum[i]);
-    *reinterpret_cast<OutV *>(out + (size_t)t * ldo + c) = o;
+    for (int q = 0; q < CH; q++)
+#pragma unroll
+        for (int i = 0; i < V; i++) sum[q][i] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < topk; k++) {
+        const int p = s_at[k];
+        if (p < 0) continue;
+        const float f = s_w[k];
+        const IN *row = rows + (size_t)p * ldr + c0;
+        InV in[CH];
+#pragma unroll
+        for (int q = 0; q < CH; q++) if (c0 + q * 256 * V < cols) in[q] = *reinterpret_cast<const InV *>(row + q * 256 * V);
+#pragma unroll
+        for (int q = 0; q < CH; q++)
+#pragma unroll
+            for (int i = 0; i < V; i++) sum[q][i] = fmaf(f, row_value(&in[q].v[i]), sum[q][i]);
+    }
+#pragma unroll
+    for (int q = 0; q < CH; q++) {
+        if (c0 + q * 256 * V >= cols) continue;
+        OutV o;
+#pragma unroll
+        for (int i = 0; i < V; i++) row_store(&o.v[i], sum[q][i]);
+        *reinterpret_cast<OutV *>(out + (size_t)t * ldo + c0 + q * 256 * V) = o;
+    }
 }
 
 template <typename IN, typename OUT>
@@ -215,10 +249,17 @@ static void combine_as(cudaStream_t st, const void *rows, size_t ldr, const int 
     OUT *o = static_cast<OUT *>(out);
     const bool wide = reinterpret_cast<uintptr_t>(rows) % (V * sizeof(IN)) == 0 && reinterpret_cast<uintptr_t>(out) % (V * sizeof(OUT)) == 0 &&
                       ldr % V == 0 && ldo % V == 0 && cols % V == 0;
-    const dim3 grid(T, (cols + 256 * (wide ? V : 1) - 1) / (256 * (wide ? V : 1)));
-    if (wide && early)  G5B_LAUNCH_PDL((expert_combine_kernel<IN, OUT, V>), grid, dim3(256), 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
-    else if (wide)      G5B_LAUNCH((expert_combine_kernel<IN, OUT, V>), grid, 256, 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
-    else                G5B_LAUNCH((expert_combine_kernel<IN, OUT, 1>), grid, 256, 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
+    // few tokens: a load a thread and pick, so that more CTAs share a row
+    auto launch = [&](auto v, auto ch) {
+        constexpr int W = decltype(v)::value, CH = decltype(ch)::value;
+        const dim3 grid(T, (cols + 256 * W * CH - 1) / (256 * W * CH));
+        if (early) G5B_LAUNCH_PDL((expert_combine_kernel<IN, OUT, W, CH>), grid, dim3(256), 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
+        else       G5B_LAUNCH((expert_combine_kernel<IN, OUT, W, CH>), grid, 256, 0, st, in, ldr, place, E, w, topk, cols, o, ldo);
+    };
+    using std::integral_constant;
+    if (!wide) launch(integral_constant<int, 1>(), integral_constant<int, 1>());
+    else if (T <= 256) launch(integral_constant<int, V>(), integral_constant<int, 1>());
+    else launch(integral_constant<int, V>(), integral_constant<int, 16 / V>());
 }
 
 void expert_combine(cudaStream_t st, const void *rows, int rows_dt, size_t ldr, const int *place, int E, const float *w, int T, int topk, int cols,

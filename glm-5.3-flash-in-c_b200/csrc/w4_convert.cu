@@ -80,13 +80,14 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
     const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
     const float s = __bfloat162float(sb);
     const bool live = finite && s > 0.f;
-    // 1 / s of a small s may be infinite: the quotient is then taken of both times 2^64
-    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
+    // 1 / s of a small s may be infinite: the quotient is then taken of both times 2^64 (the long way)
+    const bool tiny = s < 0x1p-100f;
+    const float up = tiny ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
     // Rounded by adding 1.5 2^23 + 8, in whose low bits the code then lies; eight codes are put together by multiplications, the same pipe. A
     // quotient over 7.5 (of a scale rounded to a few bits) and residuals from half a step on take the long way, eight weights at a time.
     constexpr float MAGIC = 12582912.0f + 8.0f;
     constexpr uint32_t MAGIC_BITS = 0x4b400000u, ONES = 0x11111111u;
-    const bool clamp = __uint_as_float(m) * up > 7.5f * su;
+    const bool clamp = tiny || __uint_as_float(m) > 7.5f * s;
     __align__(16) uint32_t packed[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -94,8 +95,8 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
         float far = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const float x = v[i][k] * up, t = fmaf(x, r, MAGIC), q = t - MAGIC;
-            far = fmaxf(far, fabsf(fmaf(-q, su, x)));
+            const float t = fmaf(v[i][k], r, MAGIC), q = t - MAGIC;
+            far = fmaxf(far, fabsf(fmaf(-q, su, v[i][k])));
             word += __float_as_uint(t) << (4 * k);
         }
         if (clamp || far >= half) {
