@@ -161,11 +161,13 @@ int expert_sort(cudaStream_t st, const int *idx, int T, int topk, int E, int *or
 // bytes of one load, four of which a thread has on their way.
 template <typename PIECE>
 __global__ void __launch_bounds__(256) expert_gather_kernel(const uint8_t *x, size_t row_bytes, size_t ldx, size_t ldr, const int *order,
-                                                            const int *offsets, int topk, int E, uint8_t *rows)
+                                                            const int *offsets, int picks, int topk, int E, uint8_t *rows)
 {
-    const int n = __ldg(offsets + E), pieces = (int)(row_bytes / sizeof(PIECE));
+    const int n = min(__ldg(offsets + E), picks), pieces = (int)(row_bytes / sizeof(PIECE));
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const PIECE *src = reinterpret_cast<const PIECE *>(x + (size_t)(__ldg(order + i) / topk) * ldx);
+        const int p = __ldg(order + i);
+        if (p < 0 || p >= picks) continue;                      // (not an order that the sort wrote)
+        const PIECE *src = reinterpret_cast<const PIECE *>(x + (size_t)(p / topk) * ldx);
         PIECE *dst = reinterpret_cast<PIECE *>(rows + (size_t)i * ldr);
         for (int c0 = threadIdx.x; c0 < pieces; c0 += 1024) {
             PIECE v[4];
@@ -184,9 +186,9 @@ void expert_gather(cudaStream_t st, const void *x, size_t row_bytes, size_t x_by
     const uint8_t *src = static_cast<const uint8_t *>(x);
     uint8_t *dst = static_cast<uint8_t *>(rows);
     const int grid = n < 8 * dev_sms() ? n : 8 * dev_sms();
-    if (all % 16 == 0) G5B_LAUNCH(expert_gather_kernel<uint4>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
-    else if (all % 4 == 0) G5B_LAUNCH(expert_gather_kernel<uint32_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
-    else G5B_LAUNCH(expert_gather_kernel<uint16_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, topk, E, dst);
+    if (all % 16 == 0) G5B_LAUNCH(expert_gather_kernel<uint4>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, n, topk, E, dst);
+    else if (all % 4 == 0) G5B_LAUNCH(expert_gather_kernel<uint32_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, n, topk, E, dst);
+    else G5B_LAUNCH(expert_gather_kernel<uint16_t>, grid, 256, 0, st, src, row_bytes, x_bytes, out_bytes, order, offsets, n, topk, E, dst);
 }
 
 __device__ __forceinline__ float row_value(const float *p) { return *p; }
@@ -208,6 +210,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, siz
     if (threadIdx.x < topk) {
         int p = __ldg(place + (size_t)t * topk + threadIdx.x);
         if (E) p = p >= 0 && p < E ? t * topk + (int)threadIdx.x : -1;
+        else if (p >= (int)gridDim.x * topk) p = -1;            // (not a place that the sort wrote)
         s_at[threadIdx.x] = p;
         s_w[threadIdx.x] = w ? __ldg(w + (size_t)t * topk + threadIdx.x) : 1.0f;
     }

@@ -31,8 +31,8 @@ int launched(const char *op)
     return rc == cudaSuccess ? 0 : fail("%s: launch failed: %s", op, cudaGetErrorString(rc));
 }
 
-// Whether p is memory of the device `dev`: 1 yes, 0 no (`at`: which device's it is, -1 for the host's), -1 unknown. The driver's call takes a
-// fifth of the runtime's 0.35 us, and a product asks about five addresses.
+// Whether p is memory of the device `dev`: 1 yes, 0 no (`at`: which device's it is, -1 for the host's), -1 unknown. Asked of the
+// driver: 0.04 us less an address than the runtime's call, and a product asks about five.
 typedef CUresult (*PointerAttributesFn)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
 int on_device(const void *p, int dev, int &at)
 {

@@ -437,7 +437,7 @@ int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *s
 
 /* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Products are exact, sums FP32 or
  * exact integers. An F32 activation is held to 2^-22 of the largest of the 128 columns it lies in (from a multiple of 128 on) or
- * better; a BF16 one to 2^-14 of it in calls of a few rows, which is a sixteenth of what rounding to BF16 takes, else exactly. A row
+ * better; a BF16 one to 2^-14 of it in calls of a few rows (one that is the largest keeps 2^-8 of itself as BF16), else exactly. A row
  * of x with an infinity or NaN gives NaN in all of its outputs. */
 size_t g5b_w4_matmul_workspace(const g5b_w4 *w, int dtype, int T);
 int g5b_w4_matmul(const g5b_w4 *w, const void *x, int dtype, int T, size_t ldx, void *y, size_t ldy, void *workspace,
@@ -449,11 +449,12 @@ int g5b_w4_matmul(const g5b_w4 *w, const void *x, int dtype, int T, size_t ldx, 
  * the first position of every expert, and last their number. */
 int g5b_expert_sort(const int32_t *idx, int T, int topk, int n_experts, int32_t *order, int32_t *place, int32_t *offsets,
                     void *stream);
-/* rows[i] = x[order[i] / topk] for the offsets[n_experts] sorted picks; rows behind them stay as they were. */
+/* rows[i] = x[order[i] / topk] for the offsets[n_experts] sorted picks; rows behind them stay as they were, and so do those
+ * whose order is no pick's number. */
 int g5b_expert_gather(const void *x, int dtype, int T, int cols, size_t ldx, const int32_t *order, const int32_t *offsets,
                       int topk, int n_experts, void *rows, size_t ldr, void *stream);
 /* out[t] = sum over k of weights[t][k] * rows[place[t][k]], in FP32 in the order of k; a pick left out adds nothing, a token
- * without picks is zero. weights NULL: all one. */
+ * without picks is zero. weights NULL: all one. A place outside [0, T * topk) is a pick left out. */
 int g5b_expert_combine(const void *rows, int dtype, size_t ldr, const int32_t *place, const float *weights, int T, int topk,
                        int cols, void *out, size_t ldo, void *stream);
 

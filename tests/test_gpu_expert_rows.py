@@ -81,6 +81,41 @@ def test_gather_and_combine(gpu_lib, T, K, E, cols, pad, how, dtype):
         assert bool((out.cpu()[:, cols:] == 2.0).all())
 
 
+def test_numbers_far_outside(gpu_lib):
+    """The smallest and largest integers are nobody's experts; orders and places that no sort wrote are left out."""
+    big, small = 2 ** 31 - 1, -2 ** 31
+    idx = torch.tensor([[big, 0], [small, -1], [1, 2]], dtype=torch.int32)
+    for got, want in zip(_sort(idx, 2), _sorted(idx, 2)):
+        assert torch.equal(got.cpu(), want)
+    x = torch.arange(3 * 8, dtype=torch.float32).view(3, 8).cuda()
+    rows = torch.full((6, 8), 5.0, device="cuda")
+    t = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")       # noqa: E731
+    pkg.expert_gather(x, t(4, big, small, 6, -1, 0), t(0, 100), rows)
+    assert torch.equal(rows[0], x[2]) and torch.equal(rows[5], x[0]) and bool((rows[1:5] == 5.0).all())
+    out = torch.full((3, 8), 9.0, device="cuda")
+    pkg.expert_combine(rows, t(0, big, small, 6, 5, -7).view(3, 2), None, out)
+    assert torch.equal(out[0], rows[0]) and bool((out[1] == 0).all()) and torch.equal(out[2], rows[5])
+
+
+@pytest.mark.parametrize("K", [1, 64])
+def test_no_tokens_and_many_picks(gpu_lib, K):
+    E = 3
+    none = torch.zeros((0, K), dtype=torch.int32)
+    order, place, offsets = _sort(none, E)
+    assert offsets.cpu().tolist() == [0] * (E + 1)
+    idx = _picks(torch.Generator().manual_seed(K), 5, K, E, "outside")
+    order, place, offsets = _sort(idx, E)
+    x = torch.randn((5, 40), generator=torch.Generator().manual_seed(1)).cuda()
+    rows = torch.zeros((5 * K, 40), device="cuda")
+    pkg.expert_gather(x, order, offsets, rows)
+    out = torch.empty_like(x)
+    pkg.expert_combine(rows, place, None, out)
+    here = ((idx >= 0) & (idx < E)).sum(1).double()
+    # every pick of a token has the token's own row: K sums, each off by half of 2^-23 of at most the whole
+    want = x.cpu().double() * here[:, None]
+    assert bool(((out.cpu().double() - want).abs() <= want.abs() * K * 2.0 ** -24).all())
+
+
 def test_combine_does_not_read_rows_left_out(gpu_lib):
     """NaN in the rows of picks that are not here, and weights that are not numbers beside them, reach nothing."""
     idx = torch.tensor([[0, -1, 2], [5, 9, -7]], dtype=torch.int32)
@@ -124,6 +159,25 @@ def test_experts(gpu_lib, T, K, E, H, I, group, limit, how, dtype):
     want, off = ref.experts(x.double(), idx, weights, g, u, d, limit, dtype == torch.float32)
     worst = ((got.double() - want).abs() / (off + ref.rounded(want, dtype))).max()
     assert worst <= 1.0, float(worst)
+
+
+def test_experts_without_numbers_and_far_outside(gpu_lib):
+    """A token with an infinity is NaN, its neighbours are not; picks far outside add nothing; a token without picks is zero."""
+    rng = torch.Generator().manual_seed(21)
+    E, H, I = 5, 96, 64
+    (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, 32), _stack(rng, E, I, H, 32), _stack(rng, E, H, I, 32)
+    for T in (3, 12, 60):                                  # picks one by one, a few rows to an expert, many
+        idx = torch.randint(0, E, (T, 2), generator=rng, dtype=torch.int32)
+        idx[0] = torch.tensor([2 ** 31 - 1, -2 ** 31])
+        x = torch.randn((T, H), generator=rng)
+        x[1, 5] = float("inf")
+        weights = torch.rand((T, 2), generator=rng)
+        got = _experts((gate, up, down), x.cuda(), idx, weights, 10.0)
+        assert bool((got[0] == 0).all()) and bool(torch.isnan(got[1]).all())
+        want, off = ref.experts(x[2:].double(), idx[2:], weights[2:], g, u, d, 10.0, True)
+        assert bool(((got[2:].double() - want).abs() <= off + ref.rounded(want, torch.float32)).all())
+    none = torch.zeros((0, 2), dtype=torch.int32)
+    assert _experts((gate, up, down), torch.zeros((0, H), device="cuda"), none, torch.zeros((0, 2)), 10.0).shape == (0, H)
 
 
 def test_a_checkpoint_expert_layer_in_four_bits(gpu_lib):

@@ -45,6 +45,65 @@ def test_product(gpu_lib, rows, cols, group, T, dtype):
     _check(_run(codes, scales, rows, cols, group, x.cuda(), pad=T % 3), ref.values(codes, scales, cols, group), x)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,group", [(33, 128, 32), (260, 640, 64), (144, 1100, 128), (50, 4224, 32), (300, 8192, 128), (20, 16384, 64)])
+def test_small_integers_come_out_exactly(gpu_lib, rows, cols, group, dtype):
+    """Integers, and scales that are powers of two: every product and sum is a number that FP32 holds, so whatever the order of additions
+    the result is the integer one. |x| <= 8, |code - 8| <= 8, scales from 1 to 8 and 16384 columns: below 2^23."""
+    rng = torch.Generator().manual_seed(rows)
+    codes, scales = ref.make(rng, rows, cols, group)
+    groups = -(-cols // group)
+    scales[:, :groups] = torch.exp2(torch.randint(0, 4, (rows, groups), generator=rng).float()).to(torch.bfloat16)
+    w = ref.values(codes, scales, cols, group)
+    for T in (1, 2, 3, 4, 5, 16, 17, 33, 64, 65, 129):
+        x = torch.randint(-8, 9, (T, cols), generator=rng).to(dtype)
+        y = _run(codes, scales, rows, cols, group, x.cuda())
+        want = x.double() @ w.t()
+        assert torch.equal(y.double(), want.to(dtype).double()), T
+
+
+@pytest.mark.parametrize("T", [1, 4, 30, 100])
+def test_zero_weights_give_zero(gpu_lib, T):
+    rows, cols, group = 70, 500, 32
+    codes, scales = ref.make(torch.Generator().manual_seed(1), rows, cols, group)
+    codes[:] = 0x88
+    codes[3, 7] = 0x98                                      # one weight (row 3, column 15) that is not
+    x = torch.randn((T, cols), generator=torch.Generator().manual_seed(2)) * 1e3
+    y = _run(codes, scales, rows, cols, group, x.cuda())
+    keep = torch.arange(rows) != 3
+    assert bool((y[:, keep] == 0).all())
+    _check(y, ref.values(codes, scales, cols, group), x)
+
+
+def test_no_rows(gpu_lib):
+    codes, scales = ref.make(torch.Generator().manual_seed(1), 8, 64, 32)
+    y = _run(codes, scales, 8, 64, 32, torch.zeros((0, 64), device="cuda"))
+    assert y.shape == (0, 8)
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_matrix_over_four_gigabytes(gpu_lib, T):
+    """Rows on both sides of 2^31 and 2^32 bytes of codes, and the last ones."""
+    rows, cols, group = (1 << 20) + 4101, 8448, 128
+    pitch, sp = pkg.w4_pitch(cols), pkg.w4_scale_pitch(cols, group)
+    codes = torch.full((rows, pitch), 0x88, dtype=torch.uint8, device="cuda")
+    scales = torch.ones((rows, sp), dtype=torch.bfloat16, device="cuda")
+    rng = torch.Generator().manual_seed(9)
+    at = sorted({0, 1, (1 << 31) // pitch, (1 << 31) // pitch + 1, (1 << 32) // pitch, (1 << 32) // pitch + 1, rows - 2, rows - 1})
+    some = torch.randint(0, 256, (len(at), pitch), generator=rng, dtype=torch.int32).to(torch.uint8)
+    codes[at] = some.cuda()
+    x = torch.randint(-4, 5, (T, cols), generator=rng).float()
+    w = pkg.W4(codes, scales, rows, cols, group)
+    y = torch.empty((T, rows), device="cuda")
+    ws = torch.empty(pkg.w4_matmul_workspace(w, x.cuda()), dtype=torch.uint8, device="cuda")
+    pkg.w4_matmul(w, x.cuda(), y, ws)
+    pkg.w4_status()
+    want = x.double() @ ref.values(some, torch.ones((len(at), sp), dtype=torch.bfloat16), cols, group).t()
+    assert torch.equal(y[:, at].cpu().double(), want)
+    y[:, at] = 0
+    assert int(y.count_nonzero()) == 0
+
+
 @pytest.mark.parametrize("T", [1, 7, 40, 150])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_apart_and_off_every_alignment(gpu_lib, dtype, T):

@@ -110,3 +110,21 @@ def test_python_checks():
         pkg.expert_sort(idx, 3, idx.flatten(), idx, torch.zeros(3, dtype=torch.int32), stream=0)
     with pytest.raises(ValueError):
         pkg.expert_gather(torch.zeros((4, 8)), idx.flatten(), torch.zeros(4, dtype=torch.int32), torch.zeros((8, 9)), stream=0)
+
+
+def test_experts_refusals():
+    """Matrices that do not belong together, limits that are none, workspaces that are too small: before anything is launched."""
+    L, a = pkg.lib(), 1 << 20
+    m = lambda rows, cols, group=32, count=4: C.byref(_w4(a, a, rows, cols, group, count))       # noqa: E731
+
+    def call(gate, up, down, limit=10.0, topk=2, T=1, dtype=0, ld=64):
+        return L.g5b_w4_experts(gate, up, down, a, dtype, T, ld, a, a, topk, limit, a, ld, a, 1 << 30, None)
+    # (without a device the addresses are refused first: then only that they are refused can be seen)
+    device = L.g5b_device_count() > 0
+    for args, kw, word in (((m(32, 64), m(32, 64, 64), m(64, 32)), {}, "belong together"), ((m(32, 64), m(33, 64), m(64, 32)), {}, "belong together"),
+                           ((m(32, 64), m(32, 64), m(64, 33)), {}, "belong together"), ((m(32, 64), m(32, 64, 32, 3), m(64, 32)), {}, "matrices"),
+                           ((m(32, 64), m(32, 64), m(64, 32)), {"limit": 0.0}, "limit"), ((m(32, 64), m(32, 64), m(64, 32)), {"limit": float("nan")}, "limit"),
+                           ((m(32, 64), m(32, 64), m(64, 32)), {"topk": 65}, "picks"), ((m(32, 64), m(32, 64), m(64, 32)), {"ld": 63}, "apart"),
+                           ((m(32, 64), m(32, 64), m(64, 32)), {"dtype": 2}, "dtype")):
+        assert call(*args, **kw) == -1
+        assert not device or word in _err() or "device" in _err()
