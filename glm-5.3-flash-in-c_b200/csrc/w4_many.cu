@@ -175,7 +175,6 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
     __shared__ float s_down[WM_RING][2][128];               // what takes a row's power of two off again
     int *err = &g_many_err;
 
-    pdl_trigger();
     if (threadIdx.x == 0) {
         for (int i = 0; i < WS; i++) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
         for (int i = 0; i < XS; i++) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 2); }
@@ -189,6 +188,7 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_trigger();                                          // (only now: whatever starts early may want tensor memory of its own, and this kernel has it)
     const uint32_t tmem = s_tmem;
     // sums of block b, accumulator i: columns 128 b + 64 i; converted block b of stage s: columns 256 + 128 s + 64 b
     if (a.mode != W4_DENSE) pdl_wait();                     // (the slots are another kernel's)

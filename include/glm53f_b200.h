@@ -435,10 +435,11 @@ int g5b_w4_quantize(const g5b_tensor *src, int br, int bc, const g5b_w4 *dst, vo
 /* The values of a matrix: out [rows][cols] of dtype, BF16 rounded to nearest. */
 int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *stream);
 
-/* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Products are exact, sums FP32 or
- * exact integers. An F32 activation is held to 2^-22 of the largest of the 128 columns it lies in (from a multiple of 128 on) or
- * better; a BF16 one to 2^-14 of it in calls of a few rows (one that is the largest keeps 2^-8 of itself as BF16), else exactly. A row
- * of x with an infinity or NaN gives NaN in all of its outputs. */
+/* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Sums are FP32 or exact integers. What an activation
+ * is held to: in calls of a few rows 2^-22 (BF16 rows 2^-14) of the largest of the 128 columns it lies in, from a multiple of 128 on, or
+ * better; in calls of many rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
+ * scales within 128 columns differ by more than 2^28 has products off by up to 2^-36 of the largest scale times the
+ * activation; all others are exact. A row of x with an infinity or NaN gives NaN in all of its outputs. */
 size_t g5b_w4_matmul_workspace(const g5b_w4 *w, int dtype, int T);
 int g5b_w4_matmul(const g5b_w4 *w, const void *x, int dtype, int T, size_t ldx, void *y, size_t ldy, void *workspace,
                   size_t workspace_bytes, void *stream);

@@ -62,6 +62,45 @@ def test_small_integers_come_out_exactly(gpu_lib, rows, cols, group, dtype):
         assert torch.equal(y.double(), want.to(dtype).double()), T
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [1, 4, 30, 100])
+def test_small_columns_beside_large_ones(gpu_lib, T, dtype):
+    """The first 128 columns of x are 2^24 times the others and have zero weights. What many rows are held to is 2^-38 of the row's
+    largest then (half a step of 2^-24 beside at least 2^13), which is above 2^-22 of the others."""
+    rows, cols, group = 50, 384, 64
+    rng = torch.Generator().manual_seed(T)
+    codes, scales = ref.make(rng, rows, cols, group)
+    codes[:, :64] = 0x88
+    x = torch.randn((T, cols), generator=rng)
+    x[:, :128] *= 2.0 ** 24
+    x = x.to(dtype)
+    w, xd = ref.values(codes, scales, cols, group), x.double()
+    y, want = _run(codes, scales, rows, cols, group, x.cuda()).double(), xd @ w.t()
+    off = ref.product_bound(w, xd, dtype == torch.float32) + ref.rounded(want, dtype) + 2.0 ** -38 * xd.abs().amax(1)[:, None] * w.abs().sum(1)
+    assert bool(((y - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("T", [1, 4, 30, 100])
+def test_scales_far_apart(gpu_lib, T, group, dtype):
+    """Neighbouring groups' scales from 1 down to 2^-12 (exact), 2^-27 (exact), or 2^-40 of each other, the large ones' weights zero: 2^-36 of
+    the largest scale (half a step of F16's 2^-24 beside 2^11 at least) is what a product may then be off in many rows."""
+    rows, cols = 96, 256
+    rng = torch.Generator().manual_seed(T + group)
+    codes, scales = ref.make(rng, rows, cols, group)
+    at = torch.arange(cols // group) % 2 == 1
+    ratio = 2.0 ** -torch.tensor([12.0, 27.0, 40.0])[torch.arange(rows) % 3]
+    scales[:, :cols // group] = torch.where(at[None], ratio[:, None].expand(rows, cols // group), torch.ones(rows, cols // group)).to(torch.bfloat16)
+    codes.view(rows, cols // group, group // 2)[:, ~at] = 0x88
+    x = torch.randn((T, cols), generator=rng).to(dtype)
+    w, xd = ref.values(codes, scales, cols, group), x.double()
+    y, want = _run(codes, scales, rows, cols, group, x.cuda()).double(), xd @ w.t()
+    off = ref.product_bound(w, xd, dtype == torch.float32) + ref.rounded(want, dtype)
+    off[:, 2::3] += 2.0 ** -36 * xd.abs().sum(1)[:, None]
+    assert bool(((y - want).abs() <= off).all())
+
+
 @pytest.mark.parametrize("T", [1, 4, 30, 100])
 def test_zero_weights_give_zero(gpu_lib, T):
     rows, cols, group = 70, 500, 32
