@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     pdl_wait();
     int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), uses = 0, s = 0, ph = 0;      // s, ph: the team's stage, and the parity of its uses
     bool fresh = true;
+    int have = -1;                                        // picks, gate/up: the row of x whose digits are there
     FewItem it{};
     // Lane row g is weight row wr: the two rows of a quarter of a warp are four apart, so that their pieces lie in different banks.
     const int wr = (g >> 1) | ((g & 1) << 2);
@@ -248,7 +249,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     for (long long i = i0; i < i1; i++) {
         if (fresh) {
             it = few_item<MODE>(a, slot, tile);
-            if (it.count) {
+            const int src = MODE == W4_GATEUP && a.idx ? it.first / a.topk : -1;      // (a token's picks: the same row)
+            if (it.count && (src < 0 || src != have)) {
+                have = src;
                 if (MODE == W4_DOWN || TERMS == 3) few_digits<TERMS, MODE, WHOLE, NS, float>(a, it, blocks);
                 else                               few_digits<TERMS, MODE, WHOLE, NS, uint16_t>(a, it, blocks);
             }
