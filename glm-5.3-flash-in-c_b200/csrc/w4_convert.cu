@@ -1,13 +1,16 @@
 // w4_convert.cu - a matrix to 4-bit codes with group scales, and its values back.
 //
 // Per row and group m = max |w|, s = bf16(m / 7), code = 8 + clamp(round(w / s), -7, 7), halves to even, both roundings of s to
-// nearest even. The quotient is taken exactly: the product with 1 / s decides, and where it lies near a half the residual w - q s
-// does, which is exact there (q s has 12 significant bits; within half a step of it the difference loses none). A
-// division instead is twenty instructions a weight, as many as the SM can issue while HBM delivers an FP8 weight.
+// nearest even. The quotient is taken exactly. A BF16 weight's (both have 8 significant bits) is a half or at least 2^-10 away from one, so
+// the product with 1 / s, 2^-21 off at most, is first rounded to a multiple of 2^-11 and then to an integer. Of FP32 values the product
+// decides, and where it lies near a half the residual w - q s does, which is exact there (q s has 12 significant bits; within half a step
+// of it the difference loses none). A division instead is twenty instructions a weight, as many as the SM can issue while HBM delivers
+// an FP8 weight.
 //
-// Both directions are bound by HBM, the first nearly by the instructions a weight takes (9). There a lane takes 32 columns, so that what
+// Both directions are bound by HBM, the first nearly by the instructions a weight takes. There a lane takes 32 columns, so that what
 // is paid per group - the division, the reciprocal, the maximum's shuffles - is paid once for 32 weights, and its codes are one store;
-// eight columns a lane paid it four times, converted to integers by the slow instruction, and took 72 us for 12288 x 4096 BF16 weights.
+// eight columns a lane paid it four times, converted to integers by the slow instruction, and took 72 us for 12288 x 4096 BF16 weights. (With
+// residuals for BF16 weights too, every second warp met an exact half: 42 us.)
 #include "w4.cuh"
 
 namespace g5b {
@@ -70,11 +73,12 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
         }
     }
     // the largest magnitude as bits: infinities and NaN are above every number
-    uint32_t m = 0;
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) m = max(m, __float_as_uint(v[i][k]) & 0x7fffffffu);
+        for (int k = 0; k < 8; k++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[i][k])));
+    uint32_t m = __float_as_uint(most);
     for (int o = 1; o < per; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const bool finite = m < 0x7f800000u;
     const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.0f));
@@ -84,9 +88,10 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
     const bool tiny = s < 0x1p-100f;
     const float up = tiny ? 0x1p64f : 1.0f, su = s * up, r = live ? __frcp_rn(su) : 0.f, half = 0.5f * su;
     // Rounded by adding 1.5 2^23 + 8, in whose low bits the code then lies; eight codes are put together by multiplications, the same pipe. A
-    // quotient over 7.5 (of a scale rounded to a few bits) and residuals from half a step on take the long way, eight weights at a time.
+    // quotient over 7.5 (of a scale rounded to a few bits) and FP32 residuals from half a step on take the long way, eight weights at a time.
     constexpr float MAGIC = 12582912.0f + 8.0f;
     constexpr uint32_t MAGIC_BITS = 0x4b400000u, ONES = 0x11111111u;
+    constexpr float STEP = 6144.0f;                          // 1.5 2^12, from where on FP32 numbers are 2^-11 apart
     const bool clamp = tiny || __uint_as_float(m) > 7.5f * s;
     __align__(16) uint32_t packed[4];
 #pragma unroll
@@ -95,11 +100,15 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_quantize_kernel(W4Mat w, uin
         float far = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const float t = fmaf(v[i][k], r, MAGIC), q = t - MAGIC;
-            far = fmaxf(far, fabsf(fmaf(-q, su, v[i][k])));
+            float t;
+            if (DT == DT_BF16) t = __fadd_rn(fmaf(v[i][k], r, STEP), MAGIC - STEP);
+            else {
+                t = fmaf(v[i][k], r, MAGIC);
+                far = fmaxf(far, fabsf(fmaf(-(t - MAGIC), su, v[i][k])));
+            }
             word += __float_as_uint(t) << (4 * k);
         }
-        if (clamp || far >= half) {
+        if (clamp || (DT != DT_BF16 && far >= half)) {
             word = 0u;
 #pragma unroll
             for (int k = 0; k < 8; k++) {

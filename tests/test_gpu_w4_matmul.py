@@ -301,3 +301,19 @@ def test_quantize_borders(gpu_lib):
         v[r, 4 * group:] = torch.linspace(-1, 1, group) * 2.0 ** (-149 + 2 * r if r < 40 else 127 - (r - 40))
     v[5, 3 * group + 3], v[6, 3 * group + 31], v[7, 3 * group] = float("nan"), float("inf"), float("-inf")
     _compare(v, _convert(v, rows, 5 * group, group), rows, 5 * group, group)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("exponent", [-130, -101, -20, 100])
+def test_quantize_every_quotient_of_bf16(gpu_lib, kind, exponent):
+    """Every BF16 number from a 64th of a scale on, of both signs, beside every significand of the largest (and so all of the scale's):
+    exact halves and what lies nearest to them."""
+    group = 128
+    top = (128 + torch.arange(128)).double() * 2.0 ** (exponent - 7)
+    others = torch.cat([(128 + torch.arange(128)).double() * 2.0 ** (exponent - 7 - d) for d in range(9)])
+    others = torch.cat((others, -others))
+    others = torch.nn.functional.pad(others, (0, -len(others) % (group - 1))).view(-1, group - 1)
+    rows, groups = len(top), len(others)
+    v = torch.cat((top[:, None, None].expand(rows, groups, 1), others.expand(rows, groups, group - 1)), 2)
+    v = torch.where(v.abs() <= top[:, None, None], v, torch.zeros(())).view(rows, groups * group).to(torch.bfloat16)
+    _compare(v.float(), _convert(v if kind == "bf16" else v.float(), rows, groups * group, group), rows, groups * group, group)
