@@ -6,7 +6,9 @@
 // columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand as they are, two AND to eight of them, where
 // F16 values took five logical and four packed operations; activations are 8-bit digits of a fixed-point number; sums are exact.
 // One CTA per SM, persistent. Work comes in items of 16 weight rows (gate/up: eight gate rows and the eight up rows that go with them),
-// in pieces of 4096 columns; a CTA takes a contiguous share of them.
+// in pieces of 4096 columns; a CTA takes a contiguous share of them. Of up to 2048 columns an item is 32 rows: with two blocks of 128
+// columns to a warp its waits and the sums' meeting were most of an item (down products of 64 tokens' experts 282 us at 4.5 TB/s;
+// all three products 736 -> 648 us, BF16 rows 545 -> 505, 32768 x 800 past two rows 12.9 -> 11.2).
 //   warp 16   brings an item's rows into a ring in shared memory, one TMA load for the codes and one for the scales (gate/up: two
 //             each), as many ahead as fit: they wait for nothing but room, so HBM is busy while sums are put together and rows change.
 //             (A bulk copy per row was 125 cycles of issue each: 2.3 TB/s.)
@@ -35,7 +37,8 @@ constexpr int FW_COLS = 8;                           // activation columns of an
 constexpr int FW_PIECE = 4096;                       // weight columns of a stage at most (half of them where that leaves too few stages): 16 chunks of 128 bytes
 constexpr int FW_DIGIT_BYTES = 88 * 1024;            // room for the digits
 constexpr int FW_MAX_STAGES = 12;
-constexpr int FW_SMEM = 206 * 1024;                  // for stages and digits with 16 KB of sums beside them
+constexpr int FW_SUMS = 16 * 1024;                   // sums of a sixteen of weight rows
+constexpr int FW_SMEM = 206 * 1024;                  // for stages and digits with the sums of a sixteen beside them
 
 static __device__ int g_few_err;                     // a wait that ran out: its code (0: none)
 
@@ -56,6 +59,7 @@ struct FewArgs {
     float limit;
     int whole_rows;                // rows of codes are whole chunks: one load brings all of a stage's
     int piece;                     // blocks of 128 columns of a stage
+    int sixteens;                  // of weight rows of an item
     int chunks, scale_cols;        // of a stage at most
     int scale_pitch;               // scales of a stage's row: eight more, so that eight rows lie in different banks
     int stages, stage_bytes, stage_tx;      // (stages of a team)
@@ -163,11 +167,11 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
     bar_sync(1, FW_WARPS * 32);
 }
 
-// TERMS: digits of an activation. WHOLE: groups of 128. NS: columns that there is room for.
-template <int TERMS, int MODE, bool WHOLE, int NS>
+// TERMS: digits of an activation. WHOLE: groups of 128. NS: columns that there is room for. U: sixteens of weight rows of an item.
+template <int TERMS, int MODE, bool WHOLE, int NS, int U>
 __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_constant__ FewMaps maps, const FewArgs a)
 {
-    constexpr int HALVES = MODE == W4_GATEUP ? 2 : 1, HALF_ROWS = 16 / HALVES;
+    constexpr int HALVES = MODE == W4_GATEUP ? 2 : 1, HALF_ROWS = 16 * U / HALVES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *ring = smem;                                                             // [team][stages][half][chunk][row][128] codes, [half][row][scale_pitch] scales
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     Block *blocks = reinterpret_cast<Block *>(smem + (size_t)2 * a.stages * a.stage_bytes);
     // A team waits for every use of its stages, so none of its waits can take an earlier use's phase for the one it waits for.
     __shared__ uint64_t full[2][FW_MAX_STAGES], empty[2][FW_MAX_STAGES];
-    __shared__ float s_sum[2][2][8][16][FW_COLS];                                // [team][item's parity][warp][row][column]
+    __shared__ float s_sum[2][2][8][16 * U][FW_COLS];                                // [team][item's parity][warp][row][column]
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     int *err = &g_few_err;
     pdl_trigger();
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                             else
                                 for (int c = 0; c < a.chunks; c++)
                                     tma_load_3d(half + c * (HALF_ROWS * 128), &maps.codes[h], p * (a.piece * 64) + c * 128, it.tile * HALF_ROWS, it.e, bar);
-                            tma_load_3d(to + a.chunks * 2048 + h * (HALF_ROWS * 2) * a.scale_pitch, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, bar);
+                            tma_load_3d(to + a.chunks * (2048 * U) + h * (HALF_ROWS * 2) * a.scale_pitch, &maps.scales[h], p * a.scale_cols, it.tile * HALF_ROWS, it.e, bar);
                         }
                         issued[turn]++;
                         if (++st == a.stages) { st = 0; parity[turn] ^= 1; }
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
         it.tile = tile;
         if (it.count) {
             if (turn == team) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                float acc[U][4] = {};
 #pragma unroll 1
                 for (int p = 0; p < pieces; p++) {
                     const uint8_t *st = ring + (size_t)(team * a.stages + s) * a.stage_bytes;
@@ -269,11 +273,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                     // This warp's blocks are gw, gw + 8, ...: half a chunk of 128 bytes each, chunks HALF_ROWS * 128 apart, a row's 16-byte
                     // pieces at piece ^ (row & 7). Whatever does not change from block to block is taken out of the loop.
                     const uint8_t *cg = st + (gw >> 1) * (HALF_ROWS * 128) + wr * 128, *ch = cg + (MODE == W4_GATEUP ? a.chunks * 1024 : 1024);
-                    const uint16_t *sg = reinterpret_cast<const uint16_t *>(st + a.chunks * 2048) + wr * a.scale_pitch + (WHOLE ? gw : (4 * gw) >> wlog), *sh = sg + 8 * a.scale_pitch;
+                    const uint16_t *sg = reinterpret_cast<const uint16_t *>(st + a.chunks * (2048 * U)) + wr * a.scale_pitch + (WHOLE ? gw : (4 * gw) >> wlog), *sh = sg + 8 * a.scale_pitch;
                     const Block *bp = blocks + p * a.piece + gw;
                     const int first_group = (4 * (p * a.piece + gw)) >> wlog;
-                    auto block = [&](int i) {
-                        const uint8_t *pg = cg + i * (4 * HALF_ROWS * 128), *ph_ = ch + i * (4 * HALF_ROWS * 128);
+                    auto block = [&](int i, int sixteen, float (&acc)[4]) {
+                        const uint8_t *pg = cg + i * (4 * HALF_ROWS * 128) + sixteen * 2048, *ph_ = ch + i * (4 * HALF_ROWS * 128) + sixteen * 2048;
+                        const uint16_t *s_g = sg + sixteen * 16 * a.scale_pitch, *s_h = sh + sixteen * 16 * a.scale_pitch;
                         const Block &x = bp[8 * i];
                         uint4 vg, vh;
                         if (WHOLE) {
@@ -289,12 +294,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                         // the block's scales (of four, two or one group) of rows g and g + 8
                         float fg[4], fh[4];
                         if (WHOLE) {
-                            fg[0] = bf16_to_f32(sg[8 * i]) * 0.0625f; fh[0] = bf16_to_f32(sh[8 * i]) * 0.0625f;      // (the sums are 16 times theirs)
+                            fg[0] = bf16_to_f32(s_g[8 * i]) * 0.0625f; fh[0] = bf16_to_f32(s_h[8 * i]) * 0.0625f;      // (the sums are 16 times theirs)
                         } else if (wlog) {
-                            const uint32_t g2 = *reinterpret_cast<const uint32_t *>(sg + 16 * i), h2 = *reinterpret_cast<const uint32_t *>(sh + 16 * i);
+                            const uint32_t g2 = *reinterpret_cast<const uint32_t *>(s_g + 16 * i), h2 = *reinterpret_cast<const uint32_t *>(s_h + 16 * i);
                             bf16x2_to_f32(g2, fg[0], fg[1]); bf16x2_to_f32(h2, fh[0], fh[1]);
                         } else {
-                            const uint2 g4 = *reinterpret_cast<const uint2 *>(sg + 32 * i), h4 = *reinterpret_cast<const uint2 *>(sh + 32 * i);
+                            const uint2 g4 = *reinterpret_cast<const uint2 *>(s_g + 32 * i), h4 = *reinterpret_cast<const uint2 *>(s_h + 32 * i);
                             bf16x2_to_f32(g4.x, fg[0], fg[1]); bf16x2_to_f32(g4.y, fg[2], fg[3]);
                             bf16x2_to_f32(h4.x, fh[0], fh[1]); bf16x2_to_f32(h4.y, fh[2], fh[3]);
                         }
@@ -343,20 +348,24 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                         for (int q = 0; q < 4; q++) acc[q] = fmaf(sum[q], q & 1 ? worth.y : worth.x, acc[q]);
                     };
 #pragma unroll
-                    for (int i = 0; i < FW_PIECE / 1024; i++) {
+                    for (int i = 0; i < FW_PIECE / 1024 / U; i++) {
                         if (gw + 8 * i >= nb) break;
-                        block(i);
+#pragma unroll
+                        for (int k = 0; k < U; k++) block(i, k, acc[k]);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[team][s]);
                     if (++s == a.stages) { s = 0; ph ^= 1; }
                 }
-                float (*sum)[16][FW_COLS] = s_sum[team][uses & 1];
+                float (*sum)[16 * U][FW_COLS] = s_sum[team][uses & 1];
                 uses++;
-                *reinterpret_cast<float2 *>(&sum[gw][wr][2 * t]) = make_float2(acc[0], acc[1]);
-                *reinterpret_cast<float2 *>(&sum[gw][wr + 8][2 * t]) = make_float2(acc[2], acc[3]);
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    *reinterpret_cast<float2 *>(&sum[gw][16 * k + wr][2 * t]) = make_float2(acc[k][0], acc[k][1]);
+                    *reinterpret_cast<float2 *>(&sum[gw][16 * k + wr + 8][2 * t]) = make_float2(acc[k][2], acc[k][3]);
+                }
                 bar_sync(2 + team, 256);
-                constexpr int OUT = MODE == W4_GATEUP ? 8 : 16;           // outputs of a row of x
+                constexpr int OUT = MODE == W4_GATEUP ? 8 : 16 * U;           // outputs of a row of x
                 if (gt < OUT * it.count) {
                     const int r = gt & (OUT - 1), k = gt / OUT, col = k * TERMS;
                     float v = 0.f, u = 0.f;
@@ -382,27 +391,30 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     }
 }
 
-template <int TERMS, int MODE, bool WHOLE, int NS>
+template <int TERMS, int MODE, bool WHOLE, int NS, int U>
 static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
     static SmemGrant grant;
     const int digit_bytes = (int)sizeof(FewBlock<NS, WHOLE>) * a.blocks;
-    a.stages = std::min((FW_SMEM - digit_bytes) / a.stage_bytes / 2, FW_MAX_STAGES);
+    a.stages = std::min((FW_SMEM - (U - 1) * FW_SUMS - digit_bytes) / a.stage_bytes / 2, FW_MAX_STAGES);
     const size_t smem = 1024 + (size_t)2 * a.stages * a.stage_bytes + digit_bytes;
     if (a.stages < 1) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
     // (what counts is this and the sums: more than 48 KB of them must be asked for)
-    if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
+    if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS, U>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
     const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
-    if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
-    else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS>), grid, FW_THREADS, smem, st, m, a);
+    if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS, U>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
+    else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS, U>), grid, FW_THREADS, smem, st, m, a);
     return 0;
 }
 constexpr int few_one(int terms) { return terms == 3 ? 4 : 2; }          // columns of a single row, with one to spare
 template <int TERMS, int MODE, bool WHOLE>
 static int few_columns(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
-    return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS)>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS>(st, m, a, early);
+    if constexpr (MODE != W4_GATEUP)
+        if (a.sixteens == 2)
+            return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS), 2>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS, 2>(st, m, a, early);
+    return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS), 1>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS, 1>(st, m, a, early);
 }
 template <int TERMS, int MODE>
 static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
@@ -429,10 +441,13 @@ int w4_few(cudaStream_t st, const W4Job &j)
     const int size = j.x_dt == DT_F32 ? 4 : 2;
     a.w = j.w; a.x = j.x; a.ldx = j.ldx; a.x_dt = j.x_dt; a.cols = j.w.cols; a.blocks = w4_kp(j.w.cols) / 128;
     a.wide = reinterpret_cast<uintptr_t>(j.x) % 16 == 0 && j.ldx * size % 16 == 0;
-    a.tiles = (j.w.rows + (j.mode == W4_GATEUP ? 7 : 15)) / (j.mode == W4_GATEUP ? 8 : 16);
     a.rows = j.T; a.per = j.mode == W4_DENSE ? j.T : j.idx ? 1 : j.slots.rows; a.order = j.order; a.idx = j.idx; a.topk = j.topk; a.E = j.count; a.n = j.T; a.slots = j.slots;
     a.y = j.y; a.ldy = j.ldy; a.y_dt = j.y_dt; a.limit = j.limit;
-    const int half_rows = j.mode == W4_GATEUP ? 8 : 16;
+    const int slots = j.mode == W4_DENSE ? 1 : j.idx ? j.T : j.slots.max;
+    // (two sixteens to an item wherever it has two blocks of 128 columns to a warp at most, and a CTA still has two such items)
+    a.sixteens = j.mode != W4_GATEUP && a.blocks <= FW_PIECE / 256 && (long long)slots * j.w.rows >= 64ll * dev_sms() ? 2 : 1;
+    const int half_rows = j.mode == W4_GATEUP ? 8 : 16 * a.sixteens;
+    a.tiles = (j.w.rows + half_rows - 1) / half_rows;
     a.whole_rows = j.w.pitch % 128 == 0;
     // Two stages of each team at least: with many digits beside them in pieces of half the columns.
     const size_t digits = (size_t)a.blocks * few_block(bf16 ? DT_BF16 : DT_F32, a.per);
@@ -440,9 +455,9 @@ int w4_few(cudaStream_t st, const W4Job &j)
         a.chunks = std::min(a.piece / 2, (j.w.pitch + 127) / 128);
         a.scale_cols = std::min(a.piece * 128 / j.w.group, j.w.sp);
         a.scale_pitch = a.scale_cols + 8;
-        a.stage_tx = a.chunks * 2048 + 32 * a.scale_pitch;
+        a.stage_tx = (a.chunks * 2048 + 32 * a.scale_pitch) * a.sixteens;
         a.stage_bytes = (a.stage_tx + 1023) / 1024 * 1024;
-        if (a.piece < FW_PIECE / 128 || 4 * (size_t)a.stage_bytes + digits <= (size_t)FW_SMEM) break;
+        if (a.piece < FW_PIECE / 128 || 4 * (size_t)a.stage_bytes + (a.sixteens - 1) * FW_SUMS + digits <= (size_t)FW_SMEM) break;
     }
     FewMaps m;
     for (int h = 0; h < 2; h++) {

@@ -148,7 +148,8 @@ def _experts(handles, x, idx, weights, limit, pad=0):
 @pytest.mark.parametrize("T,K,E,H,I,group,limit,how", [
     (1, 8, 12, 256, 128, 128, 10.0, "even"), (1, 1, 1, 33, 17, 32, 1.0, "even"), (5, 4, 6, 200, 96, 64, float("inf"), "outside"),
     (40, 3, 4, 130, 257, 32, 0.5, "skewed"), (90, 2, 3, 384, 128, 128, 2.0, "even"), (70, 2, 5, 100, 300, 64, 10.0, "one"),
-    (3, 2, 4, 64, 64, 32, 10.0, "none"), (33, 4, 40, 160, 160, 32, 3.0, "outside")])
+    (3, 2, 4, 64, 64, 32, 10.0, "none"), (33, 4, 40, 160, 160, 32, 3.0, "outside"),
+    (16, 4, 64, 256, 130, 32, 10.0, "even"), (2, 8, 20, 700, 130, 64, 10.0, "skewed")])
 def test_experts(gpu_lib, T, K, E, H, I, group, limit, how, dtype):
     rng = torch.Generator().manual_seed(T * 13 + H)
     (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, group), _stack(rng, E, I, H, group), _stack(rng, E, H, I, group)

@@ -63,6 +63,16 @@ def test_small_integers_come_out_exactly(gpu_lib, rows, cols, group, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,group,T", [(9473, 100, 32, 1), (9500, 2048, 128, 2), (20011, 1050, 64, 4), (12288, 1920, 32, 3), (9999, 129, 128, 1)])
+def test_many_short_rows(gpu_lib, rows, cols, group, T, dtype):
+    rng = torch.Generator().manual_seed(rows + T)
+    codes, scales = ref.make(rng, rows, cols, group)
+    x = torch.randn((T, cols), generator=rng).to(dtype)
+    _check(_run(codes, scales, rows, cols, group, x.cuda(), pad=T % 3), ref.values(codes, scales, cols, group), x)
+
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T", [1, 4, 30, 100])
 def test_small_columns_beside_large_ones(gpu_lib, T, dtype):
     """The first 128 columns of x are 2^24 times the others and have zero weights. What many rows are held to is 2^-38 of the row's
