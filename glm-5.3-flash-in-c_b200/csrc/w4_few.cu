@@ -3,8 +3,8 @@
 // keeps blocks apart. Experts of 64 tokens 805 us against 700.)
 //
 // Bound by HBM: half a byte and a scale's share per weight. The integer matrix instruction does the products (16 weight rows x 32
-// columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand as they are, two AND to eight of them, where
-// F16 values took five logical and four packed operations; activations are 8-bit digits of a fixed-point number; sums are exact.
+// columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand nearly as they are, where
+// F16 values took five logical and four packed operations to eight of them; activations are 8-bit digits of a fixed-point number; sums are exact.
 // One CTA per SM, persistent. Work comes in items of 16 weight rows (gate/up: eight gate rows and the eight up rows that go with them),
 // in pieces of 4096 columns; a CTA takes a contiguous share of them. Of up to 2048 columns an item is 32 rows: with two blocks of 128
 // columns to a warp its waits and the sums' meeting were most of an item (down products of 64 tokens' experts 282 us at 4.5 TB/s;
@@ -14,17 +14,19 @@
 //             (A bulk copy per row was 125 cycles of issue each: 2.3 TB/s.)
 //   0-7, 8-15 take items in turn, from rings of their own; the eight warps of a team share an item's blocks of 128 columns, and their sums meet in shared
 //             memory in a fixed order
-//   codes     a lane takes 16 bytes of rows g and g + 8 (lane = 4 g + t), a quad 64 bytes: 128 columns of each. Low nibbles are one
-//             operand, high nibbles - in place, 16 times their value - another with sums of its own. Which column stands for which
-//             k of an MMA does not matter as long as both operands agree, and the digits lie in that order. What the codes' offset of
-//             8 adds is the digits' sum times 8: the sums start at minus that.
+//   codes     a lane takes 16 bytes of rows g and g + 8 (lane = 4 g + t), a quad 64 bytes: 128 columns of each. Which column stands for
+//             which k of an MMA does not matter as long as both operands agree, and the digits lie in that order. In groups of 128 a
+//             byte is an operand as it is, 16 h + l, past the odd columns' digits o, and its low nibble another, past digits of
+//             e - o / 16: l e + h o = (16 h + l) o / 16 + l (e - o / 16), one AND to eight codes. (High nibbles masked too, eight moves
+//             and a multiplication of each scale: 770 us for the experts of 64 tokens at the power limit's 1.6 GHz, where instructions bound them.) What the codes' offset of
+//             8 adds is known from the digits: the sums start at minus that.
 //   scales    in FP32, once per group, on the sums of the group. A quad's 128 columns are one group of 128; for smaller groups
 //             a lane takes its words 16 bytes apart, so that an MMA is 32 columns of one group.
 //   x         becomes digits in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
 //             which the lanes read them: per row and block of 128 columns the power of two below which its values lie, and
 //             integers of 23 bits and a sign in three digits (BF16 rows: 15 bits in two), one bit less where the largest needs it.
 // Group sums are exact integers, taken into FP32 by the exponent trick (they start at the bits of 1.5 2^23, so that their bits are the
-// float 1.5 2^23 + sum, |sum| < 2^22); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
+// float 1.5 2^23 + sum, |sum| < 2^22; in groups of 128 sixteenths of 1.5 2^19); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
 
 #include "tc_ptx.cuh"
@@ -79,14 +81,19 @@ __device__ __forceinline__ FewItem few_item(const FewArgs &a, int slot, int tile
 }
 
 // (not volatile: two blocks' chains of these are put side by side)
+__device__ __forceinline__ void few_mma(int (&c)[4], uint32_t g0, uint32_t h0, uint32_t g1, uint32_t h1, uint32_t b0, uint32_t b1, int s0, int s1, int s2, int s3)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(g0), "r"(h0), "r"(g1), "r"(h1), "r"(b0), "r"(b1), "r"(s0), "r"(s1), "r"(s2), "r"(s3));
+}
 __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t g0, uint32_t h0, uint32_t g1, uint32_t h1, uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(g0), "r"(h0), "r"(g1), "r"(h1), "r"(b0), "r"(b1));
+    few_mma(c, g0, h0, g1, h1, b0, b1, c[0], c[1], c[2], c[3]);
 }
 __device__ __forceinline__ float few_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
-constexpr int FW_MAGIC = 0x4b400000;                 // the bits of 1.5 2^23
-__device__ __forceinline__ float few_float(int v) { return __fsub_rn(__int_as_float(v), 12582912.0f); }
+// The bits of 1.5 2^23, or for sums of sixteenths of 1.5 2^19.
+template <bool WHOLE> constexpr int few_magic = WHOLE ? 0x49400000 : 0x4b400000;
+template <bool WHOLE> __device__ __forceinline__ float few_float(int v) { return __fsub_rn(__int_as_float(v), WHOLE ? 786432.0f : 12582912.0f); }
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -126,18 +133,26 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
             // One more bit where the largest leaves the highest digit below 128.
             const int e = max((int)(m >> 23), 1) - 126, bits = TERMS == 3 ? 22 : 14;
             const float most = TERMS == 3 ? 127.0f * 65536.0f + 127.0f * 256.0f + 127.0f : 127.0f * 256.0f + 127.0f;
-            const int up = bits - e + (__uint_as_float(m) * few_pow2((bits + 1 - e) >> 1) * few_pow2(bits + 1 - e - ((bits + 1 - e) >> 1)) <= most);   // -114 <= up <= 148
+            const int up = bits - e + (__uint_as_float(m) * few_pow2((bits + 1 - e) >> 1) * few_pow2(bits + 1 - e - ((bits + 1 - e) >> 1)) * (WHOLE ? 1.0625f : 1.0f) <= most);   // -114 <= up <= 148
             const float scale = few_pow2(up >> 1), scale2 = few_pow2(up - (up >> 1));
+            if (!finite)
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = v[k] * scale * scale2;
+            if (WHOLE)
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) v[k] = fmaf(v[k + 1], -0.0625f, v[k]);
             uint32_t even[TERMS] = {}, odd[TERMS] = {};  // digits of columns 0 2 4 6 and 1 3 5 7
             int sum[TERMS] = {};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                int x = finite ? __float2int_rn(v[k] * scale * scale2) : 0;
+                int x = __float2int_rn(v[k]);
 #pragma unroll
                 for (int d = 0; d < TERMS; d++) {
                     const int digit = d + 1 < TERMS ? (int)(int8_t)x : x;
                     x = (x - digit) >> 8;
-                    sum[d] += digit;
+                    sum[d] += digit * (WHOLE ? (k & 1 ? 136 : 128) : 8);
                     (k & 1 ? odd : even)[d] |= (uint32_t)(digit & 255) << (8 * (k >> 1));
                 }
             }
@@ -152,10 +167,10 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
                 if (WHOLE) {
                     reinterpret_cast<uint32_t *>(&b.digits[0][col + d][t])[j] = even[d];
                     reinterpret_cast<uint32_t *>(&b.digits[1][col + d][t])[j] = odd[d];
-                    if (w == 0) b.start[0][col + d] = -8 * sum[d];
+                    if (w == 0) b.start[0][col + d] = few_magic<WHOLE> - sum[d];
                 } else {
                     reinterpret_cast<uint2 *>(&b.digits[j >> 1][col + d][t])[j & 1] = make_uint2(even[d], odd[d]);
-                    if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = FW_MAGIC - 8 * sum[d];
+                    if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = few_magic<WHOLE> - sum[d];
                 }
                 // (2^-148 at least, a subnormal FP32 number)
                 if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(-(up - (up >> 1))) * (d == 0 ? 1.0f : d == 1 ? 256.0f : 65536.0f)
@@ -290,11 +305,11 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                             vh = make_uint4(*reinterpret_cast<const uint32_t *>(ph_ + off[0]), *reinterpret_cast<const uint32_t *>(ph_ + off[1]),
                                             *reinterpret_cast<const uint32_t *>(ph_ + off[2]), *reinterpret_cast<const uint32_t *>(ph_ + off[3]));
                         }
-                        constexpr uint32_t LOW = 0x0f0f0f0fu, HIGH = 0xf0f0f0f0u;
+                        constexpr uint32_t LOW = 0x0f0f0f0fu;
                         // the block's scales (of four, two or one group) of rows g and g + 8
                         float fg[4], fh[4];
                         if (WHOLE) {
-                            fg[0] = bf16_to_f32(s_g[8 * i]) * 0.0625f; fh[0] = bf16_to_f32(s_h[8 * i]) * 0.0625f;      // (the sums are 16 times theirs)
+                            fg[0] = bf16_to_f32(s_g[8 * i]); fh[0] = bf16_to_f32(s_h[8 * i]);
                         } else if (wlog) {
                             const uint32_t g2 = *reinterpret_cast<const uint32_t *>(s_g + 16 * i), h2 = *reinterpret_cast<const uint32_t *>(s_h + 16 * i);
                             bf16x2_to_f32(g2, fg[0], fg[1]); bf16x2_to_f32(h2, fh[0], fh[1]);
@@ -316,13 +331,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                         float sum[4];
                         if (WHOLE) {
                             const int2 start = *reinterpret_cast<const int2 *>(&x.start[0][2 * t]);
-                            int lo[4] = {start.x, start.y, start.x, start.y}, hi[4] = {FW_MAGIC, FW_MAGIC, FW_MAGIC, FW_MAGIC};
-                            few_mma(lo, vg.x & LOW, vh.x & LOW, vg.y & LOW, vh.y & LOW, x0.x, x0.y);
-                            few_mma(hi, vg.x & HIGH, vh.x & HIGH, vg.y & HIGH, vh.y & HIGH, x1.x, x1.y);
+                            int lo[4], hi[4];
+                            few_mma(lo, vg.x & LOW, vh.x & LOW, vg.y & LOW, vh.y & LOW, x0.x, x0.y, 0, 0, 0, 0);
+                            few_mma(hi, vg.x, vh.x, vg.y, vh.y, x1.x, x1.y, start.x, start.y, start.x, start.y);
                             few_mma(lo, vg.z & LOW, vh.z & LOW, vg.w & LOW, vh.w & LOW, x0.z, x0.w);
-                            few_mma(hi, vg.z & HIGH, vh.z & HIGH, vg.w & HIGH, vh.w & HIGH, x1.z, x1.w);
+                            few_mma(hi, vg.z, vh.z, vg.w, vh.w, x1.z, x1.w);
 #pragma unroll
-                            for (int q = 0; q < 4; q++) sum[q] = few_float(hi[q] + 16 * lo[q]) * (q < 2 ? fg[0] : fh[0]);
+                            for (int q = 0; q < 4; q++) sum[q] = few_float<true>(hi[q] + 16 * lo[q]) * (q < 2 ? fg[0] : fh[0]);
                         } else {
                             int c[4];
 #pragma unroll
@@ -339,7 +354,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                                 if (wlog == 0 || (j & 1)) {
                                     const float sg_ = wlog ? fg[j >> 1] : fg[j], sh_ = wlog ? fh[j >> 1] : fh[j];
 #pragma unroll
-                                    for (int q = 0; q < 4; q++) sum[q] = fmaf(few_float(c[q]), q < 2 ? sg_ : sh_, sum[q]);
+                                    for (int q = 0; q < 4; q++) sum[q] = fmaf(few_float<false>(c[q]), q < 2 ? sg_ : sh_, sum[q]);
                                 }
                             }
                         }
@@ -347,12 +362,19 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
 #pragma unroll
                         for (int q = 0; q < 4; q++) acc[q] = fmaf(sum[q], q & 1 ? worth.y : worth.x, acc[q]);
                     };
+constexpr int MOST = FW_PIECE / 1024 / U;
+                    if (nb == 8 * MOST) {                // (no branch keeps the blocks apart)
 #pragma unroll
-                    for (int i = 0; i < FW_PIECE / 1024 / U; i++) {
-                        if (gw + 8 * i >= nb) break;
+                        for (int i = 0; i < MOST; i++)
 #pragma unroll
-                        for (int k = 0; k < U; k++) block(i, k, acc[k]);
-                    }
+                            for (int k = 0; k < U; k++) block(i, k, acc[k]);
+                    } else
+#pragma unroll 1
+                        for (int i = 0; i < MOST; i++) {
+                            if (gw + 8 * i >= nb) break;
+#pragma unroll
+                            for (int k = 0; k < U; k++) block(i, k, acc[k]);
+                        }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[team][s]);
                     if (++s == a.stages) { s = 0; ph ^= 1; }
