@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
 {
     extern __shared__ int sm[];
     int *count = sm, *total = sm + SORT_WARPS * E;
-    __shared__ int s_part[2][SORT_WARPS];
+    __shared__ int s_part[2][SORT_WARPS], s_valid[SORT_WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = ctas > 1 ? (int)cluster_cta_rank() : 0;
     // this warp's picks: a multiple of 32 of them
     const int share = (n + ctas * SORT_WARPS * 32 - 1) / (ctas * SORT_WARPS * 32) * 32;
@@ -91,7 +91,16 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
                 }
             }
     // sums over the experts: of the picks, and of the tiles they make
-    const int rows = slots.n ? slots.rows : 1;
+    int rows = slots.n ? slots.rows : 1, here = 0;
+    bool many = false;
+    if (slots.n && slots.many_rows) {
+        const int mine_here = __reduce_add_sync(0xffffffffu, all[0] + all[1]);
+        if (lane == 0) s_valid[warp] = mine_here;
+        __syncthreads();
+        for (int w = 0; w < SORT_WARPS; w++) here += s_valid[w];
+        many = here > slots.few_most;
+        if (many) rows = slots.many_rows;
+    }
     const int tiles[2] = {(all[0] + rows - 1) / rows, (all[1] + rows - 1) / rows};
     int sum = all[0] + all[1], tsum = tiles[0] + tiles[1];
 #pragma unroll
@@ -118,7 +127,10 @@ __global__ void __launch_bounds__(SORT_THREADS) expert_sort_kernel(const int *id
                     slots.first[tile[i] + k] = first[i] + k * rows;
                     slots.count[tile[i] + k] = min(rows, all[i] - k * rows);
                 }
-                if (e0 + i == E - 1) *slots.n = tile[i] + tiles[i];
+                if (e0 + i == E - 1) {
+                    slots.n[0] = many ? 0 : tile[i] + tiles[i];
+                    if (slots.many_rows) { slots.n[1] = many ? tile[i] + tiles[i] : 0; slots.n[2] = many ? here : 0; }
+                }
             }
         }
     }

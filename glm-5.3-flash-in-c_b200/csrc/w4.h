@@ -37,6 +37,9 @@ void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t l
 struct W4Slots {
     int *n, *expert, *first, *count;
     int max, rows;              // slots at most; rows of a tile at most
+    // many_rows > 0: the sort chooses. Up to few_most picks of experts here make slots of `rows`; with more, slots of many_rows, and then
+    // their number is n[1], that of the picks n[2], and n[0] is 0 (else n[1] and n[2] are).
+    int many_rows, few_most;
 };
 enum { W4_DENSE = 0, W4_GATEUP = 1, W4_DOWN = 2 };
 struct W4Job {
@@ -47,7 +50,7 @@ struct W4Job {
     int T;                      // rows of activations (experts: picks, at most)
     const void *x; int x_dt; size_t ldx;        // w4_few: the activations (dense, gate/up: the caller's; down: F32 rows of picks)
     const int *order; int topk;                 // w4_few, gate/up: the activation row of sorted row i is order[i] / topk
-    const int *idx;             // w4_few: not sorted, every pick a slot of its own (slots and order are not used then)
+    const int *idx;             // w4_few: not sorted, every pick a slot of its own (32 at most; slots and order are not used then)
     bool half;                  // w4_few, down: the caller's rows are BF16
     bool early;                 // w4_few: may be scheduled while the kernel before it drains
     W4Terms terms;              // w4_many: the activations as terms, in the order of the rows

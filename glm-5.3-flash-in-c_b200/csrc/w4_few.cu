@@ -1,8 +1,9 @@
 // w4_few.cu - 4-bit weights times a few rows of activations: a decoded token or two, the few tokens of an expert in a batch. Eight columns at
-// a time: two F32 rows, four of BF16. (Four F32 rows in sixteen columns were slower than the weights twice: the second product's branch
-// keeps blocks apart. Experts of 64 tokens 805 us against 700.)
+// a time: two F32 rows, four of BF16. (Four F32 rows in two sets of columns: an item of three or four rows takes 1.5 times as long as one of
+// two, and CTAs that have such items end last. Experts of 64 tokens 831 us against 752.)
 //
-// Bound by HBM: half a byte and a scale's share per weight. The integer matrix instruction does the products (16 weight rows x 32
+// Bound by HBM: half a byte and a scale's share per weight (154880 x 4096 past one row 54.3 us, 6.0 TB/s; a launch's start and end are 4 of them,
+// and all of the 5 us that 4096 x 2048 takes). The integer matrix instruction does the products (16 weight rows x 32
 // columns x 8 activation columns, twice the F16 one's): codes are the unsigned operand nearly as they are, where
 // F16 values took five logical and four packed operations to eight of them; activations are 8-bit digits of a fixed-point number; sums are exact.
 // One CTA per SM, persistent. Work comes in items of 16 weight rows (gate/up: eight gate rows and the eight up rows that go with them),
@@ -67,15 +68,17 @@ struct FewArgs {
     int stages, stage_bytes, stage_tx;      // (stages of a team)
 };
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
+// here: picks of experts that are here (idx: a bit each)
 template <int MODE>
-__device__ __forceinline__ int few_slots(const FewArgs &a) { return MODE == W4_DENSE ? 1 : a.idx ? a.n : __ldg(a.slots.n); }
+__device__ __forceinline__ int few_slots(const FewArgs &a, uint32_t here) { return MODE == W4_DENSE ? 1 : a.idx ? __popc(here) : __ldg(a.slots.n); }
 template <int MODE>
-__device__ __forceinline__ FewItem few_item(const FewArgs &a, int slot, int tile)
+__device__ __forceinline__ FewItem few_item(const FewArgs &a, uint32_t here, int slot, int tile)
 {
     if (MODE == W4_DENSE) return FewItem{0, 0, a.rows, tile};
     if (a.idx) {
-        const int e = __ldg(a.idx + slot);
-        return FewItem{e, slot, e >= 0 && e < a.E ? 1 : 0, tile};
+        for (int k = 0; k < slot; k++) here &= here - 1;
+        const int pick = __ffs(here) - 1;
+        return pick < 0 ? FewItem{} : FewItem{__ldg(a.idx + pick), pick, 1, tile};
     }
     return FewItem{__ldg(a.slots.expert + slot), __ldg(a.slots.first + slot), __ldg(a.slots.count + slot), tile};
 }
@@ -206,7 +209,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     __syncthreads();
     if (MODE != W4_DENSE && !a.idx) pdl_wait();           // (the slots are another kernel's)
     const int pieces = (a.blocks + a.piece - 1) / a.piece;
-    const long long items = (long long)few_slots<MODE>(a) * a.tiles;
+    uint32_t here = 0;
+    if (MODE != W4_DENSE && a.idx) {
+        const int e = lane < a.n ? __ldg(a.idx + lane) : -1;
+        here = __ballot_sync(0xffffffffu, e >= 0 && e < a.E);
+    }
+    const long long items = (long long)few_slots<MODE>(a, here) * a.tiles;
     const long long i0 = items * blockIdx.x / gridDim.x, i1 = items * (blockIdx.x + 1) / gridDim.x;
     bool ok = true;
     int turn = 0;                                         // the team that takes the item
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
         // ------------------------------------------------------------------- weights ----
         if (elect_one()) {
             int slot = (int)(i0 / a.tiles), tile = (int)(i0 - (long long)slot * a.tiles), stage[2] = {0, 0}, parity[2] = {1, 1}, issued[2] = {0, 0};
-            FewItem it = i0 < i1 ? few_item<MODE>(a, slot, tile) : FewItem{};
+            FewItem it = i0 < i1 ? few_item<MODE>(a, here, slot, tile) : FewItem{};
 #pragma unroll 1
             for (long long i = i0; i < i1 && ok; i++) {
                 if (it.count) {
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                     }
                     turn ^= 1;
                 }
-                if (++tile == a.tiles && i + 1 < i1) { tile = 0; it = few_item<MODE>(a, ++slot, 0); }
+                if (++tile == a.tiles && i + 1 < i1) { tile = 0; it = few_item<MODE>(a, here, ++slot, 0); }
                 it.tile = tile;
             }
             // copies in flight must land before shared memory goes away
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
 #pragma unroll 1
     for (long long i = i0; i < i1; i++) {
         if (fresh) {
-            it = few_item<MODE>(a, slot, tile);
+            it = few_item<MODE>(a, here, slot, tile);
             const int src = MODE == W4_GATEUP && a.idx ? it.first / a.topk : -1;      // (a token's picks: the same row)
             if (it.count && (src < 0 || src != have)) {
                 have = src;

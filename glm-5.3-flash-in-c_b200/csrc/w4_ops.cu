@@ -116,16 +116,22 @@ int check_ws(const char *op, const void *ws, size_t have, size_t need)
     return have >= need ? 0 : fail("%s: the workspace has %zu bytes, %zu are needed", op, have, need);
 }
 
-// How a call of the experts goes: PICKS (a token or two: every pick on its own, nothing is sorted), FEW (w4_few on sorted picks) or MANY.
-// It goes by the rows that an expert would have if all picks were here and spread evenly.
-enum { PICKS, FEW, MANY };
+// How a call of the experts goes: PICKS (every pick on its own, nothing is sorted), FEW (w4_few on sorted picks), MANY (w4_many) or EITHER.
+// PICKS saves the sort, 7 us, and reads an expert twice that two picks have, 2 us each: n picks of E experts have n^2 / 2E such pairs
+// (three tokens of 288 experts 70.2 -> 63.6 us, four 84.5 -> 77.2).
+// FEW reads an expert's weights for every two F32 rows or four of BF16, MANY once, at the speed of its conversion: 1 row to an expert 604 against 835 us,
+// 2 (F32) 818 against 968, 2.8 the same; BF16 2.8 rows 712 against 944, 4 889 against 982, 5.3 1092 against 1003.
+// How many picks are here only the device knows: of a rank's call one in eight may be. EITHER: the sort chooses, and the other kind's
+// kernels find nothing to do, 4 us in all (a rank of 36 experts: 32 tokens 135 us by w4_many, 101 so; 64 tokens 160 and 139, BF16 145 and 117).
+enum { PICKS, FEW, MANY, EITHER };
 struct ExpertsPlan { int how, rows; };           // rows of a slot at most
-constexpr int PICKS_MOST = 16;
+constexpr int PICKS_ALWAYS = 16, PICKS_MOST = 32, RANKS = 8;
 ExpertsPlan experts_plan(int dt, int T, int topk, int E, int H, int I)
 {
     const int n = T * topk, h = w4_few_rows(dt, H), i = w4_few_rows(dt, I), rows = h < i ? h : i;
-    if (rows && n <= PICKS_MOST) return {PICKS, 1};
+    if (rows && n <= PICKS_MOST && (n <= PICKS_ALWAYS || n * n <= 4 * E)) return {PICKS, 1};
     if (rows > 1 && n <= rows * E) return {FEW, rows};
+    if (rows > 1 && n <= RANKS * rows * E) return {EITHER, rows};
     return {MANY, W4_MANY_ROWS};
 }
 struct ExpertsWs {
@@ -141,11 +147,12 @@ ExpertsWs experts_ws(Pieces &ws, const ExpertsPlan &plan, int n_terms, int T, in
     if (plan.how != PICKS) {
         w.order = ws.take<int>(n); w.place = ws.take<int>(n); w.offsets = ws.take<int>(E + 1);
         w.slots.rows = plan.rows;
+        if (plan.how == EITHER) { w.slots.many_rows = W4_MANY_ROWS; w.slots.few_most = plan.rows * E; }
         w.slots.max = (int)(n / plan.rows + (n < (size_t)E ? n : (size_t)E));
-        w.slots.n = ws.take<int>(1);
+        w.slots.n = ws.take<int>(3);
         w.slots.expert = ws.take<int>(w.slots.max); w.slots.first = ws.take<int>(w.slots.max); w.slots.count = ws.take<int>(w.slots.max);
     }
-    if (plan.how == MANY) {
+    if (plan.how == MANY || plan.how == EITHER) {
         w.x = terms_of(ws, n_terms, H, n);
         w.h = terms_of(ws, n_terms, I, n);
     }
@@ -305,17 +312,25 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     W4Job j{};
     j.count = E; j.n_terms = n_terms; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
     if (plan.how != PICKS && expert_sort(st, idx, T, topk, E, ws.order, ws.place, ws.offsets, &ws.slots)) return launched(op), -1;
-    if (plan.how == MANY) w4_split(st, ws.x, x, dtype, ldx, n, H, ws.offsets + E, ws.order, topk, false);
+    const bool few = plan.how != MANY, many = plan.how == MANY || plan.how == EITHER;
+    W4Slots many_slots = ws.slots;
+    const int *many_n = ws.offsets + E;                        // picks that the products of many rows take
+    if (plan.how == EITHER) { many_slots.n = ws.slots.n + 1; many_slots.rows = W4_MANY_ROWS; many_n = ws.slots.n + 2; }
+    if (many) w4_split(st, ws.x, x, dtype, ldx, n, H, many_n, ws.order, topk, false);
     // The first of the kernels that may start early (their weights, which no kernel before them in this call writes) comes behind one that
     // was launched the ordinary way: whatever the stream held before the call is over by then.
     j.mode = W4_GATEUP; j.w = wg; j.up = wu; j.y = ws.act; j.ldy = I;
     j.x = x; j.x_dt = dtype; j.ldx = ldx; j.terms = ws.x;
     j.idx = plan.how == PICKS ? idx : nullptr; j.early = plan.how != PICKS;
-    if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
-    if (plan.how == MANY) w4_split(st, ws.h, ws.act, DT_F32, I, n, I, ws.offsets + E, nullptr, 1, true);
+    W4Job jm = j;
+    jm.slots = many_slots;
+    if ((few && w4_few(st, j)) || (many && w4_many(st, jm, nullptr))) return -1;
+    if (many) w4_split(st, ws.h, ws.act, DT_F32, I, n, I, many_n, nullptr, 1, true);
     j.mode = W4_DOWN; j.w = wd; j.y = ws.rows; j.ldy = H;
     j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true; j.half = dtype == DT_BF16;
-    if (plan.how == MANY ? w4_many(st, j, nullptr) : w4_few(st, j)) return -1;
+    jm = j;
+    jm.slots = many_slots;
+    if ((few && w4_few(st, j)) || (many && w4_many(st, jm, nullptr))) return -1;
     expert_combine(st, ws.rows, DT_F32, H, plan.how == PICKS ? idx : ws.place, plan.how == PICKS ? E : 0, weights, T, topk, H, out, dtype, ldo, true);
     return launched(op);
 }

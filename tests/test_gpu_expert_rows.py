@@ -38,6 +38,8 @@ def _picks(rng, T, K, E, how):
         return torch.full((T, K), -1, dtype=torch.int32)
     if how == "outside":          # half of them other ranks', on both sides
         return torch.randint(-E // 2 - 1, E + E // 2 + 1, (T, K), generator=rng, dtype=torch.int32)
+    if how == "elsewhere":        # seven of eight
+        return torch.randint(0, 8 * E, (T, K), generator=rng, dtype=torch.int32)
     if how == "skewed":
         return (E * torch.rand((T, K), generator=rng) ** 4).to(torch.int32).clamp(max=E - 1)
     return torch.randint(0, E, (T, K), generator=rng, dtype=torch.int32)
@@ -149,7 +151,10 @@ def _experts(handles, x, idx, weights, limit, pad=0):
     (1, 8, 12, 256, 128, 128, 10.0, "even"), (1, 1, 1, 33, 17, 32, 1.0, "even"), (5, 4, 6, 200, 96, 64, float("inf"), "outside"),
     (40, 3, 4, 130, 257, 32, 0.5, "skewed"), (90, 2, 3, 384, 128, 128, 2.0, "even"), (70, 2, 5, 100, 300, 64, 10.0, "one"),
     (3, 2, 4, 64, 64, 32, 10.0, "none"), (33, 4, 40, 160, 160, 32, 3.0, "outside"),
-    (16, 4, 64, 256, 130, 32, 10.0, "even"), (2, 8, 20, 700, 130, 64, 10.0, "skewed")])
+    (16, 4, 64, 256, 130, 32, 10.0, "even"), (2, 8, 20, 700, 130, 64, 10.0, "skewed"),
+    (4, 8, 256, 64, 48, 32, 10.0, "even"), (4, 8, 256, 72, 48, 32, 10.0, "outside"), (3, 8, 256, 64, 48, 32, 10.0, "none"),
+    (60, 4, 40, 130, 96, 64, 10.0, "even"), (70, 8, 40, 130, 96, 32, 10.0, "elsewhere"), (100, 4, 40, 96, 130, 128, 10.0, "elsewhere"),
+    (78, 8, 40, 64, 64, 64, 10.0, "elsewhere"), (90, 8, 40, 64, 64, 64, 10.0, "none")])
 def test_experts(gpu_lib, T, K, E, H, I, group, limit, how, dtype):
     rng = torch.Generator().manual_seed(T * 13 + H)
     (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, group), _stack(rng, E, I, H, group), _stack(rng, E, H, I, group)
