@@ -251,3 +251,25 @@ def test_experts_repeat_and_replay(gpu_lib):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out.cpu(), first)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_replay_with_other_picks(gpu_lib, dtype):
+    """One captured call, replayed with picks of which all, one in eight and none are here: each time what an eager call gives."""
+    rng = torch.Generator().manual_seed(5)
+    E, H, I, T, K = 40, 128, 96, 60, 4
+    (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, 32), _stack(rng, E, I, H, 32), _stack(rng, E, H, I, 32)
+    x = torch.randn((T, H), generator=rng).to(dtype).cuda()
+    weights = torch.rand((T, K), generator=rng).cuda()
+    picks = [_picks(rng, T, K, E, how).cuda() for how in ("even", "elsewhere", "none", "skewed")]
+    want = [_experts((gate, up, down), x, p, weights, 10.0) for p in picks]
+    idx, out = picks[0].clone(), torch.zeros_like(x)
+    ws = torch.empty(pkg.w4_experts_workspace(gate, up, down, x, idx), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.w4_experts(gate, up, down, x, idx, weights, 10.0, out, ws)
+    for k in (0, 1, 2, 3, 1, 0):
+        idx.copy_(picks[k])
+        graph.replay()
+        assert torch.equal(out.cpu(), want[k])
+    pkg.w4_status()
