@@ -18,48 +18,91 @@ namespace g5b {
 constexpr int CV_WARPS = 8;
 constexpr int CV_COLS = 1024;      // columns a warp takes
 
-// Eight values from column c0 on (zero behind the last column); whole: 16-byte loads of eight that exist
+// Eight values from column c0 on, of rows that allow 16-byte loads (8 of FP8): zero behind the last column, which no load crosses.
 template <int DT>
-__device__ __forceinline__ void load8(float (&v)[8], const void *src, size_t at, int c0, int cols, bool whole)
+__device__ __forceinline__ void load8(float (&v)[8], const void *src, size_t at, int c0, int cols)
 {
-    if (whole && c0 + 8 <= cols) {
-        if (DT == DT_F32) {
-            const float4 a = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at));
-            const float4 b = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at + 4));
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else if (DT == DT_BF16) {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(src) + at));
-            bf16x2_to_f32(a.x, v[0], v[1]); bf16x2_to_f32(a.y, v[2], v[3]); bf16x2_to_f32(a.z, v[4], v[5]); bf16x2_to_f32(a.w, v[6], v[7]);
-        } else {
-            const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(src) + at));
-            e4m3x4_to_f32(a.x, v[0], v[1], v[2], v[3]);
-            e4m3x4_to_f32(a.y, v[4], v[5], v[6], v[7]);
-        }
-        return;
-    }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = 0.f;
-        if (c0 + i < cols)
-            v[i] = DT == DT_F32 ? static_cast<const float *>(src)[at + i] : DT == DT_BF16 ? bf16_to_f32(static_cast<const uint16_t *>(src)[at + i])
-                                                                                       : e4m3_to_f32(static_cast<const uint8_t *>(src)[at + i]);
+    for (int i = 0; i < 8; i++) v[i] = 0.f;
+    if (c0 >= cols) return;
+    if (DT == DT_F32) {
+        const float4 a = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at));
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        if (c0 + 4 >= cols) return;
+        const float4 b = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at + 4));
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else if (DT == DT_BF16) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(src) + at));
+        bf16x2_to_f32(a.x, v[0], v[1]); bf16x2_to_f32(a.y, v[2], v[3]); bf16x2_to_f32(a.z, v[4], v[5]); bf16x2_to_f32(a.w, v[6], v[7]);
+    } else {
+        const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(src) + at));
+        e4m3x4_to_f32(a.x, v[0], v[1], v[2], v[3]);
+        e4m3x4_to_f32(a.y, v[4], v[5], v[6], v[7]);
     }
+}
+// A lane's 32 values of rows that lie anyhow: the warp brings its piece of the row into shared memory in words, as they lie in memory, and a lane shifts
+// its own out of them, S words and a part of one more. A word of padding to S keeps lanes in different banks. (An element at a time, the lanes 32
+// columns apart: 6319 x 2649 BF16 weights there and back 80 us.)
+template <int DT> constexpr int cv_words = DT == DT_F32 ? 32 : DT == DT_BF16 ? 16 : 8;
+template <int DT> constexpr int cv_room = 33 * (cv_words<DT> + 1);
+template <int DT>
+__device__ __forceinline__ void load32(float (&v)[4][8], const uint8_t *src, size_t bytes, size_t row_at, int p0, int cols, uint32_t *room)
+{
+    constexpr int SIZE = DT == DT_F32 ? 4 : DT == DT_BF16 ? 2 : 1, S = cv_words<DT>, LOG = DT == DT_F32 ? 5 : DT == DT_BF16 ? 4 : 3;
+    const int lane = threadIdx.x & 31, n = min(CV_COLS, cols - p0);
+    const uint8_t *first = src + row_at + (size_t)p0 * SIZE;
+    const int off = (int)(reinterpret_cast<uintptr_t>(first) & 3u), words = n > 0 ? (off + n * SIZE + 3) / 4 : 0;
+    const uint8_t *base = first - off;
+    // (where the matrix begins or ends within a word, that one's bytes singly)
+    const int w0 = base < src, w1 = words - (words > 0 && base + 4 * (size_t)words > src + bytes);
+#pragma unroll 8
+    for (int w = w0 + lane; w < w1; w += 32) room[w + (w >> LOG)] = __ldcs(reinterpret_cast<const uint32_t *>(base) + w);
+    if (lane < 2 && words > 0 && (lane ? w1 < words : w0 > 0)) {
+        const int w = lane ? words - 1 : 0;
+        uint32_t x = 0;
+        for (int b = 0; b < 4; b++) {
+            const uint8_t *at = base + 4 * (size_t)w + b;
+            if (at >= src && at < src + bytes) x |= (uint32_t)*at << (8 * b);
+        }
+        room[w + (w >> LOG)] = x;
+    }
+    __syncwarp();
+    const uint32_t shift = 8u * (uint32_t)off;
+    uint32_t a = room[lane * (S + 1)];
+    float *out = &v[0][0];
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+        const int next = lane * S + k + 1;
+        const uint32_t b = SIZE == 4 && off == 0 && k + 1 == S ? 0u : room[next + (next >> LOG)], u = __funnelshift_r(a, b, shift);
+        if (DT == DT_F32) out[k] = __uint_as_float(u);
+        else if (DT == DT_BF16) bf16x2_to_f32(u, out[2 * k], out[2 * k + 1]);
+        else e4m3x4_to_f32(u, out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+        a = b;
+    }
+    if (p0 + lane * 32 + 32 > cols)
+#pragma unroll
+        for (int k = 0; k < 32; k++) if (p0 + lane * 32 + k >= cols) out[k] = 0.f;
 }
 
 // (five CTAs to an SM: 12288 x 4096 FP8 weights there and back 73.8 -> 70.2 us; six spill)
-template <int DT>
+template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(CV_WARPS * 32, 5) w4_quantize_kernel(W4Mat w, uint8_t *codes, uint16_t *scales, const void *src, const float *inv,
-                                                                    int br, int bc, int scols, unsigned pieces, bool whole)
+                                                                    int br, int bc, int scols, unsigned pieces)
 {
     const int lane = threadIdx.x & 31;
     const unsigned unit = blockIdx.x * CV_WARPS + (threadIdx.x >> 5), row_ = unit / pieces;
-    const int row = (int)row_, c0 = (int)(unit - row_ * pieces) * CV_COLS + lane * 32, per = w.group / 32;
+    const int row = (int)row_, p0 = (int)(unit - row_ * pieces) * CV_COLS, c0 = p0 + lane * 32, per = w.group / 32;
     if (row >= w.rows) return;
     float v[4][8];
+    if constexpr (!WHOLE) {
+        __shared__ uint32_t room[CV_WARPS][cv_room<DT>];
+        constexpr int SIZE = DT == DT_F32 ? 4 : DT == DT_BF16 ? 2 : 1;
+        load32<DT>(v, static_cast<const uint8_t *>(src), (size_t)w.rows * w.cols * SIZE, (size_t)row * w.cols * SIZE, p0, w.cols, room[threadIdx.x >> 5]);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int c = c0 + 8 * i;
-        load8<DT>(v[i], src, (size_t)row * w.cols + c, c, w.cols, whole);
+        if constexpr (WHOLE) load8<DT>(v[i], src, (size_t)row * w.cols + c, c, w.cols);
         if (DT == DT_FP8) {
             // the weight is the FP32 product of code and block scale
             const float *irow = inv + (size_t)(row / br) * scols;
@@ -139,12 +182,19 @@ void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const
     uint8_t *codes = const_cast<uint8_t *>(w.codes);
     uint16_t *scales = const_cast<uint16_t *>(w.scales);
     const int grid = (int)((units + CV_WARPS - 1) / CV_WARPS), scols = bc > 0 ? (w.cols + bc - 1) / bc : 0;
-    if (dt == DT_F32)       G5B_LAUNCH(w4_quantize_kernel<DT_F32>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
-    else if (dt == DT_BF16) G5B_LAUNCH(w4_quantize_kernel<DT_BF16>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
-    else                    G5B_LAUNCH(w4_quantize_kernel<DT_FP8>, grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, whole);
+#define QUANTIZE(DT)                                                                                                                            \
+    do {                                                                                                                                        \
+        if (whole) G5B_LAUNCH((w4_quantize_kernel<DT, true>), grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces);  \
+        else       G5B_LAUNCH((w4_quantize_kernel<DT, false>), grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces); \
+    } while (0)
+    if (dt == DT_F32)       QUANTIZE(DT_F32);
+    else if (dt == DT_BF16) QUANTIZE(DT_BF16);
+    else                    QUANTIZE(DT_FP8);
+#undef QUANTIZE
 }
 
-// A lane takes four columns at a time, so that a warp's store is 512 contiguous bytes of FP32 (eight columns a lane: 52 us for 12288 x 4096).
+// A lane takes four columns at a time, so that a warp's store is 512 contiguous bytes of FP32 (eight columns a lane: 52 us for 12288 x 4096); of
+// rows that do not allow that one column, the next lane the next.
 template <int DT>
 __global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, void *out, size_t ldo, unsigned pieces, bool whole)
 {
@@ -152,6 +202,20 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, v
     const unsigned unit = blockIdx.x * CV_WARPS + (threadIdx.x >> 5), row_ = unit / pieces;
     const int row = (int)row_, c_first = (int)(unit - row_ * pieces) * CV_COLS + lane * 4, log = w.group == 128 ? 7 : w.group == 64 ? 6 : 5;
     if (row >= w.rows) return;
+    if (!whole) {
+        const int p0 = c_first - lane * 4, n = min(CV_COLS, w.cols - p0);
+        const uint8_t *codes = w.codes + (size_t)row * w.pitch + p0 / 2;
+        const uint16_t *scales = w.scales + (size_t)row * w.sp;
+#pragma unroll 8
+        for (int c = lane; c < n; c += 32) {
+            const int q = (int)(((uint32_t)__ldg(codes + (c >> 1)) >> (4 * (c & 1))) & 15u) - 8;
+            const float v = __fmul_rn((float)q, bf16_to_f32(__ldg(scales + ((p0 + c) >> log))));
+            const size_t at = (size_t)row * ldo + p0 + c;
+            if (DT == DT_F32) __stcs(static_cast<float *>(out) + at, v);
+            else static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+        }
+        return;
+    }
     uint32_t code[CV_COLS / 128];
     float s[CV_COLS / 128];
 #pragma unroll
@@ -173,13 +237,13 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, v
         const size_t at = (size_t)row * ldo + c0;
         if (DT == DT_F32) {
             float *o = static_cast<float *>(out) + at;
-            if (whole && c0 + 4 <= w.cols) __stcs(reinterpret_cast<float4 *>(o), make_float4(v[0], v[1], v[2], v[3]));
+            if (c0 + 4 <= w.cols) __stcs(reinterpret_cast<float4 *>(o), make_float4(v[0], v[1], v[2], v[3]));
             else
                 for (int k = 0; k < 4 && c0 + k < w.cols; k++) o[k] = v[k];
         } else {
             // (3 significant bits times 8: rounded to BF16's 8, halves to even)
             __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(out) + at;
-            if (whole && c0 + 4 <= w.cols) {
+            if (c0 + 4 <= w.cols) {
                 __align__(8) const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
                 __stcs(reinterpret_cast<uint2 *>(o), *reinterpret_cast<const uint2 *>(h));
             } else

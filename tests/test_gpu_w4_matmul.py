@@ -295,6 +295,25 @@ def test_quantize_and_back(gpu_lib, rows, cols, group, kind):
     _compare(v, _convert(src, rows, cols, group), rows, cols, group)
 
 
+@pytest.mark.parametrize("kind,shifts", [("f32", (0, 1, 2, 3)), ("bf16", (0, 1, 3, 7)), ("fp8", (0, 1, 2, 3, 5))])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 3), (5, 31), (4, 1023), (3, 1025), (6, 2049), (37, 1282), (2, 4100)])
+def test_quantize_rows_that_lie_anyhow(gpu_lib, rows, cols, kind, shifts):
+    """Sources from any element on, beside numbers that would show (NaN); F32 and BF16 values back into rows of any distance."""
+    rng = torch.Generator().manual_seed(rows + cols)
+    v, scale = 0.02 * torch.randn((rows, cols), generator=rng), None
+    if kind == "bf16":
+        v = v.to(torch.bfloat16)
+    elif kind == "fp8":
+        scale = 1e-4 * (1 + torch.rand((-(-rows // 16), -(-cols // 12)), generator=rng))
+        v = (v * 5000).to(torch.float8_e4m3fn)
+    for shift in shifts:
+        buf = torch.full((rows * cols + 16,), float("nan"), device="cuda").to(v.dtype)
+        src = buf[shift:shift + rows * cols].view(rows, cols)
+        src.copy_(v)
+        vv = v.float() * scale.repeat_interleave(16, 0)[:rows].repeat_interleave(12, 1)[:, :cols] if kind == "fp8" else v.float()
+        _compare(vv, _convert(src, rows, cols, 64, scale, (16, 12)), rows, cols, 64)
+
+
 def test_quantize_borders(gpu_lib):
     """Quotients at, and one FP32 step to either side of, every half; groups of zeros, of subnormal and of huge values, and without numbers."""
     group, rows = 32, 64
