@@ -40,17 +40,17 @@ __device__ __forceinline__ void load8(float (&v)[8], const void *src, size_t at,
         e4m3x4_to_f32(a.y, v[4], v[5], v[6], v[7]);
     }
 }
-// A lane's 32 values of rows that lie anyhow: the warp brings its piece of the row into shared memory in words, as they lie in memory, and a lane shifts
-// its own out of them, S words and a part of one more. A word of padding to S keeps lanes in different banks. (An element at a time, the lanes 32
+// A lane's 32 values of rows that lie anyhow: the warp brings its n elements from e0 on into shared memory in words, as they lie in memory, and a lane
+// shifts its own out of them, from element `start` of those on, S words and a part of one more; zero behind the first `valid`. A word of padding to S keeps lanes in different banks. (An element at a time, the lanes 32
 // columns apart: 6319 x 2649 BF16 weights there and back 80 us.)
 template <int DT> constexpr int cv_words = DT == DT_F32 ? 32 : DT == DT_BF16 ? 16 : 8;
 template <int DT> constexpr int cv_room = 33 * (cv_words<DT> + 1);
 template <int DT>
-__device__ __forceinline__ void load32(float (&v)[4][8], const uint8_t *src, size_t bytes, size_t row_at, int p0, int cols, uint32_t *room)
+__device__ __forceinline__ void load32(float (&v)[4][8], const uint8_t *src, size_t bytes, size_t e0, int n, int start, int valid, uint32_t *room)
 {
     constexpr int SIZE = DT == DT_F32 ? 4 : DT == DT_BF16 ? 2 : 1, S = cv_words<DT>, LOG = DT == DT_F32 ? 5 : DT == DT_BF16 ? 4 : 3;
-    const int lane = threadIdx.x & 31, n = min(CV_COLS, cols - p0);
-    const uint8_t *first = src + row_at + (size_t)p0 * SIZE;
+    const int lane = threadIdx.x & 31;
+    const uint8_t *first = src + e0 * SIZE;
     const int off = (int)(reinterpret_cast<uintptr_t>(first) & 3u), words = n > 0 ? (off + n * SIZE + 3) / 4 : 0;
     const uint8_t *base = first - off;
     // (where the matrix begins or ends within a word, that one's bytes singly)
@@ -67,52 +67,60 @@ __device__ __forceinline__ void load32(float (&v)[4][8], const uint8_t *src, siz
         room[w + (w >> LOG)] = x;
     }
     __syncwarp();
-    const uint32_t shift = 8u * (uint32_t)off;
-    uint32_t a = room[lane * (S + 1)];
+    const int at = off + start * SIZE, word = at >> 2;
+    const uint32_t shift = 8u * (uint32_t)(at & 3);
+    uint32_t a = room[word + (word >> LOG)];
     float *out = &v[0][0];
 #pragma unroll
     for (int k = 0; k < S; k++) {
-        const int next = lane * S + k + 1;
-        const uint32_t b = SIZE == 4 && off == 0 && k + 1 == S ? 0u : room[next + (next >> LOG)], u = __funnelshift_r(a, b, shift);
+        const int next = word + k + 1;
+        const uint32_t b = room[next + (next >> LOG)], u = __funnelshift_r(a, b, shift);
         if (DT == DT_F32) out[k] = __uint_as_float(u);
         else if (DT == DT_BF16) bf16x2_to_f32(u, out[2 * k], out[2 * k + 1]);
         else e4m3x4_to_f32(u, out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
         a = b;
     }
-    if (p0 + lane * 32 + 32 > cols)
+    if (valid < 32)
 #pragma unroll
-        for (int k = 0; k < 32; k++) if (p0 + lane * 32 + k >= cols) out[k] = 0.f;
+        for (int k = 0; k < 32; k++) if (k >= valid) out[k] = 0.f;
 }
 
 // (five CTAs to an SM: 12288 x 4096 FP8 weights there and back 73.8 -> 70.2 us; six spill)
-template <int DT, bool WHOLE>
+template <int DT, bool WHOLE, bool NARROW>
 __global__ void __launch_bounds__(CV_WARPS * 32, 5) w4_quantize_kernel(W4Mat w, uint8_t *codes, uint16_t *scales, const void *src, const float *inv,
-                                                                    int br, int bc, int scols, unsigned pieces)
+                                                                    int br, int bc, int scols, unsigned pieces, int narrow_log)
 {
     const int lane = threadIdx.x & 31;
     const unsigned unit = blockIdx.x * CV_WARPS + (threadIdx.x >> 5), row_ = unit / pieces;
-    const int row = (int)row_, p0 = (int)(unit - row_ * pieces) * CV_COLS, c0 = p0 + lane * 32, per = w.group / 32;
-    if (row >= w.rows) return;
+    // Rows of up to 512 columns (NARROW) share a warp: 2^narrow_log lanes to one (16357 x 161 FP8 weights there and back in a warp each 35.0 us, so 18.7).
+    const int lanes_log = NARROW ? narrow_log : 5;
+    const int per_warp = 32 >> lanes_log, row0 = (int)row_ * per_warp, p0 = (int)(unit - row_ * pieces) * CV_COLS;
+    if (row0 >= w.rows) return;
+    const int own = lane >> lanes_log, c0 = p0 + (lane - (own << lanes_log)) * 32, per = w.group / 32;
+    const bool exists = row0 + own < w.rows;
+    const int row = exists ? row0 + own : w.rows - 1, cols = exists ? w.cols : 0;         // (a lane without a row takes zeros)
     float v[4][8];
     if constexpr (!WHOLE) {
         __shared__ uint32_t room[CV_WARPS][cv_room<DT>];
         constexpr int SIZE = DT == DT_F32 ? 4 : DT == DT_BF16 ? 2 : 1;
-        load32<DT>(v, static_cast<const uint8_t *>(src), (size_t)w.rows * w.cols * SIZE, (size_t)row * w.cols * SIZE, p0, w.cols, room[threadIdx.x >> 5]);
+        const int n = per_warp == 1 ? min(CV_COLS, w.cols - p0) : min(per_warp, w.rows - row0) * w.cols;
+        load32<DT>(v, static_cast<const uint8_t *>(src), (size_t)w.rows * w.cols * SIZE, (size_t)row0 * w.cols + p0, n, own * w.cols + c0 - p0, cols - c0,
+                   room[threadIdx.x >> 5]);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int c = c0 + 8 * i;
-        if constexpr (WHOLE) load8<DT>(v[i], src, (size_t)row * w.cols + c, c, w.cols);
+        if constexpr (WHOLE) load8<DT>(v[i], src, (size_t)row * w.cols + c, c, cols);
         if (DT == DT_FP8) {
             // the weight is the FP32 product of code and block scale
             const float *irow = inv + (size_t)(row / br) * scols;
             if (bc % 8 == 0) {
-                const float s = c < w.cols ? __ldg(irow + c / bc) : 0.f;
+                const float s = c < cols ? __ldg(irow + c / bc) : 0.f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[i][k] = __fmul_rn(v[i][k], s);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) if (c + k < w.cols) v[i][k] = __fmul_rn(v[i][k], __ldg(irow + (c + k) / bc));
+                for (int k = 0; k < 8; k++) if (c + k < cols) v[i][k] = __fmul_rn(v[i][k], __ldg(irow + (c + k) / bc));
             }
         }
     }
@@ -165,32 +173,39 @@ __global__ void __launch_bounds__(CV_WARPS * 32, 5) w4_quantize_kernel(W4Mat w, 
         }
         packed[i] = live ? word : 0x88888888u;
     }
+    if (!exists) return;
     if (c0 / 2 < w.pitch) *reinterpret_cast<uint4 *>(codes + (size_t)row * w.pitch + c0 / 2) = *reinterpret_cast<const uint4 *>(packed);
     const int group = c0 / w.group;
     if ((lane & (per - 1)) == 0 && group < w.sp)
         scales[(size_t)row * w.sp + group] = group >= w.groups ? (uint16_t)0 : finite ? __bfloat16_as_ushort(sb) : (uint16_t)0x7fc0;
+    if (per_warp > 1)                             // (scales behind what these lanes cover)
+        for (int g = (1 << lanes_log) / per + (c0 >> 5); g < w.sp; g += 1 << lanes_log) scales[(size_t)row * w.sp + g] = 0;
 }
 
 void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const float *scale, int br, int bc)
 {
     // the pieces cover the codes' and the scales' padding too, so that no byte of either is left undefined
-    const unsigned pieces = (max(w.pitch * 2, w.sp * w.group) + CV_COLS - 1) / CV_COLS;
-    const long long units = (long long)w.rows * pieces;
+    const int lanes_log = w.cols <= 128 ? 2 : w.cols <= 256 ? 3 : w.cols <= 512 ? 4 : 5;
+    const unsigned pieces = lanes_log < 5 ? 1 : (max(w.pitch * 2, w.sp * w.group) + CV_COLS - 1) / CV_COLS;
+    const long long units = (w.rows + (32 >> lanes_log) - 1ll) / (32 >> lanes_log) * pieces;
     const int size = dt == DT_F32 ? 4 : dt == DT_BF16 ? 2 : 1;
     const size_t align = dt == DT_FP8 ? 8 : 16;
     const bool whole = (reinterpret_cast<uintptr_t>(src) % align) == 0 && ((size_t)w.cols * size) % align == 0;
     uint8_t *codes = const_cast<uint8_t *>(w.codes);
     uint16_t *scales = const_cast<uint16_t *>(w.scales);
     const int grid = (int)((units + CV_WARPS - 1) / CV_WARPS), scols = bc > 0 ? (w.cols + bc - 1) / bc : 0;
-#define QUANTIZE(DT)                                                                                                                            \
-    do {                                                                                                                                        \
-        if (whole) G5B_LAUNCH((w4_quantize_kernel<DT, true>), grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces);  \
-        else       G5B_LAUNCH((w4_quantize_kernel<DT, false>), grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces); \
+    const bool narrow = lanes_log < 5;
+#define QUANTIZE_AS(DT, W, N) G5B_LAUNCH((w4_quantize_kernel<DT, W, N>), grid, CV_WARPS * 32, 0, st, w, codes, scales, src, scale, br, bc, scols, pieces, lanes_log)
+#define QUANTIZE(DT)                                                                  \
+    do {                                                                              \
+        if (whole) { if (narrow) QUANTIZE_AS(DT, true, true); else QUANTIZE_AS(DT, true, false); }    \
+        else       { if (narrow) QUANTIZE_AS(DT, false, true); else QUANTIZE_AS(DT, false, false); }  \
     } while (0)
     if (dt == DT_F32)       QUANTIZE(DT_F32);
     else if (dt == DT_BF16) QUANTIZE(DT_BF16);
     else                    QUANTIZE(DT_FP8);
 #undef QUANTIZE
+#undef QUANTIZE_AS
 }
 
 // A lane takes four columns at a time, so that a warp's store is 512 contiguous bytes of FP32 (eight columns a lane: 52 us for 12288 x 4096); of

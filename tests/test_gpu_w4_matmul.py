@@ -296,7 +296,8 @@ def test_quantize_and_back(gpu_lib, rows, cols, group, kind):
 
 
 @pytest.mark.parametrize("kind,shifts", [("f32", (0, 1, 2, 3)), ("bf16", (0, 1, 3, 7)), ("fp8", (0, 1, 2, 3, 5))])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 3), (5, 31), (4, 1023), (3, 1025), (6, 2049), (37, 1282), (2, 4100)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 3), (5, 31), (4, 1023), (3, 1025), (6, 2049), (37, 1282), (2, 4100),
+                                       (130, 20), (70, 100), (33, 128), (37, 161), (9, 256), (17, 504), (33, 511), (19, 512), (5, 513)])
 def test_quantize_rows_that_lie_anyhow(gpu_lib, rows, cols, kind, shifts):
     """Sources from any element on, beside numbers that would show (NaN); F32 and BF16 values back into rows of any distance."""
     rng = torch.Generator().manual_seed(rows + cols)
@@ -311,7 +312,8 @@ def test_quantize_rows_that_lie_anyhow(gpu_lib, rows, cols, kind, shifts):
         src = buf[shift:shift + rows * cols].view(rows, cols)
         src.copy_(v)
         vv = v.float() * scale.repeat_interleave(16, 0)[:rows].repeat_interleave(12, 1)[:, :cols] if kind == "fp8" else v.float()
-        _compare(vv, _convert(src, rows, cols, 64, scale, (16, 12)), rows, cols, 64)
+        group = (32, 64, 128)[shift % 3]
+        _compare(vv, _convert(src, rows, cols, group, scale, (16, 12)), rows, cols, group)
 
 
 def test_quantize_borders(gpu_lib):
