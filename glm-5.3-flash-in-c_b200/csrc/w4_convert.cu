@@ -10,7 +10,7 @@
 // Both directions are bound by HBM, the first nearly by the instructions a weight takes. There a lane takes 32 columns, so that what
 // is paid per group - the division, the reciprocal, the maximum's shuffles - is paid once for 32 weights, and its codes are one store;
 // eight columns a lane paid it four times, converted to integers by the slow instruction, and took 72 us for 12288 x 4096 BF16 weights. (With
-// residuals for BF16 weights too, every second warp met an exact half: 42 us.)
+// residuals for BF16 weights too, every second warp met an exact half: 42 us.) Both directions of those together take 55.8 us, 6.3 TB/s.
 #include "w4.cuh"
 
 namespace g5b {
@@ -209,7 +209,7 @@ void w4_quantize(cudaStream_t st, const W4Mat &w, const void *src, int dt, const
 }
 
 // A lane takes four columns at a time, so that a warp's store is 512 contiguous bytes of FP32 (eight columns a lane: 52 us for 12288 x 4096); of
-// rows that do not allow that one column, the next lane the next.
+// rows that do not allow that one column, the next lane the next (6319 x 2649 there and back 45 us in F32, 37 in BF16).
 template <int DT>
 __global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, void *out, size_t ldo, unsigned pieces, bool whole)
 {
@@ -218,17 +218,29 @@ __global__ void __launch_bounds__(CV_WARPS * 32) w4_dequantize_kernel(W4Mat w, v
     const int row = (int)row_, c_first = (int)(unit - row_ * pieces) * CV_COLS + lane * 4, log = w.group == 128 ? 7 : w.group == 64 ? 6 : 5;
     if (row >= w.rows) return;
     if (!whole) {
-        const int p0 = c_first - lane * 4, n = min(CV_COLS, w.cols - p0);
-        const uint8_t *codes = w.codes + (size_t)row * w.pitch + p0 / 2;
-        const uint16_t *scales = w.scales + (size_t)row * w.sp;
-#pragma unroll 8
-        for (int c = lane; c < n; c += 32) {
-            const int q = (int)(((uint32_t)__ldg(codes + (c >> 1)) >> (4 * (c & 1))) & 15u) - 8;
-            const float v = __fmul_rn((float)q, bf16_to_f32(__ldg(scales + ((p0 + c) >> log))));
-            const size_t at = (size_t)row * ldo + p0 + c;
-            if (DT == DT_F32) __stcs(static_cast<float *>(out) + at, v);
-            else static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+        // a lane's word holds the codes of eight columns and goes round by shuffles; 32 columns have one scale
+        const int p0 = c_first - lane * 4, words = w.pitch / 4 - p0 / 8;
+        const uint32_t *codes = reinterpret_cast<const uint32_t *>(w.codes + (size_t)row * w.pitch) + p0 / 8;
+        uint32_t word[CV_COLS / 256];
+        float scale[CV_COLS / 256];
+#pragma unroll
+        for (int q = 0; q < CV_COLS / 256; q++) {
+            const int c = p0 + q * 256 + (lane & 7) * 32;
+            word[q] = q * 32 + lane < words ? __ldg(codes + q * 32 + lane) : 0u;
+            scale[q] = c < w.cols ? bf16_to_f32(__ldg(w.scales + (size_t)row * w.sp + (c >> log))) : 0.f;
         }
+#pragma unroll
+        for (int q = 0; q < CV_COLS / 256; q++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int c = p0 + q * 256 + k * 32 + lane;
+                if (c - lane >= w.cols) break;
+                const uint32_t from = __shfl_sync(0xffffffffu, word[q], 4 * k + (lane >> 3));
+                const float s = __shfl_sync(0xffffffffu, scale[q], k), v = __fmul_rn((float)((int)((from >> (4 * (lane & 7))) & 15u) - 8), s);
+                if (c >= w.cols) continue;
+                if (DT == DT_F32) __stcs(static_cast<float *>(out) + (size_t)row * ldo + c, v);
+                else static_cast<__nv_bfloat16 *>(out)[(size_t)row * ldo + c] = __float2bfloat16_rn(v);
+            }
         return;
     }
     uint32_t code[CV_COLS / 128];
