@@ -313,33 +313,18 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
                         sc.x &= last > 1 ? 0xffffffffu : 0xffffu;
                         sc.y &= last > 3 ? 0xffffffffu : last > 2 ? 0xffffu : 0u;
                     }
-                    // the largest scale's exponent, far from FP32's ends so that no power of two leaves it, and whether none is below 2^-8 of it (a
-                    // zero counts as one that is)
-                    const uint32_t x0 = sc.x & 0x7fff7fffu, y0 = sc.y & 0x7fff7fffu, m2 = __vmaxu2(x0, y0);
-                    const int top = max((int)(max(m2 & 0xffffu, m2 >> 16) >> 7), 1);
-                    const uint32_t least = (uint32_t)max(top - 8, 0) * 0x00800080u;
-                    fused = __all_sync(0xffffffffu, __vmaxu2(x0, least) == x0 && __vmaxu2(y0, least) == y0 && top >= 40 && top <= 220);
-                    if (fused) {
-                        // BF16's exponent becomes F16's, 30 for the largest: two scales by one subtraction and a shift
-                        const uint32_t base = (uint32_t)(top - 30) * 0x00800080u;
-                        const uint32_t h0 = ((x0 - base) << 3) | (sc.x & 0x80008000u), h1 = ((y0 - base) << 3) | (sc.y & 0x80008000u);
-                        s_down[step & (WM_RING - 1)][b][r] = pow2(24 - (15 + 127 - top));
+                    // exponents of the largest scale and the smallest that is not zero; far from FP32's ends, so that no power of two leaves it
+                    const uint32_t x0 = sc.x & 0x7fff7fffu, y0 = sc.y & 0x7fff7fffu, m2 = __vmaxu2(x0, y0), l2 = __vminu2(__vsub2(x0, 0x00010001u), __vsub2(y0, 0x00010001u));
+                    const int top = max((int)(max(m2 & 0xffffu, m2 >> 16) >> 7), 1), low = (int)((min(l2 & 0xffffu, l2 >> 16) + 1) >> 7);
+                    fused = __all_sync(0xffffffffu, top - low <= 8 && top >= 40 && top <= 220);
+                    const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 126);
+                    const float up = pow2(e);
+                    s_down[step & (WM_RING - 1)][b][r] = fused ? pow2(24 - e) : pow2(-e);
 #pragma unroll
-                        for (int piece = 0; piece < 4; piece++) {
-                            const int g = (4 * kb + piece) >> per;
-                            const uint32_t twice = __byte_perm(g & 2 ? h1 : h0, 0u, g & 1 ? 0x3232u : 0x1010u);
-                            s2[piece] = *reinterpret_cast<const __half2 *>(&twice);
-                        }
-                    } else {
-                        const int e = min(11 + 127 - top, 126);
-                        const float up = pow2(e);
-                        s_down[step & (WM_RING - 1)][b][r] = pow2(-e);
-#pragma unroll
-                        for (int piece = 0; piece < 4; piece++) {
-                            const int g = (4 * kb + piece) >> per;
-                            const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
-                            s2[piece] = __float2half2_rn(bf16_to_f32((uint16_t)raw) * up);
-                        }
+                    for (int piece = 0; piece < 4; piece++) {
+                        const int g = (4 * kb + piece) >> per;
+                        const uint32_t raw = (g & 2 ? sc.y : sc.x) >> (g & 1 ? 16 : 0);
+                        s2[piece] = __float2half2_rn(bf16_to_f32((uint16_t)raw) * up);
                     }
                 }
                 uint64_t *full = &w_full[ws], *free_ = &a_empty[b][as];
