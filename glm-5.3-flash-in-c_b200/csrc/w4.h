@@ -51,7 +51,6 @@ struct W4Job {
     const void *x; int x_dt; size_t ldx;        // w4_few: the activations (dense, gate/up: the caller's; down: F32 rows of picks)
     const int *order; int topk;                 // w4_few, gate/up: the activation row of sorted row i is order[i] / topk
     const int *idx;             // w4_few: not sorted, every pick a slot of its own (32 at most; slots and order are not used then)
-    bool half;                  // w4_few, down: the caller's rows are BF16
     bool early;                 // w4_few: may be scheduled while the kernel before it drains
     W4Terms terms;              // w4_many: the activations as terms, in the order of the rows
     W4Slots slots;
@@ -59,9 +58,9 @@ struct W4Job {
     float limit;
 };
 // Rows that w4_few takes at a time, of a matrix of so many columns (0: none). Dense products of up to as many are its (past three
-// or four F32 rows the weights twice take 20.8 us for 12288 x 4096 in groups of 32, w4_many 17.6).
-int  w4_few_rows(int dt, int cols);
-inline bool w4_few_takes(int dt, int cols, int T) { return T <= w4_few_rows(dt, cols); }
+// or four rows the weights twice take 20.8 us for 12288 x 4096 in groups of 32, w4_many 17.6).
+int  w4_few_rows(int cols);
+inline bool w4_few_takes(int cols, int T) { return T <= w4_few_rows(cols); }
 int  w4_few(cudaStream_t st, const W4Job &job);
 int  w4_few_status(cudaStream_t st);
 constexpr int W4_MANY_ROWS = 64;

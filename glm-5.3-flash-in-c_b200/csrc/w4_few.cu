@@ -1,5 +1,5 @@
 // w4_few.cu - 4-bit weights times a few rows of activations: a decoded token or two, the few tokens of an expert in a batch. Eight columns at
-// a time: two F32 rows, four of BF16. (Four F32 rows in two sets of columns: an item of three or four rows takes 1.5 times as long as one of
+// a time: two rows of four digits, F32 or BF16. (Four rows in two sets of columns: an item of three or four rows takes 1.5 times as long as one of
 // two, and CTAs that have such items end last. Experts of 64 tokens 831 us against 752.)
 //
 // Bound by HBM: half a byte and a scale's share per weight (154880 x 4096 past one row 54.3 us, 6.0 TB/s; a launch's start and end are 4 of them,
@@ -25,7 +25,10 @@
 //             a lane takes its words 16 bytes apart, so that an MMA is 32 columns of one group.
 //   x         becomes digits in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
 //             which the lanes read them: per row and block of 128 columns the power of two below which its values lie, and
-//             integers of 23 bits and a sign in three digits (BF16 rows: 15 bits in two), one bit less where the largest needs it.
+//             integers of 31 bits and a sign in four digits, one bit less where the largest needs it: an FP32 number down to 2^-6 of the block's largest and a
+//             BF16 one down to 2^-22 as they are, what is smaller off by one unit, 2^-29 of the largest, at most. (Three digits of F32 rows and two of BF16
+//             ones, four of which then fit, were off by 2^-22 and 2^-14 of the largest: by 3e-5 and 8e-3 of a product whose weights of columns a
+//             thousand times the others are small. The fourth digit takes a column that was idle.)
 // Group sums are exact integers, taken into FP32 by the exponent trick (they start at the bits of 1.5 2^23, so that their bits are the
 // float 1.5 2^23 + sum, |sum| < 2^22; in groups of 128 sixteenths of 1.5 2^19); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
@@ -37,6 +40,8 @@ namespace g5b {
 
 constexpr int FW_WARPS = 16, FW_THREADS = (FW_WARPS + 1) * 32;
 constexpr int FW_COLS = 8;                           // activation columns of an MMA
+constexpr int FW_DIGITS = 4;                         // of an activation, a column each
+constexpr int FW_ROWS = FW_COLS / FW_DIGITS;
 constexpr int FW_PIECE = 4096;                       // weight columns of a stage at most (half of them where that leaves too few stages): 16 chunks of 128 bytes
 constexpr int FW_DIGIT_BYTES = 88 * 1024;            // room for the digits
 constexpr int FW_MAX_STAGES = 12;
@@ -110,18 +115,18 @@ template <int NS, bool WHOLE> struct FewBlock {
 };
 
 // The 512 consumer threads: rows of an item as digits; 16 lanes hold a block.
-template <int TERMS, int MODE, bool WHOLE, int NS, typename IN>
+template <int MODE, bool WHOLE, int NS, typename IN>
 __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, FewBlock<NS, WHOLE> *blocks)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = it.count <= 1 ? 1 : it.count <= 2 ? 2 : 4, per = FW_WARPS / rows;    // warps to a row
+    const int rows = it.count <= 1 ? 1 : FW_ROWS, per = FW_WARPS / rows;    // warps to a row
     const int i = warp / per;
     bar_sync(1, FW_WARPS * 32);                          // nobody reads the digits of the rows before any more
     if (i < it.count) {
         const int at = it.first + i;
         const int src = MODE != W4_GATEUP ? at : (a.idx ? at : __ldg(a.order + at)) / a.topk;
         const IN *row = static_cast<const IN *>(a.x) + (size_t)src * a.ldx;
-        const int col = i * TERMS;
+        const int col = i * FW_DIGITS;
         for (int c0 = (warp - i * per) * 256; c0 < a.blocks * 128; c0 += per * 256) {
             const int c = c0 + lane * 8;
             float v[8];
@@ -132,29 +137,28 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             const bool finite = m < 0x7f800000u;
-            // 2^(e - 1) <= max < 2^e (a subnormal one counts as 2^-126)
-            // One more bit where the largest leaves the highest digit below 128.
-            const int e = max((int)(m >> 23), 1) - 126, bits = TERMS == 3 ? 22 : 14;
-            const float most = TERMS == 3 ? 127.0f * 65536.0f + 127.0f * 256.0f + 127.0f : 127.0f * 256.0f + 127.0f;
-            const int up = bits - e + (__uint_as_float(m) * few_pow2((bits + 1 - e) >> 1) * few_pow2(bits + 1 - e - ((bits + 1 - e) >> 1)) * (WHOLE ? 1.0625f : 1.0f) <= most);   // -114 <= up <= 148
+            // 2^(e - 1) <= max < 2^e (a subnormal one counts as 2^-126). One more bit where the largest leaves the highest digit below 128. (A unit
+            // is 2^-149 at least, the smallest FP32 number, of which all others are multiples.)
+            const int e = max((int)(m >> 23), 1) - 126;
+            constexpr float MOST = 127.0f * 16777216.0f + 127.0f * 65536.0f + 127.0f * 256.0f;
+            const float largest = __uint_as_float(m) * few_pow2((31 - e) >> 1) * few_pow2(31 - e - ((31 - e) >> 1));
+            const int up = min(30 - e + (largest * (WHOLE ? 1.0625f : 1.0f) <= MOST), 149);          // -98 <= up
             const float scale = few_pow2(up >> 1), scale2 = few_pow2(up - (up >> 1));
-            if (!finite)
+            int x[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = 0.f;
+            for (int k = 0; k < 8; k++) x[k] = finite ? __float2int_rn(v[k] * scale * scale2) : 0;
+            if (WHOLE)                                   // (the odd columns' integers, so that what they are off goes with their own weights alone)
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = v[k] * scale * scale2;
-            if (WHOLE)
-#pragma unroll
-                for (int k = 0; k < 8; k += 2) v[k] = fmaf(v[k + 1], -0.0625f, v[k]);
-            uint32_t even[TERMS] = {}, odd[TERMS] = {};  // digits of columns 0 2 4 6 and 1 3 5 7
-            int sum[TERMS] = {};
+                for (int k = 0; k < 8; k += 2) x[k] -= (x[k + 1] + 8) >> 4;
+            uint32_t even[FW_DIGITS] = {}, odd[FW_DIGITS] = {};  // digits of columns 0 2 4 6 and 1 3 5 7
+            int sum[FW_DIGITS] = {};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                int x = __float2int_rn(v[k]);
+                int rest = x[k];
 #pragma unroll
-                for (int d = 0; d < TERMS; d++) {
-                    const int digit = d + 1 < TERMS ? (int)(int8_t)x : x;
-                    x = (x - digit) >> 8;
+                for (int d = 0; d < FW_DIGITS; d++) {
+                    const int digit = d + 1 < FW_DIGITS ? (int)(int8_t)rest : rest;
+                    rest = (rest - digit) >> 8;
                     sum[d] += digit * (WHOLE ? (k & 1 ? 136 : 128) : 8);
                     (k & 1 ? odd : even)[d] |= (uint32_t)(digit & 255) << (8 * (k >> 1));
                 }
@@ -164,7 +168,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
             const int w = (c & 127) >> 3, j = WHOLE ? w & 3 : w >> 2, t = WHOLE ? w >> 2 : w & 3;
             const int span = a.w.group == 128 ? 16 : a.w.group == 64 ? 8 : 4;          // lanes of a group
 #pragma unroll
-            for (int d = 0; d < TERMS; d++) {
+            for (int d = 0; d < FW_DIGITS; d++) {
                 for (int o = 1; o < span; o <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], o);
                 if (!here) continue;
                 if (WHOLE) {
@@ -175,9 +179,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
                     reinterpret_cast<uint2 *>(&b.digits[j >> 1][col + d][t])[j & 1] = make_uint2(even[d], odd[d]);
                     if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = few_magic<WHOLE> - sum[d];
                 }
-                // (2^-148 at least, a subnormal FP32 number)
-                if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(-(up - (up >> 1))) * (d == 0 ? 1.0f : d == 1 ? 256.0f : 65536.0f)
-                                                            : __int_as_float(0x7fc00000);
+                if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(8 * d - (up - (up >> 1))) : __int_as_float(0x7fc00000);
             }
         }
     }
@@ -185,8 +187,8 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
     bar_sync(1, FW_WARPS * 32);
 }
 
-// TERMS: digits of an activation. WHOLE: groups of 128. NS: columns that there is room for. U: sixteens of weight rows of an item.
-template <int TERMS, int MODE, bool WHOLE, int NS, int U>
+// IN: of activations. WHOLE: groups of 128. NS: columns that there is room for. U: sixteens of weight rows of an item.
+template <typename IN, int MODE, bool WHOLE, int NS, int U>
 __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_constant__ FewMaps maps, const FewArgs a)
 {
     constexpr int HALVES = MODE == W4_GATEUP ? 2 : 1, HALF_ROWS = 16 * U / HALVES;
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
     Block *blocks = reinterpret_cast<Block *>(smem + (size_t)2 * a.stages * a.stage_bytes);
     // A team waits for every use of its stages, so none of its waits can take an earlier use's phase for the one it waits for.
     __shared__ uint64_t full[2][FW_MAX_STAGES], empty[2][FW_MAX_STAGES];
-    __shared__ float s_sum[2][2][8][16 * U][FW_COLS];                                // [team][item's parity][warp][row][column]
+    __shared__ __align__(16) float s_sum[2][2][8][16 * U][FW_COLS];                                // [team][item's parity][warp][row][column]
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     int *err = &g_few_err;
     pdl_trigger();
@@ -279,8 +281,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
             const int src = MODE == W4_GATEUP && a.idx ? it.first / a.topk : -1;      // (a token's picks: the same row)
             if (it.count && (src < 0 || src != have)) {
                 have = src;
-                if (MODE == W4_DOWN || TERMS == 3) few_digits<TERMS, MODE, WHOLE, NS, float>(a, it, blocks);
-                else                               few_digits<TERMS, MODE, WHOLE, NS, uint16_t>(a, it, blocks);
+                few_digits<MODE, WHOLE, NS, IN>(a, it, blocks);
             }
             fresh = false;
         }
@@ -397,15 +398,18 @@ constexpr int MOST = FW_PIECE / 1024 / U;
                 bar_sync(2 + team, 256);
                 constexpr int OUT = MODE == W4_GATEUP ? 8 : 16 * U;           // outputs of a row of x
                 if (gt < OUT * it.count) {
-                    const int r = gt & (OUT - 1), k = gt / OUT, col = k * TERMS;
-                    float v = 0.f, u = 0.f;
+                    const int r = gt & (OUT - 1), k = gt / OUT, col = k * FW_DIGITS;
+                    auto total = [&](int r) {            // digit by digit, the least first
+                        float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int w = 0; w < 8; w++)
-#pragma unroll
-                        for (int m = 0; m < TERMS; m++) {
-                            v += sum[w][r][col + m];
-                            if (MODE == W4_GATEUP) u += sum[w][r + 8][col + m];
+                        for (int w = 0; w < 8; w++) {
+                            const float4 in = *reinterpret_cast<const float4 *>(&sum[w][r][col]);
+                            d.x += in.x; d.y += in.y; d.z += in.z; d.w += in.w;
                         }
+                        return ((d.x + d.y) + d.z) + d.w;
+                    };
+                    float v = total(r);
+                    const float u = MODE == W4_GATEUP ? total(r + 8) : 0.f;
                     if (MODE == W4_GATEUP) v = swiglu_value(v, u, a.limit);
                     const int row = it.tile * OUT + r;
                     const size_t at = (size_t)(it.first + k) * a.ldy + row;
@@ -421,7 +425,7 @@ constexpr int MOST = FW_PIECE / 1024 / U;
     }
 }
 
-template <int TERMS, int MODE, bool WHOLE, int NS, int U>
+template <typename IN, int MODE, bool WHOLE, int NS, int U>
 static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
     static SmemGrant grant;
@@ -430,44 +434,39 @@ static int few_launch(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
     const size_t smem = 1024 + (size_t)2 * a.stages * a.stage_bytes + digit_bytes;
     if (a.stages < 1) { set_last_error("a 4-bit product has no room for its stages"); return -1; }
     // (what counts is this and the sums: more than 48 KB of them must be asked for)
-    if (!dev_opt_in_smem((const void *)w4_few_kernel<TERMS, MODE, WHOLE, NS, U>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
+    if (!dev_opt_in_smem((const void *)w4_few_kernel<IN, MODE, WHOLE, NS, U>, std::max(smem, (size_t)64 * 1024), grant)) return -1;
     const long long items = (long long)a.tiles * (MODE == W4_DENSE ? 1 : a.idx ? a.n : a.slots.max);
     const int grid = (int)std::min<long long>(items, dev_sms());
-    if (early) G5B_LAUNCH_PDL((w4_few_kernel<TERMS, MODE, WHOLE, NS, U>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
-    else       G5B_LAUNCH((w4_few_kernel<TERMS, MODE, WHOLE, NS, U>), grid, FW_THREADS, smem, st, m, a);
+    if (early) G5B_LAUNCH_PDL((w4_few_kernel<IN, MODE, WHOLE, NS, U>), dim3(grid), dim3(FW_THREADS), smem, st, m, a);
+    else       G5B_LAUNCH((w4_few_kernel<IN, MODE, WHOLE, NS, U>), grid, FW_THREADS, smem, st, m, a);
     return 0;
 }
-constexpr int few_one(int terms) { return terms == 3 ? 4 : 2; }          // columns of a single row, with one to spare
-template <int TERMS, int MODE, bool WHOLE>
+template <typename IN, int MODE, bool WHOLE>
 static int few_columns(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
     if constexpr (MODE != W4_GATEUP)
         if (a.sixteens == 2)
-            return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS), 2>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS, 2>(st, m, a, early);
-    return a.per == 1 ? few_launch<TERMS, MODE, WHOLE, few_one(TERMS), 1>(st, m, a, early) : few_launch<TERMS, MODE, WHOLE, FW_COLS, 1>(st, m, a, early);
+            return a.per == 1 ? few_launch<IN, MODE, WHOLE, FW_DIGITS, 2>(st, m, a, early) : few_launch<IN, MODE, WHOLE, FW_COLS, 2>(st, m, a, early);
+    return a.per == 1 ? few_launch<IN, MODE, WHOLE, FW_DIGITS, 1>(st, m, a, early) : few_launch<IN, MODE, WHOLE, FW_COLS, 1>(st, m, a, early);
 }
-template <int TERMS, int MODE>
+template <typename IN, int MODE>
 static int few_group(cudaStream_t st, const FewMaps &m, FewArgs &a, bool early)
 {
-    return a.w.group == 128 ? few_columns<TERMS, MODE, true>(st, m, a, early) : few_columns<TERMS, MODE, false>(st, m, a, early);
+    return a.w.group == 128 ? few_columns<IN, MODE, true>(st, m, a, early) : few_columns<IN, MODE, false>(st, m, a, early);
 }
 
-// What a block's digits take: of one row (with a column to spare), of what eight columns hold.
-static size_t few_block(int dt, int rows)
-{
-    return rows > 1 ? sizeof(FewBlock<FW_COLS, false>) : dt == DT_F32 ? sizeof(FewBlock<few_one(3), false>) : sizeof(FewBlock<few_one(2), false>);
-}
-// Rows of a tile for a matrix of so many columns: what eight columns hold if there is room for their digits, else one row or none.
-int w4_few_rows(int dt, int cols)
+// What a block's digits take: of one row, of two.
+static size_t few_block(int rows) { return rows > 1 ? sizeof(FewBlock<FW_COLS, false>) : sizeof(FewBlock<FW_DIGITS, false>); }
+// Rows of a tile for a matrix of so many columns: two if there is room for their digits, else one or none.
+int w4_few_rows(int cols)
 {
     const size_t blocks = w4_kp(cols) / 128;
-    return blocks * few_block(dt, 2) <= (size_t)FW_DIGIT_BYTES ? (dt == DT_F32 ? 2 : 4) : blocks * few_block(dt, 1) <= (size_t)FW_DIGIT_BYTES ? 1 : 0;
+    return blocks * few_block(FW_ROWS) <= (size_t)FW_DIGIT_BYTES ? FW_ROWS : blocks * few_block(1) <= (size_t)FW_DIGIT_BYTES ? 1 : 0;
 }
 
 int w4_few(cudaStream_t st, const W4Job &j)
 {
     FewArgs a{};
-    const bool bf16 = j.x_dt == DT_BF16 || (j.mode == W4_DOWN && j.half);
     const int size = j.x_dt == DT_F32 ? 4 : 2;
     a.w = j.w; a.x = j.x; a.ldx = j.ldx; a.x_dt = j.x_dt; a.cols = j.w.cols; a.blocks = w4_kp(j.w.cols) / 128;
     a.wide = reinterpret_cast<uintptr_t>(j.x) % 16 == 0 && j.ldx * size % 16 == 0;
@@ -480,7 +479,7 @@ int w4_few(cudaStream_t st, const W4Job &j)
     a.tiles = (j.w.rows + half_rows - 1) / half_rows;
     a.whole_rows = j.w.pitch % 128 == 0;
     // Two stages of each team at least: with many digits beside them in pieces of half the columns.
-    const size_t digits = (size_t)a.blocks * few_block(bf16 ? DT_BF16 : DT_F32, a.per);
+    const size_t digits = (size_t)a.blocks * few_block(a.per);
     for (a.piece = FW_PIECE / 128;; a.piece /= 2) {
         a.chunks = std::min(a.piece / 2, (j.w.pitch + 127) / 128);
         a.scale_cols = std::min(a.piece * 128 / j.w.group, j.w.sp);
@@ -505,9 +504,9 @@ int w4_few(cudaStream_t st, const W4Job &j)
             return -1;
         }
     }
-    if (bf16)
-        return j.mode == W4_DENSE ? few_group<2, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<2, W4_GATEUP>(st, m, a, j.early) : few_group<2, W4_DOWN>(st, m, a, j.early);
-    return j.mode == W4_DENSE ? few_group<3, W4_DENSE>(st, m, a, j.early) : j.mode == W4_GATEUP ? few_group<3, W4_GATEUP>(st, m, a, j.early) : few_group<3, W4_DOWN>(st, m, a, j.early);
+    if (j.mode == W4_DOWN) return few_group<float, W4_DOWN>(st, m, a, j.early);
+    if (j.x_dt == DT_BF16) return j.mode == W4_DENSE ? few_group<uint16_t, W4_DENSE>(st, m, a, j.early) : few_group<uint16_t, W4_GATEUP>(st, m, a, j.early);
+    return j.mode == W4_DENSE ? few_group<float, W4_DENSE>(st, m, a, j.early) : few_group<float, W4_GATEUP>(st, m, a, j.early);
 }
 
 int w4_few_status(cudaStream_t st) { return w4_flag(g_few_err, st); }

@@ -119,16 +119,16 @@ int check_ws(const char *op, const void *ws, size_t have, size_t need)
 // How a call of the experts goes: PICKS (every pick on its own, nothing is sorted), FEW (w4_few on sorted picks), MANY (w4_many) or EITHER.
 // PICKS saves the sort, 7 us, and reads an expert twice that two picks have, 2 us each: n picks of E experts have n^2 / 2E such pairs
 // (three tokens of 288 experts 70.2 -> 63.6 us, four 84.5 -> 77.2).
-// FEW reads an expert's weights for every two F32 rows or four of BF16, MANY once, at the speed of its conversion: 1 row to an expert 604 against 835 us,
-// 2 (F32) 818 against 968, 2.8 the same; BF16 2.8 rows 712 against 944, 4 889 against 982, 5.3 1092 against 1003.
+// FEW reads an expert's weights for every two rows, MANY once, at the speed of its conversion: 1 row to an expert 604 against 835 us,
+// 2 818 against 968, 2.8 the same (F32).
 // How many picks are here only the device knows: of a rank's call one in eight may be. EITHER: the sort chooses, and the other kind's
-// kernels find nothing to do, 4 us in all (a rank of 36 experts: 32 tokens 135 us by w4_many, 101 so; 64 tokens 160 and 139, BF16 145 and 117).
+// kernels find nothing to do, 4 us in all (a rank of 36 experts: 32 tokens 135 us by w4_many, 101 so; 64 tokens 160 and 139, BF16 145 and 141).
 enum { PICKS, FEW, MANY, EITHER };
 struct ExpertsPlan { int how, rows; };           // rows of a slot at most
 constexpr int PICKS_ALWAYS = 16, PICKS_MOST = 32, RANKS = 8;
-ExpertsPlan experts_plan(int dt, int T, int topk, int E, int H, int I)
+ExpertsPlan experts_plan(int T, int topk, int E, int H, int I)
 {
-    const int n = T * topk, h = w4_few_rows(dt, H), i = w4_few_rows(dt, I), rows = h < i ? h : i;
+    const int n = T * topk, h = w4_few_rows(H), i = w4_few_rows(I), rows = h < i ? h : i;
     if (rows && n <= PICKS_MOST && (n <= PICKS_ALWAYS || n * n <= 4 * E)) return {PICKS, 1};
     if (rows > 1 && n <= rows * E) return {FEW, rows};
     if (rows > 1 && n <= RANKS * rows * E) return {EITHER, rows};
@@ -205,7 +205,7 @@ extern "C" size_t g5b_w4_matmul_workspace(const g5b_w4 *m, int dtype, int T)
     if (!m || m->cols < 1 || m->cols > W4_MAX_COLS || T < 0 || T > W4_MAX_TOKENS) return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2;
-    if (w4_few_takes(dtype, m->cols, T)) return WS_ALIGN;
+    if (w4_few_takes(m->cols, T)) return WS_ALIGN;
     terms_of(ws, n_terms, m->cols, T);
     ws.take<float>(w4_many_part_floats(m->rows, m->cols, T));
     return ws.used;
@@ -226,7 +226,7 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     Pieces ws{static_cast<uint8_t *>(workspace)};
     j.mode = W4_DENSE; j.T = T; j.count = 1; j.n_terms = dtype == DT_BF16 ? 1 : 2;
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
-    if (w4_few_takes(dtype, j.w.cols, T)) {
+    if (w4_few_takes(j.w.cols, T)) {
         j.x = x; j.x_dt = dtype; j.ldx = ldx;
         return w4_few(st, j) ? -1 : launched(op);
     }
@@ -285,7 +285,7 @@ extern "C" size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *dow
         return 0;
     Pieces ws{nullptr};
     const int n_terms = dtype == DT_BF16 ? 1 : 2, rows = T < 1 ? 1 : T;
-    experts_ws(ws, experts_plan(dtype, rows, topk, gate->count, gate->cols, down->cols), n_terms, rows, topk, gate->count, gate->cols, down->cols);
+    experts_ws(ws, experts_plan(rows, topk, gate->count, gate->cols, down->cols), n_terms, rows, topk, gate->count, gate->cols, down->cols);
     return ws.used;
 }
 
@@ -307,7 +307,7 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int E = gate->count, H = wg.cols, I = wg.rows, n = T * topk, n_terms = dtype == DT_BF16 ? 1 : 2;
     Pieces pieces{static_cast<uint8_t *>(workspace)};
-    const ExpertsPlan plan = experts_plan(dtype, T, topk, E, H, I);
+    const ExpertsPlan plan = experts_plan(T, topk, E, H, I);
     const ExpertsWs ws = experts_ws(pieces, plan, n_terms, T, topk, E, H, I);
     W4Job j{};
     j.count = E; j.n_terms = n_terms; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
@@ -327,7 +327,7 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     if ((few && w4_few(st, j)) || (many && w4_many(st, jm, nullptr))) return -1;
     if (many) w4_split(st, ws.h, ws.act, DT_F32, I, n, I, many_n, nullptr, 1, true);
     j.mode = W4_DOWN; j.w = wd; j.y = ws.rows; j.ldy = H;
-    j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true; j.half = dtype == DT_BF16;
+    j.x = ws.act; j.x_dt = DT_F32; j.ldx = I; j.terms = ws.h; j.early = true;
     jm = j;
     jm.slots = many_slots;
     if ((few && w4_few(st, j)) || (many && w4_many(st, jm, nullptr))) return -1;

@@ -436,8 +436,8 @@ int g5b_w4_quantize(const g5b_tensor *src, int br, int bc, const g5b_w4 *dst, vo
 int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *stream);
 
 /* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Sums are FP32 or exact integers. What an activation
- * is held to: in calls of a few rows 2^-22 (BF16 rows 2^-14) of the largest of the 128 columns it lies in, from a multiple of 128 on, or
- * better; in calls of many rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
+ * is held to: in calls of one or two rows 2^-29 of the largest of the 128 columns it lies in, from a multiple of 128 on, or
+ * better; in calls of more rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
  * scales within 128 columns differ by more than 2^28 has products off by up to 2^-36 of the largest scale times the
  * activation; all others are exact. A row of x with an infinity or NaN gives NaN in all of its outputs. */
 size_t g5b_w4_matmul_workspace(const g5b_w4 *w, int dtype, int T);
@@ -461,7 +461,8 @@ int g5b_expert_combine(const void *rows, int dtype, size_t ldr, const int32_t *p
 
 /* Routed experts in 4 bits (the routed part of g5b_op_moe): gate and up [count][inter][hidden], down [count][hidden][inter];
  * out[t] = sum over k of weights[t][k] down_e (silu(min(gate_e x, limit)) clamp(up_e x, -limit, limit)), e = idx[t][k], with the sort
- * and the sum above. limit: infinity for no clamp. Between the products rows are F32 (22 bits as a factor; BF16 rows: 11). */
+ * and the sum above. limit: infinity for no clamp. Between the products rows are F32; as factors
+ * they are held to 2^-29 of the largest of their 128 columns where an expert's rows are taken by one or two, else to 2^-22 of themselves (BF16 rows: 2^-12). */
 size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *down, int dtype, int T, int topk);
 int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4 *down, const void *x, int dtype, int T, size_t ldx,
                    const int32_t *idx, const float *weights, int topk, float limit, void *out, size_t ldo, void *workspace,

@@ -91,6 +91,31 @@ def test_small_columns_beside_large_ones(gpu_lib, T, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 40])
+def test_columns_far_above_their_neighbours(gpu_lib, T, group, dtype):
+    """In each 128 columns two, an even and an odd one, are 2^13 times the others and have zero weights: what their neighbours are off must not
+    show in the product. An activation is held to 2^-29 of the largest of its 128 columns in calls of one or two rows, else to 2^-22 of
+    itself (BF16: exactly) and 2^-38 of its row's largest; that few numbers are added makes the sums' own share small."""
+    rows, cols = 300, 256
+    rng = torch.Generator().manual_seed(T + group)
+    codes, scales = ref.make(rng, rows, cols, group)
+    x = torch.randn((T, cols), generator=rng)
+    for c in (18, 77, 128 + 1, 128 + 126):
+        x[:, c] = 2.0 ** 13 * (1.0 + torch.rand(T, generator=rng))
+        at = codes[:, c // 2]
+        codes[:, c // 2] = (at & 15) | 0x80 if c % 2 else (at & 0xf0) | 8
+    x = x.to(dtype)
+    w, xd = ref.values(codes, scales, cols, group), x.double()
+    y, want = _run(codes, scales, rows, cols, group, x.cuda()).double(), xd @ w.t()
+    steps = 2 * (cols // 16 + 1) + cols // 32 + 16
+    block = xd.abs().view(T, -1, 128).amax(2).repeat_interleave(128, 1)
+    off = (xd.abs() @ w.abs().t()) * (steps * 2.0 ** -23 + (2.0 ** -22 if dtype == torch.float32 else 0.0))
+    off = off + (block * 2.0 ** -29 + xd.abs().amax(1, keepdim=True) * 2.0 ** -38) @ w.abs().t() + ref.rounded(want, dtype)
+    assert bool(((y - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 64])
 @pytest.mark.parametrize("T", [1, 4, 30, 100])
 def test_scales_far_apart(gpu_lib, T, group, dtype):
