@@ -29,8 +29,10 @@
 //             BF16 one down to 2^-22 as they are, what is smaller off by one unit, 2^-29 of the largest, at most. (Three digits of F32 rows and two of BF16
 //             ones, four of which then fit, were off by 2^-22 and 2^-14 of the largest: by 3e-5 and 8e-3 of a product whose weights of columns a
 //             thousand times the others are small. The fourth digit takes a column that was idle.)
-// Group sums are exact integers, taken into FP32 by the exponent trick (they start at the bits of 1.5 2^23, so that their bits are the
-// float 1.5 2^23 + sum, |sum| < 2^22; in groups of 128 sixteenths of 1.5 2^19); sums across groups are FP32. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
+// Group sums are exact integers, taken into FP32 by the exponent trick: they start at the bits of 48, so that their bits are the float
+// 48 + sum 2^-18, |sum| < 2^18 (in groups of 128 at those of 3, in sixteenths); sums across groups are FP32. Whatever the scales and
+// activations, no intermediate leaves FP32's range where the sums of a result's magnitudes do not: sum 2^-18 < 1 times a scale, times
+// a digit's worth 2^5 < 2^128, and 2^13 once an output's sums are complete. At the other end a product is off by 2^-139 of the largest activation, a sum by 2^-136. Every wait is bounded: one that runs out sets a flag (g5b_w4_status).
 #include <algorithm>
 
 #include "tc_ptx.cuh"
@@ -99,15 +101,16 @@ __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t g0, uint32_t h0, u
     few_mma(c, g0, h0, g1, h1, b0, b1, c[0], c[1], c[2], c[3]);
 }
 __device__ __forceinline__ float few_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
-// The bits of 1.5 2^23, or for sums of sixteenths of 1.5 2^19.
-template <bool WHOLE> constexpr int few_magic = WHOLE ? 0x49400000 : 0x4b400000;
-template <bool WHOLE> __device__ __forceinline__ float few_float(int v) { return __fsub_rn(__int_as_float(v), WHOLE ? 786432.0f : 12582912.0f); }
+// The bits of 48, whose last is worth 2^-18, or for sums of sixteenths of 3.
+template <bool WHOLE> constexpr int few_magic = WHOLE ? 0x40400000 : 0x42400000;
+template <bool WHOLE> __device__ __forceinline__ float few_float(int v) { return __fsub_rn(__int_as_float(v), WHOLE ? 3.0f : 48.0f); }
+constexpr float FW_REST = 8192.0f;                   // what is left of 2^18 when 2^5 are part of a digit's worth
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // A block of 128 columns: [part][column][t] 16 bytes of digits as the lanes read them, then for each of the eight columns where the sums
-// start (WHOLE: of the block; else of each 32 columns, with groups of 64 those of both halves in the first) and what a digit stands for.
+// start (WHOLE: of the block; else of each 32 columns, with groups of 64 those of both halves in the first) and what a digit stands for, times 2^5.
 template <int NS, bool WHOLE> struct FewBlock {
     uint4 digits[2][NS][4];
     int   start[WHOLE ? 1 : 4][FW_COLS];
@@ -179,7 +182,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
                     reinterpret_cast<uint2 *>(&b.digits[j >> 1][col + d][t])[j & 1] = make_uint2(even[d], odd[d]);
                     if ((lane & (span - 1)) == 0) b.start[WHOLE ? 0 : j][col + d] = few_magic<WHOLE> - sum[d];
                 }
-                if (w == 0) b.worth[col + d] = finite ? few_pow2(-(up >> 1)) * few_pow2(8 * d - (up - (up >> 1))) : __int_as_float(0x7fc00000);
+                if (w == 0) b.worth[col + d] = finite ? few_pow2(5 - (up >> 1)) * few_pow2(8 * d - (up - (up >> 1))) : __int_as_float(0x7fc00000);
             }
         }
     }
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) w4_few_kernel(const __grid_cons
                                 }
                             }
                         }
-                        // (a digit's worth comes last: times a scale alone it may be too small for FP32)
+                        // (a digit's worth comes last: times a scale alone it may be too small or too large for FP32)
 #pragma unroll
                         for (int q = 0; q < 4; q++) acc[q] = fmaf(sum[q], q & 1 ? worth.y : worth.x, acc[q]);
                     };
@@ -406,7 +409,7 @@ constexpr int MOST = FW_PIECE / 1024 / U;
                             const float4 in = *reinterpret_cast<const float4 *>(&sum[w][r][col]);
                             d.x += in.x; d.y += in.y; d.z += in.z; d.w += in.w;
                         }
-                        return ((d.x + d.y) + d.z) + d.w;
+                        return (((d.x + d.y) + d.z) + d.w) * FW_REST;
                     };
                     float v = total(r);
                     const float u = MODE == W4_GATEUP ? total(r + 8) : 0.f;

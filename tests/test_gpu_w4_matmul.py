@@ -203,6 +203,32 @@ def test_magnitudes_far_apart(gpu_lib, T, group):
     _check(_run(codes, scales, rows, cols, group, x.cuda()), ref.values(codes, scales, cols, group), x)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T", [1, 2])
+def test_scales_and_activations_of_every_magnitude(gpu_lib, T, group, dtype):
+    """Rows of W with scales from 2^-125 to 2^124, rows of x from 2^-120 to 2^120: wherever the magnitudes of a result's products add up to less
+    than the largest number, it is as exact as others, but for what falls below FP32's range: 2^-127 of the activations, and 2^-126."""
+    rows, cols = 96, 640
+    rng = torch.Generator().manual_seed(T + group)
+    codes, scales = ref.make(rng, rows, cols, group, scale=1.0)
+    groups = cols // group
+    k = torch.tensor([-125, -100, -50, 0, 50, 90, 110, 124])[torch.arange(rows) % 8]
+    scales[:, :groups] = (scales[:, :groups].double().clamp(max=8.0) * torch.exp2(k.double())[:, None]).to(torch.bfloat16)
+    assert bool(torch.isfinite(scales[:, :groups]).all())
+    w = ref.values(codes, scales, cols, group)
+    seen = 0
+    for j in (-120, -90, -40, 0, 30, 70, 105, 120):
+        x = (torch.randn((T, cols), generator=rng).double() * torch.exp2(j + 4.0 * (torch.arange(T) % 2).double())[:, None]).to(dtype)
+        xd = x.double()
+        y, want, sums = _run(codes, scales, rows, cols, group, x.cuda()).double(), xd @ w.t(), xd.abs() @ w.abs().t()
+        off = ref.product_bound(w, xd, dtype == torch.float32) + ref.rounded(want, dtype) + 2.0 ** -127 * xd.abs().sum(1, keepdim=True)
+        inside = sums < 2.0 ** 127.9
+        seen += int(inside.sum())
+        assert bool(((y - want).abs() <= off)[inside].all())
+    assert seen > 3 * T * rows
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_rows_without_numbers(gpu_lib, T):
     """A row of zeros is zero; one with an infinity or NaN is NaN in all outputs; its neighbours do not see it."""
