@@ -12,12 +12,14 @@
 //          smallest's products above F16's last bit. Otherwise 1024 + code, minus 1032, times the scale, whose largest is brought below
 //          2^12: two operations, exact over 2^28 (groups of 32, eight rows past 154880 x 4096: 132 us).
 //          (A power of two for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
-//          F32 rows past groups of 128: the codes alone, and the scale on a step's sums.
+//          Groups of 128: the codes alone (times 2^-17), and the scale on a step's sums.
 //   products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
 //          same sums one after the other, so that a converted block is used twice.
-//   sums, four warps to a block: take a step's sums out of tensor memory, take the power of two off (F32 or BF16 rows past groups of
-//          128: put the scale on) and add them in registers, because the tensor cores cut off when they add; two accumulators in turn.
-//          At a tile's end the rows' powers of two come off, and the rows are stored.
+//   sums, four warps to a block: take a step's sums out of tensor memory, take the power of two off (groups of 128: put the
+//          scale on) and add them in registers, because the tensor cores cut off when they add; two accumulators in turn.
+//          Sums in registers are 2^-35 of what they stand for: rows of x below 2^14 past 2^17 columns of codes below 2^3 and a finite scale
+//          stay within FP32. At a tile's end that and the rows' powers of two come off, and the rows are stored. (At the other end a product is
+//          off by 2^-128 of its row's largest activation.)
 // BF16 rows have one term, a converted block is used once, and the conversion is most of a step: two groups of warps take steps in turn (2048
 // rows past 12288 x 4096 288 -> 226 us; of F32 rows, whose sums then lack registers, 300 -> 327).
 // A converted block and its sums live in tensor memory (256 columns each); shared memory only holds what TMA brings, which it
@@ -105,17 +107,21 @@ __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTi
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-// Eight codes of a word as four pairs in the terms' order: (code - 8) (WHOLE), or times the scale (twice in s).
+// Eight codes of a word as four pairs in the terms' order: (code - 8) 2^-17 (WHOLE: half of the 2^-35 that sums are held in, for nothing; subnormal
+// F16 numbers are as exact as others), or times the scale (twice in s). That a nibble in the low bits of 1024 is the number 1024 + nibble, and in
+// those of 2^-7 2^-7 + nibble 2^-17, is the usual way of taking such codes to F16. (A multiplication by 2^-17 instead: 64 rows 21 -> 22.6 us.)
 template <bool WHOLE>
 __device__ __forceinline__ void many_convert(uint32_t v, __half2 s, uint32_t *f)
 {
+    constexpr uint32_t BASE = WHOLE ? 0x20002000u : 0x64006400u;
+    constexpr float P = WHOLE ? 0x1p-17f : 1.0f;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         uint32_t a, b;
-        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(v));       // (v & mask) | 1024
-        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(v));
-        const __half2 lo = __hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f));
-        const __half2 hi = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+        asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(a) : "r"(v), "n"(BASE));       // (v & mask) | base
+        asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(b) : "r"(v), "n"(BASE));
+        const __half2 lo = __hadd2(*reinterpret_cast<__half2 *>(&a), __float2half2_rn(-1032.f * P));
+        const __half2 hi = __hfma2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.f * P));
         f[2 * i] = h2_bits(WHOLE ? lo : __hmul2(lo, s));
         f[2 * i + 1] = h2_bits(WHOLE ? hi : __hmul2(hi, s));
         v >>= 8;
@@ -317,9 +323,10 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
                     const uint32_t x0 = sc.x & 0x7fff7fffu, y0 = sc.y & 0x7fff7fffu, m2 = __vmaxu2(x0, y0), l2 = __vminu2(__vsub2(x0, 0x00010001u), __vsub2(y0, 0x00010001u));
                     const int top = max((int)(max(m2 & 0xffffu, m2 >> 16) >> 7), 1), low = (int)((min(l2 & 0xffffu, l2 >> 16) + 1) >> 7);
                     fused = __all_sync(0xffffffffu, top - low <= 8 && top >= 40 && top <= 220);
-                    const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 126);
+                    // (2^114 takes the least scale's last bit to 2^-19, which F16 holds, and 2^-114 2^-35 is the least FP32 number)
+                    const int e = fused ? 15 + 127 - top : min(11 + 127 - top, 114);
                     const float up = pow2(e);
-                    s_down[step & (WM_RING - 1)][b][r] = fused ? pow2(24 - e) : pow2(-e);
+                    s_down[step & (WM_RING - 1)][b][r] = (fused ? pow2(24 - e) : pow2(-e)) * 0x1p-35f;
 #pragma unroll
                     for (int piece = 0; piece < 4; piece++) {
                         const int g = (4 * kb + piece) >> per;
@@ -386,7 +393,8 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
         pdl_wait();
 #pragma unroll 1
         while (many_next(a, walk, t)) {
-            const float i0 = lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f, i1 = lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f;
+            // what the rows' finished sums are multiplied by: 2^35 and their powers of two, 2^-126 to 2^114
+            float i0 = (lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f) * 0x1p35f, i1 = (lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f) * 0x1p35f;
             F2 acc[WM_ROWS / 2];
 #pragma unroll
             for (int k = 0; k < WM_ROWS / 2; k++) acc[k] = f2(0.f, 0.f);
@@ -399,7 +407,7 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
 #pragma unroll 1
             for (int kb = t.k0; kb < t.k1; kb++, steps++) {
                 const int buf = steps & 1;
-                float sc = bf16_to_f32(next);
+                float sc = bf16_to_f32(next) * 0x1p-18f;
                 if (WHOLE && kb + 1 < t.k1) next = __ldg(srow + kb + 1);
                 if (!(ok = mbar_wait_all(&d_full[b][buf], (uint32_t)(steps >> 1) & 1, err, 11))) break;
                 if (!WHOLE) sc = s_down[steps & (WM_RING - 1)][b][r];
@@ -434,6 +442,21 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
             }
             many_all(true, bar, bar_threads);
             const int row0 = (GATEUP ? t.rt * 128 : t.rt * 256 + b * 128) + lane * 4;
+            if (__any_sync(0xffffffffu, isinf(i0) || isinf(i1))) {
+                // (rows with activations from 2^106 on, whose factor FP32 does not hold: 2^35 goes into the sums here. Apart from the loop below,
+                // in which every instruction counts: a second factor there was 2 % of 2048 rows past 12288 x 4096.)
+#pragma unroll 1
+                for (int k = GATEUP ? warp : quarter; k < t.np; k += GATEUP ? 8 : 4)
+                    if (isinf(__shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31)))
+#pragma unroll 1
+                        for (int q = 0; q < 4; q++) {
+                            float *at = (GATEUP ? exch : sums) + k * 128 + lane * 4 + q;
+                            *at *= 0x1p35f;
+                            if (GATEUP) at[WM_ROWS * 128] *= 0x1p35f;
+                        }
+                if (isinf(i0)) i0 = __ldg(a.inv + t.first + lane);
+                if (isinf(i1)) i1 = __ldg(a.inv + t.first + lane + 32);
+            }
 #pragma unroll 1
             for (int k = GATEUP ? warp : quarter; k < t.np; k += GATEUP ? 8 : 4) {
                 const float inv = __shfl_sync(0xffffffffu, k < 32 ? i0 : i1, k & 31);

@@ -439,7 +439,8 @@ int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *s
  * is held to: in calls of one or two rows 2^-29 of the largest of the 128 columns it lies in, from a multiple of 128 on, or
  * better; in calls of more rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
  * scales within 128 columns differ by more than 2^28 has products off by up to 2^-36 of the largest scale times the
- * activation; all others are exact. A row of x with an infinity or NaN gives NaN in all of its outputs. */
+ * activation; all others are exact. Scales and activations may have any finite magnitude: a result is a number where the magnitudes of its
+ * products add up to one, and a product is off by 2^-127 of its row's largest activation at most where FP32's range ends. A row of x with an infinity or NaN gives NaN in all of its outputs. */
 size_t g5b_w4_matmul_workspace(const g5b_w4 *w, int dtype, int T);
 int g5b_w4_matmul(const g5b_w4 *w, const void *x, int dtype, int T, size_t ldx, void *y, size_t ldy, void *workspace,
                   size_t workspace_bytes, void *stream);

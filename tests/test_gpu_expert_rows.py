@@ -186,6 +186,25 @@ def test_experts_without_numbers_and_far_outside(gpu_lib):
     assert _experts((gate, up, down), torch.zeros((0, H), device="cuda"), none, torch.zeros((0, 2)), 10.0).shape == (0, H)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("T,K,E", [(3, 2, 5), (9, 3, 20), (12, 2, 5), (60, 2, 5)])
+def test_experts_of_huge_rows_and_small_weights(gpu_lib, T, K, E, group, dtype):
+    """Some rows of x about 2^110, gate and up weights about 2^-100, and as large ones the other way round: all results are numbers."""
+    rng = torch.Generator().manual_seed(T + group)
+    H, I = 200, 150
+    for big, small, down_ in ((110, -100, 1.0), (-100, 110, 2.0 ** 80)):
+        made = [(ref.make(rng, r, c, group, E, scale=s), r, c) for r, c, s in ((I, H, 2.0 ** small), (I, H, 2.0 ** small), (H, I, down_))]
+        handles, (g, u, d) = [ref.handle(*m, r, c, group) for m, r, c in made], [ref.values(*m, c, group) for m, r, c in made]
+        idx = torch.randint(0, E, (T, K), generator=rng, dtype=torch.int32)
+        x = (torch.randn((T, H), generator=rng) * torch.where(torch.arange(T) % 3 == 1, 1.0, 2.0 ** big)[:, None]).to(dtype)
+        weights = torch.rand((T, K), generator=rng)
+        got = _experts(handles, x.cuda(), idx, weights, float("inf"))
+        want, off = ref.experts(x.double(), idx, weights, g, u, d, float("inf"), dtype == torch.float32)
+        fine = want.abs() < 2.0 ** 120                     # (rows of ordinary size past huge weights: their products leave FP32)
+        assert int(fine.sum()) >= H and bool(((got.double() - want).abs() <= off + ref.rounded(want, dtype))[fine].all())
+
+
 def test_a_checkpoint_expert_layer_in_four_bits(gpu_lib):
     """As they are used together: FP8 experts converted one matrix at a time into stacks, a prompt and then single tokens through
     them; the layer put together from the sort, the gather, the products and the combination gives the same."""

@@ -205,7 +205,7 @@ def test_magnitudes_far_apart(gpu_lib, T, group):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("T", [1, 2])
+@pytest.mark.parametrize("T", [1, 2, 5, 40, 70])
 def test_scales_and_activations_of_every_magnitude(gpu_lib, T, group, dtype):
     """Rows of W with scales from 2^-125 to 2^124, rows of x from 2^-120 to 2^120: wherever the magnitudes of a result's products add up to less
     than the largest number, it is as exact as others, but for what falls below FP32's range: 2^-127 of the activations, and 2^-126."""
