@@ -46,7 +46,6 @@ struct W4Job {
     int mode;
     W4Mat w, up;                // gate/up: w is the gate
     int count;                  // matrices of the stack
-    int n_terms;                // terms of an activation
     int T;                      // rows of activations (experts: picks, at most)
     const void *x; int x_dt; size_t ldx;        // w4_few: the activations (dense, gate/up: the caller's; down: F32 rows of picks)
     const int *order; int topk;                 // w4_few, gate/up: the activation row of sorted row i is order[i] / topk

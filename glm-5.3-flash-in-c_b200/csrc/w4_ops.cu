@@ -154,7 +154,7 @@ ExpertsWs experts_ws(Pieces &ws, const ExpertsPlan &plan, int n_terms, int T, in
     }
     if (plan.how == MANY || plan.how == EITHER) {
         w.x = terms_of(ws, n_terms, H, n);
-        w.h = terms_of(ws, n_terms, I, n);
+        w.h = terms_of(ws, 2, I, n);                // (FP32 rows, whatever the caller's are)
     }
     w.act = ws.take<float>(n * I);
     w.rows = ws.take<float>(n * H);
@@ -224,13 +224,13 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     if (check_ws(op, workspace, workspace_bytes, g5b_w4_matmul_workspace(m, dtype, T))) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Pieces ws{static_cast<uint8_t *>(workspace)};
-    j.mode = W4_DENSE; j.T = T; j.count = 1; j.n_terms = dtype == DT_BF16 ? 1 : 2;
+    j.mode = W4_DENSE; j.T = T; j.count = 1;
     j.y = y; j.ldy = ldy; j.y_dt = dtype;
     if (w4_few_takes(j.w.cols, T)) {
         j.x = x; j.x_dt = dtype; j.ldx = ldx;
         return w4_few(st, j) ? -1 : launched(op);
     }
-    j.terms = terms_of(ws, j.n_terms, j.w.cols, T);
+    j.terms = terms_of(ws, dtype == DT_BF16 ? 1 : 2, j.w.cols, T);
     w4_split(st, j.terms, x, dtype, ldx, T, j.w.cols, nullptr, nullptr, 1, false);
     return w4_many(st, j, ws.take<float>(w4_many_part_floats(j.w.rows, j.w.cols, T))) ? -1 : launched(op);
 }
@@ -310,7 +310,7 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     const ExpertsPlan plan = experts_plan(T, topk, E, H, I);
     const ExpertsWs ws = experts_ws(pieces, plan, n_terms, T, topk, E, H, I);
     W4Job j{};
-    j.count = E; j.n_terms = n_terms; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
+    j.count = E; j.T = n; j.order = ws.order; j.topk = topk; j.slots = ws.slots; j.limit = limit; j.y_dt = DT_F32;
     if (plan.how != PICKS && expert_sort(st, idx, T, topk, E, ws.order, ws.place, ws.offsets, &ws.slots)) return launched(op), -1;
     const bool few = plan.how != MANY, many = plan.how == MANY || plan.how == EITHER;
     W4Slots many_slots = ws.slots;

@@ -80,7 +80,6 @@ void w4_split(cudaStream_t st, const W4Terms &t, const void *x, int dt, size_t l
         else       G5B_LAUNCH((w4_split_kernel<IN, TERMS>), grid, 256, 0, st, t, p, ldx, rows, cols, n_rows, order, topk, wide);                 \
     } while (0)
     if (dt == DT_BF16) SPLIT(uint16_t, 1, h);
-    else if (t.n_terms == 1) SPLIT(float, 1, f);
     else SPLIT(float, 2, f);
 #undef SPLIT
 }

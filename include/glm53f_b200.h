@@ -463,7 +463,7 @@ int g5b_expert_combine(const void *rows, int dtype, size_t ldr, const int32_t *p
 /* Routed experts in 4 bits (the routed part of g5b_op_moe): gate and up [count][inter][hidden], down [count][hidden][inter];
  * out[t] = sum over k of weights[t][k] down_e (silu(min(gate_e x, limit)) clamp(up_e x, -limit, limit)), e = idx[t][k], with the sort
  * and the sum above. limit: infinity for no clamp. Between the products rows are F32; as factors
- * they are held to 2^-29 of the largest of their 128 columns where an expert's rows are taken by one or two, else to 2^-22 of themselves (BF16 rows: 2^-12). */
+ * they are held to 2^-29 of the largest of their 128 columns where an expert's rows are taken by one or two, else to 2^-22 of themselves. */
 size_t g5b_w4_experts_workspace(const g5b_w4 *gate, const g5b_w4 *down, int dtype, int T, int topk);
 int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4 *down, const void *x, int dtype, int T, size_t ldx,
                    const int32_t *idx, const float *weights, int topk, float limit, void *out, size_t ldo, void *workspace,

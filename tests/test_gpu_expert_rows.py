@@ -187,6 +187,27 @@ def test_experts_without_numbers_and_far_outside(gpu_lib):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E", [(3, 2), (18, 20), (20, 2), (40, 2)])
+def test_hidden_rows_keep_what_fp32_holds(gpu_lib, T, E, dtype):
+    """Integers past weights that are multiples of 2^-6: gate and up are exact, the hidden row is off by what the sigmoid (1.53 units of 2^-23) and two
+    products are, and the down product by its additions and 2^-22 of a factor, in calls that take picks one by one, by two, and by 64."""
+    rng = torch.Generator().manual_seed(T)
+    H, I = 64, 32
+    stack = lambda r, c, s: ref.make(rng, r, c, 32, E, spread=0.0, scale=s)        # noqa: E731
+    made = [(stack(r, c, s), r, c) for r, c, s in ((I, H, 2.0 ** -6), (I, H, 2.0 ** -6), (H, I, 0.03))]
+    handles, (g, u, d) = [ref.handle(*m, r, c, 32) for m, r, c in made], [ref.values(*m, c, 32) for m, r, c in made]
+    idx = torch.randint(0, E, (T, 1), generator=rng, dtype=torch.int32)
+    x = torch.randint(-8, 9, (T, H), generator=rng).to(dtype)
+    got = _experts(handles, x.cuda(), idx, torch.ones((T, 1)), 10.0).double()
+    at = idx[:, 0].long()
+    h = ref.swiglu(torch.einsum("th,tih->ti", x.double(), g[at]), torch.einsum("th,tih->ti", x.double(), u[at]), 10.0)
+    want = torch.einsum("ti,thi->th", h, d[at])
+    steps = 2 * (I // 16 + 1) + I // 32 + 16
+    off = torch.einsum("ti,thi->th", h.abs(), d[at].abs()) * (steps + 4 + 2) * 2.0 ** -23 + ref.rounded(want, dtype)
+    assert bool(((got - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 128])
 @pytest.mark.parametrize("T,K,E", [(3, 2, 5), (9, 3, 20), (12, 2, 5), (60, 2, 5)])
 def test_experts_of_huge_rows_and_small_weights(gpu_lib, T, K, E, group, dtype):
