@@ -48,6 +48,9 @@ extern unsigned long long g_launches;
 
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What the kernel in front writes, in one that may be launched early: an ordinary load. (The read-only path wants memory that nobody writes
+// while the kernel runs, and this one runs beside that; the compiler may also move such loads over the wait.)
+template <typename T> __device__ __forceinline__ T load_new(const T *p) { return __ldca(p); }
 
 // 16-byte streaming load: weights are read once per token, so they bypass L1 allocation and
 // leave it to the activations that every row re-reads.

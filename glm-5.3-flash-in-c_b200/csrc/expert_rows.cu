@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const IN *rows, siz
     struct __align__(sizeof(OUT) * V) OutV { OUT v[V]; };
     const int t = blockIdx.x, c0 = (blockIdx.y * 256 * CH + threadIdx.x) * V;
     if (threadIdx.x < topk) {
-        int p = __ldg(place + (size_t)t * topk + threadIdx.x);
+        int p = load_new(place + (size_t)t * topk + threadIdx.x);
         if (E) p = p >= 0 && p < E ? t * topk + (int)threadIdx.x : -1;
         else if (p >= (int)gridDim.x * topk) p = -1;            // (not a place that the sort wrote)
         s_at[threadIdx.x] = p;

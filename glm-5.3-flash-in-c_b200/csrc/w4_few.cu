@@ -77,7 +77,7 @@ struct FewArgs {
 struct FewItem { int e, first, count, tile; };       // expert; sorted rows (dense: rows of x); row tile
 // here: picks of experts that are here (idx: a bit each)
 template <int MODE>
-__device__ __forceinline__ int few_slots(const FewArgs &a, uint32_t here) { return MODE == W4_DENSE ? 1 : a.idx ? __popc(here) : __ldg(a.slots.n); }
+__device__ __forceinline__ int few_slots(const FewArgs &a, uint32_t here) { return MODE == W4_DENSE ? 1 : a.idx ? __popc(here) : load_new(a.slots.n); }
 template <int MODE>
 __device__ __forceinline__ FewItem few_item(const FewArgs &a, uint32_t here, int slot, int tile)
 {
@@ -87,7 +87,7 @@ __device__ __forceinline__ FewItem few_item(const FewArgs &a, uint32_t here, int
         const int pick = __ffs(here) - 1;
         return pick < 0 ? FewItem{} : FewItem{__ldg(a.idx + pick), pick, 1, tile};
     }
-    return FewItem{__ldg(a.slots.expert + slot), __ldg(a.slots.first + slot), __ldg(a.slots.count + slot), tile};
+    return FewItem{load_new(a.slots.expert + slot), load_new(a.slots.first + slot), load_new(a.slots.count + slot), tile};
 }
 
 // (not volatile: two blocks' chains of these are put side by side)
@@ -127,7 +127,7 @@ __device__ __forceinline__ void few_digits(const FewArgs &a, const FewItem &it, 
     bar_sync(1, FW_WARPS * 32);                          // nobody reads the digits of the rows before any more
     if (i < it.count) {
         const int at = it.first + i;
-        const int src = MODE != W4_GATEUP ? at : (a.idx ? at : __ldg(a.order + at)) / a.topk;
+        const int src = MODE != W4_GATEUP ? at : (a.idx ? at : load_new(a.order + at)) / a.topk;
         const IN *row = static_cast<const IN *>(a.x) + (size_t)src * a.ldx;
         const int col = i * FW_DIGITS;
         for (int c0 = (warp - i * per) * 256; c0 < a.blocks * 128; c0 += per * 256) {

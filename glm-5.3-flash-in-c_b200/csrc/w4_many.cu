@@ -76,7 +76,7 @@ struct ManyTile {
 struct ManyWalk { int u, end; };
 __device__ __forceinline__ ManyWalk many_walk(const ManyArgs &a)
 {
-    return ManyWalk{(int)blockIdx.x, a.mode == W4_DENSE ? a.whole + (a.RT * a.TT - a.whole) * a.parts : a.RT * __ldg(a.slots.n)};
+    return ManyWalk{(int)blockIdx.x, a.mode == W4_DENSE ? a.whole + (a.RT * a.TT - a.whole) * a.parts : a.RT * load_new(a.slots.n)};
 }
 __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTile &t)
 {
@@ -97,7 +97,7 @@ __device__ __forceinline__ bool many_next(const ManyArgs &a, ManyWalk &w, ManyTi
     } else {
         const int slot = w.u / a.RT;
         t.rt = w.u - slot * a.RT;
-        t.e = __ldg(a.slots.expert + slot); t.first = __ldg(a.slots.first + slot); t.np = __ldg(a.slots.count + slot);
+        t.e = load_new(a.slots.expert + slot); t.first = load_new(a.slots.first + slot); t.np = load_new(a.slots.count + slot);
     }
     t.n = (t.np + 15) & ~15;
     w.u += gridDim.x;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
 #pragma unroll 1
         while (many_next(a, walk, t)) {
             // what the rows' finished sums are multiplied by: 2^35 and their powers of two, 2^-126 to 2^114
-            float i0 = (lane < t.np ? __ldg(a.inv + t.first + lane) : 0.f) * 0x1p35f, i1 = (lane + 32 < t.np ? __ldg(a.inv + t.first + lane + 32) : 0.f) * 0x1p35f;
+            float i0 = (lane < t.np ? load_new(a.inv + t.first + lane) : 0.f) * 0x1p35f, i1 = (lane + 32 < t.np ? load_new(a.inv + t.first + lane + 32) : 0.f) * 0x1p35f;
             F2 acc[WM_ROWS / 2];
 #pragma unroll
             for (int k = 0; k < WM_ROWS / 2; k++) acc[k] = f2(0.f, 0.f);
@@ -454,8 +454,8 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
                             *at *= 0x1p35f;
                             if (GATEUP) at[WM_ROWS * 128] *= 0x1p35f;
                         }
-                if (isinf(i0)) i0 = __ldg(a.inv + t.first + lane);
-                if (isinf(i1)) i1 = __ldg(a.inv + t.first + lane + 32);
+                if (isinf(i0)) i0 = load_new(a.inv + t.first + lane);
+                if (isinf(i1)) i1 = load_new(a.inv + t.first + lane + 32);
             }
 #pragma unroll 1
             for (int k = GATEUP ? warp : quarter; k < t.np; k += GATEUP ? 8 : 4) {

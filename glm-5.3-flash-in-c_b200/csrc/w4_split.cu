@@ -14,10 +14,10 @@ __global__ void __launch_bounds__(256) w4_split_kernel(W4Terms t, const IN *x, s
     __shared__ uint32_t s_max[2][8];
     pdl_trigger();
     pdl_wait();
-    if (n_rows) rows = min(rows, __ldg(n_rows));
+    if (n_rows) rows = min(rows, load_new(n_rows));
     int turn = 0;
     for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
-        const IN *xr = x + (size_t)(order ? __ldg(order + row) / topk : row) * ldx;
+        const IN *xr = x + (size_t)(order ? load_new(order + row) / topk : row) * ldx;
         // the first 4096 columns stay in registers
         float first[2][8];
         uint32_t m = 0;
