@@ -75,6 +75,7 @@ int check_ptr(const char *op, const char *what, const void *p, size_t align)
 int elt(int dt) { return dt == DT_F32 ? 4 : 2; }
 int check_dtype(const char *op, int dt) { return dt == DT_F32 || dt == DT_BF16 ? 0 : fail("%s: rows are F32 or BF16, not dtype %d", op, dt); }
 
+// Every entry point looks at sizes, types and distances first, then at the workspace's size, and at addresses last.
 int check_mat(const char *op, const char *what, const g5b_w4 *m, int count, W4Mat &w)
 {
     if (!m) return fail("%s: %s is null", op, what);
@@ -82,13 +83,16 @@ int check_mat(const char *op, const char *what, const g5b_w4 *m, int count, W4Ma
         return fail("%s: %s of %d x %d is outside 1 x 1 .. %d x %d", op, what, m->rows, m->cols, W4_MAX_ROWS, W4_MAX_COLS);
     if (m->group != 32 && m->group != 64 && m->group != 128) return fail("%s: groups of %s have 32, 64 or 128 columns, not %d", op, what, m->group);
     if (m->count < 1 || m->count > G5B_MAX_EXPERTS || (count && m->count != count)) return fail("%s: %s holds %d matrices", op, what, m->count);
-    if (check_ptr(op, what, m->codes, 16) || check_ptr(op, what, m->scales, 16)) return -1;
     w.codes = m->codes; w.scales = m->scales;
     w.rows = m->rows; w.cols = m->cols; w.group = m->group;
     w.pitch = (int)g5b_w4_pitch(m->cols); w.sp = (int)g5b_w4_scale_pitch(m->cols, m->group);
     w.groups = (m->cols + m->group - 1) / m->group;
     w.codes_stride = (size_t)w.rows * w.pitch; w.scales_stride = (size_t)w.rows * w.sp;
     return 0;
+}
+int check_mat_ptr(const char *op, const char *what, const W4Mat &w)
+{
+    return check_ptr(op, what, w.codes, 16) || check_ptr(op, what, w.scales, 16) ? -1 : 0;
 }
 
 // Pieces of a workspace, one after the other; without memory behind it a count of the bytes.
@@ -110,9 +114,8 @@ W4Terms terms_of(Pieces &ws, int n_terms, int cols, size_t rows)
     t.inv = ws.take<float>(rows);
     return t;
 }
-int check_ws(const char *op, const void *ws, size_t have, size_t need)
+int check_ws(const char *op, size_t have, size_t need)
 {
-    if (check_ptr(op, "the workspace", ws, 256)) return -1;
     return have >= need ? 0 : fail("%s: the workspace has %zu bytes, %zu are needed", op, have, need);
 }
 
@@ -181,11 +184,9 @@ extern "C" int g5b_w4_quantize(const g5b_tensor *src, int br, int bc, const g5b_
     if (!src || !src->on_device) return fail("%s: the source must be a device tensor", op);
     if (src->rows != w.rows || src->cols != w.cols) return fail("%s: a source of %d x %d for a matrix of %d x %d", op, src->rows, src->cols, w.rows, w.cols);
     if (src->dtype != DT_F32 && src->dtype != DT_BF16 && src->dtype != DT_FP8) return fail("%s: dtype %d of the source", op, src->dtype);
-    if (check_ptr(op, "the source", src->data, src->dtype == DT_F32 ? 4 : src->dtype == DT_BF16 ? 2 : 1)) return -1;
-    if (src->dtype == DT_FP8) {
-        if (br < 1 || bc < 1) return fail("%s: scale blocks of %d x %d", op, br, bc);
-        if (check_ptr(op, "the scale grid", src->scale_inv, 4)) return -1;
-    }
+    if (src->dtype == DT_FP8 && (br < 1 || bc < 1)) return fail("%s: scale blocks of %d x %d", op, br, bc);
+    if (check_mat_ptr(op, "the matrix", w) || check_ptr(op, "the source", src->data, src->dtype == DT_F32 ? 4 : src->dtype == DT_BF16 ? 2 : 1)) return -1;
+    if (src->dtype == DT_FP8 && check_ptr(op, "the scale grid", src->scale_inv, 4)) return -1;
     w4_quantize(static_cast<cudaStream_t>(stream), w, src->data, src->dtype, src->scale_inv, br, bc);
     return launched(op);
 }
@@ -194,8 +195,9 @@ extern "C" int g5b_w4_dequantize(const g5b_w4 *m, int dtype, void *out, size_t l
 {
     const char *op = "g5b_w4_dequantize";
     W4Mat w;
-    if (check_mat(op, "the matrix", m, 1, w) || check_dtype(op, dtype) || check_ptr(op, "the output", out, elt(dtype))) return -1;
+    if (check_mat(op, "the matrix", m, 1, w) || check_dtype(op, dtype)) return -1;
     if (ldo < (size_t)w.cols) return fail("%s: rows %zu apart for %d columns", op, ldo, w.cols);
+    if (check_mat_ptr(op, "the matrix", w) || check_ptr(op, "the output", out, elt(dtype))) return -1;
     w4_dequantize(static_cast<cudaStream_t>(stream), w, out, dtype, ldo);
     return launched(op);
 }
@@ -218,10 +220,11 @@ extern "C" int g5b_w4_matmul(const g5b_w4 *m, const void *x, int dtype, int T, s
     W4Job j{};
     if (check_mat(op, "the matrix", m, 1, j.w) || check_dtype(op, dtype)) return -1;
     if (T < 0 || T > W4_MAX_TOKENS) return fail("%s: %d rows are outside 0 .. %d", op, T, W4_MAX_TOKENS);
+    if (T && (ldx < (size_t)j.w.cols || ldy < (size_t)j.w.rows)) return fail("%s: rows %zu and %zu apart for a matrix of %d x %d", op, ldx, ldy, j.w.rows, j.w.cols);
+    if (T && check_ws(op, workspace_bytes, g5b_w4_matmul_workspace(m, dtype, T))) return -1;
+    if (check_mat_ptr(op, "the matrix", j.w)) return -1;
     if (T == 0) return 0;
-    if (check_ptr(op, "x", x, elt(dtype)) || check_ptr(op, "y", y, elt(dtype))) return -1;
-    if (ldx < (size_t)j.w.cols || ldy < (size_t)j.w.rows) return fail("%s: rows %zu and %zu apart for a matrix of %d x %d", op, ldx, ldy, j.w.rows, j.w.cols);
-    if (check_ws(op, workspace, workspace_bytes, g5b_w4_matmul_workspace(m, dtype, T))) return -1;
+    if (check_ptr(op, "x", x, elt(dtype)) || check_ptr(op, "y", y, elt(dtype)) || check_ptr(op, "the workspace", workspace, WS_ALIGN)) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Pieces ws{static_cast<uint8_t *>(workspace)};
     j.mode = W4_DENSE; j.T = T; j.count = 1;
@@ -301,9 +304,12 @@ extern "C" int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4
     if (check_picks(op, T, topk, gate->count) || check_dtype(op, dtype)) return -1;
     if (!(limit > 0.f)) return fail("%s: the clamp's limit must be above zero (infinity for none)", op);
     if (ldx < (size_t)wg.cols || ldo < (size_t)wg.cols) return fail("%s: rows %zu and %zu apart for %d columns", op, ldx, ldo, wg.cols);
+    if (T && check_ws(op, workspace_bytes, g5b_w4_experts_workspace(gate, down, dtype, T, topk))) return -1;
+    if (check_mat_ptr(op, "gate", wg) || check_mat_ptr(op, "up", wu) || check_mat_ptr(op, "down", wd)) return -1;
     if (T == 0) return 0;
-    if (check_ptr(op, "x", x, elt(dtype)) || check_ptr(op, "idx", idx, 4) || check_ptr(op, "weights", weights, 4) || check_ptr(op, "out", out, elt(dtype))) return -1;
-    if (check_ws(op, workspace, workspace_bytes, g5b_w4_experts_workspace(gate, down, dtype, T, topk))) return -1;
+    if (check_ptr(op, "x", x, elt(dtype)) || check_ptr(op, "idx", idx, 4) || check_ptr(op, "weights", weights, 4) || check_ptr(op, "out", out, elt(dtype)) ||
+        check_ptr(op, "the workspace", workspace, WS_ALIGN))
+        return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int E = gate->count, H = wg.cols, I = wg.rows, n = T * topk, n_terms = dtype == DT_BF16 ? 1 : 2;
     Pieces pieces{static_cast<uint8_t *>(workspace)};

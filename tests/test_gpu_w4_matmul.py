@@ -284,6 +284,29 @@ def test_same_bits_every_time_on_any_stream_and_in_a_graph(gpu_lib, T):
     assert torch.equal(outs[0].cpu(), first) and torch.equal(outs[1].cpu(), second)
 
 
+@pytest.mark.parametrize("T", [1, 2, 5, 70])
+def test_refused_calls_write_nothing(gpu_lib, T):
+    """A workspace a byte short or off its alignment, a matrix or a row on the host: an error that says so, and y stays as it was."""
+    rows, cols, group = 40, 96, 32
+    codes, scales = ref.make(torch.Generator().manual_seed(T), rows, cols, group)
+    w = ref.handle(codes, scales, rows, cols, group)
+    x, y = torch.ones((T, cols), device="cuda"), torch.full((T, rows), 3.0, device="cuda")
+    need = pkg.w4_matmul_workspace(w, x)
+    space = torch.empty(need + 512, dtype=torch.uint8, device="cuda")
+    with pytest.raises(RuntimeError, match=f"has {need - 1} bytes, {need} are needed"):
+        pkg.w4_matmul(w, x, y, space[:need - 1])
+    with pytest.raises(RuntimeError, match="workspace must lie on a multiple of 256 bytes"):
+        pkg.w4_matmul(w, x, y, space[16:])
+    with pytest.raises(RuntimeError, match="the matrix is not device memory"):
+        pkg._call_w4("g5b_w4_matmul", pkg.W4(codes, scales, rows, cols, group).ref, x.data_ptr(), 0, T, cols, y.data_ptr(), rows, space.data_ptr(), need, 0)
+    with pytest.raises(RuntimeError, match="x is not device memory"):
+        pkg._call_w4("g5b_w4_matmul", w.ref, x.cpu().data_ptr(), 0, T, cols, y.data_ptr(), rows, space.data_ptr(), need, 0)
+    torch.cuda.synchronize()
+    assert bool((y == 3.0).all())
+    pkg.w4_matmul(w, x, y, space[:need])
+    _check(y.cpu(), ref.values(codes, scales, cols, group), x)
+
+
 # ------------------------------------------------------------------ conversion ----
 def _quantized(v, group):
     """(codes as numbers 0..15 [rows][cols], scales [rows][groups]) of FP32 values, quotients in FP64."""

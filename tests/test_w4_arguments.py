@@ -128,3 +128,48 @@ def test_experts_refusals():
                            ((m(32, 64), m(32, 64), m(64, 32)), {"dtype": 2}, "dtype")):
         assert call(*args, **kw) == -1
         assert not device or word in _err() or "device" in _err()
+
+
+def test_experts_refusals_say_what_is_wrong():
+    """Every rule of the routed experts by its own message, whether there is a device or not: nothing but the addresses is wrong besides, and they are
+    looked at last."""
+    L, a = pkg.lib(), 1 << 20
+    m = lambda rows, cols, group=32, count=4: C.byref(_w4(a, a, rows, cols, group, count))       # noqa: E731
+    good = dict(gate=(32, 64), up=(32, 64), down=(64, 32), limit=10.0, topk=2, T=1, dtype=0, ldx=64, ldo=64, ws=1 << 30)
+
+    def call(**kw):
+        k = {**good, **kw}
+        return L.g5b_w4_experts(m(*k["gate"]), m(*k["up"]), m(*k["down"]), a, k["dtype"], k["T"], k["ldx"], a, a, k["topk"], k["limit"], a, k["ldo"], a, k["ws"], None)
+    for kw, word in (({"up": (32, 64, 64)}, "belong together"), ({"up": (33, 64)}, "belong together"), ({"up": (32, 65)}, "belong together"),
+                     ({"down": (64, 33)}, "belong together"), ({"down": (65, 32)}, "belong together"), ({"up": (32, 64, 32, 3)}, "up holds 3 matrices"),
+                     ({"down": (64, 32, 32, 5)}, "down holds 5 matrices"), ({"limit": 0.0}, "limit"), ({"limit": -1.0}, "limit"), ({"limit": float("nan")}, "limit"),
+                     ({"topk": 0}, "picks"), ({"topk": 65}, "picks"), ({"T": -1}, "outside"), ({"T": (1 << 19) + 1}, "outside"), ({"ldx": 63}, "apart"), ({"ldo": 63}, "apart"),
+                     ({"dtype": 2}, "dtype 2"), ({"gate": (32, 64, 48)}, "32, 64 or 128"), ({"gate": (0, 64)}, "outside")):
+        assert call(**kw) == -1 and word in _err(), (kw, _err())
+    for T in (1, 20, 100):                                 # picks one by one, by two, by 64
+        need = L.g5b_w4_experts_workspace(m(32, 64), m(64, 32), 0, T, 2)
+        assert call(T=T, ws=need - 1) == -1 and f"has {need - 1} bytes, {need} are needed" in _err()
+        assert call(T=T, ws=need) == -1 and "device" in _err()
+    assert call() == -1 and "device" in _err()
+    assert call(down=(64, 32, 128)) == -1 and "device" in _err()          # groups of another size in the down matrix are fine
+
+
+def test_product_refusals_say_what_is_wrong():
+    L, a = pkg.lib(), 1 << 20
+    w = C.byref(_w4(a, a, 16, 64, 32))
+
+    def call(dtype=0, T=1, ldx=64, ldy=16, ws=1 << 30):
+        return L.g5b_w4_matmul(w, a, dtype, T, ldx, a, ldy, a, ws, None)
+    for kw, word in (({"dtype": 2}, "dtype 2"), ({"T": -1}, "outside"), ({"T": (1 << 19) + 1}, "outside"), ({"ldx": 63}, "apart"), ({"ldy": 15}, "apart")):
+        assert call(**kw) == -1 and word in _err(), (kw, _err())
+    for T in (1, 2, 5, 100):
+        need = L.g5b_w4_matmul_workspace(w, 0, T)
+        assert call(T=T, ws=need - 1) == -1 and f"has {need - 1} bytes, {need} are needed" in _err()
+        assert call(T=T, ws=need) == -1 and "device" in _err()
+    assert L.g5b_w4_dequantize(w, 0, a, 63, None) == -1 and "apart" in _err()
+    assert L.g5b_w4_dequantize(w, 2, a, 64, None) == -1 and "dtype 2" in _err()
+    src = lambda rows=16, cols=64, dtype=0, on=1: C.byref(pkg.Tensor(a, a, dtype, rows, cols, on))       # noqa: E731
+    for t, blocks, word in ((src(on=0), (128, 128), "device tensor"), (src(rows=17), (128, 128), "17 x 64"), (src(cols=63), (128, 128), "16 x 63"),
+                            (src(dtype=7), (128, 128), "dtype 7"), (src(dtype=pkg.DT_FP8), (0, 128), "scale blocks"), (src(dtype=pkg.DT_FP8), (128, -1), "scale blocks")):
+        assert L.g5b_w4_quantize(t, *blocks, w, None) == -1 and word in _err(), _err()
+    assert L.g5b_w4_quantize(src(), 128, 128, w, None) == -1 and "device" in _err()
