@@ -813,6 +813,11 @@ def w4_experts(gate: W4, up: W4, down: W4, x, idx, weights, limit: float, out, w
              _check("weights", weights, (T, topk), "float32", device), topk, limit, q, ldo, space, size, _stream(stream, device))
 
 
-def w4_status(stream=0):
-    """Waits for the stream and raises if a wait inside a 4-bit product ran out since the last look (g5b_w4_status)."""
+def w4_status(stream=None):
+    """Waits for the stream (None: torch's current one of the current device) and raises if a wait inside a 4-bit product ran out on the
+    device since the last look (g5b_w4_status). Products of other streams count as far as they are over by then."""
+    if stream is None:
+        import sys
+        torch = sys.modules.get("torch")
+        stream = _stream(None, torch.cuda.current_device()) if torch is not None else 0
     _call_w4("g5b_w4_status", stream)

@@ -470,7 +470,8 @@ int g5b_w4_experts(const g5b_w4 *gate, const g5b_w4 *up, const g5b_w4 *down, con
                    size_t workspace_bytes, void *stream);
 
 /* Waits for `stream`, and says whether a wait inside a kernel of the two products above ran out on the current device since the
- * last look (all waits are bounded; none is expected to): -1 and a message then, and results since are undefined. */
+ * last look (all waits are bounded; none is expected to): -1 and a message then, and results since are undefined. What the look covers is one of the
+ * device: products of `stream` all, of other streams those that are over by then, so the last stream that has any is the one to give. */
 int g5b_w4_status(void *stream);
 
 #ifdef __cplusplus

@@ -307,6 +307,25 @@ def test_refused_calls_write_nothing(gpu_lib, T):
     _check(y.cpu(), ref.values(codes, scales, cols, group), x)
 
 
+def test_status_waits_for_the_current_stream(gpu_lib):
+    """A product behind some milliseconds of work on a side stream: the look, which is given no stream, comes after it."""
+    rows, cols, group = 300, 512, 128
+    codes, scales = ref.make(torch.Generator().manual_seed(1), rows, cols, group)
+    w, x, y = ref.handle(codes, scales, rows, cols, group), torch.ones((40, cols), device="cuda"), torch.empty((40, rows), device="cuda")
+    space = torch.empty(pkg.w4_matmul_workspace(w, x), dtype=torch.uint8, device="cuda")
+    big = torch.ones((8192, 8192), device="cuda", dtype=torch.bfloat16)
+    side, out = torch.cuda.Stream(), torch.empty_like(big)
+    for n in (1, 40):                                      # (what is set up at a first use waits for the device)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(n):
+                torch.mm(big, big, out=out)
+            pkg.w4_matmul(w, x, y, space)
+            pkg.w4_status()
+            assert side.query()
+    _check(y.cpu(), ref.values(codes, scales, cols, group), x)
+
+
 # ------------------------------------------------------------------ conversion ----
 def _quantized(v, group):
     """(codes as numbers 0..15 [rows][cols], scales [rows][groups]) of FP32 values, quotients in FP64."""

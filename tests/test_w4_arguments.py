@@ -173,3 +173,15 @@ def test_product_refusals_say_what_is_wrong():
                             (src(dtype=7), (128, 128), "dtype 7"), (src(dtype=pkg.DT_FP8), (0, 128), "scale blocks"), (src(dtype=pkg.DT_FP8), (128, -1), "scale blocks")):
         assert L.g5b_w4_quantize(t, *blocks, w, None) == -1 and word in _err(), _err()
     assert L.g5b_w4_quantize(src(), 128, 128, w, None) == -1 and "device" in _err()
+
+
+def test_status_looks_on_the_current_stream(monkeypatch):
+    """Where no stream is given: torch's current one of the current device, as for the calls whose waits it looks at."""
+    asked = []
+    monkeypatch.setattr(pkg, "_call_w4", lambda name, *args: asked.append((name, *args)))
+    monkeypatch.setattr(pkg, "_raw_stream", lambda device: 1000 + device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    pkg.w4_status()
+    pkg.w4_status(0)
+    pkg.w4_status(stream=77)
+    assert asked == [("g5b_w4_status", 1003), ("g5b_w4_status", 0), ("g5b_w4_status", 77)]
