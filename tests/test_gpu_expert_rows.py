@@ -167,6 +167,26 @@ def test_experts(gpu_lib, T, K, E, H, I, group, limit, how, dtype):
     assert worst <= 1.0, float(worst)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,E,H,I,group,down_group,how", [
+    (2, 2, 3, 4096, 40, 128, 64, "even"), (9, 4, 20, 4096, 24, 32, 128, "even"), (20, 4, 8, 4096, 24, 128, 32, "elsewhere"), (20, 4, 8, 4096, 24, 128, 64, "even"),
+    (40, 1, 2, 4224, 40, 64, 32, "even"), (3, 2, 3, 5000, 33, 128, 32, "skewed"), (9, 4, 20, 5000, 24, 64, 64, "outside"),
+    (3, 2, 3, 9728, 24, 64, 128, "even"), (9, 4, 20, 9728, 24, 128, 64, "skewed"), (3, 2, 3, 9856, 40, 32, 128, "even"), (20, 2, 3, 9856, 24, 128, 32, "even"),
+    (2, 2, 3, 17280, 24, 64, 128, "even"), (2, 2, 3, 48, 4224, 64, 128, "even"), (9, 4, 20, 40, 9856, 32, 64, "even"), (3, 2, 3, 40, 9856, 128, 32, "even")])
+def test_wide_experts(gpu_lib, T, K, E, H, I, group, down_group, how, dtype):
+    """A piece of 4096 columns, one and a part of the next, several; the widest that two rows' digits fit beside (9728 columns), one row's, none's; the
+    down matrix in groups of another size. Few experts and channels, the released width."""
+    rng = torch.Generator().manual_seed(T * 7 + H + I)
+    (gate, g), (up, u), (down, d) = _stack(rng, E, I, H, group), _stack(rng, E, I, H, group), _stack(rng, E, H, I, down_group)
+    idx = _picks(rng, T, K, E, how)
+    weights = torch.rand((T, K), generator=rng) * 2 - 0.5
+    x = (0.2 * torch.randn((T, H), generator=rng)).to(dtype)
+    got = _experts((gate, up, down), x.cuda(), idx, weights, 10.0, pad=T % 2)
+    want, off = ref.experts(x.double(), idx, weights, g, u, d, 10.0, dtype == torch.float32)
+    worst = ((got.double() - want).abs() / (off + ref.rounded(want, dtype))).max()
+    assert worst <= 1.0, float(worst)
+
+
 def test_experts_without_numbers_and_far_outside(gpu_lib):
     """A token with an infinity is NaN, its neighbours are not; picks far outside add nothing; a token without picks is zero."""
     rng = torch.Generator().manual_seed(21)

@@ -63,6 +63,17 @@ def test_small_integers_come_out_exactly(gpu_lib, rows, cols, group, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,group,T", [(40, 9728, 32, 2), (40, 9729, 128, 2), (33, 9729, 64, 1), (30, 17152, 32, 1), (30, 17153, 128, 1),
+                                               (20, 27649, 64, 1), (300, 131072, 128, 1), (17, 131072, 32, 1), (20, 131071, 64, 3)])
+def test_wide_rows(gpu_lib, rows, cols, group, T, dtype):
+    """Columns on both sides of where two rows' digits no longer fit, and one row's, up to the most that there may be."""
+    rng = torch.Generator().manual_seed(cols + T)
+    codes, scales = ref.make(rng, rows, cols, group)
+    x = torch.randn((T, cols), generator=rng).to(dtype)
+    _check(_run(codes, scales, rows, cols, group, x.cuda(), pad=T % 3), ref.values(codes, scales, cols, group), x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,cols,group,T", [(9473, 100, 32, 1), (9500, 2048, 128, 2), (20011, 1050, 64, 4), (12288, 1920, 32, 3), (9999, 129, 128, 1)])
 def test_many_short_rows(gpu_lib, rows, cols, group, T, dtype):
     rng = torch.Generator().manual_seed(rows + T)
