@@ -746,7 +746,7 @@ def w4_dequantize(w: W4, out, stream=None):
 
 
 def w4_matmul_workspace(w: W4, x) -> int:
-    """Bytes of workspace of w4_matmul for this x (g5b_w4_matmul_workspace)."""
+    """Bytes of workspace of w4_matmul for this x (g5b_w4_matmul_workspace); fewer rows can need more of it than many."""
     return lib().g5b_w4_matmul_workspace(w.ref, _rows("x", x, None)[1], x.shape[0])
 
 

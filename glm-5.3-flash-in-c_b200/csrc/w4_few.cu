@@ -9,7 +9,7 @@
 // One CTA per SM, persistent. Work comes in items of 16 weight rows (gate/up: eight gate rows and the eight up rows that go with them),
 // in pieces of 4096 columns; a CTA takes a contiguous share of them. Of up to 2048 columns an item is 32 rows: with two blocks of 128
 // columns to a warp its waits and the sums' meeting were most of an item (down products of 64 tokens' experts 282 us at 4.5 TB/s;
-// all three products 736 -> 648 us, BF16 rows 545 -> 505, 32768 x 800 past two rows 12.9 -> 11.2).
+// all three products 736 -> 648 us in short runs, 32768 x 800 past two rows 12.9 -> 10.3).
 //   warp 16   brings an item's rows into a ring in shared memory, one TMA load for the codes and one for the scales (gate/up: two
 //             each), as many ahead as fit: they wait for nothing but room, so HBM is busy while sums are put together and rows change.
 //             (A bulk copy per row was 125 cycles of issue each: 2.3 TB/s.)
@@ -26,7 +26,7 @@
 //   x         becomes digits in shared memory whenever the rows change (dense: once; experts: with the expert), in the order in
 //             which the lanes read them: per row and block of 128 columns the power of two below which its values lie, and
 //             integers of 31 bits and a sign in four digits, one bit less where the largest needs it: an FP32 number down to 2^-6 of the block's largest and a
-//             BF16 one down to 2^-22 as they are, what is smaller off by one unit, 2^-29 of the largest, at most. (Three digits of F32 rows and two of BF16
+//             BF16 one down to 2^-22 as they are (in groups of 128 even columns are off by half a unit), what is smaller by a unit, 2^-29 of the largest, at most. (Three digits of F32 rows and two of BF16
 //             ones, four of which then fit, were off by 2^-22 and 2^-14 of the largest: by 3e-5 and 8e-3 of a product whose weights of columns a
 //             thousand times the others are small. The fourth digit takes a column that was idle.)
 // Group sums are exact integers, taken into FP32 by the exponent trick: they start at the bits of 48, so that their bits are the float

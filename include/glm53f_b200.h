@@ -414,7 +414,8 @@ int g5b_engine_profile_read(g5b_engine *e, float *ms, int n, long *count, int re
  * a call can be captured into a graph. Rows are F32 or BF16 (G5B_DT_F32, G5B_DT_BF16), `ld` elements apart, unless noted.
  * Outputs must not overlap inputs. A workspace (device memory on a multiple of 256 bytes, as many bytes as the
  * _workspace function says) holds nothing between calls; calls that may run at the same time - on different
- * streams, or two captured graphs - each need their own. Results do not depend on what else is in a workspace, and are the same in
+ * streams, or two captured graphs - each need their own. Fewer rows can need more of it than many (parts of sums that many do without):
+ * a workspace for calls of several sizes has the largest of what each asks for. Results do not depend on what else is in a workspace, and are the same in
  * every run. Calls with no rows (T = 0) do nothing. Limits: 2^22 rows, 2^17 columns, 2^19 activation
  * rows, G5B_MAX_EXPERTS matrices, G5B_MAX_TOPK picks; beyond them, and for what does not fit together, -1 and a message. */
 typedef struct g5b_w4 {
@@ -436,8 +437,8 @@ int g5b_w4_quantize(const g5b_tensor *src, int br, int bc, const g5b_w4 *dst, vo
 int g5b_w4_dequantize(const g5b_w4 *w, int dtype, void *out, size_t ldo, void *stream);
 
 /* y[T][rows] = W x[T][cols], x and y of dtype (g5b_op_matvec of this format). Sums are FP32 or exact integers. What an activation
- * is held to: in calls of one or two rows 2^-29 of the largest of the 128 columns it lies in, from a multiple of 128 on, or
- * better; in calls of more rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
+ * is held to: in calls of one or two rows (past 9728 columns one, past 17152 none) 2^-29 of the largest of the 128 columns it lies in,
+ * from a multiple of 128 on, or better; in calls of more rows 2^-22 of itself (BF16: exactly), but no finer than 2^-38 of its row's largest. There a row of W whose
  * scales within 128 columns differ by more than 2^28 has products off by up to 2^-36 of the largest scale times the
  * activation; all others are exact. Scales and activations may have any finite magnitude: a result is a number where the magnitudes of its
  * products add up to one, and a product is off by 2^-127 of its row's largest activation at most where FP32's range ends. A row of x with an infinity or NaN gives NaN in all of its outputs. */
