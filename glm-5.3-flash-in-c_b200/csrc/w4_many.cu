@@ -14,7 +14,8 @@
 //          (A power of two for a whole row needs all its scales before the first product: 7000 cycles a tile in groups of 32.)
 //          Groups of 128: the codes alone (times 2^-17), and the scale on a step's sums.
 //   products, one warp to a block: D[128 rows of W][rows of x] += A * terms^T; the two terms of an F32 row go into the
-//          same sums one after the other, so that a converted block is used twice.
+//          same sums, so that a converted block is used twice: a step's lower terms all before its upper ones, because each instruction cuts
+//          what it adds to (products 2.5e-7 off 64 bits with the terms in turn, 1.0e-7 so; groups of 64 3.5e-7 and 1.8e-7).
 //   sums, four warps to a block: take a step's sums out of tensor memory, take the power of two off (groups of 128: put the
 //          scale on) and add them in registers, because the tensor cores cut off when they add; two accumulators in turn.
 //          Sums in registers are 2^-35 of what they stand for: rows of x below 2^14 past 2^17 columns of codes below 2^3 and a finite scale
@@ -267,11 +268,11 @@ __global__ void __launch_bounds__(many_threads<TERMS>(), 1) w4_many_kernel(const
                         const uint32_t d = tmem + (uint32_t)(b * 128 + buf * 64), ab = tmem + 256u + (uint32_t)(as * 128 + b * 64);
                         const uint32_t xb = smem_u32(xst) + (uint32_t)(xs * XB);
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
+                        for (int m = TERMS - 1; m >= 0; m--)
 #pragma unroll
-                            for (int m = 0; m < TERMS; m++) {
+                            for (int k = 0; k < 8; k++) {
                                 const uint64_t bd = tc_smem_desc(xb + (uint32_t)(((k >> 2) * TERMS + m) * a.n * 128)) + 2 * (k & 3);
-                                tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, k || m ? 1u : 0u);
+                                tc_mma_f16_ts(d, ab + (uint32_t)(k * 8), bd, idesc, k || m != TERMS - 1 ? 1u : 0u);
                             }
                         tc_commit(&a_empty[b][as]);
                         tc_commit(&x_empty[xs]);

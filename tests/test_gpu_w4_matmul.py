@@ -147,6 +147,22 @@ def test_scales_far_apart(gpu_lib, T, group, dtype):
     assert bool(((y - want).abs() <= off).all())
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T", [1, 3, 40, 70])
+def test_low_bits_beside_a_large_sum(gpu_lib, T, group):
+    """2^17 and then 7 times 16 columns of 32 + 29 2^-15, all weights one. In F16 terms the upper ones are multiples of the sum's unit, 2^-6, the lower ones of
+    16 columns 0.9 of it: a matrix instruction that adds those to the sum cuts them off, 6.3 units in all. Added up before the large ones they are cut
+    once, by less than a unit for each of an instruction's two cuts."""
+    rows, cols = 70, 128
+    codes, scales = ref.make(torch.Generator().manual_seed(1), rows, cols, group)
+    codes[:] = 0x99
+    scales[:, :cols // group] = 1.0
+    x = torch.full((T, cols), 32.0 + 29 * 2.0 ** -15)
+    x[:, :16] = 2.0 ** 13
+    y = _run(codes, scales, rows, cols, group, x.cuda()).double()
+    assert bool(((y - x[0].double().sum()).abs() <= 2 * 2.0 ** -6).all())
+
+
 @pytest.mark.parametrize("T", [1, 4, 30, 100])
 def test_zero_weights_give_zero(gpu_lib, T):
     rows, cols, group = 70, 500, 32
