@@ -6,6 +6,8 @@
 // single static: every answer belongs to the device that is current when it is asked for.
 #include <stdio.h>
 
+#include <mutex>
+
 #include "kernels.h"
 
 namespace g5b {
@@ -45,6 +47,10 @@ bool dev_opt_in_smem(const void *kernel, size_t bytes, SmemGrant &grant)
 {
     if (bytes <= 48 * 1024) return true;
     const int dev = dev_now();
+    if (grant.bytes[dev] >= bytes) return true;
+    // (one thread at a time, and never less than another was granted meanwhile: it may be about to launch with that)
+    static std::mutex one;
+    const std::lock_guard<std::mutex> hold(one);
     if (grant.bytes[dev] >= bytes) return true;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
         cudaGetLastError();

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/glm53f_b200.h"
 
 namespace g5b {
@@ -24,7 +26,7 @@ struct DMat {
 // Facts about, and one-time kernel set-up on, the device that is current at the call. Nothing is
 // cached across devices: a process may hold engines on several GPUs.
 constexpr int G5B_MAX_DEVICES = 64;
-struct SmemGrant { size_t bytes[G5B_MAX_DEVICES] = {}; };   // per kernel: what each device has granted
+struct SmemGrant { std::atomic<size_t> bytes[G5B_MAX_DEVICES]; };   // per kernel, in static storage: what each device has granted
 int  dev_now();
 int  dev_sms();
 bool dev_cooperative();

@@ -1,4 +1,6 @@
 """Products with 4-bit weights and group scales, and the conversion to them, against FP64 on the CPU."""
+import threading
+
 import pytest
 import torch
 
@@ -332,6 +334,40 @@ def test_refused_calls_write_nothing(gpu_lib, T):
     assert bool((y == 3.0).all())
     pkg.w4_matmul(w, x, y, space[:need])
     _check(y.cpu(), ref.values(codes, scales, cols, group), x)
+
+
+def test_threads_of_their_own(gpu_lib):
+    """Threads that call at once, each on a stream and with a workspace of its own, with products that want more shared memory one after the other:
+    what one thread alone gets, bit for bit."""
+    rng = torch.Generator().manual_seed(3)
+    work = []
+    for rows, cols, group in ((200, 320, 32), (300, 4096, 128), (100, 9000, 64)):
+        codes, scales = ref.make(rng, rows, cols, group)
+        for T in (1, 2, 5, 70):
+            work.append((ref.handle(codes, scales, rows, cols, group), torch.randn((T, cols), generator=rng).cuda()))
+
+    def run(order, out):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for i in order:
+                w, x = work[i]
+                y = torch.empty((x.shape[0], w.rows), device="cuda")
+                pkg.w4_matmul(w, x, y, torch.empty(pkg.w4_matmul_workspace(w, x), dtype=torch.uint8, device="cuda"))
+                out[i] = y
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    got = [{} for _ in range(6)]
+    threads = [threading.Thread(target=run, args=([(i * step + k) % len(work) for i in range(len(work))], got[k])) for k, step in enumerate((1, 5, 7, 11, 1, 5))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    alone = {}
+    run(range(len(work)), alone)
+    pkg.w4_status()
+    for out in got:
+        assert len(out) == len(work) and all(torch.equal(out[i], alone[i]) for i in alone)
 
 
 def test_status_waits_for_the_current_stream(gpu_lib):
